@@ -147,6 +147,133 @@ int knj_attention_step(const float* q, const float* k, const float* v, const flo
                        int n_head_kv, int head_dim, int n_ctx, uint16_t* k_cache, uint16_t* v_cache,
                        float* out, void* stream);
 
+/* ------------------------------------------------------------ speculative step
+ * The operators around a step that verifies drafted tokens: rotary positions of
+ * any layout and scaling, a cache in f16 or 8 bits written and read back, the
+ * attention of a tree of drafts over that cache, and the log probabilities of
+ * given tokens.  No counterpart in the reference, which decodes one token at a
+ * time.  These calls queue their kernels on `stream` and return: they allocate
+ * nothing, synchronise nothing and keep nothing between calls (scratch is the
+ * caller's `workspace`), so they can be captured into a HIP graph; two calls
+ * that may run at once need a workspace each.  All pointers are memory of the
+ * device opened by knj_device_open, which must be the calling thread's current
+ * one (KNJ_E_STATE otherwise).  `type` is that of the activations: KNJ_TYPE_F32,
+ * KNJ_TYPE_F16 or KNJ_TYPE_BF16; arithmetic is f32 (angles f64), rounded once.
+ * Rows of activations and caches start on 16-byte boundaries, their strides
+ * count elements; anything else is refused.  head_dim is 64 or 128. */
+
+/* knj_rope: every head of rows q [n_rows][n_head][head_dim] (and k
+ *   [n_rows][n_head_kv][head_dim]; n_head_kv 0: none) RMS-normalised with its
+ *   norm weight (NULL: not) and rotated at position pos[row]: the first n_rot
+ *   dims (a multiple of 8) in pairs (i, i + n_rot/2) (KNJ_ROPE_HALF) or
+ *   (2i, 2i + 1) (KNJ_ROPE_INTERLEAVED) by the angle pos * inv_freq[i], cos and
+ *   sin times mscale; the other dims pass.  Angles are formed in f64 (the decode
+ *   step's own tables hold f32 angles: they part by up to pos * 2^-24 radians).
+ *   An output may be its own input (the same pointer and stride).
+ * knj_rope_freqs (host only): the n_rot/2 frequencies base^(-2i/n_rot) under a
+ *   scaling for contexts `factor` (>= 1) times orig_ctx, to be copied to the
+ *   device, and mscale.  KNJ_ROPE_LINEAR: / factor.  KNJ_ROPE_NTK: base times
+ *   factor^(n_rot/(n_rot-2)).  KNJ_ROPE_YARN: a ramp between the two over the
+ *   dims whose wavelength turns p0 (beta_fast, e.g. 32) to p1 (beta_slow, e.g. 1)
+ *   times in orig_ctx, mscale 0.1 ln(factor) + 1.  KNJ_ROPE_LLAMA3: / factor for
+ *   wavelengths above orig_ctx/p0 (low_freq_factor), kept below orig_ctx/p1
+ *   (high_freq_factor), interpolated between. */
+#define KNJ_ROPE_HALF 0
+#define KNJ_ROPE_INTERLEAVED 1
+#define KNJ_ROPE_NONE 0
+#define KNJ_ROPE_LINEAR 1
+#define KNJ_ROPE_NTK 2
+#define KNJ_ROPE_YARN 3
+#define KNJ_ROPE_LLAMA3 4
+int knj_rope_freqs(int n_rot, double base, int scaling, double factor, int orig_ctx, double p0,
+                   double p1, double* inv_freq, float* mscale);
+int knj_rope(int type, int layout, int n_rot, const double* inv_freq, float mscale,
+             const int32_t* pos, int n_rows, int head_dim, const void* q, int n_head,
+             uint64_t q_stride, const float* q_norm, void* q_out, uint64_t q_out_stride,
+             const void* k, int n_head_kv, uint64_t k_stride, const float* k_norm, void* k_out,
+             uint64_t k_out_stride, float eps, void* stream);
+
+/* One layer's cache of n_seq sequences: k and v [n_head_kv][n_ctx][head_dim] per
+ *   sequence, sequence s at element s * seq_stride (the layout of the model's own
+ *   f16 cache; seq_stride 0: back to back), in one of three formats.  The 8-bit
+ *   ones hold a scale per (slot, kv head) in k_scale and v_scale [n_head_kv][n_ctx]
+ *   per sequence, sequence s at s * seq_stride / head_dim:
+ *   KNJ_KV_I8: scale = amax/127, codes rint(x * 127/amax);
+ *   KNJ_KV_F8: scale = amax/448, codes e4m3(x * 448/amax).
+ *   Codes are those of the exact quotient, ties to even.  A row whose largest
+ *   magnitude is below 2^-119 is stored as zeros; a row that holds an infinity or
+ *   a NaN reads back as NaN (KNJ_KV_F16 keeps them as they are).
+ * knj_kv_store: rows t < counts[s] (NULL: n_rows) of sequence s, k and v
+ *   [n_seq][n_rows][n_head_kv][head_dim] with row_stride elements from a row to
+ *   the next (of both), go to slots start[s] + t.  Rows that would fall outside
+ *   [0, n_ctx) are not stored.
+ * knj_kv_load: slots[s][t] (NULL: slot t) of the cache into rows k and v of the
+ *   same form, as code * scale rounded to `type`; rows whose slot is outside
+ *   [0, n_ctx) are left as they were.  Loaded as f32 and stored again, a row keeps
+ *   its codes, and its scale to a rounding: how an accepted path of drafts moves
+ *   to the end of the prefix. */
+#define KNJ_KV_F16 0
+#define KNJ_KV_F8 1
+#define KNJ_KV_I8 2
+typedef struct knj_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale; /* NULL with KNJ_KV_F16 */
+  float* v_scale;
+  uint64_t seq_stride;
+  int32_t format;
+  int32_t n_seq, n_head_kv, n_ctx, head_dim;
+} knj_kv_cache;
+int knj_kv_store(const knj_kv_cache* cache, int type, const void* k, const void* v,
+                 uint64_t row_stride, const int32_t* start, const int32_t* counts, int n_rows,
+                 void* stream);
+int knj_kv_load(const knj_kv_cache* cache, int type, const int32_t* slots, int n_rows, void* k,
+                void* v, uint64_t row_stride, void* stream);
+
+/* knj_attention_tree: attention of up to n_rows drafts per sequence over the
+ *   cache, which already holds the drafts' keys and values: draft t of sequence s
+ *   is in slot prefix[s] + t (t < counts[s]; NULL: n_rows) and sees the slots
+ *   before prefix[s] and those drafts u < counts[s] whose bit u % 64 of word u / 64
+ *   of its mask row is set: mask [n_seq][n_rows][ceil(n_rows/64)] words, one
+ *   [n_rows][..] for all sequences with mask_shared, NULL for a chain (u <= t).
+ *   q, out: [n_seq][n_rows][n_head][head_dim] with q_stride and out_stride
+ *   elements per row; out = softmax(scale * q.k) v over the slots seen.  Whatever
+ *   unseen slots hold counts for nothing, NaN included; a draft that sees nothing
+ *   gives zeros; rows past counts[s] are left as they were.  A draft that sees a
+ *   draft whose value row holds an infinity or a NaN gives NaN (all of its dims).
+ *   prefix[s] is held to [0, max_prefix] and counts[s] to [0, n_rows]; max_prefix +
+ *   n_rows <= n_ctx, n_rows <= 1024, scale in [1e-6, 1e6], n_head a multiple of n_head_kv.
+ *   out may be q.  With f32 activations the queries and the softmax's weights
+ *   keep 22 bits, with 16-bit ones the weights 11 (the outputs' own rounding).
+ * knj_attention_tree_workspace: bytes its workspace needs for these sizes (0 for
+ *   arguments that it refuses); any contents. */
+int knj_attention_tree(const knj_kv_cache* cache, int type, const void* q, uint64_t q_stride,
+                       int n_head, int n_rows, const int32_t* prefix, int max_prefix,
+                       const int32_t* counts, const uint64_t* mask, int mask_shared, float scale,
+                       void* out, uint64_t out_stride, void* workspace, uint64_t workspace_bytes,
+                       void* stream);
+uint64_t knj_attention_tree_workspace(const knj_kv_cache* cache, int n_head, int n_rows,
+                                      int max_prefix);
+
+/* knj_token_logprobs: of rows of logits [n_rows][n_vocab] (row_stride elements
+ *   from a row to the next, any alignment of `type`'s own), with x = logits /
+ *   temperature and lse = log sum exp(x):
+ *   logprob[row] = x[tokens[row]] - lse (tokens and logprob: both or neither; 0
+ *     where the token is negative, NaN where it is n_vocab or above);
+ *   entropy[row] = -sum p log p, p = exp(x - lse) (NULL: not computed);
+ *   top_idx, top_logprob [n_rows][n_top]: the n_top largest logits, largest first,
+ *     ties to the lowest index, with their log probabilities (n_top 0: none; at
+ *     most 32 and n_vocab).
+ *   -inf rules a token out.  A row with nothing left gives log probabilities of
+ *   -inf and an entropy of 0; a row that holds a NaN or +inf gives NaN (in top_idx a
+ *   NaN ranks as -inf).  n_vocab <= 2^20, n_rows * n_vocab / 2048 < 2^31.
+ * knj_token_logprobs_workspace: bytes of its workspace; any contents. */
+int knj_token_logprobs(int type, const void* logits, uint64_t row_stride, int n_rows, int n_vocab,
+                       float temperature, const int32_t* tokens, float* logprob, float* entropy,
+                       int n_top, int32_t* top_idx, float* top_logprob, void* workspace,
+                       uint64_t workspace_bytes, void* stream);
+uint64_t knj_token_logprobs_workspace(int n_rows, int n_vocab);
+
 /* ------------------------------------------------------------ model step
  * The device counterpart of knj::Model (/root/reference/src/model/model.h:55-80):
  * open -> forward(tokens, n) -> logits of the last token, reset(), pos().

@@ -25,12 +25,18 @@ LIB_PATH = os.path.join(HERE, "libkanjoos_amd.so")
 TYPE_F32, TYPE_F16, TYPE_Q4_K, TYPE_Q6_K, TYPE_BF16 = 0, 1, 12, 14, 30
 KNJ_OK, KNJ_E_CORRECTNESS, KNJ_E_ARCH, KNJ_E_ENV, KNJ_E_HIP, KNJ_E_ARG, KNJ_E_STATE = 0, 5, 6, 7, 9, 22, 23
 
+# rotary layouts and scalings (knj_rope, knj_rope_freqs), cache formats (knj_kv_cache)
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_NONE, ROPE_LINEAR, ROPE_NTK, ROPE_YARN, ROPE_LLAMA3 = 0, 1, 2, 3, 4
+KV_F16, KV_F8, KV_I8 = 0, 1, 2
+
 # every entry point include/knj_capi.h declares
 EXPORTS = (
     "knj_device_open", "knj_device_close", "knj_device_caps_get", "knj_check_arch",
     "knj_built_arch", "knj_last_error", "knj_malloc", "knj_free", "knj_memcpy_h2d",
     "knj_memcpy_d2h", "knj_memset_zero", "knj_synchronize", "knj_dequant", "knj_gemv",
-    "knj_rmsnorm", "knj_moe_router", "knj_moe_decode_layer", "knj_moe_decode_layer_noalloc", "knj_moe_batch_layer", "knj_attention_step", "knj_model_create_synthetic", "knj_model_create_from_image",
+    "knj_rmsnorm", "knj_rope_freqs", "knj_rope", "knj_kv_store", "knj_kv_load", "knj_attention_tree",
+    "knj_attention_tree_workspace", "knj_token_logprobs", "knj_token_logprobs_workspace", "knj_moe_router", "knj_moe_decode_layer", "knj_moe_decode_layer_noalloc", "knj_moe_batch_layer", "knj_attention_step", "knj_model_create_synthetic", "knj_model_create_from_image",
     "knj_model_free", "knj_model_image_bytes", "knj_model_image_device", "knj_model_layer_offsets", "knj_model_fill_kv", "knj_gguf_probe",
     "knj_model_create_from_gguf", "knj_model_config_get",
     "knj_model_download_image", "knj_model_reset", "knj_model_pos", "knj_model_set_pos",
@@ -91,6 +97,13 @@ class Span(C.Structure):
                 ("stream", C.c_int32), ("start_ns", C.c_uint64), ("end_ns", C.c_uint64)]
 
 
+class KvCacheDesc(C.Structure):
+    """``knj_kv_cache`` (include/knj_capi.h)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("seq_stride", C.c_uint64), ("format", C.c_int32), ("n_seq", C.c_int32), ("n_head_kv", C.c_int32),
+                ("n_ctx", C.c_int32), ("head_dim", C.c_int32)]
+
+
 class DeviceCaps(C.Structure):
     _fields_ = [
         ("gcn_arch", C.c_char * 32), ("name", C.c_char * 64), ("wave_size", C.c_int32),
@@ -104,6 +117,7 @@ class DeviceCaps(C.Structure):
 _P = C.c_void_p
 _i = C.c_int
 _f = C.c_float
+_d = C.c_double
 _u64 = C.c_uint64
 _SIGS = {
     "knj_device_open": (_i, [_i]),
@@ -129,6 +143,14 @@ _SIGS = {
     "knj_moe_batch_layer": (_i, [_P, _P, _f, _P, _P, _P, _P, _i, _i, _i, _i, _i, _i, _i, _P, _P,
                                   _P, _P, _P, _P]),
     "knj_attention_step": (_i, [_P, _P, _P, _P, _P, _f, _f, _i, _i, _i, _i, _i, _P, _P, _P, _P]),
+    "knj_rope_freqs": (_i, [_i, _d, _i, _d, _i, _d, _d, _P, C.POINTER(_f)]),
+    "knj_rope": (_i, [_i, _i, _i, _P, _f, _P, _i, _i, _P, _i, _u64, _P, _P, _u64, _P, _i, _u64, _P, _P, _u64, _f, _P]),
+    "knj_kv_store": (_i, [_P, _i, _P, _P, _u64, _P, _P, _i, _P]),
+    "knj_kv_load": (_i, [_P, _i, _P, _i, _P, _P, _u64, _P]),
+    "knj_attention_tree": (_i, [_P, _i, _P, _u64, _i, _i, _P, _i, _P, _P, _i, _f, _P, _u64, _P, _u64, _P]),
+    "knj_attention_tree_workspace": (_u64, [_P, _i, _i, _i]),
+    "knj_token_logprobs": (_i, [_i, _P, _u64, _i, _i, _f, _P, _P, _P, _i, _P, _P, _P, _u64, _P]),
+    "knj_token_logprobs_workspace": (_u64, [_i, _i]),
     "knj_model_create_synthetic": (_i, [C.POINTER(ModelConfig), _u64, C.POINTER(_P)]),
     "knj_model_create_from_image": (_i, [C.POINTER(ModelConfig), _P, _u64, C.POINTER(_P)]),
     "knj_model_free": (_i, [_P]),
@@ -339,6 +361,116 @@ def attention_step(q, k, v, q_norm, k_norm, eps, rope_base, pos, n_head, n_head_
     check(lib().knj_attention_step(_p(q), _p(k), _p(v), _p(q_norm), _p(k_norm), eps, rope_base, pos,
                                    n_head, n_head_kv, head_dim, n_ctx, _p(k_cache), _p(v_cache),
                                    _p(out), None))
+
+
+# ------------------------------------------------------------------ speculative step
+#
+# Operators around a step that verifies drafted tokens (include/knj_capi.h, "speculative step").  They
+# queue on `stream` and return; buffers must live until the stream has passed them.
+
+def rope_freqs(n_rot: int, base: float, scaling: int = ROPE_NONE, factor: float = 1.0, orig_ctx: int = 0,
+               p0: float | None = None, p1: float | None = None):
+    """(inv_freq float64 [n_rot / 2], mscale) of a rotary scaling (knj_rope_freqs); p0, p1 default to the
+    published ones (YaRN 32 and 1 turns, Llama 3 factors 1 and 4)."""
+    dflt = {ROPE_YARN: (32.0, 1.0), ROPE_LLAMA3: (1.0, 4.0)}.get(scaling, (0.0, 0.0))
+    out = np.empty(max(n_rot, 0) // 2, np.float64)
+    ms = C.c_float()
+    check(lib().knj_rope_freqs(n_rot, base, scaling, factor, orig_ctx, dflt[0] if p0 is None else p0,
+                               dflt[1] if p1 is None else p1, _ptr(out), C.byref(ms)))
+    return out, ms.value
+
+
+def rope(type_id: int, q, k, pos, inv_freq, n_rows: int, n_head: int, n_head_kv: int, head_dim: int, q_out=None,
+         k_out=None, n_rot: int | None = None, layout: int = ROPE_HALF, mscale: float = 1.0, q_norm=None, k_norm=None,
+         eps: float = 1e-6, q_stride: int | None = None, k_stride: int | None = None, q_out_stride: int | None = None,
+         k_out_stride: int | None = None, stream=None) -> None:
+    """Normalises (with a norm weight) and rotates rows of queries and keys (knj_rope).  Outputs default to
+    in place; strides default to packed rows (an output in place takes its input's)."""
+    q_stride = n_head * head_dim if q_stride is None else q_stride
+    k_stride = n_head_kv * head_dim if k_stride is None else k_stride
+    if q_out is None:
+        q_out, q_out_stride = q, q_stride
+    if k_out is None:
+        k_out, k_out_stride = k, k_stride
+    check(lib().knj_rope(type_id, layout, head_dim if n_rot is None else n_rot, _p(inv_freq), mscale, _p(pos), n_rows,
+                         head_dim, _p(q), n_head, q_stride, _p(q_norm), _p(q_out),
+                         n_head * head_dim if q_out_stride is None else q_out_stride, _p(k), n_head_kv, k_stride,
+                         _p(k_norm), _p(k_out), n_head_kv * head_dim if k_out_stride is None else k_out_stride, eps,
+                         stream))
+
+
+class KvCache:
+    """A layer's cache of several sequences in f16 or 8 bits (knj_kv_cache) over given buffers, or with
+    :meth:`allocate` over its own."""
+
+    def __init__(self, format: int, n_seq: int, n_head_kv: int, n_ctx: int, head_dim: int, k, v, k_scale=None,
+                 v_scale=None, seq_stride: int = 0):
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.desc = KvCacheDesc(_p(k), _p(v), _p(k_scale), _p(v_scale), seq_stride, format, n_seq, n_head_kv, n_ctx,
+                                head_dim)
+        self.ref = C.addressof(self.desc)
+
+    @classmethod
+    def allocate(cls, format: int, n_seq: int, n_head_kv: int, n_ctx: int, head_dim: int) -> "KvCache":
+        rows = n_seq * n_head_kv * n_ctx
+        bufs = [DeviceBuffer(rows * head_dim * (2 if format == KV_F16 else 1)) for _ in range(2)]
+        bufs += [None, None] if format == KV_F16 else [DeviceBuffer(4 * rows) for _ in range(2)]
+        for b in bufs:
+            if b is not None:
+                b.zero()
+        return cls(format, n_seq, n_head_kv, n_ctx, head_dim, *bufs)
+
+
+def kv_store(cache: KvCache, type_id: int, k, v, start, n_rows: int, counts=None, row_stride: int | None = None,
+             stream=None) -> None:
+    """Rows t < counts[s] of every sequence into slots start[s] + t (knj_kv_store)."""
+    d = cache.desc
+    check(lib().knj_kv_store(cache.ref, type_id, _p(k), _p(v),
+                             d.n_head_kv * d.head_dim if row_stride is None else row_stride, _p(start), _p(counts),
+                             n_rows, stream))
+
+
+def kv_load(cache: KvCache, type_id: int, k, v, n_rows: int, slots=None, row_stride: int | None = None,
+            stream=None) -> None:
+    """Slots of every sequence (slots [n_seq][n_rows]; None: slot t) read back into rows k and v (knj_kv_load)."""
+    d = cache.desc
+    check(lib().knj_kv_load(cache.ref, type_id, _p(slots), n_rows, _p(k), _p(v),
+                            d.n_head_kv * d.head_dim if row_stride is None else row_stride, stream))
+
+
+def attention_tree_workspace(cache: KvCache, n_head: int, n_rows: int, max_prefix: int) -> int:
+    """Bytes of workspace that attention_tree needs for these sizes (0: none)."""
+    return lib().knj_attention_tree_workspace(cache.ref, n_head, n_rows, max_prefix)
+
+
+def attention_tree(cache: KvCache, type_id: int, q, out, n_head: int, n_rows: int, prefix, max_prefix: int,
+                   workspace: DeviceBuffer | None = None, counts=None, mask=None, mask_shared: bool = False,
+                   scale: float | None = None, q_stride: int | None = None, out_stride: int | None = None,
+                   stream=None) -> None:
+    """Attention of a tree of drafts per sequence over the cache (knj_attention_tree); scale defaults to
+    1 / sqrt(head_dim)."""
+    d = cache.desc
+    width = n_head * d.head_dim
+    check(lib().knj_attention_tree(cache.ref, type_id, _p(q), width if q_stride is None else q_stride, n_head, n_rows,
+                                   _p(prefix), max_prefix, _p(counts), _p(mask), int(mask_shared),
+                                   d.head_dim ** -0.5 if scale is None else scale, _p(out),
+                                   width if out_stride is None else out_stride, _p(workspace),
+                                   workspace.nbytes if workspace is not None else 0, stream))
+
+
+def token_logprobs_workspace(n_rows: int, n_vocab: int) -> int:
+    """Bytes of workspace that token_logprobs needs."""
+    return lib().knj_token_logprobs_workspace(n_rows, n_vocab)
+
+
+def token_logprobs(type_id: int, logits, n_rows: int, n_vocab: int, workspace: DeviceBuffer, tokens=None, logprob=None,
+                   entropy=None, n_top: int = 0, top_idx=None, top_logprob=None, temperature: float = 1.0,
+                   row_stride: int | None = None, stream=None) -> None:
+    """Log probabilities of given tokens, the rows' entropy and their n_top largest logits (knj_token_logprobs)."""
+    check(lib().knj_token_logprobs(type_id, _p(logits), n_vocab if row_stride is None else row_stride, n_rows, n_vocab,
+                                   temperature, _p(tokens), _p(logprob), _p(entropy), n_top, _p(top_idx),
+                                   _p(top_logprob), _p(workspace), workspace.nbytes if workspace is not None else 0,
+                                   stream))
 
 
 # ------------------------------------------------------------------ model

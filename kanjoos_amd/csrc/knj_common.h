@@ -37,6 +37,21 @@ int hip_fail(hipError_t e, const char* what);
 // Refuses launches before knj_device_open() has passed the arch guard.
 int require_open();
 
+// The same, and the calling thread's current device is the opened one (calls
+// that take device memory of any stream without a scratch of the library's).
+int require_device();
+
+// Bytes of an activation of `type` (KNJ_TYPE_F32, F16 or BF16), 0 for another type.
+inline int act_bytes(int type) {
+  return type == KNJ_TYPE_F32 ? 4 : type == KNJ_TYPE_F16 || type == KNJ_TYPE_BF16 ? 2 : 0;
+}
+// Rows that 16-byte loads can take: base and row stride on 16-byte boundaries.
+inline bool rows_aligned(const void* p, uint64_t stride, int elem_bytes) {
+  return ((uintptr_t)p & 15) == 0 && (stride * (uint64_t)elem_bytes & 15) == 0;
+}
+// KNJ_E_ARG, with the reason, for a cache description that is not one.
+int check_kv_cache(const knj_kv_cache* c);
+
 // Per-device scratch owned by the library (partials, counters); grown on
 // demand, never shrunk, released at knj_device_close().
 void* device_scratch(uint64_t bytes, hipStream_t stream);
@@ -264,6 +279,61 @@ bool prefill_attention_ok(int n_head, int n_head_kv, int head_dim);
 // Scratch the prompt-pass attention needs for up to max_rows rows.
 uint64_t prefill_partial_bytes(int n_head, int n_head_kv, int head_dim, int max_rows);
 hipError_t launch_prefill_attention(const PrefillAttnArgs& a, hipStream_t s);
+
+// ---------------------------------------------------------------- speculative step
+struct RopeArgs {
+  const void *q, *k;          // [n_rows][n_head][D], [n_rows][n_head_kv][D]
+  void *q_out, *k_out;
+  uint64_t q_stride, k_stride, q_out_stride, k_out_stride;  // elements per row
+  const float *q_norm, *k_norm;  // optional [D]
+  float eps;
+  const double* inv_freq;     // [n_rot / 2]
+  float mscale;
+  const int32_t* pos;         // [n_rows]
+  int n_rows, n_head, n_head_kv, n_rot;
+};
+hipError_t launch_rope(int type, int layout, int head_dim, const RopeArgs& a, hipStream_t s);
+
+struct KvRowsArgs {
+  knj_kv_cache c;             // seq_stride filled in
+  void *k, *v;                // activation rows [n_seq][n_rows][n_head_kv][D] (read by the store)
+  uint64_t row_stride;
+  const int32_t* index;       // store: start [n_seq]; load: slots [n_seq][n_rows] or null
+  const int32_t* counts;      // store: [n_seq] or null
+  int n_rows;
+};
+hipError_t launch_kv_store(int type, const KvRowsArgs& a, hipStream_t s);
+hipError_t launch_kv_load(int type, const KvRowsArgs& a, hipStream_t s);
+
+struct TreeArgs {
+  knj_kv_cache c;             // seq_stride filled in
+  const void* q;              // [n_seq][n_rows][n_head][D]
+  void* out;
+  uint64_t q_stride, out_stride;
+  const int32_t* prefix;      // [n_seq]
+  const int32_t* counts;      // [n_seq] or null
+  const uint64_t* mask;       // [n_seq or 1][n_rows][words] or null (chain)
+  float* partial;             // split records
+  float scale;
+  int n_head, n_rows, max_prefix, mask_shared;
+  int type;                   // of q and out
+};
+uint64_t tree_partial_bytes(const knj_kv_cache& c, int n_head, int n_rows, int max_prefix);
+hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t s);
+
+struct LogprobArgs {
+  const void* logits;
+  uint64_t row_stride;
+  int n_rows, n_vocab, n_top;
+  double inv_temp;
+  const int32_t* tokens;
+  float *logprob, *entropy;
+  int32_t* top_idx;
+  float* top_logprob;
+  void* records;              // logprob_record_bytes
+};
+uint64_t logprob_record_bytes(int n_rows, int n_vocab);
+hipError_t launch_token_logprobs(int type, const LogprobArgs& a, hipStream_t s);
 
 // Decode-step control block in device memory: the token fed to the step, its
 // position, the index into the output token ring, and the packed argmax of the

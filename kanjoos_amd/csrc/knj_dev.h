@@ -57,6 +57,16 @@ __device__ __forceinline__ uint16_t f2h(float v) {
   return __builtin_bit_cast(unsigned short, (_Float16)v);
 }
 
+// Two f32 as 16-bit activations of TYPE (f16 or bf16, round to nearest even), the
+// first in the low half.
+template <int TYPE>
+__device__ __forceinline__ uint32_t pack_act(float a, float b) {
+  if constexpr (TYPE == KNJ_TYPE_F16) return (uint32_t)f2h(a) | ((uint32_t)f2h(b) << 16);
+  else
+    return (uint32_t)__builtin_bit_cast(unsigned short, (__bf16)a) |
+           ((uint32_t)__builtin_bit_cast(unsigned short, (__bf16)b) << 16);
+}
+
 // ---- cross-lane moves without the LDS crossbar.  Rows of 16 lanes exchange
 // through DPP (quad permutes, the 8- and 16-lane mirrors, row rotation); rows
 // and half-waves through the gfx950 permlane swaps.  Every lane of the group

@@ -52,6 +52,18 @@ int require_open() {
   return KNJ_OK;
 }
 
+int require_device() {
+  const int rc = require_open();
+  if (rc) return rc;
+  int dev = -1;
+  KNJ_HIP(hipGetDevice(&dev));
+  if (dev != g_device) {
+    set_error("the current device is not the one knj_device_open opened");
+    return KNJ_E_STATE;
+  }
+  return KNJ_OK;
+}
+
 void* device_scratch(uint64_t bytes, hipStream_t stream) {
   std::lock_guard<std::mutex> g(g_mu);
   if (bytes > g_scratch_bytes) {

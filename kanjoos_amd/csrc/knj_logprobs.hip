@@ -1,0 +1,339 @@
+// kanjoos_amd/csrc/knj_logprobs.hip -- log probabilities of given tokens over rows of logits, with
+// the rows' entropy and their largest entries.
+//
+// Two launches.  The first reads every logit once: a wave takes 2048 of a row
+// into registers and leaves a record of them -- the largest (value and index),
+// the sum of the others' exponentials relative to it, and the entropy's sum.
+// The second, a workgroup per row, joins a row's records in f64 and finds the
+// n largest logits: only the n pieces with the largest maxima can hold any, so
+// those n (of 75 at a vocabulary of 151,936) are read again.
+#include <string>
+
+#include "knj_common.h"
+#include "knj_dev.h"
+
+namespace knj {
+namespace {
+
+using namespace dev;
+
+constexpr int kPiece = 2048;   // logits of one wave
+constexpr int kPer = kPiece / 64;
+constexpr int kMaxTop = 32;
+constexpr int kMaxVocab = 1 << 20;
+constexpr int kMaxPieces = kMaxVocab / kPiece;  // 512
+constexpr int kJoin = 512;     // threads of the joining workgroup
+
+struct Record {
+  uint32_t key;   // order_key of the piece's largest logit
+  uint32_t idx;   // its index in the row
+  float rest;     // sum over the piece's other logits of 2^((x - max) c); NaN: the piece holds a NaN or +inf
+  float ent;      // sum over them of 2^((x - max) c) (x - max) c
+};
+
+// Unsigned keys in the order of the floats (+0 and -0 alike); at least
+// 0x007FFFFF (-inf), so 0 is below every logit.
+__device__ __forceinline__ uint32_t order_key(float v) {
+  const uint32_t u = __float_as_uint(v + 0.0f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float order_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
+}
+
+// Where lane l's value i of a piece stands in the row.
+template <int TYPE>
+__device__ __forceinline__ int piece_index(int piece, int lane, int i) {
+  constexpr int V = TYPE == KNJ_TYPE_F32 ? 4 : 8;  // values per 16 bytes
+  return piece * kPiece + ((i / V) * 64 + lane) * V + i % V;
+}
+
+// A piece of a row, kPer values per lane, -inf past the row's end; 16-byte loads
+// at the alignment of the type (the device runs with unaligned access on).
+template <int TYPE>
+__device__ __forceinline__ void load_piece(const void* logits, uint64_t row_at, int piece, int n_vocab, int lane,
+                                           float (&v)[kPer]) {
+  constexpr int V = TYPE == KNJ_TYPE_F32 ? 4 : 8, EB = 16 / V;
+  const char* base = (const char*)logits + row_at * EB;
+#pragma unroll
+  for (int j = 0; j < kPer / V; ++j) {
+    const int at = piece_index<TYPE>(piece, lane, j * V);
+    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+    if (at + V <= n_vocab) {
+      __builtin_memcpy(&w, base + (uint64_t)at * EB, 16);
+    } else if (at < n_vocab) {
+      uint32_t t[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (at + i < n_vocab) {
+          if constexpr (EB == 4) t[i] = ((const uint32_t*)base)[at + i];
+          else t[i / 2] |= (uint32_t)((const uint16_t*)base)[at + i] << (16 * (i & 1));
+        }
+      }
+      w = make_uint4(t[0], t[1], t[2], t[3]);
+    }
+    const uint32_t t[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float x;
+      if constexpr (TYPE == KNJ_TYPE_F32) x = __uint_as_float(t[i]);
+      else if constexpr (TYPE == KNJ_TYPE_F16) x = h2f(t[i / 2] >> (16 * (i & 1)));
+      else x = __uint_as_float((i & 1) ? (t[i / 2] & 0xFFFF0000u) : (t[i / 2] << 16));
+      v[j * V + i] = at + i < n_vocab ? x : -INFINITY;
+    }
+  }
+}
+
+// Record of one piece per wave.  With the largest logit m of the piece and
+// d = (x - m) log2(e) / T <= 0: rest = sum 2^d, ent = sum 2^d d over all but the
+// largest itself, so that a row with one likely token keeps log(1 + rest) to the
+// rest's own precision.  log2(e)/T comes as two floats (its rounding would be a
+// common error of every term).
+template <int TYPE>
+__global__ __launch_bounds__(kBlock) void k_logprob_pieces(LogprobArgs a, int n_pieces, float c_hi, float c_lo) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t w = blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6);
+  const uint32_t row = w / (uint32_t)n_pieces, piece = w - row * (uint32_t)n_pieces;
+  if (row >= (uint32_t)a.n_rows) return;
+  float v[kPer];
+  load_piece<TYPE>(a.logits, (uint64_t)row * a.row_stride, piece, a.n_vocab, lane, v);
+  bool bad = false;
+  float best = -INFINITY;
+  int bi = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    bad |= v[i] != v[i] || v[i] == INFINITY;
+    v[i] = v[i] == v[i] ? v[i] : -INFINITY;
+    if (v[i] > best) {
+      best = v[i];
+      bi = i;
+    }
+  }
+  const uint32_t idx = piece_index<TYPE>(piece, lane, bi);
+  const unsigned long long top =
+      wave_max_u64(((unsigned long long)order_key(best) << 32) | (0xFFFFFFFFu - idx));
+  const uint32_t top_idx = 0xFFFFFFFFu - (uint32_t)top;
+  const float m = order_value((uint32_t)(top >> 32));
+  const int skip = idx == top_idx ? bi : -1;
+  float rest = 0.0f, ent = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const float t = v[i] - m;
+    // (-inf, and -inf - -inf, weigh nothing: held where 2^d is 0 and d finite)
+    const float d = fmaxf(fmaf(t, c_hi, t * c_lo), -16384.0f);
+    const float e = i == skip ? 0.0f : __builtin_amdgcn_exp2f(d);
+    rest += e;
+    ent = fmaf(e, d, ent);
+  }
+  rest = group_sum<64>(rest);
+  ent = group_sum<64>(ent);
+  bad = __ballot(bad) != 0;
+  if (lane == 0)
+    ((Record*)a.records)[w] = Record{(uint32_t)(top >> 32), top_idx, bad ? NAN : rest, ent};
+}
+
+// A row's records joined.  With M the row's largest logit, f = 2^((m - M) c) of
+// each piece: rest = sum over the pieces of f (1 + rest_p), without the 1 of the
+// piece that holds M, and ent = sum of f (ent_p + (1 + rest_p) (m - M) c); then
+// log sum e^(x - M) = log1p(rest), the entropy log1p(rest) - ln 2 ent / (1 + rest).
+template <int TYPE>
+__global__ __launch_bounds__(kJoin) void k_logprob_join(LogprobArgs a, int n_pieces, double c) {
+  constexpr int W = kJoin / 64;
+  __shared__ unsigned long long keys[kMaxPieces];
+  __shared__ unsigned long long cand[kMaxTop * (kMaxTop + 1) / 2];
+  __shared__ unsigned long long red_key[W];
+  __shared__ double red_rest[W], red_ent[W];
+  __shared__ int red_bad[W], chosen[kMaxTop];
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const Record* rec = (const Record*)a.records + (uint64_t)row * n_pieces;
+  Record r{0u, 0u, 0.0f, 0.0f};
+  unsigned long long key = 0;
+  if (tid < n_pieces) {  // n_pieces <= kMaxPieces = kJoin
+    r = rec[tid];
+    key = ((unsigned long long)r.key << 32) | (0xFFFFFFFFu - r.idx);
+  }
+  keys[tid] = key;
+  const unsigned long long wk = wave_max_u64(key);
+  if (lane == 0) red_key[wave] = wk;
+  __syncthreads();
+  unsigned long long top = red_key[0];
+#pragma unroll
+  for (int i = 1; i < W; ++i) top = red_key[i] > top ? red_key[i] : top;
+  const float M = order_value((uint32_t)(top >> 32));
+  double rest = 0.0, ent = 0.0;
+  bool bad = tid < n_pieces && r.rest != r.rest;
+  const float m = order_value(r.key);
+  if (tid < n_pieces && m > -INFINITY && M < INFINITY && !bad) {
+    const double d = ((double)m - (double)M) * c;
+    const double f = exp2(d);
+    const double own = (double)r.rest + (key == top ? 0.0 : 1.0);
+    rest = f * own;
+    ent = f * ((double)r.ent + (1.0 + (double)r.rest) * d);
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    rest += __shfl_xor(rest, o);
+    ent += __shfl_xor(ent, o);
+  }
+  bad = __ballot(bad) != 0;
+  if (lane == 0) {
+    red_rest[wave] = rest;
+    red_ent[wave] = ent;
+    red_bad[wave] = bad;
+  }
+  __syncthreads();
+  rest = ent = 0.0;
+  bad = false;
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    rest += red_rest[i];
+    ent += red_ent[i];
+    bad |= red_bad[i] != 0;
+  }
+  const bool none = M == -INFINITY;  // nothing left in the row
+  const double lse = log1p(rest);    // above M / T
+  // log probability of a logit x of this row
+  auto logp = [&](float x) -> float {
+    if (bad) return NAN;
+    if (none || x == -INFINITY) return -INFINITY;
+    return (float)(((double)x - (double)M) * a.inv_temp - lse);
+  };
+  if (tid == 0) {
+    if (a.entropy) a.entropy[row] = bad ? NAN : none ? 0.0f : (float)(lse - 0.6931471805599453 * ent / (1.0 + rest));
+    if (a.logprob) {
+      const int t = a.tokens[row];
+      float lp = t < 0 ? 0.0f : NAN;
+      if (t >= 0 && t < a.n_vocab) {
+        const uint64_t at = (uint64_t)row * a.row_stride + t;
+        float x;
+        if constexpr (TYPE == KNJ_TYPE_F32) x = ((const float*)a.logits)[at];
+        else if constexpr (TYPE == KNJ_TYPE_F16) x = h2f(((const uint16_t*)a.logits)[at]);
+        else x = __uint_as_float((uint32_t)((const uint16_t*)a.logits)[at] << 16);
+        lp = logp(x);
+      }
+      a.logprob[row] = lp;
+    }
+  }
+  const int n = a.n_top;
+  if (n == 0) return;
+  // the n pieces with the largest keys, by rank (keys differ: their indexes do)
+  if (tid < n_pieces) {
+    int rank = 0;
+    for (int j = 0; j < n_pieces; ++j) rank += keys[j] > key;
+    if (rank < n) chosen[rank] = tid;
+  }
+  for (int i = tid; i < kMaxTop * (kMaxTop + 1) / 2; i += kJoin) cand[i] = 0;
+  __syncthreads();
+  const int n_sel = min(n, n_pieces);
+  // every one of the n largest logits is at least the n-th piece's largest
+  const unsigned long long least = n_pieces >= n ? keys[chosen[n - 1]] : 1ull;
+  // wave by wave: the chosen piece of rank q holds at most n - q of them, taken
+  // out one after the other into its own places
+  for (int q = wave; q < n_sel; q += W) {
+    const int piece = chosen[q];
+    float v[kPer];
+    load_piece<TYPE>(a.logits, (uint64_t)row * a.row_stride, piece, a.n_vocab, lane, v);
+    uint32_t u[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      u[i] = piece_index<TYPE>(piece, lane, i) < a.n_vocab ? order_key(v[i] == v[i] ? v[i] : -INFINITY) : 0u;
+    const int at = q * n - q * (q - 1) / 2;
+    for (int t = 0; t < n - q; ++t) {
+      uint32_t best = 0;
+      int bi = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (u[i] > best) {
+          best = u[i];
+          bi = i;
+        }
+      const uint32_t idx = piece_index<TYPE>(piece, lane, bi);
+      const unsigned long long mine = best ? ((unsigned long long)best << 32) | (0xFFFFFFFFu - idx) : 0ull;
+      const unsigned long long big = wave_max_u64(mine);
+      if (big < least) break;  // (uniform; also when the piece is used up)
+      if (lane == 0) cand[at + t] = big;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) u[i] = (mine == big && i == bi) ? 0u : u[i];
+    }
+  }
+  __syncthreads();
+  const int n_cand = n_sel * n - n_sel * (n_sel - 1) / 2;
+  for (int i = tid; i < n_cand; i += kJoin) {
+    const unsigned long long mine = cand[i];
+    if (!mine) continue;
+    int rank = 0;
+    for (int j = 0; j < n_cand; ++j) rank += cand[j] > mine;
+    if (rank < n) {
+      a.top_idx[(uint64_t)row * n + rank] = (int32_t)(0xFFFFFFFFu - (uint32_t)mine);
+      a.top_logprob[(uint64_t)row * n + rank] = logp(order_value((uint32_t)(mine >> 32)));
+    }
+  }
+}
+
+int pieces_of(int n_vocab) { return (n_vocab + kPiece - 1) / kPiece; }
+
+}  // namespace
+
+uint64_t logprob_record_bytes(int n_rows, int n_vocab) {
+  return (uint64_t)n_rows * pieces_of(n_vocab) * sizeof(Record);
+}
+
+hipError_t launch_token_logprobs(int type, const LogprobArgs& a, hipStream_t s) {
+  const int n_pieces = pieces_of(a.n_vocab);
+  const uint64_t waves = (uint64_t)a.n_rows * n_pieces;
+  const dim3 grid((unsigned)((waves + kBlock / 64 - 1) / (kBlock / 64)));
+  const double c = 1.4426950408889634 * a.inv_temp;
+  const float c_hi = (float)c, c_lo = (float)(c - (double)c_hi);
+#define KNJ_LOGPROBS(TYPE)                                                                            \
+  do {                                                                                                \
+    KNJ_LAUNCH(k_logprob_pieces<TYPE>, grid, dim3(kBlock), 0, s, a, n_pieces, c_hi, c_lo);            \
+    KNJ_LAUNCH(k_logprob_join<TYPE>, dim3(a.n_rows), dim3(kJoin), 0, s, a, n_pieces, c);              \
+  } while (0)
+  if (type == KNJ_TYPE_F32) KNJ_LOGPROBS(KNJ_TYPE_F32);
+  else if (type == KNJ_TYPE_F16) KNJ_LOGPROBS(KNJ_TYPE_F16);
+  else KNJ_LOGPROBS(KNJ_TYPE_BF16);
+#undef KNJ_LOGPROBS
+  return hipGetLastError();
+}
+
+}  // namespace knj
+
+using namespace knj;
+
+extern "C" {
+
+int knj_token_logprobs(int type, const void* logits, uint64_t row_stride, int n_rows, int n_vocab,
+                       float temperature, const int32_t* tokens, float* logprob, float* entropy,
+                       int n_top, int32_t* top_idx, float* top_logprob, void* workspace,
+                       uint64_t workspace_bytes, void* stream) {
+  const int eb = act_bytes(type);
+  KNJ_CHECK_ARG(eb, "logits must be F32, F16 or BF16");
+  KNJ_CHECK_ARG(logits, "null pointer");
+  KNJ_CHECK_ARG(((uintptr_t)logits & (eb - 1)) == 0, "the logits must be aligned to their type");
+  KNJ_CHECK_ARG(n_rows >= 0, "negative row count");
+  KNJ_CHECK_ARG(n_vocab > 0 && n_vocab <= kMaxVocab, "n_vocab must be in [1, 2^20]");
+  KNJ_CHECK_ARG(row_stride >= (uint64_t)n_vocab, "the row stride is below the row's width");
+  KNJ_CHECK_ARG((uint64_t)n_rows * pieces_of(n_vocab) < (1ull << 31), "too many rows for one call");
+  KNJ_CHECK_ARG(temperature >= 1e-4f && temperature <= 1e4f, "the temperature must be in [1e-4, 1e4]");
+  KNJ_CHECK_ARG(!tokens == !logprob, "tokens and logprob go together");
+  KNJ_CHECK_ARG(n_top >= 0 && n_top <= kMaxTop && n_top <= n_vocab, "n_top must be in [0, min(32, n_vocab)]");
+  KNJ_CHECK_ARG(n_top == 0 || (top_idx && top_logprob), "null top_idx or top_logprob");
+  const uint64_t need = logprob_record_bytes(n_rows, n_vocab);
+  if (n_rows && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) {
+    set_error("knj_token_logprobs: these sizes need a 16-byte aligned workspace of " + std::to_string(need) + " bytes");
+    return KNJ_E_ARG;
+  }
+  const int rc = require_device();
+  if (rc || n_rows == 0) return rc;
+  LogprobArgs a{logits, row_stride, n_rows, n_vocab, n_top, 1.0 / (double)temperature, tokens, logprob, entropy,
+                top_idx, top_logprob, workspace};
+  KNJ_HIP(launch_token_logprobs(type, a, (hipStream_t)stream));
+  return KNJ_OK;
+}
+
+uint64_t knj_token_logprobs_workspace(int n_rows, int n_vocab) {
+  if (n_rows <= 0 || n_vocab <= 0 || n_vocab > kMaxVocab) return 0;
+  return logprob_record_bytes(n_rows, n_vocab);
+}
+
+}  // extern "C"
