@@ -318,7 +318,7 @@ struct TreeArgs {
   int n_head, n_rows, max_prefix, mask_shared;
   int type;                   // of q and out
 };
-uint64_t tree_partial_bytes(const knj_kv_cache& c, int n_head, int n_rows, int max_prefix);
+uint64_t tree_partial_bytes(const knj_kv_cache& c, int type, int n_head, int n_rows, int max_prefix);
 hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t s);
 
 struct LogprobArgs {

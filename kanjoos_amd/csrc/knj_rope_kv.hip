@@ -5,6 +5,7 @@
 // elements a lane, so a head's reductions (the norm's sum, the largest
 // magnitude) stay inside the group's DPP moves and every element is read and
 // written once.
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -452,8 +453,8 @@ int knj_attention_tree(const knj_kv_cache* cache, int type, const void* q, uint6
   KNJ_CHECK_ARG(eb, "activations must be F32, F16 or BF16");
   KNJ_CHECK_ARG(q && out && prefix, "null pointer");
   KNJ_CHECK_ARG(n_rows >= 0 && n_rows <= 1024, "n_rows must be in [0, 1024]");
-  KNJ_CHECK_ARG(n_head > 0 && n_head <= 4096 && n_head % cache->n_head_kv == 0,
-                "n_head must be a positive multiple of n_head_kv, at most 4096");
+  KNJ_CHECK_ARG(n_head > 0 && n_head <= 1024 && n_head % cache->n_head_kv == 0,
+                "n_head must be a positive multiple of n_head_kv, at most 1024");
   KNJ_CHECK_ARG(max_prefix >= 0 && (int64_t)max_prefix + n_rows <= cache->n_ctx,
                 "max_prefix and the drafts must fit into n_ctx");
   KNJ_CHECK_ARG(scale >= 1e-6f && scale <= 1e6f, "the scale must be in [1e-6, 1e6]");
@@ -462,7 +463,7 @@ int knj_attention_tree(const knj_kv_cache* cache, int type, const void* q, uint6
   KNJ_CHECK_ARG(q_stride >= width && out_stride >= width, "a row stride is below the row's width");
   KNJ_CHECK_ARG(rows_aligned(q, q_stride, eb) && rows_aligned(out, out_stride, eb),
                 "rows must start on 16-byte boundaries");
-  const uint64_t need = n_rows ? tree_partial_bytes(*cache, n_head, n_rows, max_prefix) : 0;
+  const uint64_t need = n_rows ? tree_partial_bytes(*cache, type, n_head, n_rows, max_prefix) : 0;
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) {
     set_error("knj_attention_tree: these sizes need a 16-byte aligned workspace of " + std::to_string(need) + " bytes");
     return KNJ_E_ARG;
@@ -476,10 +477,12 @@ int knj_attention_tree(const knj_kv_cache* cache, int type, const void* q, uint6
 }
 
 uint64_t knj_attention_tree_workspace(const knj_kv_cache* cache, int n_head, int n_rows, int max_prefix) {
-  if (check_kv_cache(cache) || n_head <= 0 || n_head > 4096 || n_head % cache->n_head_kv || n_rows <= 0 ||
+  if (check_kv_cache(cache) || n_head <= 0 || n_head > 1024 || n_head % cache->n_head_kv || n_rows <= 0 ||
       n_rows > 1024 || max_prefix < 0 || (int64_t)max_prefix + n_rows > cache->n_ctx)
     return 0;
-  return tree_partial_bytes(*cache, n_head, n_rows, max_prefix);
+  // (enough for every type)
+  return std::max(tree_partial_bytes(*cache, KNJ_TYPE_F32, n_head, n_rows, max_prefix),
+                  tree_partial_bytes(*cache, KNJ_TYPE_F16, n_head, n_rows, max_prefix));
 }
 
 }  // extern "C"

@@ -7,17 +7,28 @@
 // once for all drafts and heads of a tile.
 #pragma once
 
+#include <type_traits>
+
 #include "knj_common.h"
 #include "knj_dev.h"
 #include "knj_mfma.h"
 
 namespace knj {
 
+// n / d by one multiplication, for n d < 2^32.
+struct FastDiv {
+  uint32_t d, m;  // m = ceil(2^32 / d), 0 for d = 1
+  FastDiv() = default;
+  explicit FastDiv(uint32_t v) : d(v), m(v > 1 ? (uint32_t)(((1ull << 32) + v - 1) / v) : 0u) {}
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return m ? __umulhi(n, m) : n; }
+};
+
 struct TreePlan {
   int cps;       // chunks per split of the slots
   int n_split;   // splits of the longest sequence
   int n_tiles;   // column tiles of a full set of drafts
   int units;     // n_seq * n_split * n_head_kv
+  FastDiv by_nk, by_split, by_group;  // n_head_kv, n_split, query heads per kv head
 };
 
 namespace tree {
@@ -42,53 +53,71 @@ __device__ __forceinline__ uint2 codes4_h(uint32_t w) {
   }
 }
 
-// The f16 of a word that are infinite or NaN replaced by zero; true if any was.
+// Of four codes (slot 0 dims 0, 1, slot 1 dims 0, 1 in one word, slots 2, 3 in the
+// other) the even and the odd dim's four slots as f16.
+template <int FORMAT>
+__device__ __forceinline__ void pairs_h(u32x2 w, uint2& even, uint2& odd) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  if constexpr (FORMAT == KNJ_KV_F8) {
+    const uint32_t x = __builtin_amdgcn_perm(0u, w.x, 0x03010200u), y = __builtin_amdgcn_perm(0u, w.y, 0x03010200u);
+    const uint2 a = codes4_h<FORMAT>(x), b = codes4_h<FORMAT>(y);
+    even = make_uint2(a.x, b.x);
+    odd = make_uint2(a.y, b.y);
+  } else {
+    const uint32_t x = w.x ^ 0x80808080u, y = w.y ^ 0x80808080u;
+    const h2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+    auto half = [&](uint32_t u, uint32_t sel) {
+      return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, sel)) - off);
+    };
+    even = make_uint2(half(x, 0x04020400u), half(y, 0x04020400u));
+    odd = make_uint2(half(x, 0x04030401u), half(y, 0x04030401u));
+  }
+}
+
+// The elements of a word that are infinite or NaN replaced by zero; true if any was.
+template <int FORMAT>
 __device__ __forceinline__ bool drop_nonfinite(uint32_t& w) {
-  const bool lo = (w & 0x7C00u) == 0x7C00u, hi = (w & 0x7C000000u) == 0x7C000000u;
-  if (lo) w &= 0xFFFF0000u;
-  if (hi) w &= 0x0000FFFFu;
-  return lo || hi;
+  if constexpr (FORMAT == KNJ_KV_F8) {  // codes 0x7F and 0xFF
+    const uint32_t m = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+    w &= ~(m | (m - (m >> 7)));
+    return m != 0;
+  } else {
+    const bool lo = (w & 0x7C00u) == 0x7C00u, hi = (w & 0x7C000000u) == 0x7C000000u;
+    if (lo) w &= 0xFFFF0000u;
+    if (hi) w &= 0x0000FFFFu;
+    return lo || hi;
+  }
 }
 
 // Four transposed f16 (see lds_tr16) by the builtin: its waits are the compiler's.
-__device__ __forceinline__ u32x2 lds_tr16_at(const uint8_t* p) {
+__device__ __forceinline__ u32x2 lds_tr16_at(uint32_t p) {
   typedef short s4 __attribute__((__vector_size__(8)));
   typedef __attribute__((address_space(3))) s4 lds_s4;
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)p));
 }
 
-// Weights (and their sum) are held times 2^14: the largest stay below f16's
-// 65,504 and f16 keeps all of a weight's bits down to 2^-28 of the largest.
-constexpr float kLift = 14.0f;
+// Weights are formed relative to a reference that follows the running maximum
+// only when that has passed it by 2^7 (the accumulators are rescaled then, which
+// after a column's first slots is rare), and held times 2^7: at most 2^14, or 2^15
+// with a value scale's factor, below f16's 65,504, and f16 keeps all of a weight's
+// bits down to 2^-21 of the reference.
+constexpr float kLift = 7.0f, kLag = 7.0f;
 
-template <int TYPE>
-__device__ __forceinline__ void store4(void* p, uint64_t i, float4 v) {
-  if constexpr (TYPE == KNJ_TYPE_F32) *reinterpret_cast<float4*>((float*)p + i) = v;
-  else *reinterpret_cast<uint2*>((uint16_t*)p + i) = make_uint2(pack_act<TYPE>(v.x, v.y), pack_act<TYPE>(v.z, v.w));
-}
-__device__ __forceinline__ void store4(int type, void* p, uint64_t i, float4 v) {
-  if (type == KNJ_TYPE_F32) store4<KNJ_TYPE_F32>(p, i, v);
-  else if (type == KNJ_TYPE_F16) store4<KNJ_TYPE_F16>(p, i, v);
-  else store4<KNJ_TYPE_BF16>(p, i, v);
+// Maximum that carries a NaN (a NaN score makes its column NaN); the instruction
+// takes three, without the quieting of its inputs that fmaxf asks for.
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// 16 bytes at an LDS address.
+__device__ __forceinline__ uint4 lds_b128(uint32_t p) {
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) const u32x4 lds_v4;
+  return __builtin_bit_cast(uint4, *(lds_v4*)(uintptr_t)p);
 }
 
-// Eight activations as f32.
-__device__ __forceinline__ void load8(int type, const void* p, uint64_t i, float4& a, float4& b) {
-  if (type == KNJ_TYPE_F32) {
-    a = *reinterpret_cast<const float4*>((const float*)p + i);
-    b = *reinterpret_cast<const float4*>((const float*)p + i + 4);
-    return;
-  }
-  const uint4 u = *reinterpret_cast<const uint4*>((const uint16_t*)p + i);
-  if (type == KNJ_TYPE_F16) {
-    a = make_float4(h2f(u.x), h2f(u.x >> 16), h2f(u.y), h2f(u.y >> 16));
-    b = make_float4(h2f(u.z), h2f(u.z >> 16), h2f(u.w), h2f(u.w >> 16));
-  } else {
-    a = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
-                    __uint_as_float(u.y & 0xFFFF0000u));
-    b = make_float4(__uint_as_float(u.z << 16), __uint_as_float(u.z & 0xFFFF0000u), __uint_as_float(u.w << 16),
-                    __uint_as_float(u.w & 0xFFFF0000u));
-  }
+// Four results as activations.
+__device__ __forceinline__ uint2 pack4(int type, float4 v) {
+  if (type == KNJ_TYPE_F16) return make_uint2(pack_act<KNJ_TYPE_F16>(v.x, v.y), pack_act<KNJ_TYPE_F16>(v.z, v.w));
+  return make_uint2(pack_act<KNJ_TYPE_BF16>(v.x, v.y), pack_act<KNJ_TYPE_BF16>(v.z, v.w));
 }
 
 // Prefix and drafts of a sequence, held to what the host checked.
@@ -112,124 +141,157 @@ __device__ __forceinline__ uint64_t seen64(const uint64_t* row, int words, int t
   return v;
 }
 
-// A column's result or split record, four dims at a time: the maximum in base-2
-// units, the sum and the weighted values.
-template <int D>
-__device__ __forceinline__ void emit(const TreeArgs& a, const TreePlan& p, int s, int kvh, int split, int n_cols, int G,
-                                     int N, int col, int d, float M, float L, float4 o) {
-  if (col >= N * G) return;
-  if (p.n_split > 1) {
-    float* rec = a.partial + ((((uint64_t)s * a.c.n_head_kv + kvh) * p.n_split + split) * n_cols + col) * (D + 4);
-    if (d == 0) {
-      rec[0] = M;
-      rec[1] = L;
-    }
-    *reinterpret_cast<float4*>(rec + 4 + d) = o;
-    return;
-  }
-  const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // nothing seen: zeros
-  const int t = col / G;
-  store4(a.type, a.out, ((uint64_t)s * a.n_rows + t) * a.out_stride + (uint64_t)(kvh * G + col - t * G) * D + d,
-         make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+// LDS DMA of 16 bytes per lane, as dma16, from a wave-uniform address and each lane's offset.
+__device__ __forceinline__ void dma16_at(const void* g, uint32_t off, uint32_t base) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(g), "s"(base) : "memory");
 }
 
-// Workgroup = (sequence, split of the slots, kv head, tile of WC * NT * 16 columns).
-// Wave (wc, ws) holds NT tiles of 16 columns -- queries as the B operand in
-// registers -- against SW of the chunk's WS * SW slots:
+// LDS DMA of 4 bytes per lane, as dma16.
+__device__ __forceinline__ void dma4(const void* g, uint32_t base) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(g), "s"(base) : "memory");
+}
+
+typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
+
+// Workgroup = (sequence, split of the slots, kv head, tile of WC * NT * 16 columns)
+// of WC * WS waves.  Wave (wc, ws) holds NT tiles of 16 columns -- queries as the B
+// operand in registers -- against SW of the chunk's C = WS * SW slots:
 //   scores  S[slot][col] = K (16 slots x 32 dims) x Q (32 dims x 16 columns); lane
 //           (r = l % 16, kq = l / 16) ends with column r's slots 16 st + 4 kq + i;
 //   values  O^T[d][col] = V^T (16 dims x 32 slots) x E (32 slots x 16 columns), the
 //           weights as the lane holds them, V^T by transposed LDS reads.
-// With few columns the waves share the slots instead (WS > 1, each with running
-// statistics of its own, joined at the end).  Chunks go through registers to
-// LDS as f16, the next one's loads in flight while one is computed; 8-bit codes
-// are exact in f16 and their scales stay out of the products: a score is
-// multiplied by its slot's, a weight by its slot's over the running largest of
-// the scales its column has seen (a power of two; a weight then stays in f16's
-// range whatever the cache's units).  Queries are scaled by a power of two per
-// row, so that f16 holds any of them.  SPLIT keeps queries and weights as f16
-// high parts and remainders (22 bits), for f32 activations.
-template <int D, int FORMAT, bool SPLIT, int NT, int WC, int SW>
-__global__ __launch_bounds__(kBlock, 2) void k_tree(TreeArgs a, TreePlan p) {
-  constexpr int WS = 4 / WC, C = WS * SW, COLS = WC * NT * 16, ST = SW / 16;
-  constexpr int RB = 2 * D, RPB = 256 / RB, NSLOT = RB / 16, NPAIR = RB / 32, CB = C * RB;
+// Waves that share the columns (WS > 1) keep running statistics of their own and
+// join them at the end, through LDS, in pairs.
+//
+// Chunks reach LDS by DMA, as the cache holds them, NST - 1 chunks ahead, one
+// barrier a chunk; 16-byte pieces (K) and 32-byte pairs (V) of a row are permuted
+// by an XOR of the row index, so that the operand reads fall on distinct banks.
+// 8-bit codes become f16 (exactly) as operands.  Their scales stay out of the
+// products: a score is multiplied by its slot's, a weight by its slot's over the
+// running largest of the scales its column has seen (a power of two, so a weight
+// stays in f16's range whatever the cache's units).  Queries are scaled by a
+// power of two per row, so that f16 holds any of them.  SPLIT keeps queries and
+// weights as f16 high parts and remainders (22 bits), for f32 activations.
+//
+// The loads that need no sequence length (a chunk's rows, the queries) come
+// first; rows of a chunk past the sequence's slots hold whatever the cache does
+// there, and the chunks that reach the drafts are cleaned before use (below).
+template <int D, int FORMAT, bool SPLIT, int NT, int WC, int WS, int SW, int NST>
+__global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p) {
   constexpr bool Q8 = FORMAT != KNJ_KV_F16;
-  constexpr int NP = C * D / (Q8 ? 16 : 8) / kBlock;  // 16-byte loads per thread and matrix
-  static_assert(NP >= 1 && C * D % (16 * kBlock) == 0, "whole loads");
-  constexpr int JOIN = WS > 1 ? WS * COLS * (D + 4) * 4 : 0;
-  constexpr int LDS = 2 * CB > JOIN ? 2 * CB : JOIN;
-  auto kslot = [](int q, int sl) { return sl ^ ((q / RPB) & (NSLOT - 1)); };
-  auto vslot = [](int q, int sl) { return sl ^ (((q / RPB) & (NPAIR - 1)) << 1); };
-  __shared__ __align__(16) uint8_t lds[LDS];
-  __shared__ __align__(16) float ksc[Q8 ? C : 4], vsc[Q8 ? C : 4];
+  constexpr int NW = WC * WS, NTH = 64 * NW, C = WS * SW, COLS = WC * NT * 16, ST = SW / 16;
+  constexpr int RB = Q8 ? D : 2 * D;                     // bytes of a cache row
+  constexpr int RPB = 256 / RB, NSLOT = RB / 16, NPAIR = RB / 32, CB = C * RB;
+  constexpr bool HALVES = CB / 1024 < NW;                // half of the waves fetch K, half V
+  constexpr int NI = HALVES ? 1 : CB / 1024 / NW;        // 1 KB DMA instructions per wave and matrix
+  constexpr int NDMA = (HALVES ? 1 : 2 * NI) + (Q8 ? 1 : 0);  // of a chunk, per wave
+  constexpr int SB = 2 * CB + (Q8 ? 8 * C : 0);          // bytes of a stage: K, V, scales of both
+  constexpr int DT = D / 16;                             // accumulator tiles per column tile
+  constexpr int JOIN = WS > 1 ? WS / 2 * WC * NT * (DT * 1024 + 512) : 0;
+  constexpr int LDS = NST * SB > JOIN ? NST * SB : JOIN;
+  static_assert(HALVES ? 2 * CB == 1024 * NW : CB % (1024 * NW) == 0, "whole DMA instructions");
+  static_assert(C % 32 == 0 && NW % (C / 32) == 0, "whole DMA instructions of scales");
+  static_assert(SB % 256 == 0, "stages on whole rows");
+  static_assert(SW == 16 || SW % 32 == 0, "16 slots, or steps of 32");
+  __shared__ __align__(1024) uint8_t lds[LDS];
   __shared__ uint32_t poison[C / 32];
-  __shared__ float jm[WS > 1 ? WS * COLS : 1], jl[WS > 1 ? WS * COLS : 1];
-  uint8_t *ks = lds, *vs = lds + CB;
 
   // tiles of one unit run on one XCD, whose L2 then serves their shared slots
-  const int tile = (blockIdx.x >> 3) % p.n_tiles;
-  const int unit = ((blockIdx.x >> 3) / p.n_tiles) * 8 + (blockIdx.x & 7);
+  // (workgroups go to the eight XCDs in turn; gridDim.x is a multiple of eight)
+  const int tile = blockIdx.x >> 3, unit = blockIdx.y * 8 + (blockIdx.x & 7);
   if (unit >= p.units) return;
-  const int nk = a.c.n_head_kv, G = a.n_head / nk;
-  const int kvh = unit % nk, split = (unit / nk) % p.n_split, s = unit / (nk * p.n_split);
-  int P, N;
-  seq_lengths(a, s, P, N);
-  const int valid = P + N;
-  const int c0 = split * p.cps, c1 = min((valid + C - 1) / C, c0 + p.cps);
-  if (tile * COLS >= N * G || c0 >= c1) return;
-  const int n_cols = p.n_tiles * COLS;
-
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int nk = a.c.n_head_kv, G = p.by_group.d, n_ctx = a.c.n_ctx;
+  const int rest = p.by_nk.div(unit), kvh = unit - rest * nk;
+  const int s = p.by_split.div(rest), split = rest - s * p.n_split;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wc = wave % WC, ws = wave / WC, r = lane & 15, kq = lane >> 4;
-  const uint64_t seq_at = (uint64_t)s * a.c.seq_stride + (uint64_t)kvh * a.c.n_ctx * D;
+  const uint64_t seq_at = (uint64_t)s * a.c.seq_stride + (uint64_t)kvh * n_ctx * D;
   constexpr int EB = Q8 ? 1 : 2;
   const uint8_t* kc = (const uint8_t*)a.c.k + seq_at * EB;
   const uint8_t* vc = (const uint8_t*)a.c.v + seq_at * EB;
-  const float *kscale = nullptr, *vscale = nullptr;
-  if constexpr (Q8) {
-    kscale = a.c.k_scale + seq_at / D;
-    vscale = a.c.v_scale + seq_at / D;
-  }
 
-  // ---- a chunk's bytes into registers (zeros past the sequence's slots)
-  uint4 kr[NP], vr[NP];
-  float ksr = 0.0f, vsr = 0.0f;
-  constexpr int PR = Q8 ? D / 16 : D / 8;  // 16-byte loads per row
-  auto fetch = [&](int p0) {
+  // ---- chunk j's bytes into stage `st`: wave w's instruction i fills KB i NW + w
+  // of the chunk's K and of its V, whose rows share row 1024 w / RB + lane RB/16's
+  // permutation (rows past the cache are its last row); with 8 bits, 64 of the scales
+  const int dw = HALVES ? wave % (NW / 2) : wave;
+  const bool dv = HALVES && wave >= NW / 2;
+  const int dq = (dw * 1024 + 16 * lane) / RB, dsl = lane % NSLOT;
+  const uint32_t koff = 16 * (dsl ^ ((dq / RPB) & (NSLOT - 1)));
+  const uint32_t voff = 16 * (dsl ^ (((dq / RPB) & (NPAIR - 1)) << 1));
+  auto dma = [&](int j, int st) {
+    const int p0 = j * C;
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(lds + st * SB + dw * 1024));
+    if (__builtin_expect(p0 + C <= n_ctx, 1)) {  // uniform
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int at = tid + kBlock * i, q = at / PR, sl = at % PR;
-      const bool in = p0 + q < valid;
-      const uint64_t off = (uint64_t)(in ? p0 + q : valid - 1) * (D * EB) + 16 * sl;
-      kr[i] = *reinterpret_cast<const uint4*>(kc + off);
-      vr[i] = *reinterpret_cast<const uint4*>(vc + off);
-      if (!in) kr[i] = vr[i] = make_uint4(0u, 0u, 0u, 0u);
-    }
-    if constexpr (Q8) {
-      if (tid < C) {
-        const bool in = p0 + tid < valid;
-        ksr = in ? kscale[p0 + tid] : 0.0f;
-        vsr = in ? vscale[p0 + tid] : 0.0f;
+      for (int i = 0; i < NI; ++i) {
+        const uint64_t at = (uint64_t)p0 * RB + i * NW * 1024;
+        if (!dv) dma16_at(kc + at, dq * RB + koff, to + i * NW * 1024);
+        if (!HALVES || dv) dma16_at(vc + at, dq * RB + voff, to + CB + i * NW * 1024);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const uint64_t row = (uint64_t)min(p0 + i * (NW * 1024 / RB) + dq, n_ctx - 1) * RB;
+        if (!dv) dma16(kc + row + koff, to + i * NW * 1024);
+        if (!HALVES || dv) dma16(vc + row + voff, to + CB + i * NW * 1024);
       }
     }
+    if constexpr (Q8) {
+      // (waves beyond the scales' 2 C floats repeat: the same bytes)
+      const int x = wave % (2 * C / 64) * 64 + lane;
+      const float* sc = (x < C ? a.c.k_scale : a.c.v_scale) + seq_at / D;
+      dma4(sc + min(p0 + x % C, n_ctx - 1),
+           __builtin_amdgcn_readfirstlane(lds_addr(lds + st * SB + 2 * CB + wave % (2 * C / 64) * 256)));
+    }
   };
-  fetch(c0 * C);
+  const int c0 = split * p.cps;
+#pragma unroll
+  for (int i = 0; i < NST - 1; ++i) dma(c0 + i, i);
 
-  // ---- this lane's query columns
+  // ---- this lane's query columns.  Step c's dims 8 kq .. + 7 of 32; with 8 bits,
+  // where a 16-byte piece of a K row is two steps', dims 64 (c/2) + 16 kq + 8 (c%2)
   h16x8 qh[NT][D / 32], ql[SPLIT ? NT : 1][D / 32];
   float s2[NT];
   int tcol[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int col = min(tile * COLS + (wc * NT + nt) * 16 + r, N * G - 1);  // (past the drafts: not stored)
-    const int t = col / G;
+    const int col = min(tile * COLS + (wc * NT + nt) * 16 + r, a.n_rows * G - 1);  // (past the drafts: not stored)
+    const int t = p.by_group.div(col);
     tcol[nt] = t;
-    const uint64_t at = ((uint64_t)s * a.n_rows + t) * a.q_stride + (uint64_t)(kvh * G + col - t * G) * D + 8 * kq;
+    const uint64_t at = ((uint64_t)s * a.n_rows + t) * a.q_stride + (uint64_t)(kvh * G + col - t * G) * D;
     float4 x[D / 32], y[D / 32];
+    if constexpr (SPLIT) {
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        const float* q = (const float*)a.q + at + (Q8 ? 64 * (c >> 1) + 16 * kq + 8 * (c & 1) : 32 * c + 8 * kq);
+        x[c] = *reinterpret_cast<const float4*>(q);
+        y[c] = *reinterpret_cast<const float4*>(q + 4);
+      }
+    } else {
+      uint4 u[D / 32];
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c)
+        u[c] = *reinterpret_cast<const uint4*>((const uint16_t*)a.q + at +
+                                               (Q8 ? 64 * (c >> 1) + 16 * kq + 8 * (c & 1) : 32 * c + 8 * kq));
+      if (a.type == KNJ_TYPE_F16) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          x[c] = make_float4(h2f(u[c].x), h2f(u[c].x >> 16), h2f(u[c].y), h2f(u[c].y >> 16));
+          y[c] = make_float4(h2f(u[c].z), h2f(u[c].z >> 16), h2f(u[c].w), h2f(u[c].w >> 16));
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          x[c] = make_float4(__uint_as_float(u[c].x << 16), __uint_as_float(u[c].x & 0xFFFF0000u),
+                             __uint_as_float(u[c].y << 16), __uint_as_float(u[c].y & 0xFFFF0000u));
+          y[c] = make_float4(__uint_as_float(u[c].z << 16), __uint_as_float(u[c].z & 0xFFFF0000u),
+                             __uint_as_float(u[c].w << 16), __uint_as_float(u[c].w & 0xFFFF0000u));
+        }
+      }
+    }
     float am = 0.0f;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
-      load8(SPLIT ? KNJ_TYPE_F32 : a.type, a.q, at + 32 * c, x[c], y[c]);
       am = fmaxf(am, fmaxf(fmaxf(fabsf(x[c].x), fabsf(x[c].y)), fmaxf(fabsf(x[c].z), fabsf(x[c].w))));
       am = fmaxf(am, fmaxf(fmaxf(fabsf(y[c].x), fabsf(y[c].y)), fmaxf(fabsf(y[c].z), fabsf(y[c].w))));
     }
@@ -248,11 +310,19 @@ __global__ __launch_bounds__(kBlock, 2) void k_tree(TreeArgs a, TreePlan p) {
       if constexpr (SPLIT) ql[nt][c] = lo;
     }
   }
+  int P, N;
+  seq_lengths(a, s, P, N);
+  const int valid = P + N, n_cols = p.n_tiles * COLS;
+  const int c1 = min((valid + C - 1) / C, c0 + p.cps);
+  if (tile * COLS >= N * G || c0 >= c1) {
+    __builtin_amdgcn_s_waitcnt(0);  // the fetch lands before the workgroup ends
+    return;
+  }
 
   // (maxima in units of the stored scores, before s2)
   float m[NT], l[NT], vref[NT];
   bool spoilt[NT];
-  f32x4 acc[NT][D / 16];
+  f32x4 acc[NT][DT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     m[nt] = -INFINITY;
@@ -260,77 +330,38 @@ __global__ __launch_bounds__(kBlock, 2) void k_tree(TreeArgs a, TreePlan p) {
     vref[nt] = 0.0f;
     spoilt[nt] = false;
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt) acc[nt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int dt = 0; dt < DT; ++dt) acc[nt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
   const int words = (a.n_rows + 63) / 64;
   const uint64_t* mask = a.mask ? a.mask + (a.mask_shared ? 0 : (uint64_t)s * a.n_rows * words) : nullptr;
 
-  for (int j = c0; j < c1; ++j) {
-    const int p0 = j * C;
-    const bool drafts = p0 + C > P;  // the chunk reaches the drafts (or the end)
-    __syncthreads();                 // every wave is done with the chunk before
-    if (drafts) {
-      if (tid < C / 32) poison[tid] = 0u;
-      __syncthreads();
-    }
-    // ---- registers to LDS, as f16
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int at = tid + kBlock * i, q = at / PR, sl = at % PR;
-      uint4 kw[Q8 ? 2 : 1], vw[Q8 ? 2 : 1];
-      if constexpr (Q8) {
-        const uint2 k0 = codes4_h<FORMAT>(kr[i].x), k1 = codes4_h<FORMAT>(kr[i].y);
-        const uint2 k2 = codes4_h<FORMAT>(kr[i].z), k3 = codes4_h<FORMAT>(kr[i].w);
-        const uint2 v0 = codes4_h<FORMAT>(vr[i].x), v1 = codes4_h<FORMAT>(vr[i].y);
-        const uint2 v2 = codes4_h<FORMAT>(vr[i].z), v3 = codes4_h<FORMAT>(vr[i].w);
-        kw[0] = make_uint4(k0.x, k0.y, k1.x, k1.y);
-        kw[1] = make_uint4(k2.x, k2.y, k3.x, k3.y);
-        vw[0] = make_uint4(v0.x, v0.y, v1.x, v1.y);
-        vw[1] = make_uint4(v2.x, v2.y, v3.x, v3.y);
-      } else {
-        kw[0] = kr[i];
-        vw[0] = vr[i];
-      }
-      // a draft's value row may be unseen by some columns of the tile: what is
-      // not finite in it would reach them as 0 x inf, and is kept out
-      if (FORMAT != KNJ_KV_I8 && drafts && p0 + q >= P) {
-        bool any = false;
-#pragma unroll
-        for (int h = 0; h < (Q8 ? 2 : 1); ++h) {
-          any |= drop_nonfinite(vw[h].x);
-          any |= drop_nonfinite(vw[h].y);
-          any |= drop_nonfinite(vw[h].z);
-          any |= drop_nonfinite(vw[h].w);
-        }
-        if (any) atomicOr(&poison[q >> 5], 1u << (q & 31));
-      }
-#pragma unroll
-      for (int h = 0; h < (Q8 ? 2 : 1); ++h) {
-        const int slot = Q8 ? 2 * sl + h : sl;
-        *reinterpret_cast<uint4*>(ks + q * RB + 16 * kslot(q, slot)) = kw[h];
-        *reinterpret_cast<uint4*>(vs + q * RB + 16 * vslot(q, slot)) = vw[h];
-      }
-    }
-    if constexpr (Q8) {
-      if (tid < C) {
-        ksc[tid] = ksr;
-        vsc[tid] = vsr;
-      }
-    }
-    __syncthreads();
-    if (j + 1 < c1) fetch(p0 + C);
+  // Operand addresses within a stage.  K rows 16 st + r share row r's permutation, V
+  // rows 16 k + pa row pa's; a row starts on a multiple of its size, so piece c's
+  // (pair b's) permuted place is an XOR of the address with the first one's.
+  const uint32_t kat = (ws * SW + r) * RB + 16 * (kq ^ ((r / RPB) & (NSLOT - 1)));
+  const int pa = 4 * kq + (r >> 2);
+  const uint32_t vat = CB + (ws * SW + pa) * RB + 32 * ((pa / RPB) & (NPAIR - 1)) + 8 * (r & 3);
+  const uint32_t lds0 = lds_addr(lds);
 
-    // ---- scores
+  // ---- one chunk in stage `at`; DRAFTS: it reaches the drafts or the end
+  auto chunk = [&](auto drafts_c, const uint8_t* at, int p0) {
+    constexpr bool DRAFTS = decltype(drafts_c)::value;
+    const uint32_t k0 = lds0 + (uint32_t)(at - lds) + kat, v0at = lds0 + (uint32_t)(at - lds) + vat;
     f32x4 sc[NT][ST];
 #pragma unroll
     for (int st = 0; st < ST; ++st) {
-      const int q = ws * SW + 16 * st + r;
-      const uint8_t* krow = ks + q * RB;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) sc[nt][st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
-        const h16x8 ka = __builtin_bit_cast(h16x8, *reinterpret_cast<const uint4*>(krow + 16 * kslot(q, 4 * c + kq)));
+        h16x8 ka;
+        if constexpr (Q8) {
+          const uint4 w = lds_b128((k0 ^ (64 * (c >> 1))) + 16 * st * RB);
+          const uint2 x = codes4_h<FORMAT>((c & 1) ? w.z : w.x), y = codes4_h<FORMAT>((c & 1) ? w.w : w.y);
+          ka = __builtin_bit_cast(h16x8, make_uint4(x.x, x.y, y.x, y.y));
+        } else {
+          ka = __builtin_bit_cast(h16x8, lds_b128((k0 ^ (64 * c)) + 16 * st * RB));
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           sc[nt][st] = mfma16(ka, qh[nt][c], sc[nt][st]);
@@ -338,12 +369,18 @@ __global__ __launch_bounds__(kBlock, 2) void k_tree(TreeArgs a, TreePlan p) {
         }
       }
     }
-    float4 vq[Q8 ? ST : 1];  // value scales of this lane's slots
+    __builtin_amdgcn_sched_barrier(0);
+    float vq[Q8 ? 4 * ST : 1];  // value scales of this lane's slots
     if constexpr (Q8) {
 #pragma unroll
       for (int st = 0; st < ST; ++st) {
-        const float4 kv = *reinterpret_cast<const float4*>(ksc + ws * SW + 16 * st + 4 * kq);
-        vq[st] = *reinterpret_cast<const float4*>(vsc + ws * SW + 16 * st + 4 * kq);
+        const uint8_t* q = at + 2 * CB + 4 * (ws * SW + 16 * st + 4 * kq);
+        const float4 kv = *reinterpret_cast<const float4*>(q);
+        const float4 vv = *reinterpret_cast<const float4*>(q + 4 * C);
+        vq[4 * st] = vv.x;
+        vq[4 * st + 1] = vv.y;
+        vq[4 * st + 2] = vv.z;
+        vq[4 * st + 3] = vv.w;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           sc[nt][st][0] *= kv.x;
@@ -353,110 +390,127 @@ __global__ __launch_bounds__(kBlock, 2) void k_tree(TreeArgs a, TreePlan p) {
         }
       }
     }
-    // ---- the slots a column does not see, where the chunk reaches the drafts
-    uint32_t nib[NT][ST];  // four bits per lane and slot tile
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int st = 0; st < ST; ++st) nib[nt][st] = 15u;
-    if (drafts) {
+    // the slots a column does not see
+    uint32_t seen[NT][ST];  // four bits each
+    if constexpr (DRAFTS) {
       uint64_t bad = 0;
       if constexpr (FORMAT != KNJ_KV_I8) {
-        bad = poison[ws * (SW / 32)];
-        if constexpr (SW == 64) bad |= (uint64_t)poison[ws * (SW / 32) + 1] << 32;
+        bad = poison[(ws * SW) >> 5];
+        if constexpr (SW == 64) bad |= (uint64_t)poison[((ws * SW) >> 5) + 1] << 32;
+        if constexpr (SW == 16) bad = (bad >> ((ws * SW) & 31)) & 0xFFFFu;
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const uint64_t seen =
+        const uint64_t b =
             seen64(mask ? mask + (uint64_t)tcol[nt] * words : nullptr, words, tcol[nt], N, p0 + ws * SW - P);
-        spoilt[nt] |= (seen & bad) != 0;
+        spoilt[nt] |= (b & bad) != 0;
 #pragma unroll
         for (int st = 0; st < ST; ++st) {
-          const uint32_t b = (uint32_t)(seen >> (16 * st + 4 * kq)) & 15u;
-          nib[nt][st] = b;
+          seen[nt][st] = (uint32_t)(b >> (16 * st + 4 * kq)) & 15u;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[nt][st][i] = (b >> i) & 1u ? sc[nt][st][i] : -INFINITY;
+          for (int i = 0; i < 4; ++i) sc[nt][st][i] = (seen[nt][st] >> i) & 1u ? sc[nt][st][i] : -INFINITY;
         }
       }
     }
-    // ---- running softmax per column, and the weights as the values' operand
-    h16x8 eh[NT][ST / 2], el[SPLIT ? NT : 1][ST / 2];
-    float alpha[NT];
+    // before the drafts every column sees the same slots: one reference for all
+    float vs[Q8 ? 4 * ST : 1], vnew = 0.0f;
+    if constexpr (Q8 && !DRAFTS) {
+      float vm = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4 * ST; ++i) vm = fmaxf(vm, vq[i] < INFINITY ? vq[i] : 0.0f);
+      vm = fmaxf(vm, xor16_f(vm));
+      vm = fmaxf(vm, xor32_f(vm));
+      vnew = fmaxf(vref[0], __uint_as_float(__float_as_uint(vm) & 0x7F800000u));
+      const float inv = vnew > 0.0f ? __uint_as_float((254u << 23) - __float_as_uint(vnew)) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4 * ST; ++i) vs[i] = vq[i] * inv;
+    }
+    // running softmax per column, and the weights as the values' operand
+    constexpr int NE = SW == 16 ? 1 : ST / 2;
+    h16x8 eh[NT][NE], el[SPLIT ? NT : 1][NE];  // (SW 16: the first four)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float mx = -INFINITY;
 #pragma unroll
       for (int st = 0; st < ST; ++st)
-        mx = fmaxf(mx, fmaxf(fmaxf(sc[nt][st][0], sc[nt][st][1]), fmaxf(sc[nt][st][2], sc[nt][st][3])));
-      mx = fmaxf(mx, xor16_f(mx));
-      mx = fmaxf(mx, xor32_f(mx));
-      const float mn = fmaxf(m[nt], mx);
-      // (-inf while the column has seen nothing: exponents then from 0)
+        mx = max_nan(max_nan(max_nan(mx, sc[nt][st][0]), max_nan(sc[nt][st][1], sc[nt][st][2])), sc[nt][st][3]);
+      const float2 m16 = pair16_f(mx);
+      mx = max_nan(m16.x, m16.y);
+      const float2 m32 = pair32_f(mx);
+      mx = max_nan(m32.x, m32.y);
+      // (the reference is -inf while the column has seen nothing: exponents then from 0)
+      const float mn = (mx - m[nt]) * s2[nt] <= kLag ? m[nt] : max_nan(m[nt], mx);
       const float mr = mn == -INFINITY ? 0.0f : mn * s2[nt];
-      alpha[nt] = __builtin_amdgcn_exp2f(fmaf(m[nt], s2[nt], -mr));
+      float alpha = __builtin_amdgcn_exp2f(fmaf(m[nt], s2[nt], -mr));
       m[nt] = mn;
       float es = 0.0f;
       float w[4 * ST];
 #pragma unroll
-      for (int st = 0; st < ST; ++st)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(sc[nt][st][i], s2[nt], kLift - mr));
-          es += e;
-          w[4 * st + i] = e;
-        }
-      l[nt] = l[nt] * alpha[nt] + es;
+      for (int i = 0; i < 4 * ST; ++i) {
+        w[i] = __builtin_amdgcn_exp2f(fmaf(sc[nt][i >> 2][i & 3], s2[nt], kLift - mr));
+        es += w[i];
+      }
+      l[nt] = l[nt] * alpha + es;
       if constexpr (Q8) {
-        float vm = 0.0f;  // the largest finite scale that the column sees here
+        float ref = vnew;
+        if constexpr (DRAFTS) {
+          float vm = 0.0f;  // the largest finite scale that the column sees here
 #pragma unroll
-        for (int st = 0; st < ST; ++st) {
-          const float v[4] = {vq[st].x, vq[st].y, vq[st].z, vq[st].w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) vm = fmaxf(vm, (!drafts || (nib[nt][st] >> i) & 1u) && v[i] < INFINITY ? v[i] : 0.0f);
+          for (int i = 0; i < 4 * ST; ++i)
+            vm = fmaxf(vm, ((seen[nt][i >> 2] >> (i & 3)) & 1u) && vq[i] < INFINITY ? vq[i] : 0.0f);
+          vm = fmaxf(vm, xor16_f(vm));
+          vm = fmaxf(vm, xor32_f(vm));
+          ref = fmaxf(vref[nt], __uint_as_float(__float_as_uint(vm) & 0x7F800000u));
         }
-        vm = fmaxf(vm, xor16_f(vm));
-        vm = fmaxf(vm, xor32_f(vm));
-        const float ref = fmaxf(vref[nt], __uint_as_float(__float_as_uint(vm) & 0x7F800000u));
         const float inv = ref > 0.0f ? __uint_as_float((254u << 23) - __float_as_uint(ref)) : 0.0f;
-        alpha[nt] *= vref[nt] * inv;
+        alpha *= vref[nt] * inv;
         vref[nt] = ref;
 #pragma unroll
-        for (int st = 0; st < ST; ++st) {
-          const float v[4] = {vq[st].x, vq[st].y, vq[st].z, vq[st].w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float x = w[4 * st + i] * (v[i] * inv);
-            w[4 * st + i] = !drafts || (nib[nt][st] >> i) & 1u ? x : 0.0f;
-          }
+        for (int i = 0; i < 4 * ST; ++i) {
+          if constexpr (DRAFTS) w[i] = (seen[nt][i >> 2] >> (i & 3)) & 1u ? w[i] * (vq[i] * inv) : 0.0f;
+          else w[i] *= vs[i];
+          // (the weight itself, rounded to f32, is what is split below: formed anew
+          // inside the conversion to f16, the product could round the other way
+          // there than in the remainder, an f16 step off)
+          if constexpr (SPLIT) asm("" : "+v"(w[i]));
         }
       }
 #pragma unroll
-      for (int c = 0; c < ST / 2; ++c) {
+      for (int c = 0; c < NE; ++c) {
         h16x8 hi, lo;
         split_h8(make_float4(w[8 * c], w[8 * c + 1], w[8 * c + 2], w[8 * c + 3]),
-                 make_float4(w[8 * c + 4], w[8 * c + 5], w[8 * c + 6], w[8 * c + 7]), hi, lo);
+                 SW == 16 ? make_float4(0.f, 0.f, 0.f, 0.f)
+                          : make_float4(w[(8 * c + 4) % (4 * ST)], w[(8 * c + 5) % (4 * ST)], w[(8 * c + 6) % (4 * ST)],
+                                        w[(8 * c + 7) % (4 * ST)]),
+                 hi, lo);
         eh[nt][c] = hi;
         if constexpr (SPLIT) el[nt][c] = lo;
       }
-      if (__ballot(alpha[nt] != 1.0f) != 0) {
+      {
 #pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt)
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[nt][dt][i] *= alpha[nt];
+          for (int i = 0; i < 4; ++i) acc[nt][dt][i] *= alpha;
       }
     }
-    // ---- values: step c covers slots 32c + 4kq + i and 32c + 16 + 4kq + i; lane r's
-    // transposed read takes row 32c (+ 16) + 4kq + r/4, dims 16dt + 4(r%4) .. + 3,
-    // and receives dim 16dt + r of the four rows
-    const int pa = 4 * kq + (r >> 2), sub = 8 * (r & 3);
+    __builtin_amdgcn_sched_barrier(0);
+    // values: step c covers slots 32c + 4kq + i and 32c + 16 + 4kq + i (SW 16: the
+    // first).  Lane r's transposed read takes bytes 8 (r%4) .. + 7 of 32-byte pair b
+    // of row 4kq + r/4 and receives 16-bit element r of the pair, of four rows:
+    // dim 16b + r, or with 8 bits dims 32b + 2r (tile 2b) and 32b + 2r + 1 (2b + 1)
+    auto product = [&](int dt, uint2 v0, uint2 v1, int c) {
+      if constexpr (SW == 16) {
+        const h16x4 vv = __builtin_bit_cast(h16x4, v0);
 #pragma unroll
-    for (int c = 0; c < ST / 2; ++c) {
-      const uint8_t* vrow = vs + (ws * SW + 32 * c + pa) * RB + (sub & 15);
-#pragma unroll
-      for (int dt = 0; dt < D / 16; ++dt) {
-        // (rows pa + 16 k share the swizzle of row pa)
-        const uint8_t* at = vrow + 16 * vslot(pa, (32 * dt + sub) >> 4);
-        const u32x2 v0 = lds_tr16_at(at), v1 = lds_tr16_at(at + 16 * RB);
+        for (int nt = 0; nt < NT; ++nt) {
+          const h16x4 hi = __builtin_shufflevector(eh[nt][0], eh[nt][0], 0, 1, 2, 3);
+          acc[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x16f16(vv, hi, acc[nt][dt], 0, 0, 0);
+          if constexpr (SPLIT) {
+            const h16x4 lo = __builtin_shufflevector(el[nt][0], el[nt][0], 0, 1, 2, 3);
+            acc[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x16f16(vv, lo, acc[nt][dt], 0, 0, 0);
+          }
+        }
+      } else {
         const h16x8 vv = __builtin_bit_cast(h16x8, make_uint4(v0.x, v0.y, v1.x, v1.y));
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -464,7 +518,66 @@ __global__ __launch_bounds__(kBlock, 2) void k_tree(TreeArgs a, TreePlan p) {
           if constexpr (SPLIT) acc[nt][dt] = mfma16(vv, el[nt][c], acc[nt][dt]);
         }
       }
+    };
+#pragma unroll
+    for (int c = 0; c < NE; ++c) {
+#pragma unroll
+      for (int b = 0; b < NPAIR; ++b) {
+        const uint32_t q = (v0at ^ (32 * b)) + 32 * c * RB;
+        const u32x2 v0 = lds_tr16_at(q);
+        u32x2 v1 = v0;
+        if constexpr (SW != 16) v1 = lds_tr16_at(q + 16 * RB);
+        if constexpr (Q8) {
+          uint2 e0, o0, e1, o1;
+          pairs_h<FORMAT>(v0, e0, o0);
+          if constexpr (SW != 16) pairs_h<FORMAT>(v1, e1, o1);
+          else e1 = e0, o1 = o0;
+          product(2 * b, e0, e1, c);
+          product(2 * b + 1, o0, o1, c);
+        } else {
+          product(b, make_uint2(v0.x, v0.y), make_uint2(v1.x, v1.y), c);
+        }
+      }
     }
+  };
+
+  for (int j = c0; j < c1; ++j) {
+    const int p0 = j * C;
+    uint8_t* at = lds + (j - c0) % NST * SB;
+    // this wave's DMA of chunk j has landed (the chunks after it may be in flight);
+    // the barrier hands every wave's part over and ends the reads of chunk j - 1,
+    // whose stage chunk j + NST - 1 then refills
+    KNJ_BARRIER_AFTER(vm_lds_imm((NST - 2) * NDMA));
+    dma(j + NST - 1, (j - c0 + NST - 1) % NST);  // (past the range: fetched and not used)
+    if (__builtin_expect(p0 + C <= P, 1)) {
+      chunk(std::false_type{}, at, p0);
+      continue;
+    }
+    // A draft's value row may be unseen by some columns of the tile, and rows past
+    // the drafts are seen by none: what is not finite in them would reach a column
+    // as 0 x inf, and is replaced by zeros.  Columns that see such a draft are
+    // marked and come out as NaN.  (int8 codes are finite; their scales are
+    // selected away.)
+    if constexpr (FORMAT != KNJ_KV_I8) {
+      if (tid < C / 32) poison[tid] = 0u;
+      KNJ_BARRIER_AFTER(kLdsOnly);
+      for (int o = 16 * tid; o < CB; o += 16 * NTH) {
+        const int q = o / RB;
+        if (p0 + q < P) continue;
+        uint4* w = reinterpret_cast<uint4*>(at + CB + o);
+        uint4 v = *w;
+        bool any = false;
+        any |= drop_nonfinite<FORMAT>(v.x);
+        any |= drop_nonfinite<FORMAT>(v.y);
+        any |= drop_nonfinite<FORMAT>(v.z);
+        any |= drop_nonfinite<FORMAT>(v.w);
+        if (!any) continue;
+        *w = v;
+        if (p0 + q < valid) atomicOr(&poison[q >> 5], 1u << (q & 31));
+      }
+      KNJ_BARRIER_AFTER(kLdsOnly);
+    }
+    chunk(std::true_type{}, at, p0);
   }
 
   // ---- columns out: sums over the four lanes of a column, scales back in
@@ -476,55 +589,96 @@ __global__ __launch_bounds__(kBlock, 2) void k_tree(TreeArgs a, TreePlan p) {
     m[nt] = m[nt] == -INFINITY ? -INFINITY : m[nt] * s2[nt];
     if constexpr (Q8) {
 #pragma unroll
-      for (int dt = 0; dt < D / 16; ++dt)
+      for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[nt][dt][i] *= vref[nt];
     }
   }
-  if constexpr (WS == 1) {
+  __builtin_amdgcn_s_waitcnt(0);  // the fetches past the range land before LDS is reused or given back
+  if constexpr (WS > 1) {
+    // the waves that shared the columns, in pairs: the upper half leaves its
+    // registers in LDS, the lower half takes them in
+    constexpr int WV = WC * NT;  // column tiles of one ws
+    float4* ja = reinterpret_cast<float4*>(lds);
+    float2* jm = reinterpret_cast<float2*>(lds + WS / 2 * WV * DT * 1024);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int col = tile * COLS + (wc * NT + nt) * 16 + r;
+    for (int h = WS / 2; h >= 1; h >>= 1) {
+      __syncthreads();
+      if (ws >= h && ws < 2 * h) {
 #pragma unroll
-      for (int dt = 0; dt < D / 16; ++dt)
-        emit<D>(a, p, s, kvh, split, n_cols, G, N, col, 16 * dt + 4 * kq, m[nt], l[nt],
-                make_float4(acc[nt][dt][0], acc[nt][dt][1], acc[nt][dt][2], acc[nt][dt][3]));
-    }
-  } else {
-    // the waves that shared the slots join their columns through LDS
-    float* ja = reinterpret_cast<float*>(lds);
-    __syncthreads();
+        for (int nt = 0; nt < NT; ++nt) {
+          const int u = (ws - h) * WV + wc * NT + nt;
+          jm[u * 64 + lane] = make_float2(m[nt], l[nt]);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int col = (wc * NT + nt) * 16 + r;
-      if (kq == 0) {
-        jm[ws * COLS + col] = m[nt];
-        jl[ws * COLS + col] = l[nt];
+          for (int dt = 0; dt < DT; ++dt)
+            ja[(u * DT + dt) * 64 + lane] = make_float4(acc[nt][dt][0], acc[nt][dt][1], acc[nt][dt][2], acc[nt][dt][3]);
+        }
       }
+      __syncthreads();
+      if (ws < h) {
 #pragma unroll
-      for (int dt = 0; dt < D / 16; ++dt)
-        *reinterpret_cast<float4*>(ja + (ws * COLS + col) * (D + 4) + 16 * dt + 4 * kq) =
-            make_float4(acc[nt][dt][0], acc[nt][dt][1], acc[nt][dt][2], acc[nt][dt][3]);
-    }
-    __syncthreads();
-    for (int i = tid; i < COLS * (D / 4); i += kBlock) {
-      const int col = i / (D / 4), d = 4 * (i % (D / 4));
-      float M = -INFINITY, L = 0.0f;
+        for (int nt = 0; nt < NT; ++nt) {
+          const int u = ws * WV + wc * NT + nt;
+          const float2 ml = jm[u * 64 + lane];
+          const float M = fmaxf(m[nt], ml.x), mr = M == -INFINITY ? 0.0f : M;
+          const float fa = exp2f(m[nt] - mr), fb = exp2f(ml.x - mr);
+          m[nt] = M;
+          l[nt] = l[nt] * fa + ml.y * fb;
 #pragma unroll
-      for (int k = 0; k < WS; ++k) M = fmaxf(M, jm[k * COLS + col]);
-      const float mr = M == -INFINITY ? 0.0f : M;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int k = 0; k < WS; ++k) {
-        const float f = exp2f(jm[k * COLS + col] - mr);
-        const float4 v = *reinterpret_cast<const float4*>(ja + (k * COLS + col) * (D + 4) + d);
-        L += jl[k * COLS + col] * f;
-        o.x += v.x * f;
-        o.y += v.y * f;
-        o.z += v.z * f;
-        o.w += v.w * f;
+          for (int dt = 0; dt < DT; ++dt) {
+            const float4 v = ja[(u * DT + dt) * 64 + lane];
+            acc[nt][dt][0] = acc[nt][dt][0] * fa + v.x * fb;
+            acc[nt][dt][1] = acc[nt][dt][1] * fa + v.y * fb;
+            acc[nt][dt][2] = acc[nt][dt][2] * fa + v.z * fb;
+            acc[nt][dt][3] = acc[nt][dt][3] * fa + v.w * fb;
+          }
+        }
       }
-      emit<D>(a, p, s, kvh, split, n_cols, G, N, tile * COLS + col, d, M, L, o);
+    }
+    if (ws != 0) return;
+  }
+  // the results of a column, or its split record: the maximum in base-2 units, the
+  // sum and the weighted values.  A lane has dims 16 dt + 4 kq + i, or with 8 bits
+  // 32 b + 8 kq + 2 i of tile 2b and the dims after those of tile 2b + 1.
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int col = tile * COLS + (wc * NT + nt) * 16 + r;
+    if (col >= N * G) continue;
+    float4 o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      if constexpr (Q8) {
+        const f32x4 e = acc[nt][dt & ~1], f = acc[nt][dt | 1];
+        o[dt] = (dt & 1) ? make_float4(e[2], f[2], e[3], f[3]) : make_float4(e[0], f[0], e[1], f[1]);
+      } else {
+        o[dt] = make_float4(acc[nt][dt][0], acc[nt][dt][1], acc[nt][dt][2], acc[nt][dt][3]);
+      }
+    }
+    constexpr auto dim = [](int dt) { return Q8 ? 32 * (dt >> 1) + 4 * (dt & 1) : 16 * dt; };
+    const int d0 = (Q8 ? 8 : 4) * kq;
+    if (p.n_split > 1) {
+      float* rec = a.partial + ((((uint64_t)s * nk + kvh) * p.n_split + split) * n_cols + col) * (D + 4);
+      if (kq == 0) *reinterpret_cast<float2*>(rec) = make_float2(m[nt], l[nt]);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float4*>(rec + 4 + d0 + dim(dt)) = o[dt];
+      continue;
+    }
+    const float inv = l[nt] == 0.0f ? 0.0f : 1.0f / l[nt];  // nothing seen: zeros
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] = make_float4(o[dt].x * inv, o[dt].y * inv, o[dt].z * inv, o[dt].w * inv);
+    const int t = tcol[nt];  // (col is below N G: t is its own)
+    const uint64_t to = ((uint64_t)s * a.n_rows + t) * a.out_stride + (uint64_t)(kvh * G + col - t * G) * D + d0;
+    if constexpr (SPLIT) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float4*>((float*)a.out + to + dim(dt)) = o[dt];
+    } else if (a.type == KNJ_TYPE_F16) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        *reinterpret_cast<uint2*>((uint16_t*)a.out + to + dim(dt)) = pack4(KNJ_TYPE_F16, o[dt]);
+    } else {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        *reinterpret_cast<uint2*>((uint16_t*)a.out + to + dim(dt)) = pack4(KNJ_TYPE_BF16, o[dt]);
     }
   }
 }
@@ -537,7 +691,7 @@ hipError_t launch_format(const TreeArgs& a, const TreePlan& p, int cols, hipStre
 #define KNJ_TREE_FORMAT(FORMAT)                                                                          \
   template <>                                                                                            \
   hipError_t launch_format<FORMAT>(const TreeArgs& a, const TreePlan& p, int cols, hipStream_t s) {      \
-    const dim3 grid((unsigned)((p.units + 7) / 8 * 8 * p.n_tiles));                                      \
+    const dim3 grid(8 * p.n_tiles, (p.units + 7) / 8);                                                   \
     const bool split = a.type == KNJ_TYPE_F32;                                                           \
     if (a.c.head_dim == 128) {                                                                           \
       if (split) KNJ_TREE_COLS(128, FORMAT, true);                                                       \
@@ -548,13 +702,18 @@ hipError_t launch_format(const TreeArgs& a, const TreePlan& p, int cols, hipStre
     }                                                                                                    \
     return hipGetLastError();                                                                            \
   }
-#define KNJ_TREE_COLS(DD, FORMAT, SPLIT)                                                                 \
-  do {                                                                                                   \
-    if (cols == 16) KNJ_LAUNCH((k_tree<DD, FORMAT, SPLIT, 1, 1, 32>), grid, dim3(kBlock), 0, s, a, p);   \
-    else if (cols == 32) KNJ_LAUNCH((k_tree<DD, FORMAT, SPLIT, 2, 1, 32>), grid, dim3(kBlock), 0, s, a, p); \
-    else if (cols == 64) KNJ_LAUNCH((k_tree<DD, FORMAT, SPLIT, 2, 2, 64>), grid, dim3(kBlock), 0, s, a, p); \
-    else KNJ_LAUNCH((k_tree<DD, FORMAT, SPLIT, 2, 4, 64>), grid, dim3(kBlock), 0, s, a, p);              \
+#define KNJ_TREE_COLS(DD, FORMAT, SPLIT)                                                             \
+  do {                                                                                               \
+    if (cols == 16) KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, 1, 1, 4, 16);                                 \
+    else if (cols == 32) KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, 1, 2, 2, 32);                            \
+    else if (SPLIT) KNJ_TREE_LAUNCH(DD, FORMAT, true, 1, 4, 1, 64);                                  \
+    else if (cols == 64) KNJ_TREE_LAUNCH(DD, FORMAT, false, 2, 2, 2, 32);                            \
+    else KNJ_TREE_LAUNCH(DD, FORMAT, false, 2, 4, 1, 64);                                            \
   } while (0)
+// two stages of an f16 cache's rows fill LDS for two workgroups, three of an 8-bit one's
+#define KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, NT, WC, WS, SW)                                           \
+  KNJ_LAUNCH((k_tree<DD, FORMAT, SPLIT, NT, WC, WS, SW, FORMAT == KNJ_KV_F16 ? 2 : 3>), grid,        \
+             dim3(64 * WC * WS), 0, s, a, p)
 
 }  // namespace tree
 }  // namespace knj

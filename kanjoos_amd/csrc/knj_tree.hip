@@ -65,53 +65,57 @@ __global__ __launch_bounds__(kBlock) void k_tree_merge(TreeArgs a, TreePlan p, i
     o = make_float4(o.x + v.x * f, o.y + v.y * f, o.z + v.z * f, o.w + v.w * f);
   }
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // nothing seen: zeros
-  store4(a.type, a.out, (uint64_t)row * a.out_stride + (uint64_t)h * D + 4 * d,
-         make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+  o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  const uint64_t to = (uint64_t)row * a.out_stride + (uint64_t)h * D + 4 * d;
+  if (a.type == KNJ_TYPE_F32) *reinterpret_cast<float4*>((float*)a.out + to) = o;
+  else *reinterpret_cast<uint2*>((uint16_t*)a.out + to) = pack4(a.type, o);
 }
 
 namespace {
 
 // Columns of a tile and slots of a chunk, by the columns a kv head has in all.
 struct Shape {
-  int cols, chunk;
+  int cols, chunk, waves;
 };
-Shape shape_of(int cols) {
-  if (cols <= 16) return {16, 128};
-  if (cols <= 32) return {32, 128};
-  if (cols <= 64) return {64, 128};
-  return {128, 64};
+Shape shape_of(int cols, bool split) {
+  if (cols <= 16) return {16, 64, 4};
+  if (cols <= 32) return {32, 64, 4};
+  if (cols <= 64 || split) return {64, 64, 4};
+  return {128, 64, 4};
 }
 
-// workgroups that the slots are split for
-constexpr int kTreeWGs = 512;
+// waves that the slots are split for: two per SIMD, what the registers admit
+constexpr int kTreeWaves = 2048;
 
 struct Planned {
   TreePlan p;
   Shape sh;
 };
-Planned plan(const knj_kv_cache& c, int n_head, int n_rows, int max_prefix) {
+Planned plan(const knj_kv_cache& c, int type, int n_head, int n_rows, int max_prefix) {
   const int cols = n_rows * (n_head / c.n_head_kv);
-  const Shape sh = shape_of(cols);
+  const Shape sh = shape_of(cols, type == KNJ_TYPE_F32);
   const int tiles = (cols + sh.cols - 1) / sh.cols;
   const int chunks = (max_prefix + n_rows + sh.chunk - 1) / sh.chunk;
   const int64_t base = (int64_t)c.n_seq * c.n_head_kv * tiles;
-  const int64_t want = std::max<int64_t>(1, kTreeWGs / base);
+  const int64_t want = std::max<int64_t>(1, kTreeWaves / sh.waves / base);
   const int cps = (int)std::max<int64_t>(1, (chunks + want - 1) / want);
   const int n_split = (chunks + cps - 1) / cps;
-  return {TreePlan{cps, n_split, tiles, (int)(c.n_seq * (int64_t)c.n_head_kv * n_split)}, sh};
+  return {TreePlan{cps, n_split, tiles, (int)(c.n_seq * (int64_t)c.n_head_kv * n_split), FastDiv(c.n_head_kv),
+                   FastDiv(n_split), FastDiv(n_head / c.n_head_kv)},
+          sh};
 }
 
 }  // namespace
 }  // namespace tree
 
-uint64_t tree_partial_bytes(const knj_kv_cache& c, int n_head, int n_rows, int max_prefix) {
-  const tree::Planned q = tree::plan(c, n_head, n_rows, max_prefix);
+uint64_t tree_partial_bytes(const knj_kv_cache& c, int type, int n_head, int n_rows, int max_prefix) {
+  const tree::Planned q = tree::plan(c, type, n_head, n_rows, max_prefix);
   if (q.p.n_split == 1) return 0;
   return (uint64_t)q.p.units * q.p.n_tiles * q.sh.cols * (c.head_dim + 4) * sizeof(float);
 }
 
 hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t s) {
-  const tree::Planned q = tree::plan(a.c, a.n_head, a.n_rows, a.max_prefix);
+  const tree::Planned q = tree::plan(a.c, a.type, a.n_head, a.n_rows, a.max_prefix);
   hipError_t e;
   if (a.c.format == KNJ_KV_F16) e = tree::launch_format<KNJ_KV_F16>(a, q.p, q.sh.cols, s);
   else if (a.c.format == KNJ_KV_F8) e = tree::launch_format<KNJ_KV_F8>(a, q.p, q.sh.cols, s);
