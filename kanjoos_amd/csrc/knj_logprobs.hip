@@ -22,7 +22,10 @@ constexpr int kPer = kPiece / 64;
 constexpr int kMaxTop = 32;
 constexpr int kMaxVocab = 1 << 20;
 constexpr int kMaxPieces = kMaxVocab / kPiece;  // 512
-constexpr int kJoin = 512;     // threads of the joining workgroup
+constexpr int kCand = kMaxTop * (kMaxTop + 1) / 2;  // candidates of the largest: sum of n - q over the n pieces
+// Waves of a row's joining workgroup: sixteen hold all the pieces of the n largest
+// at once; past kJoinRows rows, four a row keep the chip busier.
+constexpr int kJoinRows = 128;
 
 struct Record {
   uint32_t key;   // order_key of the piece's largest logit
@@ -84,6 +87,13 @@ __device__ __forceinline__ void load_piece(const void* logits, uint64_t row_at, 
   }
 }
 
+// A logit's place in the order of the largest: by value, ties to the lowest
+// index; a NaN as -inf, 0 past the row's end.
+__device__ __forceinline__ unsigned long long piece_key(float v, uint32_t idx, int n_vocab) {
+  if (idx >= (uint32_t)n_vocab) return 0ull;
+  return ((unsigned long long)order_key(v == v ? v : -INFINITY) << 32) | (0xFFFFFFFFu - idx);
+}
+
 // Record of one piece per wave.  With the largest logit m of the piece and
 // d = (x - m) log2(e) / T <= 0: rest = sum 2^d, ent = sum 2^d d over all but the
 // largest itself, so that a row with one likely token keeps log(1 + rest) to the
@@ -132,60 +142,123 @@ __global__ __launch_bounds__(kBlock) void k_logprob_pieces(LogprobArgs a, int n_
     ((Record*)a.records)[w] = Record{(uint32_t)(top >> 32), top_idx, bad ? NAN : rest, ent};
 }
 
+// 2^d in f64 to f32's precision, d <= 0.
+__device__ __forceinline__ double exp2_neg(double d) {
+  const double n = rint(fmax(d, -2000.0));
+  return ldexp((double)__builtin_amdgcn_exp2f((float)(fmax(d, -2000.0) - n)), (int)n);
+}
+
+// How many of keys[0 .. n) are above `key`; n a multiple of 8 (zeros fill it).
+__device__ __forceinline__ int rank_among(const unsigned long long* keys, int n, unsigned long long key) {
+  int rank = 0;
+  for (int j = 0; j < n; j += 8) {
+    ulonglong2 k[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k[i] = *reinterpret_cast<const ulonglong2*>(keys + j + 2 * i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rank += (k[i].x > key) + (k[i].y > key);
+  }
+  return rank;
+}
+
 // A row's records joined.  With M the row's largest logit, f = 2^((m - M) c) of
 // each piece: rest = sum over the pieces of f (1 + rest_p), without the 1 of the
 // piece that holds M, and ent = sum of f (ent_p + (1 + rest_p) (m - M) c); then
 // log sum e^(x - M) = log1p(rest), the entropy log1p(rest) - ln 2 ent / (1 + rest).
-template <int TYPE>
-__global__ __launch_bounds__(kJoin) void k_logprob_join(LogprobArgs a, int n_pieces, double c) {
-  constexpr int W = kJoin / 64;
-  __shared__ unsigned long long keys[kMaxPieces];
-  __shared__ unsigned long long cand[kMaxTop * (kMaxTop + 1) / 2];
+// The pieces that can hold one of the n largest are ranked and fetched first, so
+// that the sums are formed while they are on their way.  W waves a row.
+template <int TYPE, int W>
+__global__ __launch_bounds__(64 * W) void k_logprob_join(LogprobArgs a, int n_pieces, double c) {
+  constexpr int NT = 64 * W, R = kMaxPieces > NT ? kMaxPieces / NT : 1;  // records a thread
+  __shared__ __align__(16) unsigned long long keys[kMaxPieces];
+  __shared__ __align__(16) unsigned long long cand[kCand + 8];
   __shared__ unsigned long long red_key[W];
   __shared__ double red_rest[W], red_ent[W];
   __shared__ int red_bad[W], chosen[kMaxTop];
+  __shared__ int n_cand;
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Record* rec = (const Record*)a.records + (uint64_t)row * n_pieces;
-  Record r{0u, 0u, 0.0f, 0.0f};
-  unsigned long long key = 0;
-  if (tid < n_pieces) {  // n_pieces <= kMaxPieces = kJoin
-    r = rec[tid];
-    key = ((unsigned long long)r.key << 32) | (0xFFFFFFFFu - r.idx);
+  const uint64_t row_at = (uint64_t)row * a.row_stride;
+  const int n = a.n_top, n_sel = min(n, n_pieces);
+  Record r[R];
+  unsigned long long key[R], wk = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int p = tid + i * NT;
+    r[i] = Record{0u, 0u, 0.0f, 0.0f};
+    key[i] = 0;
+    if (p < n_pieces) {
+      r[i] = rec[p];
+      key[i] = ((unsigned long long)r[i].key << 32) | (0xFFFFFFFFu - r[i].idx);
+    }
+    if (p < kMaxPieces) keys[p] = key[i];
+    wk = key[i] > wk ? key[i] : wk;
   }
-  keys[tid] = key;
-  const unsigned long long wk = wave_max_u64(key);
+  if (tid == 0) n_cand = 0;
+  wk = wave_max_u64(wk);
   if (lane == 0) red_key[wave] = wk;
   __syncthreads();
   unsigned long long top = red_key[0];
 #pragma unroll
   for (int i = 1; i < W; ++i) top = red_key[i] > top ? red_key[i] : top;
   const float M = order_value((uint32_t)(top >> 32));
-  double rest = 0.0, ent = 0.0;
-  bool bad = tid < n_pieces && r.rest != r.rest;
-  const float m = order_value(r.key);
-  if (tid < n_pieces && m > -INFINITY && M < INFINITY && !bad) {
-    const double d = ((double)m - (double)M) * c;
-    const double f = exp2(d);
-    const double own = (double)r.rest + (key == top ? 0.0 : 1.0);
-    rest = f * own;
-    ent = f * ((double)r.ent + (1.0 + (double)r.rest) * d);
-  }
+  // the n pieces with the largest keys, by rank (keys differ: their indexes do)
+  if (n) {
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    rest += __shfl_xor(rest, o);
-    ent += __shfl_xor(ent, o);
+    for (int i = 0; i < R; ++i) {
+      if (tid + i * NT >= n_pieces) break;
+      const int rank = rank_among(keys, (n_pieces + 7) & ~7, key[i]);
+      if (rank < n) chosen[rank] = tid + i * NT;
+    }
   }
-  bad = __ballot(bad) != 0;
-  if (lane == 0) {
-    red_rest[wave] = rest;
-    red_ent[wave] = ent;
-    red_bad[wave] = bad;
+  float x_tok = 0.0f;  // the given token's logit
+  const int tok = tid == 0 && a.logprob ? a.tokens[row] : -1;
+  if (tok >= 0 && tok < a.n_vocab) {
+    if constexpr (TYPE == KNJ_TYPE_F32) x_tok = ((const float*)a.logits)[row_at + tok];
+    else if constexpr (TYPE == KNJ_TYPE_F16) x_tok = h2f(((const uint16_t*)a.logits)[row_at + tok]);
+    else x_tok = __uint_as_float((uint32_t)((const uint16_t*)a.logits)[row_at + tok] << 16);
+  }
+  double rest = 0.0, ent = 0.0;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if (tid + i * NT >= n_pieces) break;
+    const bool b = r[i].rest != r[i].rest;
+    bad |= b;
+    const float m = order_value(r[i].key);
+    if (m > -INFINITY && M < INFINITY && !b) {
+      const double d = ((double)m - (double)M) * c;
+      const double f = exp2_neg(d);
+      rest += f * ((double)r[i].rest + (key[i] == top ? 0.0 : 1.0));
+      ent += f * ((double)r[i].ent + (1.0 + (double)r[i].rest) * d);
+    }
+  }
+  const int waves = min(W, (n_pieces + 63) >> 6);  // that hold records
+  if (wave < waves) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      rest += __shfl_xor(rest, o);
+      ent += __shfl_xor(ent, o);
+    }
+    bad = __ballot(bad) != 0;
+    if (lane == 0) {
+      red_rest[wave] = rest;
+      red_ent[wave] = ent;
+      red_bad[wave] = bad;
+    }
   }
   __syncthreads();
+  float v[2][kPer];  // the chosen pieces of ranks `wave` and W + wave
+  auto fetch = [&](int q0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (q0 + h * W + wave < n_sel)
+        load_piece<TYPE>(a.logits, row_at, chosen[q0 + h * W + wave], a.n_vocab, lane, v[h]);
+  };
+  fetch(0);
   rest = ent = 0.0;
   bad = false;
-#pragma unroll
-  for (int i = 0; i < W; ++i) {
+  for (int i = 0; i < waves; ++i) {
     rest += red_rest[i];
     ent += red_ent[i];
     bad |= red_bad[i] != 0;
@@ -200,69 +273,61 @@ __global__ __launch_bounds__(kJoin) void k_logprob_join(LogprobArgs a, int n_pie
   };
   if (tid == 0) {
     if (a.entropy) a.entropy[row] = bad ? NAN : none ? 0.0f : (float)(lse - 0.6931471805599453 * ent / (1.0 + rest));
-    if (a.logprob) {
-      const int t = a.tokens[row];
-      float lp = t < 0 ? 0.0f : NAN;
-      if (t >= 0 && t < a.n_vocab) {
-        const uint64_t at = (uint64_t)row * a.row_stride + t;
-        float x;
-        if constexpr (TYPE == KNJ_TYPE_F32) x = ((const float*)a.logits)[at];
-        else if constexpr (TYPE == KNJ_TYPE_F16) x = h2f(((const uint16_t*)a.logits)[at]);
-        else x = __uint_as_float((uint32_t)((const uint16_t*)a.logits)[at] << 16);
-        lp = logp(x);
-      }
-      a.logprob[row] = lp;
-    }
+    if (a.logprob) a.logprob[row] = tok < 0 ? 0.0f : tok >= a.n_vocab ? NAN : logp(x_tok);
   }
-  const int n = a.n_top;
   if (n == 0) return;
-  // the n pieces with the largest keys, by rank (keys differ: their indexes do)
-  if (tid < n_pieces) {
-    int rank = 0;
-    for (int j = 0; j < n_pieces; ++j) rank += keys[j] > key;
-    if (rank < n) chosen[rank] = tid;
-  }
-  for (int i = tid; i < kMaxTop * (kMaxTop + 1) / 2; i += kJoin) cand[i] = 0;
-  __syncthreads();
-  const int n_sel = min(n, n_pieces);
-  // every one of the n largest logits is at least the n-th piece's largest
+  // Every one of the n largest logits is at least the n-th piece's largest: the
+  // logits that are (few more than n, as a rule) become candidates, in any order.
   const unsigned long long least = n_pieces >= n ? keys[chosen[n - 1]] : 1ull;
-  // wave by wave: the chosen piece of rank q holds at most n - q of them, taken
-  // out one after the other into its own places
-  for (int q = wave; q < n_sel; q += W) {
-    const int piece = chosen[q];
-    float v[kPer];
-    load_piece<TYPE>(a.logits, (uint64_t)row * a.row_stride, piece, a.n_vocab, lane, v);
-    uint32_t u[kPer];
+  for (int q0 = 0; q0 < n_sel; q0 += 2 * W) {
+    if (q0) fetch(q0);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      u[i] = piece_index<TYPE>(piece, lane, i) < a.n_vocab ? order_key(v[i] == v[i] ? v[i] : -INFINITY) : 0u;
-    const int at = q * n - q * (q - 1) / 2;
-    for (int t = 0; t < n - q; ++t) {
-      uint32_t best = 0;
-      int bi = 0;
+    for (int h = 0; h < 2; ++h) {
+      if (q0 + h * W + wave >= n_sel) break;
+      const int piece = chosen[q0 + h * W + wave];
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (u[i] > best) {
-          best = u[i];
-          bi = i;
-        }
-      const uint32_t idx = piece_index<TYPE>(piece, lane, bi);
-      const unsigned long long mine = best ? ((unsigned long long)best << 32) | (0xFFFFFFFFu - idx) : 0ull;
-      const unsigned long long big = wave_max_u64(mine);
-      if (big < least) break;  // (uniform; also when the piece is used up)
-      if (lane == 0) cand[at + t] = big;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) u[i] = (mine == big && i == bi) ? 0u : u[i];
+      for (int i = 0; i < kPer; ++i) {
+        if (order_key(v[h][i] == v[h][i] ? v[h][i] : -INFINITY) < (uint32_t)(least >> 32)) continue;
+        const unsigned long long mine = piece_key(v[h][i], piece_index<TYPE>(piece, lane, i), a.n_vocab);
+        if (mine < least) continue;
+        const int at = atomicAdd(&n_cand, 1);
+        if (at < kCand) cand[at] = mine;
+      }
     }
   }
   __syncthreads();
-  const int n_cand = n_sel * n - n_sel * (n_sel - 1) / 2;
-  for (int i = tid; i < n_cand; i += kJoin) {
+  int nc = n_cand;
+  if (nc > kCand) {
+    // Rows whose largest logits crowd into few pieces (sorted ones, equal ones): the
+    // chosen piece of rank q holds at most n - q of the n largest, taken out one
+    // after the other.
+    __syncthreads();
+    if (tid == 0) n_cand = 0;
+    __syncthreads();
+    for (int q = wave; q < n_sel; q += W) {
+      const int piece = chosen[q];
+      load_piece<TYPE>(a.logits, row_at, piece, a.n_vocab, lane, v[0]);
+      unsigned long long last = ~0ull;  // the key taken out before
+      for (int t = 0; t < n - q; ++t) {
+        unsigned long long mine = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const unsigned long long k = piece_key(v[0][i], piece_index<TYPE>(piece, lane, i), a.n_vocab);
+          mine = k < last && k > mine ? k : mine;
+        }
+        last = wave_max_u64(mine);
+        if (last < least) break;  // (uniform; also when the piece is used up)
+        if (lane == 0) cand[atomicAdd(&n_cand, 1)] = last;
+      }
+    }
+    __syncthreads();
+    nc = n_cand;
+  }
+  if (tid < 8) cand[nc + tid] = 0;  // (whole eights for the ranking)
+  __syncthreads();
+  for (int i = tid; i < nc; i += NT) {
     const unsigned long long mine = cand[i];
-    if (!mine) continue;
-    int rank = 0;
-    for (int j = 0; j < n_cand; ++j) rank += cand[j] > mine;
+    const int rank = rank_among(cand, (nc + 7) & ~7, mine);
     if (rank < n) {
       a.top_idx[(uint64_t)row * n + rank] = (int32_t)(0xFFFFFFFFu - (uint32_t)mine);
       a.top_logprob[(uint64_t)row * n + rank] = logp(order_value((uint32_t)(mine >> 32)));
@@ -287,7 +352,10 @@ hipError_t launch_token_logprobs(int type, const LogprobArgs& a, hipStream_t s) 
 #define KNJ_LOGPROBS(TYPE)                                                                            \
   do {                                                                                                \
     KNJ_LAUNCH(k_logprob_pieces<TYPE>, grid, dim3(kBlock), 0, s, a, n_pieces, c_hi, c_lo);            \
-    KNJ_LAUNCH(k_logprob_join<TYPE>, dim3(a.n_rows), dim3(kJoin), 0, s, a, n_pieces, c);              \
+    if (a.n_rows <= kJoinRows)                                                                        \
+      KNJ_LAUNCH((k_logprob_join<TYPE, 16>), dim3(a.n_rows), dim3(1024), 0, s, a, n_pieces, c);       \
+    else                                                                                              \
+      KNJ_LAUNCH((k_logprob_join<TYPE, 4>), dim3(a.n_rows), dim3(256), 0, s, a, n_pieces, c);         \
   } while (0)
   if (type == KNJ_TYPE_F32) KNJ_LOGPROBS(KNJ_TYPE_F32);
   else if (type == KNJ_TYPE_F16) KNJ_LOGPROBS(KNJ_TYPE_F16);
