@@ -1,8 +1,8 @@
 // kanjoos_amd/csrc/knj_rope_kv.hip -- rotary positions of query and key rows, and cache rows
 // written in f16 or 8 bits and read back.
 //
-// Both are streams over rows of heads: a group of D/8 lanes holds one head, eight
-// elements a lane, so a head's reductions (the norm's sum, the largest
+// Both are streams over rows of heads: a group of D/8 lanes holds one head's row (of
+// a cache its key and its value), eight elements a lane, so a head's reductions (the norm's sum, the largest
 // magnitude) stay inside the group's DPP moves and every element is read and
 // written once.
 #include <algorithm>
@@ -109,148 +109,159 @@ __global__ __launch_bounds__(kBlock) void k_rope(RopeArgs a) {
 }
 
 // ---------------------------------------------------------------- cache rows
-// rint(x * top / amax * rstep) of the exact quotient, ties to even (rstep a
-// power of two); `inv` is top / amax in f64.  The product with it is off by 2^-52 of the quotient,
-// which decides a rounding only next to a tie: there the quotient is divided
-// out (x * top * rstep is exact, and a division that is correctly rounded gives
-// the tie itself for a quotient that is one).
-__device__ __forceinline__ double quotient_code(float x, double inv, double top, double amax, double rstep) {
-  const double z = (double)x * inv * rstep;
-  double t = rint(z);
-  if (fabs(fabs(z - t) - 0.5) < 1e-9) t = rint((double)x * top * rstep / amax);
+// rint(x * top / amax * rstep) of the exact quotient, ties to even (rstep a power
+// of two, the result at most 127); `inv` is top / amax.  The f32 product with it is
+// off by 2^-23 of itself, 1.6e-5, which decides a rounding only next to a tie:
+// there the quotient is divided out in f64 (x * top * rstep is exact, and a division
+// that is correctly rounded gives the tie itself for a quotient that is one).
+__device__ __forceinline__ float quotient_code(float x, float inv, double top, float amax, float rstep) {
+  const float z = x * inv * rstep;
+  float t = rintf(z);
+  if (fabsf(fabsf(z - t) - 0.5f) < 1e-4f) t = (float)rint((double)x * top * (double)rstep / (double)amax);
   return t;
 }
 
-// Rows of `FORMAT` from rows of activations: head-row u = ((s, t), k or v, head).
-template <int TYPE, int FORMAT, int D>
-__global__ __launch_bounds__(kBlock) void k_kv_store(KvRowsArgs a) {
-  constexpr int T = D / 8;
-  const knj_kv_cache& c = a.c;
-  const uint64_t u0 = (uint64_t)blockIdx.x * (kBlock / T) + threadIdx.x / T;
-  const int lane = threadIdx.x % T;
-  const uint64_t total = (uint64_t)c.n_seq * a.n_rows * 2 * c.n_head_kv;
-  const uint64_t u = u0 < total ? u0 : total - 1;  // every lane computes; those past the rows store nothing
-  const uint32_t per = 2 * c.n_head_kv;
-  const uint64_t row = u / per;
-  const uint32_t hv = (uint32_t)(u - row * per);
-  const bool is_v = hv >= (uint32_t)c.n_head_kv;
-  const int h = is_v ? hv - c.n_head_kv : hv;
-  const uint32_t s = (uint32_t)(row / (uint32_t)a.n_rows), t = (uint32_t)(row - (uint64_t)s * a.n_rows);
-  const int64_t slot = (int64_t)a.index[s] + t;
-  const bool keep = u0 < total && slot >= 0 && slot < c.n_ctx && (!a.counts || (int64_t)t < a.counts[s]);
-  const void* src = is_v ? a.v : a.k;
-  const uint64_t at = row * a.row_stride + (uint64_t)h * D + 8 * lane;
-  const float4 p = ld4<TYPE>(src, at), q = ld4<TYPE>(src, at + 4);
-  const float x[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
-  const uint64_t to = (uint64_t)s * c.seq_stride + ((uint64_t)h * c.n_ctx + slot) * D + 8 * lane;
-  void* dst = is_v ? c.v : c.k;
-  if constexpr (FORMAT == KNJ_KV_F16) {
-    uint4 w;
-    w.x = pack_act<KNJ_TYPE_F16>(x[0], x[1]);
-    w.y = pack_act<KNJ_TYPE_F16>(x[2], x[3]);
-    w.z = pack_act<KNJ_TYPE_F16>(x[4], x[5]);
-    w.w = pack_act<KNJ_TYPE_F16>(x[6], x[7]);
-    if (keep) *reinterpret_cast<uint4*>((uint16_t*)dst + to) = w;
-    return;
-  } else {
-    constexpr double kTop = FORMAT == KNJ_KV_I8 ? 127.0 : 448.0;
-    float amax = 0.0f;
-    bool bad = false;  // an infinity or a NaN
+// Where unit u of a sequence's rows (a row's kv head: its key and its value) lies:
+// T lanes hold eight elements of each.
+template <int T>
+struct Unit {
+  uint32_t t;  // row
+  int h, lane;
+  bool in;     // a unit there is (the lanes past the last repeat it and store nothing)
+  __device__ __forceinline__ Unit(const KvRowsArgs& a) {
+    const uint32_t nk = a.c.n_head_kv, total = (uint32_t)a.n_rows * nk;
+    const uint32_t u = blockIdx.x * (kBlock / T) + threadIdx.x / T;
+    in = u < total;
+    const uint32_t v = in ? u : total - 1;
+    t = v / nk;
+    h = (int)(v - t * nk);
+    lane = threadIdx.x % T;
+  }
+};
+
+// Eight values of a head's row as codes, and the row's scale, by its T lanes.
+template <int FORMAT, int T>
+__device__ __forceinline__ uint2 quantise8(const float (&x)[8], float& scale) {
+  constexpr double kTop = FORMAT == KNJ_KV_I8 ? 127.0 : 448.0;
+  float amax = 0.0f;
+  bool bad = false;  // an infinity or a NaN
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      amax = fmaxf(amax, fabsf(x[i]));
-      bad |= !(fabsf(x[i]) < INFINITY);
-    }
-    amax = group_max<T>(amax);
-    bad = group_max<T>(bad ? 1.0f : 0.0f) != 0.0f;
-    const bool live = !bad && amax >= 0x1p-119f;
-    const double inv = live ? kTop / (double)amax : 0.0;
+  for (int i = 0; i < 8; ++i) {
+    amax = fmaxf(amax, fabsf(x[i]));
+    bad |= !(fabsf(x[i]) < INFINITY);
+  }
+  amax = group_max<T>(amax);
+  bad = group_max<T>(bad ? 1.0f : 0.0f) != 0.0f;
+  const bool live = !bad && amax >= 0x1p-119f;
+  const float inv = live ? (float)kTop / amax : 0.0f;
+  scale = bad ? NAN : live ? amax / (float)kTop : 0.0f;
+  uint2 o;
+  if constexpr (FORMAT == KNJ_KV_I8) {
     int w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = (int)quotient_code(live ? x[i] : 0.0f, inv, kTop, amax, 1.0f);
+    o.x = (w[0] & 255) | ((w[1] & 255) << 8) | ((w[2] & 255) << 16) | ((uint32_t)w[3] << 24);
+    o.y = (w[4] & 255) | ((w[5] & 255) << 8) | ((w[6] & 255) << 16) | ((uint32_t)w[7] << 24);
+  } else {
     float f[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
+      // e4m3: three bits after the leading one, steps of 2^-9 below 2^-6
       const float xi = live ? x[i] : 0.0f;
-      if constexpr (FORMAT == KNJ_KV_I8) {
-        w[i] = (int)quotient_code(xi, inv, kTop, amax, 1.0);
-      } else {
-        // e4m3: three bits after the leading one, steps of 2^-9 below 2^-6
-        const uint64_t b = __builtin_bit_cast(uint64_t, (double)xi * inv);
-        const int e = max((int)((b >> 52) & 0x7FF) - 1023, -6);
-        const double step = __builtin_bit_cast(double, (uint64_t)(1023 + e - 3) << 52);
-        const double rstep = __builtin_bit_cast(double, (uint64_t)(1023 - e + 3) << 52);
-        f[i] = (float)(quotient_code(xi, inv, kTop, amax, rstep) * step);  // a value of e4m3
-      }
+      const int e = max((int)((__float_as_uint(xi * inv) >> 23) & 0xFF) - 127, -6);
+      const float step = __uint_as_float((uint32_t)(127 + e - 3) << 23);
+      const float rstep = __uint_as_float((uint32_t)(127 - e + 3) << 23);
+      f[i] = quotient_code(xi, inv, kTop, amax, rstep) * step;  // a value of e4m3
     }
-    uint2 o;
-    if constexpr (FORMAT == KNJ_KV_I8) {
-      o.x = (w[0] & 255) | ((w[1] & 255) << 8) | ((w[2] & 255) << 16) | ((uint32_t)w[3] << 24);
-      o.y = (w[4] & 255) | ((w[5] & 255) << 8) | ((w[6] & 255) << 16) | ((uint32_t)w[7] << 24);
-    } else {
-      int lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
-      int hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[4], f[5], 0, false);
-      o.x = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], lo, true);
-      o.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[6], f[7], hi, true);
-    }
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+    const int hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[4], f[5], 0, false);
+    o.x = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], lo, true);
+    o.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[6], f[7], hi, true);
+  }
+  return o;
+}
+
+// Rows of `FORMAT` from rows of activations; blockIdx.y is the sequence.
+template <int TYPE, int FORMAT, int D>
+__global__ __launch_bounds__(kBlock) void k_kv_store(KvRowsArgs a) {
+  const knj_kv_cache& c = a.c;
+  const Unit<D / 8> u(a);
+  const uint32_t s = blockIdx.y;
+  const uint64_t at = ((uint64_t)s * a.n_rows + u.t) * a.row_stride + (uint64_t)u.h * D + 8 * u.lane;
+  const float4 k0 = ld4<TYPE>(a.k, at), k1 = ld4<TYPE>(a.k, at + 4);
+  const float4 v0 = ld4<TYPE>(a.v, at), v1 = ld4<TYPE>(a.v, at + 4);
+  const int64_t slot = (int64_t)a.index[s] + u.t;
+  const bool keep = u.in && slot >= 0 && slot < c.n_ctx && (!a.counts || (int64_t)u.t < a.counts[s]);
+  const uint64_t row = (uint64_t)u.h * c.n_ctx + slot;
+  const uint64_t to = (uint64_t)s * c.seq_stride + row * D + 8 * u.lane;
+  const float k[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
+  const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+  if constexpr (FORMAT == KNJ_KV_F16) {
     if (!keep) return;
-    *reinterpret_cast<uint2*>((uint8_t*)dst + to) = o;
-    if (lane == 0) {
-      float* scale = (is_v ? c.v_scale : c.k_scale) + (uint64_t)s * (c.seq_stride / D) + (uint64_t)h * c.n_ctx + slot;
-      *scale = bad ? NAN : live ? amax / (float)kTop : 0.0f;
+    auto pack = [](const float (&x)[8]) {
+      return make_uint4(pack_act<KNJ_TYPE_F16>(x[0], x[1]), pack_act<KNJ_TYPE_F16>(x[2], x[3]),
+                        pack_act<KNJ_TYPE_F16>(x[4], x[5]), pack_act<KNJ_TYPE_F16>(x[6], x[7]));
+    };
+    *reinterpret_cast<uint4*>((uint16_t*)c.k + to) = pack(k);
+    *reinterpret_cast<uint4*>((uint16_t*)c.v + to) = pack(v);
+  } else {
+    float ks, vs;
+    const uint2 kw = quantise8<FORMAT, D / 8>(k, ks), vw = quantise8<FORMAT, D / 8>(v, vs);
+    if (!keep) return;
+    *reinterpret_cast<uint2*>((uint8_t*)c.k + to) = kw;
+    *reinterpret_cast<uint2*>((uint8_t*)c.v + to) = vw;
+    if (u.lane == 0) {
+      const uint64_t sc = (uint64_t)s * (c.seq_stride / D) + row;
+      c.k_scale[sc] = ks;
+      c.v_scale[sc] = vs;
     }
+  }
+}
+
+// Eight codes times their scale.
+template <int FORMAT>
+__device__ __forceinline__ void values8(uint2 w, float scale, float4& a, float4& b) {
+  if constexpr (FORMAT == KNJ_KV_I8) {
+    auto at = [](uint32_t x, int j) { return (float)(int8_t)(x >> (8 * j)); };
+    a = make_float4(at(w.x, 0) * scale, at(w.x, 1) * scale, at(w.x, 2) * scale, at(w.x, 3) * scale);
+    b = make_float4(at(w.y, 0) * scale, at(w.y, 1) * scale, at(w.y, 2) * scale, at(w.y, 3) * scale);
+  } else {
+    const auto p = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.x, false), q = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.x, true);
+    const auto r = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.y, false), t = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.y, true);
+    a = make_float4(p[0] * scale, p[1] * scale, q[0] * scale, q[1] * scale);
+    b = make_float4(r[0] * scale, r[1] * scale, t[0] * scale, t[1] * scale);
   }
 }
 
 // The reverse: rows of activations from cache slots.
 template <int TYPE, int FORMAT, int D>
 __global__ __launch_bounds__(kBlock) void k_kv_load(KvRowsArgs a) {
-  constexpr int T = D / 8;
   const knj_kv_cache& c = a.c;
-  const uint64_t u = (uint64_t)blockIdx.x * (kBlock / T) + threadIdx.x / T;
-  const int lane = threadIdx.x % T;
-  const uint32_t per = 2 * c.n_head_kv;
-  const uint64_t row = u / per;
-  if (row >= (uint64_t)c.n_seq * a.n_rows) return;
-  const uint32_t hv = (uint32_t)(u - row * per);
-  const bool is_v = hv >= (uint32_t)c.n_head_kv;
-  const int h = is_v ? hv - c.n_head_kv : hv;
-  const uint32_t s = (uint32_t)(row / (uint32_t)a.n_rows), t = (uint32_t)(row - (uint64_t)s * a.n_rows);
-  const int slot = a.index ? a.index[row] : (int)t;
-  if (slot < 0 || slot >= c.n_ctx) return;
-  const uint64_t from = (uint64_t)s * c.seq_stride + ((uint64_t)h * c.n_ctx + slot) * D + 8 * lane;
-  const void* src = is_v ? c.v : c.k;
-  float x[8];
+  const Unit<D / 8> u(a);
+  const uint32_t s = blockIdx.y;
+  const uint64_t out = (uint64_t)s * a.n_rows + u.t;
+  const int slot = a.index ? a.index[out] : (int)u.t;
+  if (!u.in || slot < 0 || slot >= c.n_ctx) return;
+  const uint64_t row = (uint64_t)u.h * c.n_ctx + slot;
+  const uint64_t from = (uint64_t)s * c.seq_stride + row * D + 8 * u.lane;
+  float4 k0, k1, v0, v1;
   if constexpr (FORMAT == KNJ_KV_F16) {
-    const uint4 w = *reinterpret_cast<const uint4*>((const uint16_t*)src + from);
-    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = h2f(v[i]);
-      x[2 * i + 1] = h2f(v[i] >> 16);
-    }
+    k0 = ld4<KNJ_TYPE_F16>(c.k, from);
+    k1 = ld4<KNJ_TYPE_F16>(c.k, from + 4);
+    v0 = ld4<KNJ_TYPE_F16>(c.v, from);
+    v1 = ld4<KNJ_TYPE_F16>(c.v, from + 4);
   } else {
-    const uint2 w = *reinterpret_cast<const uint2*>((const uint8_t*)src + from);
-    const float scale =
-        ((is_v ? c.v_scale : c.k_scale) + (uint64_t)s * (c.seq_stride / D) + (uint64_t)h * c.n_ctx)[slot];
-    const uint32_t v[2] = {w.x, w.y};
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if constexpr (FORMAT == KNJ_KV_I8) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[4 * i + j] = (float)(int8_t)(v[i] >> (8 * j)) * scale;
-      } else {
-        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)v[i], false);
-        const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)v[i], true);
-        x[4 * i] = lo[0] * scale;
-        x[4 * i + 1] = lo[1] * scale;
-        x[4 * i + 2] = hi[0] * scale;
-        x[4 * i + 3] = hi[1] * scale;
-      }
-    }
+    const uint2 kw = *reinterpret_cast<const uint2*>((const uint8_t*)c.k + from);
+    const uint2 vw = *reinterpret_cast<const uint2*>((const uint8_t*)c.v + from);
+    const uint64_t sc = (uint64_t)s * (c.seq_stride / D) + row;
+    values8<FORMAT>(kw, c.k_scale[sc], k0, k1);
+    values8<FORMAT>(vw, c.v_scale[sc], v0, v1);
   }
-  void* dst = is_v ? a.v : a.k;
-  const uint64_t to = row * a.row_stride + (uint64_t)h * D + 8 * lane;
-  st4<TYPE>(dst, to, make_float4(x[0], x[1], x[2], x[3]));
-  st4<TYPE>(dst, to + 4, make_float4(x[4], x[5], x[6], x[7]));
+  const uint64_t to = out * a.row_stride + (uint64_t)u.h * D + 8 * u.lane;
+  st4<TYPE>(a.k, to, k0);
+  st4<TYPE>(a.k, to + 4, k1);
+  st4<TYPE>(a.v, to, v0);
+  st4<TYPE>(a.v, to + 4, v1);
 }
 
 // KERNEL<TYPE, second argument, D> for a run-time type, format and head_dim.
@@ -273,9 +284,8 @@ __global__ __launch_bounds__(kBlock) void k_kv_load(KvRowsArgs a) {
   } while (0)
 
 dim3 kv_rows_grid(const KvRowsArgs& a) {
-  const uint64_t units = (uint64_t)a.c.n_seq * a.n_rows * 2 * a.c.n_head_kv;
-  const uint64_t per = kBlock / (a.c.head_dim / 8);
-  return dim3((unsigned)((units + per - 1) / per));
+  const uint32_t units = (uint32_t)a.n_rows * a.c.n_head_kv, per = kBlock / (a.c.head_dim / 8);
+  return dim3((units + per - 1) / per, a.c.n_seq);
 }
 
 }  // namespace
@@ -311,7 +321,7 @@ int check_kv_cache(const knj_kv_cache* c) {
                 "cache format must be KNJ_KV_F16, KNJ_KV_F8 or KNJ_KV_I8");
   KNJ_CHECK_ARG(c->format == KNJ_KV_F16 || (c->k_scale && c->v_scale), "an 8-bit cache needs k_scale and v_scale");
   KNJ_CHECK_ARG(c->head_dim == 64 || c->head_dim == 128, "head_dim must be 64 or 128");
-  KNJ_CHECK_ARG(c->n_seq > 0 && c->n_seq <= 65536, "n_seq must be in [1, 65536]");
+  KNJ_CHECK_ARG(c->n_seq > 0 && c->n_seq <= 65535, "n_seq must be in [1, 65535]");
   KNJ_CHECK_ARG(c->n_head_kv > 0 && c->n_head_kv <= 64, "n_head_kv must be in [1, 64]");
   KNJ_CHECK_ARG(c->n_ctx > 0, "n_ctx must be positive");
   const uint64_t seq = (uint64_t)c->n_head_kv * c->n_ctx * c->head_dim;
@@ -414,7 +424,7 @@ static int check_kv_rows(const knj_kv_cache* cache, int type, const void* k, con
   KNJ_CHECK_ARG(row_stride >= (uint64_t)cache->n_head_kv * cache->head_dim, "the row stride is below the row's width");
   KNJ_CHECK_ARG(rows_aligned(k, row_stride, eb) && rows_aligned(v, row_stride, eb),
                 "rows must start on 16-byte boundaries");
-  KNJ_CHECK_ARG((uint64_t)cache->n_seq * n_rows * 2 * cache->n_head_kv < (1ull << 34), "too many rows for one call");
+  KNJ_CHECK_ARG((uint64_t)n_rows * cache->n_head_kv < (1ull << 31), "too many rows for one call");
   return KNJ_OK;
 }
 
