@@ -29,6 +29,7 @@ struct TreePlan {
   int n_tiles;   // column tiles of a full set of drafts
   int units;     // n_seq * n_split * n_head_kv
   FastDiv by_nk, by_split, by_group;  // n_head_kv, n_split, query heads per kv head
+  FastDiv by_head, by_rows, by_cps;   // n_head, n_rows, cps
 };
 
 namespace tree {
@@ -98,10 +99,10 @@ __device__ __forceinline__ u32x2 lds_tr16_at(uint32_t p) {
 
 // Weights are formed relative to a reference that follows the running maximum
 // only when that has passed it by 2^7 (the accumulators are rescaled then, which
-// after a column's first slots is rare), and held times 2^7: at most 2^14, or 2^15
+// after a column's first slots is rare), and held times 2^6: at most 2^13, or 2^15
 // with a value scale's factor, below f16's 65,504, and f16 keeps all of a weight's
-// bits down to 2^-21 of the reference.
-constexpr float kLift = 7.0f, kLag = 7.0f;
+// bits down to 2^-20 of the reference.
+constexpr float kLift = 6.0f, kLag = 7.0f;
 
 // Maximum that carries a NaN (a NaN score makes its column NaN); the instruction
 // takes three, without the quieting of its inputs that fmaxf asks for.
@@ -343,20 +344,20 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
   const uint32_t vat = CB + (ws * SW + pa) * RB + 32 * ((pa / RPB) & (NPAIR - 1)) + 8 * (r & 3);
   const uint32_t lds0 = lds_addr(lds);
 
-  // ---- one chunk in stage `at`; DRAFTS: it reaches the drafts or the end
-  auto chunk = [&](auto drafts_c, const uint8_t* at, int p0) {
-    constexpr bool DRAFTS = decltype(drafts_c)::value;
-    const uint32_t k0 = lds0 + (uint32_t)(at - lds) + kat, v0at = lds0 + (uint32_t)(at - lds) + vat;
-    f32x4 sc[NT][ST];
+  // ---- a chunk's scores, in units of 1 / s2, and this lane's value scales
+  constexpr int NE = SW == 16 ? 1 : ST / 2;  // value steps
+  auto scores = [&](uint32_t at, f32x4 (&sc)[NT][ST], float (&vq)[Q8 ? 4 * ST : 1]) {
+    const uint32_t k0 = at + kat;
 #pragma unroll
     for (int st = 0; st < ST; ++st) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) sc[nt][st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      uint4 w = {};
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         h16x8 ka;
         if constexpr (Q8) {
-          const uint4 w = lds_b128((k0 ^ (64 * (c >> 1))) + 16 * st * RB);
+          if (c % 2 == 0) w = lds_b128((k0 ^ (64 * (c >> 1))) + 16 * st * RB);
           const uint2 x = codes4_h<FORMAT>((c & 1) ? w.z : w.x), y = codes4_h<FORMAT>((c & 1) ? w.w : w.y);
           ka = __builtin_bit_cast(h16x8, make_uint4(x.x, x.y, y.x, y.y));
         } else {
@@ -369,14 +370,11 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
         }
       }
     }
-    __builtin_amdgcn_sched_barrier(0);
-    float vq[Q8 ? 4 * ST : 1];  // value scales of this lane's slots
     if constexpr (Q8) {
 #pragma unroll
       for (int st = 0; st < ST; ++st) {
-        const uint8_t* q = at + 2 * CB + 4 * (ws * SW + 16 * st + 4 * kq);
-        const float4 kv = *reinterpret_cast<const float4*>(q);
-        const float4 vv = *reinterpret_cast<const float4*>(q + 4 * C);
+        const uint32_t q = at + 2 * CB + 4 * (ws * SW + 16 * st + 4 * kq);
+        const float4 kv = __builtin_bit_cast(float4, lds_b128(q)), vv = __builtin_bit_cast(float4, lds_b128(q + 4 * C));
         vq[4 * st] = vv.x;
         vq[4 * st + 1] = vv.y;
         vq[4 * st + 2] = vv.z;
@@ -390,194 +388,275 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
         }
       }
     }
-    // the slots a column does not see
-    uint32_t seen[NT][ST];  // four bits each
-    if constexpr (DRAFTS) {
-      uint64_t bad = 0;
-      if constexpr (FORMAT != KNJ_KV_I8) {
-        bad = poison[(ws * SW) >> 5];
-        if constexpr (SW == 64) bad |= (uint64_t)poison[((ws * SW) >> 5) + 1] << 32;
-        if constexpr (SW == 16) bad = (bad >> ((ws * SW) & 31)) & 0xFFFFu;
-      }
+  };
+  // the largest of a column's scores
+  auto largest = [&](const f32x4 (&sc)[ST]) {
+    float mx = -INFINITY;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const uint64_t b =
-            seen64(mask ? mask + (uint64_t)tcol[nt] * words : nullptr, words, tcol[nt], N, p0 + ws * SW - P);
-        spoilt[nt] |= (b & bad) != 0;
+    for (int st = 0; st < ST; ++st)
+      mx = max_nan(max_nan(max_nan(mx, sc[st][0]), max_nan(sc[st][1], sc[st][2])), sc[st][3]);
+    const float2 m16 = pair16_f(mx);
+    mx = max_nan(m16.x, m16.y);
+    const float2 m32 = pair32_f(mx);
+    return max_nan(m32.x, m32.y);
+  };
+  // Weights of a column's scores against its reference, into the values' operand; with
+  // 8 bits times w8, the slots' value scales over the column's.  Returns their sum
+  // (without those).
+  auto weights = [&](const f32x4 (&sc)[ST], float s2c, float mref, const float (&w8)[Q8 ? 4 * ST : 1], h16x8 (&eh)[NE],
+                     h16x8 (&el)[SPLIT ? NE : 1]) {
+    // (the reference is -inf while the column has seen nothing: exponents then from 0)
+    const float mr = mref == -INFINITY ? 0.0f : mref * s2c;
+    float es = 0.0f;
+    float w[4 * ST];
 #pragma unroll
-        for (int st = 0; st < ST; ++st) {
-          seen[nt][st] = (uint32_t)(b >> (16 * st + 4 * kq)) & 15u;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sc[nt][st][i] = (seen[nt][st] >> i) & 1u ? sc[nt][st][i] : -INFINITY;
-        }
+    for (int i = 0; i < 4 * ST; ++i) {
+      w[i] = __builtin_amdgcn_exp2f(fmaf(sc[i >> 2][i & 3], s2c, kLift - mr));
+      es += w[i];
+      if constexpr (Q8) {
+        w[i] *= w8[i];
+        // (the weight itself, rounded to f32, is what is split below: formed anew
+        // inside the conversion to f16, the product could round the other way
+        // there than in the remainder, an f16 step off)
+        if constexpr (SPLIT) asm("" : "+v"(w[i]));
       }
     }
-    // before the drafts every column sees the same slots: one reference for all
-    float vs[Q8 ? 4 * ST : 1], vnew = 0.0f;
-    if constexpr (Q8 && !DRAFTS) {
-      float vm = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4 * ST; ++i) vm = fmaxf(vm, vq[i] < INFINITY ? vq[i] : 0.0f);
-      vm = fmaxf(vm, xor16_f(vm));
-      vm = fmaxf(vm, xor32_f(vm));
-      vnew = fmaxf(vref[0], __uint_as_float(__float_as_uint(vm) & 0x7F800000u));
-      const float inv = vnew > 0.0f ? __uint_as_float((254u << 23) - __float_as_uint(vnew)) : 0.0f;
-#pragma unroll
-      for (int i = 0; i < 4 * ST; ++i) vs[i] = vq[i] * inv;
+    for (int c = 0; c < NE; ++c) {
+      h16x8 hi, lo;
+      split_h8(make_float4(w[8 * c], w[8 * c + 1], w[8 * c + 2], w[8 * c + 3]),
+               SW == 16 ? make_float4(0.f, 0.f, 0.f, 0.f)
+                        : make_float4(w[(8 * c + 4) % (4 * ST)], w[(8 * c + 5) % (4 * ST)], w[(8 * c + 6) % (4 * ST)],
+                                      w[(8 * c + 7) % (4 * ST)]),
+               hi, lo);
+      eh[c] = hi;
+      if constexpr (SPLIT) el[c] = lo;
     }
-    // running softmax per column, and the weights as the values' operand
-    constexpr int NE = SW == 16 ? 1 : ST / 2;
-    h16x8 eh[NT][NE], el[SPLIT ? NT : 1][NE];  // (SW 16: the first four)
+    return es;
+  };
+  // Values: step c covers slots 32c + 4kq + i and 32c + 16 + 4kq + i (SW 16: the
+  // first).  Lane r's transposed read takes bytes 8 (r%4) .. + 7 of 32-byte pair b
+  // of row 4kq + r/4 and receives 16-bit element r of the pair, of four rows:
+  // dim 16b + r, or with 8 bits dims 32b + 2r (tile 2b) and 32b + 2r + 1 (2b + 1).
+  struct VPair {
+    u32x2 x, y;
+  };
+  auto vread = [&](uint32_t at, int c, int b) {
+    const uint32_t q = ((at + vat) ^ (32 * b)) + 32 * c * RB;
+    VPair v;
+    v.x = lds_tr16_at(q);
+    v.y = v.x;
+    if constexpr (SW != 16) v.y = lds_tr16_at(q + 16 * RB);
+    return v;
+  };
+  auto product = [&](int dt, uint2 v0, uint2 v1, int c, const h16x8 (&eh)[NT][NE], const h16x8 (&el)[NT][SPLIT ? NE : 1]) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int st = 0; st < ST; ++st)
-        mx = max_nan(max_nan(max_nan(mx, sc[nt][st][0]), max_nan(sc[nt][st][1], sc[nt][st][2])), sc[nt][st][3]);
-      const float2 m16 = pair16_f(mx);
-      mx = max_nan(m16.x, m16.y);
-      const float2 m32 = pair32_f(mx);
-      mx = max_nan(m32.x, m32.y);
-      // (the reference is -inf while the column has seen nothing: exponents then from 0)
-      const float mn = (mx - m[nt]) * s2[nt] <= kLag ? m[nt] : max_nan(m[nt], mx);
-      const float mr = mn == -INFINITY ? 0.0f : mn * s2[nt];
-      float alpha = __builtin_amdgcn_exp2f(fmaf(m[nt], s2[nt], -mr));
-      m[nt] = mn;
-      float es = 0.0f;
-      float w[4 * ST];
-#pragma unroll
-      for (int i = 0; i < 4 * ST; ++i) {
-        w[i] = __builtin_amdgcn_exp2f(fmaf(sc[nt][i >> 2][i & 3], s2[nt], kLift - mr));
-        es += w[i];
-      }
-      l[nt] = l[nt] * alpha + es;
-      if constexpr (Q8) {
-        float ref = vnew;
-        if constexpr (DRAFTS) {
-          float vm = 0.0f;  // the largest finite scale that the column sees here
-#pragma unroll
-          for (int i = 0; i < 4 * ST; ++i)
-            vm = fmaxf(vm, ((seen[nt][i >> 2] >> (i & 3)) & 1u) && vq[i] < INFINITY ? vq[i] : 0.0f);
-          vm = fmaxf(vm, xor16_f(vm));
-          vm = fmaxf(vm, xor32_f(vm));
-          ref = fmaxf(vref[nt], __uint_as_float(__float_as_uint(vm) & 0x7F800000u));
-        }
-        const float inv = ref > 0.0f ? __uint_as_float((254u << 23) - __float_as_uint(ref)) : 0.0f;
-        alpha *= vref[nt] * inv;
-        vref[nt] = ref;
-#pragma unroll
-        for (int i = 0; i < 4 * ST; ++i) {
-          if constexpr (DRAFTS) w[i] = (seen[nt][i >> 2] >> (i & 3)) & 1u ? w[i] * (vq[i] * inv) : 0.0f;
-          else w[i] *= vs[i];
-          // (the weight itself, rounded to f32, is what is split below: formed anew
-          // inside the conversion to f16, the product could round the other way
-          // there than in the remainder, an f16 step off)
-          if constexpr (SPLIT) asm("" : "+v"(w[i]));
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < NE; ++c) {
-        h16x8 hi, lo;
-        split_h8(make_float4(w[8 * c], w[8 * c + 1], w[8 * c + 2], w[8 * c + 3]),
-                 SW == 16 ? make_float4(0.f, 0.f, 0.f, 0.f)
-                          : make_float4(w[(8 * c + 4) % (4 * ST)], w[(8 * c + 5) % (4 * ST)], w[(8 * c + 6) % (4 * ST)],
-                                        w[(8 * c + 7) % (4 * ST)]),
-                 hi, lo);
-        eh[nt][c] = hi;
-        if constexpr (SPLIT) el[nt][c] = lo;
-      }
-      {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[nt][dt][i] *= alpha;
-      }
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    // values: step c covers slots 32c + 4kq + i and 32c + 16 + 4kq + i (SW 16: the
-    // first).  Lane r's transposed read takes bytes 8 (r%4) .. + 7 of 32-byte pair b
-    // of row 4kq + r/4 and receives 16-bit element r of the pair, of four rows:
-    // dim 16b + r, or with 8 bits dims 32b + 2r (tile 2b) and 32b + 2r + 1 (2b + 1)
-    auto product = [&](int dt, uint2 v0, uint2 v1, int c) {
       if constexpr (SW == 16) {
         const h16x4 vv = __builtin_bit_cast(h16x4, v0);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const h16x4 hi = __builtin_shufflevector(eh[nt][0], eh[nt][0], 0, 1, 2, 3);
-          acc[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x16f16(vv, hi, acc[nt][dt], 0, 0, 0);
-          if constexpr (SPLIT) {
-            const h16x4 lo = __builtin_shufflevector(el[nt][0], el[nt][0], 0, 1, 2, 3);
-            acc[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x16f16(vv, lo, acc[nt][dt], 0, 0, 0);
-          }
+        const h16x4 hi = __builtin_shufflevector(eh[nt][0], eh[nt][0], 0, 1, 2, 3);
+        acc[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x16f16(vv, hi, acc[nt][dt], 0, 0, 0);
+        if constexpr (SPLIT) {
+          const h16x4 lo = __builtin_shufflevector(el[nt][0], el[nt][0], 0, 1, 2, 3);
+          acc[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x16f16(vv, lo, acc[nt][dt], 0, 0, 0);
         }
       } else {
         const h16x8 vv = __builtin_bit_cast(h16x8, make_uint4(v0.x, v0.y, v1.x, v1.y));
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          acc[nt][dt] = mfma16(vv, eh[nt][c], acc[nt][dt]);
-          if constexpr (SPLIT) acc[nt][dt] = mfma16(vv, el[nt][c], acc[nt][dt]);
-        }
+        acc[nt][dt] = mfma16(vv, eh[nt][c], acc[nt][dt]);
+        if constexpr (SPLIT) acc[nt][dt] = mfma16(vv, el[nt][c], acc[nt][dt]);
       }
-    };
+    }
+  };
+  // the products of a chunk, its first step's reads given; each step's operands are
+  // read while the step before is multiplied
+  auto values = [&](uint32_t at, VPair (&v)[NPAIR], const h16x8 (&eh)[NT][NE], const h16x8 (&el)[NT][SPLIT ? NE : 1]) {
 #pragma unroll
     for (int c = 0; c < NE; ++c) {
 #pragma unroll
       for (int b = 0; b < NPAIR; ++b) {
-        const uint32_t q = (v0at ^ (32 * b)) + 32 * c * RB;
-        const u32x2 v0 = lds_tr16_at(q);
-        u32x2 v1 = v0;
-        if constexpr (SW != 16) v1 = lds_tr16_at(q + 16 * RB);
         if constexpr (Q8) {
           uint2 e0, o0, e1, o1;
-          pairs_h<FORMAT>(v0, e0, o0);
-          if constexpr (SW != 16) pairs_h<FORMAT>(v1, e1, o1);
+          pairs_h<FORMAT>(v[b].x, e0, o0);
+          if constexpr (SW != 16) pairs_h<FORMAT>(v[b].y, e1, o1);
           else e1 = e0, o1 = o0;
-          product(2 * b, e0, e1, c);
-          product(2 * b + 1, o0, o1, c);
+          if (c + 1 < NE) v[b] = vread(at, c + 1, b);
+          product(2 * b, e0, e1, c, eh, el);
+          product(2 * b + 1, o0, o1, c, eh, el);
         } else {
-          product(b, make_uint2(v0.x, v0.y), make_uint2(v1.x, v1.y), c);
+          product(b, make_uint2(v[b].x.x, v[b].x.y), make_uint2(v[b].y.x, v[b].y.y), c, eh, el);
+          if (c + 1 < NE) v[b] = vread(at, c + 1, b);
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
+  // a value scale's reference: the power of two below twice the largest, which a
+  // later scale may pass twice over before it moves (weights stay below 2^15)
+  auto vref_of = [](float vm) { return __uint_as_float((__float_as_uint(vm) & 0x7F800000u) ? (__float_as_uint(vm) & 0x7F800000u) + 0x00800000u : 0u); };
+  auto inverse = [](float ref) { return ref > 0.0f ? __uint_as_float((254u << 23) - __float_as_uint(ref)) : 0.0f; };
+  auto rescale = [&](int nt, float alpha) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[nt][dt][i] *= alpha;
+  };
 
-  for (int j = c0; j < c1; ++j) {
-    const int p0 = j * C;
-    uint8_t* at = lds + (j - c0) % NST * SB;
-    // this wave's DMA of chunk j has landed (the chunks after it may be in flight);
-    // the barrier hands every wave's part over and ends the reads of chunk j - 1,
-    // whose stage chunk j + NST - 1 then refills
+  // chunk j's stage ready: this wave's DMA of it has landed (the chunks after it may
+  // be in flight); the barrier hands every wave's part over and ends the reads of
+  // chunk j - 1, whose stage chunk j + NST - 1 then refills (past the range: fetched
+  // and not used)
+  int j = c0, stage = 0;
+  auto ready = [&]() {
     KNJ_BARRIER_AFTER(vm_lds_imm((NST - 2) * NDMA));
-    dma(j + NST - 1, (j - c0 + NST - 1) % NST);  // (past the range: fetched and not used)
-    if (__builtin_expect(p0 + C <= P, 1)) {
-      chunk(std::false_type{}, at, p0);
-      continue;
-    }
-    // A draft's value row may be unseen by some columns of the tile, and rows past
-    // the drafts are seen by none: what is not finite in them would reach a column
-    // as 0 x inf, and is replaced by zeros.  Columns that see such a draft are
-    // marked and come out as NaN.  (int8 codes are finite; their scales are
-    // selected away.)
-    if constexpr (FORMAT != KNJ_KV_I8) {
-      if (tid < C / 32) poison[tid] = 0u;
-      KNJ_BARRIER_AFTER(kLdsOnly);
-      for (int o = 16 * tid; o < CB; o += 16 * NTH) {
-        const int q = o / RB;
-        if (p0 + q < P) continue;
-        uint4* w = reinterpret_cast<uint4*>(at + CB + o);
-        uint4 v = *w;
-        bool any = false;
-        any |= drop_nonfinite<FORMAT>(v.x);
-        any |= drop_nonfinite<FORMAT>(v.y);
-        any |= drop_nonfinite<FORMAT>(v.z);
-        any |= drop_nonfinite<FORMAT>(v.w);
-        if (!any) continue;
-        *w = v;
-        if (p0 + q < valid) atomicOr(&poison[q >> 5], 1u << (q & 31));
+    dma(j + NST - 1, stage == 0 ? NST - 1 : stage - 1);
+  };
+  auto next = [&]() {
+    ++j;
+    stage = stage + 1 == NST ? 0 : stage + 1;
+    if (j < c1) ready();
+  };
+  const int j_prefix = min(c1, P / C);  // chunks below lie in the prefix
+  ready();
+  while (j < c1) {
+    // ---- the first chunk, and those that reach the drafts or the end
+    {
+      const int p0 = j * C;
+      const uint32_t at = lds0 + stage * SB;
+      const bool drafts = p0 + C > P;
+      // A draft's value row may be unseen by some columns of the tile, and rows past
+      // the drafts are seen by none: what is not finite in them would reach a column
+      // as 0 x inf, and is replaced by zeros.  Columns that see such a draft are
+      // marked and come out as NaN.  (int8 codes are finite; their scales are
+      // selected away.)
+      uint64_t bad = 0;
+      if (FORMAT != KNJ_KV_I8 && drafts) {
+        if (tid < C / 32) poison[tid] = 0u;
+        KNJ_BARRIER_AFTER(kLdsOnly);
+        for (int o = 16 * tid; o < CB; o += 16 * NTH) {
+          const int q = o / RB;
+          if (p0 + q < P) continue;
+          uint4* w = reinterpret_cast<uint4*>(lds + stage * SB + CB + o);
+          uint4 v = *w;
+          bool any = false;
+          any |= drop_nonfinite<FORMAT>(v.x);
+          any |= drop_nonfinite<FORMAT>(v.y);
+          any |= drop_nonfinite<FORMAT>(v.z);
+          any |= drop_nonfinite<FORMAT>(v.w);
+          if (!any) continue;
+          *w = v;
+          if (p0 + q < valid) atomicOr(&poison[q >> 5], 1u << (q & 31));
+        }
+        KNJ_BARRIER_AFTER(kLdsOnly);
+        bad = poison[(ws * SW) >> 5];
+        if constexpr (SW == 64) bad |= (uint64_t)poison[((ws * SW) >> 5) + 1] << 32;
+        if constexpr (SW == 16) bad = (bad >> ((ws * SW) & 31)) & 0xFFFFu;
       }
-      KNJ_BARRIER_AFTER(kLdsOnly);
+      f32x4 sc[NT][ST];
+      float vq[Q8 ? 4 * ST : 1];
+      scores(at, sc, vq);
+      h16x8 eh[NT][NE], el[NT][SPLIT ? NE : 1];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        // the slots that the column sees: four bits per lane and slot tile
+        uint64_t seen = ~0ull;
+        if (drafts) seen = seen64(mask ? mask + (uint64_t)tcol[nt] * words : nullptr, words, tcol[nt], N, p0 + ws * SW - P);
+        spoilt[nt] |= (seen & bad) != 0;
+        seen >>= 4 * kq;
+        float vm = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4 * ST; ++i) {
+          const bool in = (seen >> (16 * (i >> 2) + (i & 3))) & 1u;
+          sc[nt][i >> 2][i & 3] = in ? sc[nt][i >> 2][i & 3] : -INFINITY;
+          if constexpr (Q8) vm = fmaxf(vm, in && vq[i] < INFINITY ? vq[i] : 0.0f);  // the largest finite one
+        }
+        const float mx = largest(sc[nt]);
+        const float mn = (mx - m[nt]) * s2[nt] <= kLag ? m[nt] : max_nan(m[nt], mx);
+        const float mr = mn == -INFINITY ? 0.0f : mn * s2[nt];
+        float alpha = __builtin_amdgcn_exp2f(fmaf(m[nt], s2[nt], -mr));
+        m[nt] = mn;
+        l[nt] *= alpha;
+        float w8[Q8 ? 4 * ST : 1];
+        if constexpr (Q8) {
+          vm = fmaxf(vm, xor16_f(vm));
+          vm = fmaxf(vm, xor32_f(vm));
+          const float ref = fmaxf(vref[nt], vref_of(vm));
+          const float inv = inverse(ref);
+          alpha *= vref[nt] * inv;
+          vref[nt] = ref;
+#pragma unroll
+          for (int i = 0; i < 4 * ST; ++i) w8[i] = (seen >> (16 * (i >> 2) + (i & 3))) & 1u ? vq[i] * inv : 0.0f;
+        }
+        l[nt] += weights(sc[nt], s2[nt], mn, w8, eh[nt], el[nt]);
+        rescale(nt, alpha);
+      }
+      VPair v[NPAIR];
+#pragma unroll
+      for (int b = 0; b < NPAIR; ++b) v[b] = vread(at, 0, b);
+      values(at, v, eh, el);
     }
-    chunk(std::true_type{}, at, p0);
+    next();
+    // ---- the chunks of the prefix: every column sees every slot.  A chunk whose
+    // scores (or value scales) have left the columns' references behind is begun
+    // again after a rescale.
+    int settled = -1;
+    while (j < j_prefix) {
+      float mx[NT], vm = 0.0f;
+      bool over = false;
+      for (;;) {
+        const uint32_t at = lds0 + stage * SB;
+        f32x4 sc[NT][ST];
+        float vq[Q8 ? 4 * ST : 1];
+        scores(at, sc, vq);
+        over = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mx[nt] = largest(sc[nt]);
+          over |= !((mx[nt] - m[nt]) * s2[nt] <= kLag);
+        }
+        if constexpr (Q8) {
+          vm = 0.0f;  // the largest finite scale
+#pragma unroll
+          for (int i = 0; i < 4 * ST; ++i) vm = fmaxf(vm, vq[i] < INFINITY ? vq[i] : 0.0f);
+          vm = fmaxf(vm, xor16_f(vm));
+          vm = fmaxf(vm, xor32_f(vm));
+          over |= vm >= 4.0f * vref[0];
+        }
+        if (j != settled && __ballot(over) != 0) break;
+        VPair v[NPAIR];
+#pragma unroll
+        for (int b = 0; b < NPAIR; ++b) v[b] = vread(at, 0, b);
+        float w8[Q8 ? 4 * ST : 1];
+        if constexpr (Q8) {
+          const float inv = inverse(vref[0]);  // (alike in every column)
+#pragma unroll
+          for (int i = 0; i < 4 * ST; ++i) w8[i] = vq[i] * inv;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        h16x8 eh[NT][NE], el[NT][SPLIT ? NE : 1];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) l[nt] += weights(sc[nt], s2[nt], m[nt], w8, eh[nt], el[nt]);
+        __builtin_amdgcn_sched_barrier(0);
+        values(at, v, eh, el);
+        next();
+        if (j >= j_prefix) break;
+      }
+      if (j >= j_prefix) break;
+      settled = j;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float mn = (mx[nt] - m[nt]) * s2[nt] <= kLag ? m[nt] : max_nan(m[nt], mx[nt]);
+        const float mr = mn == -INFINITY ? 0.0f : mn * s2[nt];
+        float alpha = __builtin_amdgcn_exp2f(fmaf(m[nt], s2[nt], -mr));
+        m[nt] = mn;
+        l[nt] *= alpha;
+        if constexpr (Q8) {
+          const float ref = vm >= 4.0f * vref[nt] ? vref_of(vm) : vref[nt];
+          alpha *= vref[nt] * inverse(ref);
+          vref[nt] = ref;
+        }
+        rescale(nt, alpha);
+      }
+    }
   }
 
   // ---- columns out: sums over the four lanes of a column, scales back in

@@ -14,56 +14,84 @@ template <>
 hipError_t launch_format<KNJ_KV_I8>(const TreeArgs&, const TreePlan&, int, hipStream_t);
 
 // Merge of a (draft, head)'s split records: M = max m, out = sum acc 2^(m - M) /
-// sum l 2^(m - M).  Thread = four dims of every NP-th split, the parts added in
-// order through LDS.  Only the splits that the sequence reaches hold a record.
-template <int D>
-__global__ __launch_bounds__(kBlock) void k_tree_merge(TreeArgs a, TreePlan p, int chunk, int n_cols) {
-  constexpr int ND = D / 4, NP = kBlock / ND;
-  __shared__ float pm[NP], pl[NP];
-  __shared__ float4 pa[NP][ND];
-  const int h = blockIdx.x % a.n_head;
-  const uint32_t row = blockIdx.x / a.n_head;
-  const int s = row / a.n_rows, t = row - s * a.n_rows;
+// sum l 2^(m - M).  Thread = four dims of every NP-th split, eight splits' loads at
+// once, the parts added in order through LDS (NP 1: no parts, and a workgroup
+// holds several outputs).  The loads do not wait for the sequence's length: every
+// split has its place, and those that the sequence does not reach, which hold no
+// record, are dropped afterwards.
+template <int D, int NP>
+__global__ __launch_bounds__(kBlock) void k_tree_merge(TreeArgs a, TreePlan p, int chunk, int n_cols, uint32_t n_out) {
+  constexpr int ND = D / 4, B = 8, PER = kBlock / (ND * NP);
+  __shared__ float pm[PER][NP], pl[PER][NP];
+  __shared__ float4 pa[NP > 1 ? PER : 1][NP][ND];
+  const int nk = a.c.n_head_kv, G = p.by_group.d;
+  const int slot = threadIdx.x / (ND * NP), part = threadIdx.x / ND % NP, d = threadIdx.x % ND;
+  const uint32_t at = blockIdx.x * PER + slot, out = min(at, n_out - 1);
+  const uint32_t row = p.by_head.div(out), h = out - row * a.n_head;
+  const uint32_t s = p.by_rows.div(row), t = row - s * a.n_rows, kvh = p.by_group.div(h);
+  const float* rec = a.partial + (((uint64_t)s * nk + kvh) * p.n_split * n_cols + t * G + (h - kvh * G)) * (D + 4);
+  const uint64_t stride = (uint64_t)n_cols * (D + 4);
+  float2 ml[B];
+  float4 v[B];
+  auto fetch = [&](int i0) {
+#pragma unroll
+    for (int k = 0; k < B; ++k) {
+      const int i = i0 + part + k * NP;
+      ml[k] = make_float2(-INFINITY, 0.0f);
+      if (i >= p.n_split) continue;
+      ml[k] = *reinterpret_cast<const float2*>(rec + i * stride);
+      v[k] = *reinterpret_cast<const float4*>(rec + i * stride + 4 + 4 * d);
+    }
+  };
+  fetch(0);
   int P, N;
   seq_lengths(a, s, P, N);
-  if (t >= N) return;
-  const int chunks = (P + N + chunk - 1) / chunk, used = (chunks + p.cps - 1) / p.cps;
-  const int nk = a.c.n_head_kv, G = a.n_head / nk, kvh = h / G;
-  const float* rec = a.partial + (((uint64_t)s * nk + kvh) * p.n_split * n_cols + t * G + h % G) * (D + 4);
-  const uint64_t stride = (uint64_t)n_cols * (D + 4);
-  const int part = threadIdx.x / ND, d = threadIdx.x % ND;
+  const int chunks = (P + N + chunk - 1) / chunk, used = p.by_cps.div(chunks + p.cps - 1);
   float M = -INFINITY, L = 0.0f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = part; i < used; i += NP) {
-    const float2 ml = *reinterpret_cast<const float2*>(rec + i * stride);
-    const float4 v = *reinterpret_cast<const float4*>(rec + i * stride + 4 + 4 * d);
-    const float Mn = fmaxf(M, ml.x), ref = Mn == -INFINITY ? 0.0f : Mn;
-    const float fo = exp2f(M - ref), fn = exp2f(ml.x - ref);
-    L = L * fo + ml.y * fn;
-    o = make_float4(o.x * fo + v.x * fn, o.y * fo + v.y * fn, o.z * fo + v.z * fn, o.w * fo + v.w * fn);
+  for (int i0 = 0; i0 < used; i0 += B * NP) {
+    if (i0) fetch(i0);
+    float Mn = M;
+#pragma unroll
+    for (int k = 0; k < B; ++k) {
+      if (i0 + part + k * NP >= used) ml[k] = make_float2(-INFINITY, 0.0f);
+      Mn = fmaxf(Mn, ml[k].x);
+    }
+    const float ref = Mn == -INFINITY ? 0.0f : Mn, fo = __builtin_amdgcn_exp2f(M - ref);
+    L *= fo;
+    o = make_float4(o.x * fo, o.y * fo, o.z * fo, o.w * fo);
+#pragma unroll
+    for (int k = 0; k < B; ++k) {
+      if (i0 + part + k * NP >= used) continue;
+      const float f = __builtin_amdgcn_exp2f(ml[k].x - ref);
+      L += ml[k].y * f;
+      o = make_float4(o.x + v[k].x * f, o.y + v[k].y * f, o.z + v[k].z * f, o.w + v[k].w * f);
+    }
     M = Mn;
   }
-  if (d == 0) {
-    pm[part] = M;
-    pl[part] = L;
-  }
-  pa[part][d] = o;
-  __syncthreads();
-  if (part != 0) return;
-  M = pm[0];
+  if constexpr (NP > 1) {
+    if (d == 0) {
+      pm[slot][part] = M;
+      pl[slot][part] = L;
+    }
+    pa[slot][part][d] = o;
+    __syncthreads();
+    if (part != 0) return;
+    M = pm[slot][0];
 #pragma unroll
-  for (int i = 1; i < NP; ++i) M = fmaxf(M, pm[i]);
-  const float ref = M == -INFINITY ? 0.0f : M;
-  L = 0.0f;
-  o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 1; i < NP; ++i) M = fmaxf(M, pm[slot][i]);
+    const float ref = M == -INFINITY ? 0.0f : M;
+    L = 0.0f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const float f = exp2f(pm[i] - ref);
-    const float4 v = pa[i][d];
-    L += pl[i] * f;
-    o = make_float4(o.x + v.x * f, o.y + v.y * f, o.z + v.z * f, o.w + v.w * f);
+    for (int i = 0; i < NP; ++i) {
+      const float f = __builtin_amdgcn_exp2f(pm[slot][i] - ref);
+      const float4 x = pa[slot][i][d];
+      L += pl[slot][i] * f;
+      o = make_float4(o.x + x.x * f, o.y + x.y * f, o.z + x.z * f, o.w + x.w * f);
+    }
   }
+  if (at >= n_out || (int)t >= N) return;
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // nothing seen: zeros
   o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
   const uint64_t to = (uint64_t)row * a.out_stride + (uint64_t)h * D + 4 * d;
@@ -101,7 +129,8 @@ Planned plan(const knj_kv_cache& c, int type, int n_head, int n_rows, int max_pr
   const int cps = (int)std::max<int64_t>(1, (chunks + want - 1) / want);
   const int n_split = (chunks + cps - 1) / cps;
   return {TreePlan{cps, n_split, tiles, (int)(c.n_seq * (int64_t)c.n_head_kv * n_split), FastDiv(c.n_head_kv),
-                   FastDiv(n_split), FastDiv(n_head / c.n_head_kv)},
+                   FastDiv(n_split), FastDiv(n_head / c.n_head_kv), FastDiv(n_head), FastDiv(n_rows),
+                   FastDiv(cps)},
           sh};
 }
 
@@ -121,12 +150,22 @@ hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t s) {
   else if (a.c.format == KNJ_KV_F8) e = tree::launch_format<KNJ_KV_F8>(a, q.p, q.sh.cols, s);
   else e = tree::launch_format<KNJ_KV_I8>(a, q.p, q.sh.cols, s);
   if (e != hipSuccess || q.p.n_split == 1) return e;
-  const dim3 grid((unsigned)((uint64_t)a.c.n_seq * a.n_rows * a.n_head));
+  // few outputs: their splits over the workgroup's parts, for its latency; many: the
+  // fewest threads an output that hold its splits in one batch of loads
+  const uint32_t n_out = (uint32_t)a.c.n_seq * a.n_rows * a.n_head;
   const int n_cols = q.p.n_tiles * q.sh.cols;
-  if (a.c.head_dim == 128)
-    KNJ_LAUNCH(tree::k_tree_merge<128>, grid, dim3(dev::kBlock), 0, s, a, q.p, q.sh.chunk, n_cols);
-  else
-    KNJ_LAUNCH(tree::k_tree_merge<64>, grid, dim3(dev::kBlock), 0, s, a, q.p, q.sh.chunk, n_cols);
+  const bool wide = n_out <= 512 || q.p.n_split > 8;
+#define KNJ_TREE_MERGE(DD, NP)                                                                                  \
+  KNJ_LAUNCH((tree::k_tree_merge<DD, NP>), dim3((n_out + 1024 / (DD) / (NP) - 1) / (1024 / (DD) / (NP))),        \
+             dim3(dev::kBlock), 0, s, a, q.p, q.sh.chunk, n_cols, n_out)
+  if (a.c.head_dim == 128) {
+    if (wide) KNJ_TREE_MERGE(128, 8);
+    else KNJ_TREE_MERGE(128, 1);
+  } else {
+    if (wide) KNJ_TREE_MERGE(64, 16);
+    else KNJ_TREE_MERGE(64, 1);
+  }
+#undef KNJ_TREE_MERGE
   return hipGetLastError();
 }
 
