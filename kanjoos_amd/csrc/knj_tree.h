@@ -562,12 +562,19 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
         if (drafts) seen = seen64(mask ? mask + (uint64_t)tcol[nt] * words : nullptr, words, tcol[nt], N, p0 + ws * SW - P);
         spoilt[nt] |= (seen & bad) != 0;
         seen >>= 4 * kq;
-        float vm = 0.0f;
+        float vm = 0.0f, vin[Q8 ? 4 * ST : 1];  // value scales of the slots seen, and the largest finite one
 #pragma unroll
-        for (int i = 0; i < 4 * ST; ++i) {
-          const bool in = (seen >> (16 * (i >> 2) + (i & 3))) & 1u;
-          sc[nt][i >> 2][i & 3] = in ? sc[nt][i >> 2][i & 3] : -INFINITY;
-          if constexpr (Q8) vm = fmaxf(vm, in && vq[i] < INFINITY ? vq[i] : 0.0f);  // the largest finite one
+        for (int st = 0; st < ST; ++st) {
+          const uint32_t four = (uint32_t)(seen >> (16 * st));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool in = (four & (1u << i)) != 0;
+            sc[nt][st][i] = in ? sc[nt][st][i] : -INFINITY;
+            if constexpr (Q8) {
+              vin[4 * st + i] = in ? vq[4 * st + i] : 0.0f;
+              vm = fmaxf(vm, vin[4 * st + i] < INFINITY ? vin[4 * st + i] : 0.0f);
+            }
+          }
         }
         const float mx = largest(sc[nt]);
         const float mn = (mx - m[nt]) * s2[nt] <= kLag ? m[nt] : max_nan(m[nt], mx);
@@ -584,7 +591,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
           alpha *= vref[nt] * inv;
           vref[nt] = ref;
 #pragma unroll
-          for (int i = 0; i < 4 * ST; ++i) w8[i] = (seen >> (16 * (i >> 2) + (i & 3))) & 1u ? vq[i] * inv : 0.0f;
+          for (int i = 0; i < 4 * ST; ++i) w8[i] = vin[i] * inv;
         }
         l[nt] += weights(sc[nt], s2[nt], mn, w8, eh[nt], el[nt]);
         rescale(nt, alpha);
@@ -785,8 +792,7 @@ hipError_t launch_format(const TreeArgs& a, const TreePlan& p, int cols, hipStre
   do {                                                                                               \
     if (cols == 16) KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, 1, 1, 4, 16);                                 \
     else if (cols == 32) KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, 1, 2, 2, 32);                            \
-    else if (SPLIT) KNJ_TREE_LAUNCH(DD, FORMAT, true, 1, 4, 1, 64);                                  \
-    else if (cols == 64) KNJ_TREE_LAUNCH(DD, FORMAT, false, 2, 2, 2, 32);                            \
+    else if (SPLIT || cols == 64) KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, 2, 2, 2, 32);                   \
     else KNJ_TREE_LAUNCH(DD, FORMAT, false, 2, 4, 1, 64);                                            \
   } while (0)
 // two stages of an f16 cache's rows fill LDS for two workgroups, three of an 8-bit one's

@@ -101,37 +101,37 @@ __global__ __launch_bounds__(kBlock) void k_tree_merge(TreeArgs a, TreePlan p, i
 
 namespace {
 
-// Columns of a tile and slots of a chunk, by the columns a kv head has in all.
-struct Shape {
-  int cols, chunk, waves;
-};
-Shape shape_of(int cols, bool split) {
-  if (cols <= 16) return {16, 64, 4};
-  if (cols <= 32) return {32, 64, 4};
-  if (cols <= 64 || split) return {64, 64, 4};
-  return {128, 64, 4};
-}
-
-// waves that the slots are split for: two per SIMD, what the registers admit
-constexpr int kTreeWaves = 2048;
+constexpr int kTreeChunk = 64;  // slots of a chunk in every shape
 
 struct Planned {
   TreePlan p;
-  Shape sh;
+  int cols;  // columns of a tile
 };
+
+// Tiles of 32 columns (16 where there are no more) finish a chunk soonest; wider
+// ones read and decode the cache for more columns at once and win when there is
+// work enough for every wave (64 drafts x 8 heads at 32K slots: 64 us with 128
+// columns, 81 with 32; at 4K slots 30 and 25; 25 drafts over 4K 25.7 and 21.5).
+// Two workgroups a CU where each then has several chunks, else one, with fewer
+// records to merge (16 drafts x 8 heads over 16K slots 22.3 against 25.0 us, over
+// 4K 15.0 against 14.2).
+constexpr int64_t kWideWork = 10000, kTwoWork = 2500;  // chunks of 32-column tiles, chunks of tiles
+
 Planned plan(const knj_kv_cache& c, int type, int n_head, int n_rows, int max_prefix) {
-  const int cols = n_rows * (n_head / c.n_head_kv);
-  const Shape sh = shape_of(cols, type == KNJ_TYPE_F32);
-  const int tiles = (cols + sh.cols - 1) / sh.cols;
-  const int chunks = (max_prefix + n_rows + sh.chunk - 1) / sh.chunk;
-  const int64_t base = (int64_t)c.n_seq * c.n_head_kv * tiles;
-  const int64_t want = std::max<int64_t>(1, kTreeWaves / sh.waves / base);
+  const int group = n_head / c.n_head_kv, n_cols = n_rows * group;
+  const int chunks = (max_prefix + n_rows + kTreeChunk - 1) / kTreeChunk;
+  const int64_t units = (int64_t)c.n_seq * c.n_head_kv;
+  int cols = n_cols <= 16 ? 16 : 32;
+  if (n_cols > 32 && units * ((n_cols + 31) / 32) * chunks >= kWideWork)
+    cols = n_cols <= 64 || type == KNJ_TYPE_F32 ? 64 : 128;
+  const int tiles = (n_cols + cols - 1) / cols;
+  const int64_t wgs = units * tiles * chunks >= kTwoWork ? 512 : 256;
+  const int64_t want = std::max<int64_t>(1, wgs / (units * tiles));
   const int cps = (int)std::max<int64_t>(1, (chunks + want - 1) / want);
   const int n_split = (chunks + cps - 1) / cps;
-  return {TreePlan{cps, n_split, tiles, (int)(c.n_seq * (int64_t)c.n_head_kv * n_split), FastDiv(c.n_head_kv),
-                   FastDiv(n_split), FastDiv(n_head / c.n_head_kv), FastDiv(n_head), FastDiv(n_rows),
-                   FastDiv(cps)},
-          sh};
+  return {TreePlan{cps, n_split, tiles, (int)(units * n_split), FastDiv(c.n_head_kv), FastDiv(n_split), FastDiv(group),
+                   FastDiv(n_head), FastDiv(n_rows), FastDiv(cps)},
+          cols};
 }
 
 }  // namespace
@@ -140,24 +140,24 @@ Planned plan(const knj_kv_cache& c, int type, int n_head, int n_rows, int max_pr
 uint64_t tree_partial_bytes(const knj_kv_cache& c, int type, int n_head, int n_rows, int max_prefix) {
   const tree::Planned q = tree::plan(c, type, n_head, n_rows, max_prefix);
   if (q.p.n_split == 1) return 0;
-  return (uint64_t)q.p.units * q.p.n_tiles * q.sh.cols * (c.head_dim + 4) * sizeof(float);
+  return (uint64_t)q.p.units * q.p.n_tiles * q.cols * (c.head_dim + 4) * sizeof(float);
 }
 
 hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t s) {
   const tree::Planned q = tree::plan(a.c, a.type, a.n_head, a.n_rows, a.max_prefix);
   hipError_t e;
-  if (a.c.format == KNJ_KV_F16) e = tree::launch_format<KNJ_KV_F16>(a, q.p, q.sh.cols, s);
-  else if (a.c.format == KNJ_KV_F8) e = tree::launch_format<KNJ_KV_F8>(a, q.p, q.sh.cols, s);
-  else e = tree::launch_format<KNJ_KV_I8>(a, q.p, q.sh.cols, s);
+  if (a.c.format == KNJ_KV_F16) e = tree::launch_format<KNJ_KV_F16>(a, q.p, q.cols, s);
+  else if (a.c.format == KNJ_KV_F8) e = tree::launch_format<KNJ_KV_F8>(a, q.p, q.cols, s);
+  else e = tree::launch_format<KNJ_KV_I8>(a, q.p, q.cols, s);
   if (e != hipSuccess || q.p.n_split == 1) return e;
   // few outputs: their splits over the workgroup's parts, for its latency; many: the
   // fewest threads an output that hold its splits in one batch of loads
   const uint32_t n_out = (uint32_t)a.c.n_seq * a.n_rows * a.n_head;
-  const int n_cols = q.p.n_tiles * q.sh.cols;
+  const int n_cols = q.p.n_tiles * q.cols;
   const bool wide = n_out <= 512 || q.p.n_split > 8;
 #define KNJ_TREE_MERGE(DD, NP)                                                                                  \
   KNJ_LAUNCH((tree::k_tree_merge<DD, NP>), dim3((n_out + 1024 / (DD) / (NP) - 1) / (1024 / (DD) / (NP))),        \
-             dim3(dev::kBlock), 0, s, a, q.p, q.sh.chunk, n_cols, n_out)
+             dim3(dev::kBlock), 0, s, a, q.p, tree::kTreeChunk, n_cols, n_out)
   if (a.c.head_dim == 128) {
     if (wide) KNJ_TREE_MERGE(128, 8);
     else KNJ_TREE_MERGE(128, 1);
