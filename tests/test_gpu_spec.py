@@ -545,6 +545,87 @@ def test_attention_tree_magnitudes(device, fmt, size):
     close(got, want, bound, f"size {size}")
 
 
+def store_prefix(c, kv, n):
+    """Rows [n_seq][n][nk][D] (float64) into the first n slots; their values as the cache holds them,
+    [n_seq][nk][n][D]."""
+    d = c.desc
+    bufs = [put(a.astype(np.float32)) for a in kv]
+    K.kv_store(c, F32, bufs[0], bufs[1], i32(np.zeros(d.n_seq)), n)
+    out = []
+    for a in kv:
+        code, scale = codes(a.astype(np.float32).astype(np.float64), d.format)
+        out.append(values(code, scale, d.format).transpose(0, 2, 1, 3))
+    return out
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,T,nh", [(128, 8, 48), (128, 20, 64), (64, 9, 40), (64, 33, 64)])
+def test_attention_tree_wide(device, t, fmt, D, T, nh):
+    """The column tiles of 64 and 128 that much work is given to: the bound on the
+    prefixes makes the work large, the prefixes themselves stay short."""
+    print(f"wide type {t} format {fmt} D {D} T {T} heads {nh}", flush=True)
+    rng = np.random.default_rng([t, fmt, D, T])
+    n, nk, bound_p = 8, 8, 6000
+    c = K.KvCache.allocate(fmt, n, nk, bound_p + T, D)
+    prefixes = np.array([0, 63, 64, 129, 300, 1000, 17, 700])
+    filled = 1000 + T
+    kv = store_prefix(c, [rng.normal(size=(n, filled, nk, D)) * np.exp(0.3 * rng.normal(size=(n, filled, nk)))[..., None] for _ in range(2)],
+                      filled)
+    sees = np.stack([tree_bits(rng, T) for _ in range(n)])
+    counts = np.array([T, T - 1, 1, T, 2, T, 0, T])
+    q = decode(encode(1.5 * rng.normal(size=(n, T, nh, D)), t), t)
+    got, before = run_tree(c, t, q, T, prefixes, counts, sees, nh, max_prefix=bound_p)
+    want, bound = tree64(q, kv, prefixes, counts, sees, D ** -0.5, t)
+    for s in range(n):
+        close(got[s, :counts[s]], want[s, :counts[s]], bound[s, :counts[s]], f"prefix {prefixes[s]}")
+        assert np.array_equal(got[s, counts[s]:], before[s, counts[s]:])
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("T,nh", [(1, 4), (3, 16), (12, 16)])
+@pytest.mark.parametrize("rising", [1, -1])
+def test_attention_tree_drifting(device, t, fmt, T, nh, rising):
+    """Scores and value units that rise (or fall) along the prefix, so that every
+    chunk passes (or none reaches) what the chunks before it left as reference."""
+    print(f"drift type {t} format {fmt} T {T} heads {nh} rising {rising}", flush=True)
+    rng = np.random.default_rng([t, fmt, T])
+    nk, D, P = 2, 128, 1500
+    c = make_cache(fmt, 1, nk, P + T, D)
+    ramp = np.linspace(0, 1, P + T)[::rising]
+    base = rng.normal(size=(nk, D))
+    k = (0.2 * rng.normal(size=(1, P + T, nk, D)) + 3 * ramp[None, :, None, None] * base[None, None])
+    v = rng.normal(size=(1, P + T, nk, D)) * np.exp2(12 * ramp)[None, :, None, None]
+    kv = store_prefix(c, [k, v], P + T)
+    sees = tree_bits(rng, T)[None]
+    q = 2.0 * np.repeat(base, nh // nk, axis=0)[None, None] + 0.3 * rng.normal(size=(1, T, nh, D))
+    q = decode(encode(q, t), t)
+    got, _ = run_tree(c, t, q, T, [P], None, sees, nh)
+    want, bound = tree64(q, kv, [P], [T], sees, D ** -0.5, t)
+    close(got, want, bound, "drift")
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("part", ["k", "v"])
+def test_attention_tree_nan_in_prefix(device, fmt, part):
+    """A NaN that every draft sees reaches every draft -- of a value in f16 its own
+    dim -- and the call ends."""
+    rng = np.random.default_rng(fmt)
+    nh, nk, D, T, P = 8, 2, 64, 5, 700
+    c = make_cache(fmt, 2, nk, P + T, D)
+    x = [rng.normal(size=(2, P + T, nk, D)) for _ in range(2)]
+    x[part == "v"][1, 400, :, 9] = np.nan
+    with np.errstate(invalid="ignore"):
+        kv = store_prefix(c, x, P + T)
+        q = rng.normal(size=(2, T, nh, D)).astype(np.float32).astype(np.float64)
+        sees = np.stack([tree_bits(rng, T)] * 2)
+        got, _ = run_tree(c, F32, q, T, [P, P], None, sees, nh)
+        want, bound = tree64(q, kv, [P, P], [T, T], sees, D ** -0.5, F32)
+    assert np.isnan(want[1, ..., 9]).all() and np.isfinite(want[0]).all()
+    close(got, want, np.where(np.isnan(bound), 1.0, bound), "nan")
+
+
 def test_attention_tree_long_cache(device):
     """Sequences whose cache begins past 2^32 elements."""
     rng = np.random.default_rng(1)
@@ -689,6 +770,25 @@ def test_token_logprobs_ties_and_masks(device, t):
     check_logprobs(x, raw, t, tokens, n_top, 1.0)
     tokens[:3] = [-2 ** 31, 2 ** 31 - 1, V - 1]
     check_logprobs(x, raw, t, tokens, 1, 0.6)
+
+
+@pytest.mark.parametrize("t,V,rows,n_top", [(F32, 5000, 131, 32), (BF16, 3000, 300, 7), (F16, 600000, 129, 20)])
+def test_token_logprobs_many_rows(device, t, V, rows, n_top):
+    """Rows enough for the narrower join, more pieces than it has threads among them;
+    the rows repeat a few of their own, so that ties and sorted rows come along."""
+    print(f"logprobs type {t} vocab {V} rows {rows} top {n_top}", flush=True)
+    rng = np.random.default_rng([V, rows])
+    kinds = np.stack([3 * rng.normal(size=V), np.sort(rng.integers(0, 50, V)).astype(float), np.zeros(V),
+                      np.where(rng.random(V) < 0.99, -np.inf, rng.normal(size=V))])
+    raw4 = encode(kinds, t)
+    pick = rng.integers(0, 4, rows)
+    tokens4 = rng.integers(0, V, 4)
+    want = logprobs64(decode(raw4, t), tokens4, n_top, 1.0)
+    got = run_logprobs(raw4[pick], t, V, tokens4[pick], n_top, 1.0)
+    with np.errstate(invalid="ignore"):
+        for g, w, what, d in ((got[0], want[0], "logprob", 1.0), (got[1], want[1], "entropy", 40.0), (got[3], want[3], "top", 1.0)):
+            close(g, w[pick], 48 * U * np.minimum(d, d * np.abs(w[pick])) + 2 * U * np.abs(w[pick]) + 1e-37, what)
+    assert np.array_equal(got[2], want[2][pick])
 
 
 def test_token_logprobs_parts(device):
