@@ -148,17 +148,20 @@ __device__ __forceinline__ double exp2_neg(double d) {
   return ldexp((double)__builtin_amdgcn_exp2f((float)(fmax(d, -2000.0) - n)), (int)n);
 }
 
-// How many of keys[0 .. n) are above `key`; n a multiple of 8 (zeros fill it).
-__device__ __forceinline__ int rank_among(const unsigned long long* keys, int n, unsigned long long key) {
-  int rank = 0;
-  for (int j = 0; j < n; j += 8) {
-    ulonglong2 k[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) k[i] = *reinterpret_cast<const ulonglong2*>(keys + j + 2 * i);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) rank += (k[i].x > key) + (k[i].y > key);
+// Ranks of keys[0 .. n) among themselves (how many are above), by all threads: eight
+// lanes a key, each against every eighth.  found(i, rank) on one of the eight.
+template <int NT, class F>
+__device__ __forceinline__ void rank_keys(const unsigned long long* keys, int n, F found) {
+  const int sub = threadIdx.x & 7;
+  for (int i0 = 0; i0 < n; i0 += NT / 8) {  // (uniform: the lanes' sums need all eight)
+    const int i = i0 + (threadIdx.x >> 3);
+    const unsigned long long key = keys[min(i, n - 1)];
+    int above = 0;
+#pragma unroll 4
+    for (int j = sub; j < n; j += 8) above += keys[j] > key;
+    const int rank = (int)group_sum<8>((float)above);
+    if (sub == 0 && i < n) found(i, rank);
   }
-  return rank;
 }
 
 // A row's records joined.  With M the row's largest logit, f = 2^((m - M) c) of
@@ -171,7 +174,7 @@ template <int TYPE, int W>
 __global__ __launch_bounds__(64 * W) void k_logprob_join(LogprobArgs a, int n_pieces, double c) {
   constexpr int NT = 64 * W, R = kMaxPieces > NT ? kMaxPieces / NT : 1;  // records a thread
   __shared__ __align__(16) unsigned long long keys[kMaxPieces];
-  __shared__ __align__(16) unsigned long long cand[kCand + 8];
+  __shared__ __align__(16) unsigned long long cand[kCand];
   __shared__ unsigned long long red_key[W];
   __shared__ double red_rest[W], red_ent[W];
   __shared__ int red_bad[W], chosen[kMaxTop];
@@ -203,14 +206,10 @@ __global__ __launch_bounds__(64 * W) void k_logprob_join(LogprobArgs a, int n_pi
   for (int i = 1; i < W; ++i) top = red_key[i] > top ? red_key[i] : top;
   const float M = order_value((uint32_t)(top >> 32));
   // the n pieces with the largest keys, by rank (keys differ: their indexes do)
-  if (n) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      if (tid + i * NT >= n_pieces) break;
-      const int rank = rank_among(keys, (n_pieces + 7) & ~7, key[i]);
-      if (rank < n) chosen[rank] = tid + i * NT;
-    }
-  }
+  if (n)
+    rank_keys<NT>(keys, n_pieces, [&](int i, int rank) {
+      if (rank < n) chosen[rank] = i;
+    });
   float x_tok = 0.0f;  // the given token's logit
   const int tok = tid == 0 && a.logprob ? a.tokens[row] : -1;
   if (tok >= 0 && tok < a.n_vocab) {
@@ -279,6 +278,7 @@ __global__ __launch_bounds__(64 * W) void k_logprob_join(LogprobArgs a, int n_pi
   // Every one of the n largest logits is at least the n-th piece's largest: the
   // logits that are (few more than n, as a rule) become candidates, in any order.
   const unsigned long long least = n_pieces >= n ? keys[chosen[n - 1]] : 1ull;
+  const float least_value = n_pieces >= n ? order_value((uint32_t)(least >> 32)) : -INFINITY;
   for (int q0 = 0; q0 < n_sel; q0 += 2 * W) {
     if (q0) fetch(q0);
 #pragma unroll
@@ -287,9 +287,10 @@ __global__ __launch_bounds__(64 * W) void k_logprob_join(LogprobArgs a, int n_pi
       const int piece = chosen[q0 + h * W + wave];
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        if (order_key(v[h][i] == v[h][i] ? v[h][i] : -INFINITY) < (uint32_t)(least >> 32)) continue;
+        const bool may = !(v[h][i] < least_value);  // (a NaN may, where -inf does)
+        if (__builtin_expect(__ballot(may) == 0, 1)) continue;
         const unsigned long long mine = piece_key(v[h][i], piece_index<TYPE>(piece, lane, i), a.n_vocab);
-        if (mine < least) continue;
+        if (!may || mine < least) continue;
         const int at = atomicAdd(&n_cand, 1);
         if (at < kCand) cand[at] = mine;
       }
@@ -323,16 +324,12 @@ __global__ __launch_bounds__(64 * W) void k_logprob_join(LogprobArgs a, int n_pi
     __syncthreads();
     nc = n_cand;
   }
-  if (tid < 8) cand[nc + tid] = 0;  // (whole eights for the ranking)
-  __syncthreads();
-  for (int i = tid; i < nc; i += NT) {
-    const unsigned long long mine = cand[i];
-    const int rank = rank_among(cand, (nc + 7) & ~7, mine);
-    if (rank < n) {
-      a.top_idx[(uint64_t)row * n + rank] = (int32_t)(0xFFFFFFFFu - (uint32_t)mine);
-      a.top_logprob[(uint64_t)row * n + rank] = logp(order_value((uint32_t)(mine >> 32)));
-    }
-  }
+  rank_keys<NT>(cand, nc, [&](int i, int rank) {
+    if (rank >= n) return;
+    const unsigned long long k = cand[i];
+    a.top_idx[(uint64_t)row * n + rank] = (int32_t)(0xFFFFFFFFu - (uint32_t)k);
+    a.top_logprob[(uint64_t)row * n + rank] = logp(order_value((uint32_t)(k >> 32)));
+  });
 }
 
 int pieces_of(int n_vocab) { return (n_vocab + kPiece - 1) / kPiece; }
