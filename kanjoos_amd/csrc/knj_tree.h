@@ -15,12 +15,17 @@
 
 namespace knj {
 
-// n / d by one multiplication, for n d < 2^32.
+// n / d for n < 2^31 by one multiplication: with L = ceil(log2 d) and m = ceil(2^(31 +
+// L) / d), which 32 bits hold, n m 2^-(31 + L) is above n / d by less than 1 / d.
 struct FastDiv {
-  uint32_t d, m;  // m = ceil(2^32 / d), 0 for d = 1
+  uint32_t d, m, sh;  // m 0 for d = 1
   FastDiv() = default;
-  explicit FastDiv(uint32_t v) : d(v), m(v > 1 ? (uint32_t)(((1ull << 32) + v - 1) / v) : 0u) {}
-  __device__ __forceinline__ uint32_t div(uint32_t n) const { return m ? __umulhi(n, m) : n; }
+  explicit FastDiv(uint32_t v) : d(v), m(0), sh(0) {
+    if (v == 1) return;
+    while ((1ull << (sh + 1)) < v) ++sh;  // L - 1
+    m = (uint32_t)(((1ull << (32 + sh)) + v - 1) / v);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return m ? __umulhi(n, m) >> sh : n; }
 };
 
 struct TreePlan {
@@ -164,8 +169,8 @@ typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 // Waves that share the columns (WS > 1) keep running statistics of their own and
 // join them at the end, through LDS, in pairs.
 //
-// Chunks reach LDS by DMA, as the cache holds them, NST - 1 chunks ahead, one
-// barrier a chunk; 16-byte pieces (K) and 32-byte pairs (V) of a row are permuted
+// Chunks reach LDS by DMA, as the cache holds them, the next one while one is
+// computed, one barrier a chunk; 16-byte pieces (K) and 32-byte pairs (V) of a row are permuted
 // by an XOR of the row index, so that the operand reads fall on distinct banks.
 // 8-bit codes become f16 (exactly) as operands.  Their scales stay out of the
 // products: a score is multiplied by its slot's, a weight by its slot's over the
@@ -177,7 +182,7 @@ typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 // The loads that need no sequence length (a chunk's rows, the queries) come
 // first; rows of a chunk past the sequence's slots hold whatever the cache does
 // there, and the chunks that reach the drafts are cleaned before use (below).
-template <int D, int FORMAT, bool SPLIT, int NT, int WC, int WS, int SW, int NST>
+template <int D, int FORMAT, bool SPLIT, int NT, int WC, int WS, int SW>
 __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p) {
   constexpr bool Q8 = FORMAT != KNJ_KV_F16;
   constexpr int NW = WC * WS, NTH = 64 * NW, C = WS * SW, COLS = WC * NT * 16, ST = SW / 16;
@@ -185,11 +190,10 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
   constexpr int RPB = 256 / RB, NSLOT = RB / 16, NPAIR = RB / 32, CB = C * RB;
   constexpr bool HALVES = CB / 1024 < NW;                // half of the waves fetch K, half V
   constexpr int NI = HALVES ? 1 : CB / 1024 / NW;        // 1 KB DMA instructions per wave and matrix
-  constexpr int NDMA = (HALVES ? 1 : 2 * NI) + (Q8 ? 1 : 0);  // of a chunk, per wave
   constexpr int SB = 2 * CB + (Q8 ? 8 * C : 0);          // bytes of a stage: K, V, scales of both
   constexpr int DT = D / 16;                             // accumulator tiles per column tile
   constexpr int JOIN = WS > 1 ? WS / 2 * WC * NT * (DT * 1024 + 512) : 0;
-  constexpr int LDS = NST * SB > JOIN ? NST * SB : JOIN;
+  constexpr int LDS = 2 * SB > JOIN ? 2 * SB : JOIN;
   static_assert(HALVES ? 2 * CB == 1024 * NW : CB % (1024 * NW) == 0, "whole DMA instructions");
   static_assert(C % 32 == 0 && NW % (C / 32) == 0, "whole DMA instructions of scales");
   static_assert(SB % 256 == 0, "stages on whole rows");
@@ -199,7 +203,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
 
   // tiles of one unit run on one XCD, whose L2 then serves their shared slots
   // (workgroups go to the eight XCDs in turn; gridDim.x is a multiple of eight)
-  const int tile = blockIdx.x >> 3, unit = blockIdx.y * 8 + (blockIdx.x & 7);
+  const int tile = blockIdx.x >> 3, unit = (blockIdx.z * gridDim.y + blockIdx.y) * 8 + (blockIdx.x & 7);
   if (unit >= p.units) return;
   const int nk = a.c.n_head_kv, G = p.by_group.d, n_ctx = a.c.n_ctx;
   const int rest = p.by_nk.div(unit), kvh = unit - rest * nk;
@@ -246,8 +250,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
     }
   };
   const int c0 = split * p.cps;
-#pragma unroll
-  for (int i = 0; i < NST - 1; ++i) dma(c0 + i, i);
+  dma(c0, 0);
 
   // ---- this lane's query columns.  Step c's dims 8 kq .. + 7 of 32; with 8 bits,
   // where a 16-byte piece of a K row is two steps', dims 64 (c/2) + 16 kq + 8 (c%2)
@@ -501,18 +504,18 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
       for (int i = 0; i < 4; ++i) acc[nt][dt][i] *= alpha;
   };
 
-  // chunk j's stage ready: this wave's DMA of it has landed (the chunks after it may
-  // be in flight); the barrier hands every wave's part over and ends the reads of
-  // chunk j - 1, whose stage chunk j + NST - 1 then refills (past the range: fetched
-  // and not used)
+  // chunk j's stage ready: this wave's DMA of it has landed; the barrier hands every
+  // wave's part over and ends the reads of chunk j - 1, whose stage the next chunk
+  // then refills (past the range: fetched and not used).  A third stage, a chunk more
+  // ahead, gained nothing (int8 at 32K slots 18.6 us against 17.9).
   int j = c0, stage = 0;
   auto ready = [&]() {
-    KNJ_BARRIER_AFTER(vm_lds_imm((NST - 2) * NDMA));
-    dma(j + NST - 1, stage == 0 ? NST - 1 : stage - 1);
+    KNJ_BARRIER_AFTER(vm_lds_imm(0));
+    dma(j + 1, stage ^ 1);
   };
   auto next = [&]() {
     ++j;
-    stage = stage + 1 == NST ? 0 : stage + 1;
+    stage ^= 1;
     if (j < c1) ready();
   };
   const int j_prefix = min(c1, P / C);  // chunks below lie in the prefix
@@ -777,7 +780,8 @@ hipError_t launch_format(const TreeArgs& a, const TreePlan& p, int cols, hipStre
 #define KNJ_TREE_FORMAT(FORMAT)                                                                          \
   template <>                                                                                            \
   hipError_t launch_format<FORMAT>(const TreeArgs& a, const TreePlan& p, int cols, hipStream_t s) {      \
-    const dim3 grid(8 * p.n_tiles, (p.units + 7) / 8);                                                   \
+    const unsigned eights = (p.units + 7) / 8, y = eights < 32768u ? eights : 32768u;                    \
+    const dim3 grid(8 * p.n_tiles, y, (eights + y - 1) / y);                                             \
     const bool split = a.type == KNJ_TYPE_F32;                                                           \
     if (a.c.head_dim == 128) {                                                                           \
       if (split) KNJ_TREE_COLS(128, FORMAT, true);                                                       \
@@ -795,10 +799,8 @@ hipError_t launch_format(const TreeArgs& a, const TreePlan& p, int cols, hipStre
     else if (SPLIT || cols == 64) KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, 2, 2, 2, 32);                   \
     else KNJ_TREE_LAUNCH(DD, FORMAT, false, 2, 4, 1, 64);                                            \
   } while (0)
-// two stages of an f16 cache's rows fill LDS for two workgroups, three of an 8-bit one's
-#define KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, NT, WC, WS, SW)                                           \
-  KNJ_LAUNCH((k_tree<DD, FORMAT, SPLIT, NT, WC, WS, SW, FORMAT == KNJ_KV_F16 ? 2 : 3>), grid,        \
-             dim3(64 * WC * WS), 0, s, a, p)
+#define KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, NT, WC, WS, SW) \
+  KNJ_LAUNCH((k_tree<DD, FORMAT, SPLIT, NT, WC, WS, SW>), grid, dim3(64 * WC * WS), 0, s, a, p)
 
 }  // namespace tree
 }  // namespace knj
