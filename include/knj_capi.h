@@ -169,7 +169,7 @@ int knj_attention_step(const float* q, const float* k, const float* v, const flo
  *   (2i, 2i + 1) (KNJ_ROPE_INTERLEAVED) by the angle pos * inv_freq[i], cos and
  *   sin times mscale; the other dims pass.  Angles are formed in f64 (the decode
  *   step's own tables hold f32 angles: they part by up to pos * 2^-24 radians).
- *   An output may be its own input (the same pointer and stride).
+ *   An output may be its own input (the same pointer and stride).  n_rows < 2^24.
  * knj_rope_freqs (host only): the n_rot/2 frequencies base^(-2i/n_rot) under a
  *   scaling for contexts `factor` (>= 1) times orig_ctx, to be copied to the
  *   device, and mscale.  KNJ_ROPE_LINEAR: / factor.  KNJ_ROPE_NTK: base times
@@ -206,7 +206,7 @@ int knj_rope(int type, int layout, int n_rot, const double* inv_freq, float msca
  * knj_kv_store: rows t < counts[s] (NULL: n_rows) of sequence s, k and v
  *   [n_seq][n_rows][n_head_kv][head_dim] with row_stride elements from a row to
  *   the next (of both), go to slots start[s] + t.  Rows that would fall outside
- *   [0, n_ctx) are not stored.
+ *   [0, n_ctx) are not stored.  n_rows * n_head_kv < 2^27, here and in knj_kv_load.
  * knj_kv_load: slots[s][t] (NULL: slot t) of the cache into rows k and v of the
  *   same form, as code * scale rounded to `type`; rows whose slot is outside
  *   [0, n_ctx) are left as they were.  Loaded as f32 and stored again, a row keeps
@@ -244,10 +244,11 @@ int knj_kv_load(const knj_kv_cache* cache, int type, const int32_t* slots, int n
  *   prefix[s] is held to [0, max_prefix] and counts[s] to [0, n_rows]; max_prefix +
  *   n_rows <= n_ctx, n_rows <= 1024, scale in [1e-6, 1e6], n_head a multiple of n_head_kv
  *   and at most 1024.
- *   out may be q.  With f32 activations the queries and the softmax's weights
+ *   out may be q (with out_stride = q_stride).  With f32 activations the queries and the softmax's weights
  *   keep 22 bits, with 16-bit ones the weights 11 (the outputs' own rounding).
- * knj_attention_tree_workspace: bytes its workspace needs for these sizes (0 for
- *   arguments that it refuses); any contents. */
+ * knj_attention_tree_workspace: bytes its workspace needs for these sizes (0: none,
+ *   or arguments that it refuses); any contents.  Smaller sizes can need more (their
+ *   slots are split further), but none more than 262144 * (head_dim + 4). */
 int knj_attention_tree(const knj_kv_cache* cache, int type, const void* q, uint64_t q_stride,
                        int n_head, int n_rows, const int32_t* prefix, int max_prefix,
                        const int32_t* counts, const uint64_t* mask, int mask_shared, float scale,
@@ -267,7 +268,8 @@ uint64_t knj_attention_tree_workspace(const knj_kv_cache* cache, int n_head, int
  *     most 32 and n_vocab).
  *   -inf rules a token out.  A row with nothing left gives log probabilities of
  *   -inf and an entropy of 0; a row that holds a NaN or +inf gives NaN (in top_idx a
- *   NaN ranks as -inf).  n_vocab <= 2^20, n_rows * n_vocab / 2048 < 2^31.
+ *   NaN ranks as -inf).  n_vocab <= 2^20, n_rows < 2^24 and
+ *   n_rows * ceil(n_vocab / 2048) < 2^26.
  * knj_token_logprobs_workspace: bytes of its workspace; any contents. */
 int knj_token_logprobs(int type, const void* logits, uint64_t row_stride, int n_rows, int n_vocab,
                        float temperature, const int32_t* tokens, float* logprob, float* entropy,

@@ -6,7 +6,7 @@
 // the sum of the others' exponentials relative to it, and the entropy's sum.
 // The second, a workgroup per row, joins a row's records in f64 and finds the
 // n largest logits: only the n pieces with the largest maxima can hold any, so
-// those n (of 75 at a vocabulary of 151,936) are read again.
+// those n are read again.
 #include <string>
 
 #include "knj_common.h"
@@ -378,7 +378,8 @@ int knj_token_logprobs(int type, const void* logits, uint64_t row_stride, int n_
   KNJ_CHECK_ARG(n_rows >= 0, "negative row count");
   KNJ_CHECK_ARG(n_vocab > 0 && n_vocab <= kMaxVocab, "n_vocab must be in [1, 2^20]");
   KNJ_CHECK_ARG(row_stride >= (uint64_t)n_vocab, "the row stride is below the row's width");
-  KNJ_CHECK_ARG((uint64_t)n_rows * pieces_of(n_vocab) < (1ull << 31), "too many rows for one call");
+  KNJ_CHECK_ARG(n_rows < (1 << 24) && (uint64_t)n_rows * pieces_of(n_vocab) < (1ull << 26),
+                "too many rows for one call");  // (a grid holds 2^32 threads a dim)
   KNJ_CHECK_ARG(temperature >= 1e-4f && temperature <= 1e4f, "the temperature must be in [1e-4, 1e4]");
   KNJ_CHECK_ARG(!tokens == !logprob, "tokens and logprob go together");
   KNJ_CHECK_ARG(n_top >= 0 && n_top <= kMaxTop && n_top <= n_vocab, "n_top must be in [0, min(32, n_vocab)]");

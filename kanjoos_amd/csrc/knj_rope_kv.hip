@@ -394,6 +394,7 @@ int knj_rope(int type, int layout, int n_rot, const double* inv_freq, float msca
   KNJ_CHECK_ARG(((uintptr_t)inv_freq & 7) == 0 && (((uintptr_t)q_norm | (uintptr_t)k_norm) & 15) == 0,
                 "inv_freq must be 8-byte and the norm weights 16-byte aligned");
   KNJ_CHECK_ARG(n_rows >= 0, "negative row count");
+  KNJ_CHECK_ARG(n_rows < (1 << 24), "too many rows for one call");  // (a grid holds 2^32 threads a dim)
   KNJ_CHECK_ARG(n_head > 0 && n_head <= 4096 && n_head_kv >= 0 && n_head_kv <= 4096,
                 "n_head must be in [1, 4096], n_head_kv in [0, 4096]");
   KNJ_CHECK_ARG(n_head_kv == 0 || (k && k_out), "null key pointer");
@@ -424,7 +425,7 @@ static int check_kv_rows(const knj_kv_cache* cache, int type, const void* k, con
   KNJ_CHECK_ARG(row_stride >= (uint64_t)cache->n_head_kv * cache->head_dim, "the row stride is below the row's width");
   KNJ_CHECK_ARG(rows_aligned(k, row_stride, eb) && rows_aligned(v, row_stride, eb),
                 "rows must start on 16-byte boundaries");
-  KNJ_CHECK_ARG((uint64_t)n_rows * cache->n_head_kv < (1ull << 31), "too many rows for one call");
+  KNJ_CHECK_ARG((uint64_t)n_rows * cache->n_head_kv < (1ull << 27), "too many rows for one call");
   return KNJ_OK;
 }
 

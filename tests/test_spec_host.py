@@ -178,6 +178,34 @@ def test_token_logprobs_refusals(kw, match):
     refused(lambda: K.token_logprobs(**{**a, **kw}), match)
 
 
+@pytest.mark.parametrize("n_rows,n_vocab", [(1 << 24, 8), (1 << 23, 20000)])
+def test_token_logprobs_row_limits(n_rows, n_vocab):
+    """A launch holds 2^32 threads along a dimension of its grid: 256 a row, 64 a piece."""
+    L = K.lib()
+    assert L.knj_token_logprobs(F32, A, n_vocab, n_rows, n_vocab, 1.0, None, None, A, 0, None, None, A,
+                                K.token_logprobs_workspace(n_rows, n_vocab), None) == K.KNJ_E_ARG
+    assert b"too many" in L.knj_last_error()
+
+
+def test_row_limits():
+    refused(lambda: K.rope(F32, A, A, A, A, 1 << 24, 8, 1, 128), "too many")
+    c = cache(n_ctx=1 << 25)
+    n = (1 << 27) // c.desc.n_head_kv
+    refused(lambda: K.kv_store(c, F32, A, A, A, n), "too many")
+    refused(lambda: K.kv_load(c, F32, A, A, n), "too many")
+
+
+@pytest.mark.parametrize("n_head,n_seq", [(2, 1), (8, 1), (32, 1), (32, 5), (64, 65535)])
+def test_attention_tree_workspace_bound(n_head, n_seq):
+    """No sizes need more than the documented 262144 (head_dim + 4) bytes."""
+    for n_head_kv, head_dim in ((1, 64), (2, 128)):
+        c = cache(n_head_kv=n_head_kv, head_dim=head_dim, n_seq=n_seq, n_ctx=1 << 22)
+        for n_rows in (1, 2, 7, 16, 33, 64, 100, 257, 1024):
+            for prefix in (0, 1, 100, 1000, 4096, 50000, (1 << 22) - 1024):
+                need = K.attention_tree_workspace(c, n_head, n_rows, prefix)
+                assert need <= 262144 * (head_dim + 4)
+
+
 def test_token_logprobs_workspace_size():
     need = K.token_logprobs_workspace(7, 5000)
     assert need > 0 and K.token_logprobs_workspace(14, 5000) == 2 * need
