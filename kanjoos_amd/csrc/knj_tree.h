@@ -351,20 +351,28 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
   constexpr int NE = SW == 16 ? 1 : ST / 2;  // value steps
   auto scores = [&](uint32_t at, f32x4 (&sc)[NT][ST], float (&vq)[Q8 ? 4 * ST : 1]) {
     const uint32_t k0 = at + kat;
+    constexpr int NK = Q8 ? D / 64 : D / 32;  // 16-byte reads of a K row per lane
+    uint4 w[NK][ST];
 #pragma unroll
-    for (int st = 0; st < ST; ++st) {
+    for (int c = 0; c < NK; ++c)
+#pragma unroll
+      for (int st = 0; st < ST; ++st) w[c][st] = lds_b128((k0 ^ (64 * c)) + 16 * st * RB);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int st = 0; st < ST; ++st)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) sc[nt][st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      uint4 w = {};
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
+    for (int c = 0; c < D / 32; ++c) {
+#pragma unroll
+      for (int st = 0; st < ST; ++st) {
         h16x8 ka;
         if constexpr (Q8) {
-          if (c % 2 == 0) w = lds_b128((k0 ^ (64 * (c >> 1))) + 16 * st * RB);
-          const uint2 x = codes4_h<FORMAT>((c & 1) ? w.z : w.x), y = codes4_h<FORMAT>((c & 1) ? w.w : w.y);
+          const uint4 u = w[c >> 1][st];
+          const uint2 x = codes4_h<FORMAT>((c & 1) ? u.z : u.x), y = codes4_h<FORMAT>((c & 1) ? u.w : u.y);
           ka = __builtin_bit_cast(h16x8, make_uint4(x.x, x.y, y.x, y.y));
         } else {
-          ka = __builtin_bit_cast(h16x8, lds_b128((k0 ^ (64 * c)) + 16 * st * RB));
+          ka = __builtin_bit_cast(h16x8, w[c][st]);
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
