@@ -2,9 +2,9 @@
 // written in f16 or 8 bits and read back.
 //
 // Both are streams over rows of heads: a group of D/8 lanes holds one head's row (of
-// a cache its key and its value), eight elements a lane, so a head's reductions (the norm's sum, the largest
-// magnitude) stay inside the group's DPP moves and every element is read and
-// written once.
+// a cache its key and its value), eight elements a lane, so a head's reductions (the
+// norm's sum, the largest magnitude) stay inside the group's DPP moves and every
+// element is read and written once.
 #include <algorithm>
 #include <cmath>
 #include <string>
@@ -49,6 +49,9 @@ __device__ __forceinline__ void st4(void* p, uint64_t i, float4 v) {
 // pos * f and its reduction to [-pi, pi] in f64 (an f32 product is off by
 // pos * 2^-24 radians, 0.06 at a million), the functions in f32 on the reduced
 // angle.
+//
+// Bound by memory: 4000 rows of 36 f32 heads of 128 (147 MB in and out) 30.9 us a call,
+// 4.8 TB/s, where a large copy reaches 5.1.  One row is a launch: 2.1 us on the chip.
 template <int TYPE, int LAYOUT, int D>
 __global__ __launch_bounds__(kBlock) void k_rope(RopeArgs a) {
   constexpr int T = D / 8, HPB = kBlock / T;
@@ -181,7 +184,12 @@ __device__ __forceinline__ uint2 quantise8(const float (&x)[8], float& scale) {
   return o;
 }
 
-// Rows of `FORMAT` from rows of activations; blockIdx.y is the sequence.
+// Rows of `FORMAT` from rows of activations; blockIdx.y is the sequence.  The same
+// lanes take a head's key and its value, so that the two reductions and divisions
+// run side by side (4096 rows of 4 f32 heads of 128 as e4m3 with a group for each
+// matrix: 8.9 us, so 8.2).  That is 21 MB, 4.1 us at a copy's rate: the rest is one
+// pass of latency (loads, two maxima over 16 lanes, a division, stores) of 1024
+// workgroups that are all resident at once; 32 sequences' one row 3.3 us.
 template <int TYPE, int FORMAT, int D>
 __global__ __launch_bounds__(kBlock) void k_kv_store(KvRowsArgs a) {
   const knj_kv_cache& c = a.c;
@@ -233,7 +241,9 @@ __device__ __forceinline__ void values8(uint2 w, float scale, float4& a, float4&
   }
 }
 
-// The reverse: rows of activations from cache slots.
+// The reverse: rows of activations from cache slots.  Bound by memory: 32,000 rows of
+// 4 int8 heads of 128 to f16 (99 MB) 22.0 us, 4.5 TB/s, with keys and values by the
+// same lanes (28 with a group for each); gathered rows of 32 sequences 2.6 us.
 template <int TYPE, int FORMAT, int D>
 __global__ __launch_bounds__(kBlock) void k_kv_load(KvRowsArgs a) {
   const knj_kv_cache& c = a.c;

@@ -41,7 +41,7 @@ namespace tree {
 
 using namespace dev;
 
-// Sixteen codes as f16 (exact): e4m3 by the conversion, int8 by setting the
+// Four codes as f16 (exact): e4m3 by the conversion, int8 by setting the
 // offset code under the exponent of 1024 and subtracting 1024 + 128.
 template <int FORMAT>
 __device__ __forceinline__ uint2 codes4_h(uint32_t w) {
@@ -170,8 +170,9 @@ typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 // join them at the end, through LDS, in pairs.
 //
 // Chunks reach LDS by DMA, as the cache holds them, the next one while one is
-// computed, one barrier a chunk; 16-byte pieces (K) and 32-byte pairs (V) of a row are permuted
-// by an XOR of the row index, so that the operand reads fall on distinct banks.
+// computed, one barrier a chunk; 16-byte pieces (K) and 32-byte pairs (V) of a row
+// are permuted by an XOR of the row index, so that the operand reads fall on
+// distinct banks.
 // 8-bit codes become f16 (exactly) as operands.  Their scales stay out of the
 // products: a score is multiplied by its slot's, a weight by its slot's over the
 // running largest of the scales its column has seen (a power of two, so a weight
@@ -182,6 +183,20 @@ typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 // The loads that need no sequence length (a chunk's rows, the queries) come
 // first; rows of a chunk past the sequence's slots hold whatever the cache does
 // there, and the chunks that reach the drafts are cleaned before use (below).
+//
+// What bounds it (f16, 64 drafts x 32 heads over 32,764 slots of 4 kv heads, 34 GFLOP:
+// 58.5 us a call, 0.59 PFLOP/s; 49 us here, 9 in the merge): of a wave's life the
+// matrix cores are busy for 42 %, vector instructions issue for 25 % (two waves share
+// a SIMD, so 51 % of it) and LDS delivers for 45 % of the CU's; the two waves that
+// the accumulators leave room for do not cover one another's waits.  Taken out one
+// at a time, in a copy: the exponentials change nothing, a chunk that is always in L2
+// saves 6 us, 24 of a chunk's 64 products with their reads 10.  Calls of few drafts
+// are one wave's path through a chunk, 1.7 us of conversions, reductions and waits,
+// and two launches: 9.5 us for 4 drafts over 1000 f16 slots.
+// Tried and no faster: eight waves to a tile (of 128 columns within 3 %, of 32
+// slower), a raised wave priority around the products, 768 or 1024 workgroups,
+// chunks of 128 slots, chunks through registers instead of DMA, the next chunk's DMA
+// behind this one's reads (1 to 5 % slower).
 template <int D, int FORMAT, bool SPLIT, int NT, int WC, int WS, int SW>
 __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p) {
   constexpr bool Q8 = FORMAT != KNJ_KV_F16;
