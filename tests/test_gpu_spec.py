@@ -667,6 +667,63 @@ def test_attention_tree_first_rows_of_many(device):
         assert np.array_equal(got[0, count:], before[0, count:])
 
 
+def test_attention_tree_many_units(device):
+    """More (sequence, kv head) pairs than one dimension of the grid holds in eights:
+    every pair of 4100 sequences of 64 heads gets its own answer."""
+    rng = np.random.default_rng(11)
+    n, nk, D, ctx = 4100, 64, 64, 3
+    c = make_cache(K.KV_F16, n, nk, ctx, D)
+    kv = fill_cache(c, rng)
+    prefix = rng.integers(0, ctx, n)
+    q = rng.normal(size=(n, 1, nk, D)).astype(np.float16).astype(np.float64)
+    got, _ = run_tree(c, F16, q, 1, prefix, None, None, nk, max_prefix=ctx - 1)
+    sc = np.einsum("shd,shjd->shj", q[:, 0], kv[0]) * D ** -0.5  # (a chain of one: slots up to its own)
+    A = np.einsum("shd,shjd->shj", np.abs(q[:, 0]), np.abs(kv[0])).max(-1) * D ** -0.5
+    seen = np.arange(ctx) <= prefix[:, None]
+    sc = np.where(seen[:, None], sc, -np.inf)
+    e = np.exp(sc - sc.max(-1, keepdims=True))
+    l = e.sum(-1, keepdims=True)
+    w = e / l
+    want = np.einsum("shj,shjd->shd", w, kv[1])
+    rms = np.sqrt(np.einsum("shj,shjd->shd", np.broadcast_to(seen[:, None], w.shape).astype(np.float64), kv[1] ** 2))
+    # (tree64's bound)
+    bound = (32 * U * A[..., None] + 64 * U + 2.0 ** -11) * np.einsum("shj,shjd->shd", w, np.abs(kv[1])) \
+        + 6 * 2.0 ** -25 * rms / l + HALF[F16] * np.abs(want) + 2.0 ** -25
+    close(got[:, 0], want, bound, "pairs")
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_attention_tree_many_heads(device, fmt):
+    """The most query heads over one kv head."""
+    rng = np.random.default_rng([13, fmt])
+    nh, D, T, P = 1024, 64, 3, 70
+    c = make_cache(fmt, 1, 1, P + T, D)
+    kv = fill_cache(c, rng)
+    q = rng.normal(size=(1, T, nh, D)).astype(np.float32).astype(np.float64)
+    sees = tree_bits(rng, T)[None]
+    got, _ = run_tree(c, F32, q, T, [P], None, sees, nh)
+    want, bound = tree64(q, kv, [P], [T], sees, D ** -0.5, F32)
+    close(got, want, bound, "heads")
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_kv_rows_of_most_sequences(device, fmt):
+    """The most sequences a cache may have, a row each; read back by a slot list that
+    names the same slot twice."""
+    rng = np.random.default_rng([17, fmt])
+    n, D = 65535, 64
+    c = make_cache(fmt, n, 1, 1, D)
+    x = rng.normal(size=(2, n, D)).astype(np.float32)
+    buf = [put(a) for a in x]
+    K.kv_store(c, F32, buf[0], buf[1], i32(np.zeros(n)), 1)
+    out = [K.DeviceBuffer(2 * x[0].nbytes) for _ in range(2)]
+    K.kv_load(c, F32, out[0], out[1], 2, slots=i32(np.zeros(2 * n)))
+    for a, o in zip(x, out):
+        code, scale = codes(a.astype(np.float64), fmt)
+        v = values(code, scale, fmt)[:, None]
+        close(o.download(np.float32).reshape(n, 2, D), np.broadcast_to(v, (n, 2, D)), U * np.abs(v) + 1e-45, "rows")
+
+
 # ------------------------------------------------------------------ log probabilities
 
 def logprobs64(x, tokens, n_top, T):
@@ -772,7 +829,8 @@ def test_token_logprobs_ties_and_masks(device, t):
     check_logprobs(x, raw, t, tokens, 1, 0.6)
 
 
-@pytest.mark.parametrize("t,V,rows,n_top", [(F32, 5000, 131, 32), (BF16, 3000, 300, 7), (F16, 600000, 129, 20)])
+@pytest.mark.parametrize("t,V,rows,n_top", [(F32, 5000, 131, 32), (BF16, 3000, 300, 7), (F16, 600000, 129, 20),
+                                            (F32, 5000, 257, 32), (F16, 600000, 259, 20)])
 def test_token_logprobs_many_rows(device, t, V, rows, n_top):
     """Rows enough for the narrower join, more pieces than it has threads among them;
     the rows repeat a few of their own, so that ties and sorted rows come along."""
