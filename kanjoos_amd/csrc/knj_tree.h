@@ -516,9 +516,12 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  // a value scale's reference: the power of two below twice the largest, which a
-  // later scale may pass twice over before it moves (weights stay below 2^15)
-  auto vref_of = [](float vm) { return __uint_as_float((__float_as_uint(vm) & 0x7F800000u) ? (__float_as_uint(vm) & 0x7F800000u) + 0x00800000u : 0u); };
+  // a value scale's reference: the power of two above the largest, which a later
+  // scale may pass fourfold before it moves (weights stay up to 2^15)
+  auto vref_of = [](float vm) {
+    const uint32_t e = __float_as_uint(vm) & 0x7F800000u;
+    return __uint_as_float(e ? e + 0x00800000u : 0u);
+  };
   auto inverse = [](float ref) { return ref > 0.0f ? __uint_as_float((254u << 23) - __float_as_uint(ref)) : 0.0f; };
   auto rescale = [&](int nt, float alpha) {
 #pragma unroll
@@ -652,7 +655,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
           for (int i = 0; i < 4 * ST; ++i) vm = fmaxf(vm, vq[i] < INFINITY ? vq[i] : 0.0f);
           vm = fmaxf(vm, xor16_f(vm));
           vm = fmaxf(vm, xor32_f(vm));
-          over |= vm >= 4.0f * vref[0];
+          over |= vm > 4.0f * vref[0];
         }
         if (j != settled && __ballot(over) != 0) break;
         VPair v[NPAIR];
@@ -683,7 +686,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
         m[nt] = mn;
         l[nt] *= alpha;
         if constexpr (Q8) {
-          const float ref = vm >= 4.0f * vref[nt] ? vref_of(vm) : vref[nt];
+          const float ref = vm > 4.0f * vref[nt] ? vref_of(vm) : vref[nt];
           alpha *= vref[nt] * inverse(ref);
           vref[nt] = ref;
         }

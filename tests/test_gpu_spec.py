@@ -626,6 +626,27 @@ def test_attention_tree_nan_in_prefix(device, fmt, part):
     close(got, want, np.where(np.isnan(bound), 1.0, bound), "nan")
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_attention_tree_zero_rows(device, fmt):
+    """A prefix of zero rows (scales of zero in 8 bits) that ends in ordinary ones: the
+    zeros take their equal part of the weights."""
+    rng = np.random.default_rng([19, fmt])
+    nh, nk, D, T, P = 8, 2, 64, 2, 400
+    c = make_cache(fmt, 1, nk, P + T, D)
+    x = rng.normal(size=(2, P + T, nk, D)).astype(np.float32)
+    x[:, :300] = 0
+    bufs = [put(a) for a in x]
+    K.kv_store(c, F32, bufs[0], bufs[1], i32([0]), P + T)
+    a = cache_arrays(c)
+    kv = [values(a[m], a[m + "_scale"], fmt) for m in ("k", "v")]
+    q = rng.normal(size=(1, T, nh, D)).astype(np.float32).astype(np.float64)
+    sees = tree_bits(rng, T)[None]
+    for prefix in (P, 200):  # the second sees zeros alone before its drafts' slots, which hold zeros too
+        got, _ = run_tree(c, F32, q, T, [prefix], None, sees, nh, max_prefix=P)
+        want, bound = tree64(q, kv, [prefix], [T], sees, D ** -0.5, F32)
+        close(got, want, bound, f"prefix {prefix}")
+
+
 def test_attention_tree_long_cache(device):
     """Sequences whose cache begins past 2^32 elements."""
     rng = np.random.default_rng(1)
