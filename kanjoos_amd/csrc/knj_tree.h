@@ -177,8 +177,9 @@ typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 // products: a score is multiplied by its slot's, a weight by its slot's over the
 // running largest of the scales its column has seen (a power of two, so a weight
 // stays in f16's range whatever the cache's units).  Queries are scaled by a
-// power of two per row, so that f16 holds any of them.  SPLIT keeps queries and
-// weights as f16 high parts and remainders (22 bits), for f32 activations.
+// power of two per row, so that f16 holds any of them.  Weights are f16 high parts and
+// remainders (22 bits) whatever the activations: 11 bits of a weight leave errors of
+// the size of an f16 output's own rounding.  SPLIT keeps f32 queries so too.
 //
 // The loads that need no sequence length (a chunk's rows, the queries) come
 // first; rows of a chunk past the sequence's slots hold whatever the cache does
@@ -430,7 +431,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
   // 8 bits times w8, the slots' value scales over the column's.  Returns their sum
   // (without those).
   auto weights = [&](const f32x4 (&sc)[ST], float s2c, float mref, const float (&w8)[Q8 ? 4 * ST : 1], h16x8 (&eh)[NE],
-                     h16x8 (&el)[SPLIT ? NE : 1]) {
+                     h16x8 (&el)[NE]) {
     // (the reference is -inf while the column has seen nothing: exponents then from 0)
     const float mr = mref == -INFINITY ? 0.0f : mref * s2c;
     float es = 0.0f;
@@ -444,7 +445,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
         // (the weight itself, rounded to f32, is what is split below: formed anew
         // inside the conversion to f16, the product could round the other way
         // there than in the remainder, an f16 step off)
-        if constexpr (SPLIT) asm("" : "+v"(w[i]));
+        asm("" : "+v"(w[i]));
       }
     }
 #pragma unroll
@@ -456,7 +457,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
                                       w[(8 * c + 7) % (4 * ST)]),
                hi, lo);
       eh[c] = hi;
-      if constexpr (SPLIT) el[c] = lo;
+      el[c] = lo;
     }
     return es;
   };
@@ -475,27 +476,25 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
     if constexpr (SW != 16) v.y = lds_tr16_at(q + 16 * RB);
     return v;
   };
-  auto product = [&](int dt, uint2 v0, uint2 v1, int c, const h16x8 (&eh)[NT][NE], const h16x8 (&el)[NT][SPLIT ? NE : 1]) {
+  auto product = [&](int dt, uint2 v0, uint2 v1, int c, const h16x8 (&eh)[NT][NE], const h16x8 (&el)[NT][NE]) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       if constexpr (SW == 16) {
         const h16x4 vv = __builtin_bit_cast(h16x4, v0);
         const h16x4 hi = __builtin_shufflevector(eh[nt][0], eh[nt][0], 0, 1, 2, 3);
         acc[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x16f16(vv, hi, acc[nt][dt], 0, 0, 0);
-        if constexpr (SPLIT) {
-          const h16x4 lo = __builtin_shufflevector(el[nt][0], el[nt][0], 0, 1, 2, 3);
-          acc[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x16f16(vv, lo, acc[nt][dt], 0, 0, 0);
-        }
+        const h16x4 lo = __builtin_shufflevector(el[nt][0], el[nt][0], 0, 1, 2, 3);
+        acc[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x16f16(vv, lo, acc[nt][dt], 0, 0, 0);
       } else {
         const h16x8 vv = __builtin_bit_cast(h16x8, make_uint4(v0.x, v0.y, v1.x, v1.y));
         acc[nt][dt] = mfma16(vv, eh[nt][c], acc[nt][dt]);
-        if constexpr (SPLIT) acc[nt][dt] = mfma16(vv, el[nt][c], acc[nt][dt]);
+        acc[nt][dt] = mfma16(vv, el[nt][c], acc[nt][dt]);
       }
     }
   };
   // the products of a chunk, its first step's reads given; each step's operands are
   // read while the step before is multiplied
-  auto values = [&](uint32_t at, VPair (&v)[NPAIR], const h16x8 (&eh)[NT][NE], const h16x8 (&el)[NT][SPLIT ? NE : 1]) {
+  auto values = [&](uint32_t at, VPair (&v)[NPAIR], const h16x8 (&eh)[NT][NE], const h16x8 (&el)[NT][NE]) {
 #pragma unroll
     for (int c = 0; c < NE; ++c) {
 #pragma unroll
@@ -583,7 +582,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
       f32x4 sc[NT][ST];
       float vq[Q8 ? 4 * ST : 1];
       scores(at, sc, vq);
-      h16x8 eh[NT][NE], el[NT][SPLIT ? NE : 1];
+      h16x8 eh[NT][NE], el[NT][NE];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         // the slots that the column sees: four bits per lane and slot tile
@@ -668,7 +667,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
           for (int i = 0; i < 4 * ST; ++i) w8[i] = vq[i] * inv;
         }
         __builtin_amdgcn_sched_barrier(0);
-        h16x8 eh[NT][NE], el[NT][SPLIT ? NE : 1];
+        h16x8 eh[NT][NE], el[NT][NE];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) l[nt] += weights(sc[nt], s2[nt], m[nt], w8, eh[nt], el[nt]);
         __builtin_amdgcn_sched_barrier(0);
