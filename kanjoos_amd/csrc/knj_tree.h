@@ -102,12 +102,13 @@ __device__ __forceinline__ u32x2 lds_tr16_at(uint32_t p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)p));
 }
 
-// Weights are formed relative to a reference that follows the running maximum
-// only when that has passed it by 2^7 (the accumulators are rescaled then, which
-// after a column's first slots is rare), and held times 2^6: at most 2^13, or 2^15
-// with a value scale's factor, below f16's 65,504, and f16 keeps all of a weight's
-// bits down to 2^-20 of the reference.
-constexpr float kLift = 6.0f, kLag = 7.0f;
+// A weight is 2^(s - r), its column's reference r 6 below the running maximum when it
+// was set and moved only when that has passed it by 13 (the accumulators are rescaled
+// then, which after a column's first slots is rare): at most 2^13, or 2^15 with a value
+// scale's factor, below f16's 65,504, and f16 keeps all of a weight's bits down to
+// 2^-20 of the maximum.  r is kept as the f32 that the exponents subtract, so that
+// a rescale by 2^(old - new) fits the weights on both sides, and is 1 where r stays.
+constexpr float kLift = 6.0f, kLag = 13.0f;
 
 // Maximum that carries a NaN (a NaN score makes its column NaN); the instruction
 // takes three, without the quieting of its inputs that fmaxf asks for.
@@ -339,7 +340,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
     return;
   }
 
-  // (maxima in units of the stored scores, before s2)
+  // (m: the references)
   float m[NT], l[NT], vref[NT];
   bool spoilt[NT];
   f32x4 acc[NT][DT];
@@ -433,12 +434,12 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
   auto weights = [&](const f32x4 (&sc)[ST], float s2c, float mref, const float (&w8)[Q8 ? 4 * ST : 1], h16x8 (&eh)[NE],
                      h16x8 (&el)[NE]) {
     // (the reference is -inf while the column has seen nothing: exponents then from 0)
-    const float mr = mref == -INFINITY ? 0.0f : mref * s2c;
+    const float mr = mref == -INFINITY ? 0.0f : mref;
     float es = 0.0f;
     float w[4 * ST];
 #pragma unroll
     for (int i = 0; i < 4 * ST; ++i) {
-      w[i] = __builtin_amdgcn_exp2f(fmaf(sc[i >> 2][i & 3], s2c, kLift - mr));
+      w[i] = __builtin_amdgcn_exp2f(fmaf(sc[i >> 2][i & 3], s2c, -mr));
       es += w[i];
       if constexpr (Q8) {
         w[i] *= w8[i];
@@ -522,6 +523,13 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
     return __uint_as_float(e ? e + 0x00800000u : 0u);
   };
   auto inverse = [](float ref) { return ref > 0.0f ? __uint_as_float((254u << 23) - __float_as_uint(ref)) : 0.0f; };
+  // column nt's reference moved if the largest score has passed it; the factor of what
+  // was summed before
+  auto moved = [&](int nt, float mx) {
+    const float old = m[nt];
+    if (!(fmaf(mx, s2[nt], -old) <= kLag)) m[nt] = max_nan(old, fmaf(mx, s2[nt], -kLift));
+    return __builtin_amdgcn_exp2f(old - (m[nt] == -INFINITY ? 0.0f : m[nt]));
+  };
   auto rescale = [&](int nt, float alpha) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -605,10 +613,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
           }
         }
         const float mx = largest(sc[nt]);
-        const float mn = (mx - m[nt]) * s2[nt] <= kLag ? m[nt] : max_nan(m[nt], mx);
-        const float mr = mn == -INFINITY ? 0.0f : mn * s2[nt];
-        float alpha = __builtin_amdgcn_exp2f(fmaf(m[nt], s2[nt], -mr));
-        m[nt] = mn;
+        float alpha = moved(nt, mx);
         l[nt] *= alpha;
         float w8[Q8 ? 4 * ST : 1];
         if constexpr (Q8) {
@@ -621,7 +626,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
 #pragma unroll
           for (int i = 0; i < 4 * ST; ++i) w8[i] = vin[i] * inv;
         }
-        l[nt] += weights(sc[nt], s2[nt], mn, w8, eh[nt], el[nt]);
+        l[nt] += weights(sc[nt], s2[nt], m[nt], w8, eh[nt], el[nt]);
         rescale(nt, alpha);
       }
       VPair v[NPAIR];
@@ -632,7 +637,9 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
     next();
     // ---- the chunks of the prefix: every column sees every slot.  A chunk whose
     // scores (or value scales) have left the columns' references behind is begun
-    // again after a rescale.
+    // again after a rescale, which leaves the columns that it does not move as they
+    // were.  (A column that a NaN or +inf has reached asks for none: its queries may
+    // be those of rows past the drafts, which hold anything.)
     int settled = -1;
     while (j < j_prefix) {
       float mx[NT], vm = 0.0f;
@@ -646,7 +653,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           mx[nt] = largest(sc[nt]);
-          over |= !((mx[nt] - m[nt]) * s2[nt] <= kLag);
+          over |= !(fmaf(mx[nt], s2[nt], -m[nt]) <= kLag) && m[nt] < INFINITY;
         }
         if constexpr (Q8) {
           vm = 0.0f;  // the largest finite scale
@@ -679,10 +686,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
       settled = j;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float mn = (mx[nt] - m[nt]) * s2[nt] <= kLag ? m[nt] : max_nan(m[nt], mx[nt]);
-        const float mr = mn == -INFINITY ? 0.0f : mn * s2[nt];
-        float alpha = __builtin_amdgcn_exp2f(fmaf(m[nt], s2[nt], -mr));
-        m[nt] = mn;
+        float alpha = moved(nt, mx[nt]);
         l[nt] *= alpha;
         if constexpr (Q8) {
           const float ref = vm > 4.0f * vref[nt] ? vref_of(vm) : vref[nt];
@@ -700,7 +704,6 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
     l[nt] += xor16_f(l[nt]);
     l[nt] += xor32_f(l[nt]);
     if (spoilt[nt]) l[nt] = NAN;
-    m[nt] = m[nt] == -INFINITY ? -INFINITY : m[nt] * s2[nt];
     if constexpr (Q8) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
@@ -751,7 +754,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
     }
     if (ws != 0) return;
   }
-  // the results of a column, or its split record: the maximum in base-2 units, the
+  // the results of a column, or its split record: the reference, the
   // sum and the weighted values.  A lane has dims 16 dt + 4 kq + i, or with 8 bits
   // 32 b + 8 kq + 2 i of tile 2b and the dims after those of tile 2b + 1.
 #pragma unroll
