@@ -245,7 +245,8 @@ int knj_kv_load(const knj_kv_cache* cache, int type, const int32_t* slots, int n
  *   n_rows <= n_ctx, n_rows <= 1024, scale in [1e-6, 1e6], n_head a multiple of n_head_kv
  *   and at most 1024.
  *   out may be q (with out_stride = q_stride).  On the matrix cores f32 queries, and the softmax's weights
- *   with any activations, keep 22 bits.
+ *   with any activations, keep 22 bits: with an 8-bit cache of the largest product of a
+ *   weight and a value scale, down to 2^-80 of the largest weight times the largest scale.
  * knj_attention_tree_workspace: bytes its workspace needs for these sizes (0: none,
  *   or arguments that it refuses); any contents.  Smaller sizes can need more (their
  *   slots are split further), but none more than 262144 * (head_dim + 4). */

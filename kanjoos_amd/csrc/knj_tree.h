@@ -110,6 +110,13 @@ __device__ __forceinline__ u32x2 lds_tr16_at(uint32_t p) {
 // a rescale by 2^(old - new) fits the weights on both sides, and is 1 where r stays.
 constexpr float kLift = 6.0f, kLag = 13.0f;
 
+// With 8-bit values the slot of a column's largest scale may have next to no weight, and
+// the weights that the column lives on then meet small factors: r is set further
+// below the maximum, by up to 2^80, wherever the largest product of a weight and its
+// factor would stay below 1.  (The sum of weights, in f32, has the room; the products
+// are what f16 has to hold, and are held to 65,504 from then on.)
+constexpr float kMostLift = 80.0f;
+
 // Maximum that carries a NaN (a NaN score makes its column NaN); the instruction
 // takes three, without the quieting of its inputs that fmaxf asks for.
 __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
@@ -177,7 +184,7 @@ typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 // 8-bit codes become f16 (exactly) as operands.  Their scales stay out of the
 // products: a score is multiplied by its slot's, a weight by its slot's over the
 // running largest of the scales its column has seen (a power of two, so a weight
-// stays in f16's range whatever the cache's units).  Queries are scaled by a
+// stays in f16's range whatever the cache's units; kMostLift has the other end).  Queries are scaled by a
 // power of two per row, so that f16 holds any of them.  Weights are f16 high parts and
 // remainders (22 bits) whatever the activations: 11 bits of a weight leave errors of
 // the size of an f16 output's own rounding.  SPLIT keeps f32 queries so too.
@@ -342,6 +349,8 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
 
   // (m: the references)
   float m[NT], l[NT], vref[NT];
+  float lag[Q8 ? NT : 1], top[Q8 ? NT : 1];  // kLag and the lift; a product that the column has had
+  bool lifted = false;                       // any column of the wave (uniform)
   bool spoilt[NT];
   f32x4 acc[NT][DT];
 #pragma unroll
@@ -349,6 +358,10 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
     m[nt] = -INFINITY;
     l[nt] = 0.0f;
     vref[nt] = 0.0f;
+    if constexpr (Q8) {
+      lag[nt] = kLag;
+      top[nt] = 0.0f;
+    }
     spoilt[nt] = false;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[nt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -428,39 +441,35 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
     const float2 m32 = pair32_f(mx);
     return max_nan(m32.x, m32.y);
   };
-  // Weights of a column's scores against its reference, into the values' operand; with
-  // 8 bits times w8, the slots' value scales over the column's.  Returns their sum
-  // (without those).
-  auto weights = [&](const f32x4 (&sc)[ST], float s2c, float mref, const float (&w8)[Q8 ? 4 * ST : 1], h16x8 (&eh)[NE],
-                     h16x8 (&el)[NE]) {
+  // Weights of a column's scores against its reference; with 8 bits times w8, the slots'
+  // value scales over the column's.  Returns their sum (without those).
+  auto weights = [&](const f32x4 (&sc)[ST], float s2c, float mref, const float (&w8)[Q8 ? 4 * ST : 1], float (&w)[4 * ST]) {
     // (the reference is -inf while the column has seen nothing: exponents then from 0)
     const float mr = mref == -INFINITY ? 0.0f : mref;
     float es = 0.0f;
-    float w[4 * ST];
 #pragma unroll
     for (int i = 0; i < 4 * ST; ++i) {
       w[i] = __builtin_amdgcn_exp2f(fmaf(sc[i >> 2][i & 3], s2c, -mr));
       es += w[i];
       if constexpr (Q8) {
         w[i] *= w8[i];
-        // (the weight itself, rounded to f32, is what is split below: formed anew
-        // inside the conversion to f16, the product could round the other way
+        // (the weight itself, rounded to f32, is what is split in `operand`: formed
+        // anew inside the conversion to f16, the product could round the other way
         // there than in the remainder, an f16 step off)
         asm("" : "+v"(w[i]));
       }
     }
+    return es;
+  };
+  // the same as the values' operand
+  auto operand = [&](const float (&w)[4 * ST], h16x8 (&eh)[NE], h16x8 (&el)[NE]) {
 #pragma unroll
-    for (int c = 0; c < NE; ++c) {
-      h16x8 hi, lo;
+    for (int c = 0; c < NE; ++c)
       split_h8(make_float4(w[8 * c], w[8 * c + 1], w[8 * c + 2], w[8 * c + 3]),
                SW == 16 ? make_float4(0.f, 0.f, 0.f, 0.f)
                         : make_float4(w[(8 * c + 4) % (4 * ST)], w[(8 * c + 5) % (4 * ST)], w[(8 * c + 6) % (4 * ST)],
                                       w[(8 * c + 7) % (4 * ST)]),
-               hi, lo);
-      eh[c] = hi;
-      el[c] = lo;
-    }
-    return es;
+               eh[c], el[c]);
   };
   // Values: step c covers slots 32c + 4kq + i and 32c + 16 + 4kq + i (SW 16: the
   // first).  Lane r's transposed read takes bytes 8 (r%4) .. + 7 of 32-byte pair b
@@ -525,10 +534,43 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
   auto inverse = [](float ref) { return ref > 0.0f ? __uint_as_float((254u << 23) - __float_as_uint(ref)) : 0.0f; };
   // column nt's reference moved if the largest score has passed it; the factor of what
   // was summed before
+  auto lag_of = [&](int nt) {
+    if constexpr (Q8) return lag[nt];
+    else return kLag;
+  };
   auto moved = [&](int nt, float mx) {
     const float old = m[nt];
-    if (!(fmaf(mx, s2[nt], -old) <= kLag)) m[nt] = max_nan(old, fmaf(mx, s2[nt], -kLift));
+    if (!(fmaf(mx, s2[nt], -old) <= lag_of(nt))) m[nt] = max_nan(old, fmaf(mx, s2[nt], kLag - kLift - lag_of(nt)));
     return __builtin_amdgcn_exp2f(old - (m[nt] == -INFINITY ? 0.0f : m[nt]));
+  };
+  // Largest of a column's products, and whether one is beyond f16.  (A NaN is its
+  // column's result, whatever the references.)
+  auto largest_product = [&](const float (&w)[4 * ST]) {
+    float pm = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4 * ST; i += 2) pm = max_nan(max_nan(pm, w[i]), w[i + 1]);
+    const float2 m16 = pair16_f(pm);
+    pm = max_nan(m16.x, m16.y);
+    const float2 m32 = pair32_f(pm);
+    return max_nan(m32.x, m32.y);
+  };
+  auto beyond = [](float pm) { return pm >= 65520.0f; };
+  // Whether a column's references have to move for its products: t, the largest of them
+  // as far as known (`top` before this chunk's, which are asked where that is below 1),
+  // is below 1 since they last moved, or one of this chunk's is beyond f16.
+  auto low_or_beyond = [&](float top, float pm, bool fresh, float& t) {
+    t = (fresh && !(top >= 1.0f)) || beyond(pm) ? max_nan(top, pm) : top;
+    return (fresh && t > 0.0f && t < 1.0f) || beyond(pm);
+  };
+  // Column nt's lift: the factor of what was and is summed that brings t, a product that
+  // the column has had, to between 2^6 and 2^7.
+  auto lift = [&](int nt, float t) {
+    const float e = (float)((int)(__float_as_uint(t) >> 23) - 127);
+    const float d = t < INFINITY ? fminf(fmaxf(kLift - e, kLag - lag[nt]), kMostLift + kLag - lag[nt]) : 0.0f;
+    const float old = m[nt];
+    m[nt] -= d;
+    lag[nt] += d;
+    return d == 0.0f ? 1.0f : __builtin_amdgcn_exp2f(old - m[nt]);
   };
   auto rescale = [&](int nt, float alpha) {
 #pragma unroll
@@ -554,147 +596,165 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
   const int j_prefix = min(c1, P / C);  // chunks below lie in the prefix
   ready();
   while (j < c1) {
-    // ---- the first chunk, and those that reach the drafts or the end
-    {
-      const int p0 = j * C;
-      const uint32_t at = lds0 + stage * SB;
-      const bool drafts = p0 + C > P;
-      // A draft's value row may be unseen by some columns of the tile, and rows past
-      // the drafts are seen by none: what is not finite in them would reach a column
-      // as 0 x inf, and is replaced by zeros.  Columns that see such a draft are
-      // marked and come out as NaN.  (int8 codes are finite; their scales are
-      // selected away.)
-      uint64_t bad = 0;
-      if (FORMAT != KNJ_KV_I8 && drafts) {
-        if (tid < C / 32) poison[tid] = 0u;
-        KNJ_BARRIER_AFTER(kLdsOnly);
-        for (int o = 16 * tid; o < CB; o += 16 * NTH) {
-          const int q = o / RB;
-          if (p0 + q < P) continue;
-          uint4* w = reinterpret_cast<uint4*>(lds + stage * SB + CB + o);
-          uint4 v = *w;
-          bool any = false;
-          any |= drop_nonfinite<FORMAT>(v.x);
-          any |= drop_nonfinite<FORMAT>(v.y);
-          any |= drop_nonfinite<FORMAT>(v.z);
-          any |= drop_nonfinite<FORMAT>(v.w);
-          if (!any) continue;
-          *w = v;
-          if (p0 + q < valid) atomicOr(&poison[q >> 5], 1u << (q & 31));
-        }
-        KNJ_BARRIER_AFTER(kLdsOnly);
-        bad = poison[(ws * SW) >> 5];
-        if constexpr (SW == 64) bad |= (uint64_t)poison[((ws * SW) >> 5) + 1] << 32;
-        if constexpr (SW == 16) bad = (bad >> ((ws * SW) & 31)) & 0xFFFFu;
+    // ---- the first chunk, those that reach the drafts or the end, and those of the
+    // prefix that move a reference
+    const int p0 = j * C;
+    const uint32_t at = lds0 + stage * SB;
+    const bool drafts = p0 + C > P;
+    // A draft's value row may be unseen by some columns of the tile, and rows past
+    // the drafts are seen by none: what is not finite in them would reach a column
+    // as 0 x inf, and is replaced by zeros.  Columns that see such a draft are
+    // marked and come out as NaN.  (int8 codes are finite; their scales are
+    // selected away.)
+    uint64_t bad = 0;
+    if (FORMAT != KNJ_KV_I8 && drafts) {
+      if (tid < C / 32) poison[tid] = 0u;
+      KNJ_BARRIER_AFTER(kLdsOnly);
+      for (int o = 16 * tid; o < CB; o += 16 * NTH) {
+        const int q = o / RB;
+        if (p0 + q < P) continue;
+        uint4* w = reinterpret_cast<uint4*>(lds + stage * SB + CB + o);
+        uint4 v = *w;
+        bool any = false;
+        any |= drop_nonfinite<FORMAT>(v.x);
+        any |= drop_nonfinite<FORMAT>(v.y);
+        any |= drop_nonfinite<FORMAT>(v.z);
+        any |= drop_nonfinite<FORMAT>(v.w);
+        if (!any) continue;
+        *w = v;
+        if (p0 + q < valid) atomicOr(&poison[q >> 5], 1u << (q & 31));
       }
+      KNJ_BARRIER_AFTER(kLdsOnly);
+      bad = poison[(ws * SW) >> 5];
+      if constexpr (SW == 64) bad |= (uint64_t)poison[((ws * SW) >> 5) + 1] << 32;
+      if constexpr (SW == 16) bad = (bad >> ((ws * SW) & 31)) & 0xFFFFu;
+    }
+    f32x4 sc[NT][ST];
+    float vq[Q8 ? 4 * ST : 1];
+    scores(at, sc, vq);
+    h16x8 eh[NT][NE], el[NT][NE];
+    float w[NT][4 * ST], es[NT], alpha[NT], t[Q8 ? NT : 1];
+    bool out[Q8 ? NT : 1];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      // the slots that the column sees: four bits per lane and slot tile
+      uint64_t seen = ~0ull;
+      if (drafts) seen = seen64(mask ? mask + (uint64_t)tcol[nt] * words : nullptr, words, tcol[nt], N, p0 + ws * SW - P);
+      spoilt[nt] |= (seen & bad) != 0;
+      seen >>= 4 * kq;
+      float vm = 0.0f, vin[Q8 ? 4 * ST : 1];  // value scales of the slots seen, and the largest finite one
+#pragma unroll
+      for (int st = 0; st < ST; ++st) {
+        const uint32_t four = (uint32_t)(seen >> (16 * st));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = (four & (1u << i)) != 0;
+          sc[nt][st][i] = in ? sc[nt][st][i] : -INFINITY;
+          if constexpr (Q8) {
+            vin[4 * st + i] = in ? vq[4 * st + i] : 0.0f;
+            vm = fmaxf(vm, vin[4 * st + i] < INFINITY ? vin[4 * st + i] : 0.0f);
+          }
+        }
+      }
+      const float before = m[nt];
+      alpha[nt] = moved(nt, largest(sc[nt]));
+      l[nt] *= alpha[nt];
+      bool same = true;
+      float w8[Q8 ? 4 * ST : 1];
+      if constexpr (Q8) {
+        vm = fmaxf(vm, xor16_f(vm));
+        vm = fmaxf(vm, xor32_f(vm));
+        const float ref = vm > 4.0f * vref[nt] ? vref_of(vm) : vref[nt];
+        const float inv = inverse(ref);
+        same = m[nt] == before && ref == vref[nt];
+        alpha[nt] *= vref[nt] * inv;
+        vref[nt] = ref;
+#pragma unroll
+        for (int i = 0; i < 4 * ST; ++i) w8[i] = vin[i] * inv;
+      }
+      es[nt] = weights(sc[nt], s2[nt], m[nt], w8, w[nt]);
+      if constexpr (Q8) {
+        out[nt] = low_or_beyond(top[nt] * alpha[nt], largest_product(w[nt]), !same, t[nt]);
+      }
+    }
+    if constexpr (Q8) {
+      bool any = false, any_lift = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) any |= out[nt];
+      if (__builtin_expect(__ballot(any) != 0, 0)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float f = out[nt] ? lift(nt, t[nt]) : 1.0f;
+#pragma unroll
+          for (int i = 0; i < 4 * ST; ++i) w[nt][i] *= f;
+          es[nt] *= f;
+          l[nt] *= f;
+          alpha[nt] *= f;
+          t[nt] *= f;
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        top[nt] = t[nt];
+        any_lift |= lag[nt] > kLag;
+      }
+      lifted = __ballot(any_lift) != 0;
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      l[nt] += es[nt];
+      operand(w[nt], eh[nt], el[nt]);
+      rescale(nt, alpha[nt]);
+    }
+    VPair v[NPAIR];
+#pragma unroll
+    for (int b = 0; b < NPAIR; ++b) v[b] = vread(at, 0, b);
+    values(at, v, eh, el);
+    next();
+    // ---- the chunks of the prefix: every column sees every slot.  A chunk whose
+    // scores or value scales have left the columns' references behind is done above,
+    // which leaves the columns that it does not move as they were, and so is every
+    // chunk while a column is lifted and its products have to be watched.  (A column
+    // that a NaN or +inf has reached asks for none of it: its queries may be those of
+    // rows past the drafts, which hold anything.)
+    while (j < j_prefix && !lifted) {
+      const uint32_t at = lds0 + stage * SB;
       f32x4 sc[NT][ST];
       float vq[Q8 ? 4 * ST : 1];
       scores(at, sc, vq);
-      h16x8 eh[NT][NE], el[NT][NE];
+      bool over = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        // the slots that the column sees: four bits per lane and slot tile
-        uint64_t seen = ~0ull;
-        if (drafts) seen = seen64(mask ? mask + (uint64_t)tcol[nt] * words : nullptr, words, tcol[nt], N, p0 + ws * SW - P);
-        spoilt[nt] |= (seen & bad) != 0;
-        seen >>= 4 * kq;
-        float vm = 0.0f, vin[Q8 ? 4 * ST : 1];  // value scales of the slots seen, and the largest finite one
+      for (int nt = 0; nt < NT; ++nt)
+        over |= !(fmaf(largest(sc[nt]), s2[nt], -m[nt]) <= kLag) && m[nt] < INFINITY;
+      if constexpr (Q8) {
+        float vm = 0.0f;  // the largest finite scale
 #pragma unroll
-        for (int st = 0; st < ST; ++st) {
-          const uint32_t four = (uint32_t)(seen >> (16 * st));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool in = (four & (1u << i)) != 0;
-            sc[nt][st][i] = in ? sc[nt][st][i] : -INFINITY;
-            if constexpr (Q8) {
-              vin[4 * st + i] = in ? vq[4 * st + i] : 0.0f;
-              vm = fmaxf(vm, vin[4 * st + i] < INFINITY ? vin[4 * st + i] : 0.0f);
-            }
-          }
-        }
-        const float mx = largest(sc[nt]);
-        float alpha = moved(nt, mx);
-        l[nt] *= alpha;
-        float w8[Q8 ? 4 * ST : 1];
-        if constexpr (Q8) {
-          vm = fmaxf(vm, xor16_f(vm));
-          vm = fmaxf(vm, xor32_f(vm));
-          const float ref = fmaxf(vref[nt], vref_of(vm));
-          const float inv = inverse(ref);
-          alpha *= vref[nt] * inv;
-          vref[nt] = ref;
-#pragma unroll
-          for (int i = 0; i < 4 * ST; ++i) w8[i] = vin[i] * inv;
-        }
-        l[nt] += weights(sc[nt], s2[nt], m[nt], w8, eh[nt], el[nt]);
-        rescale(nt, alpha);
+        for (int i = 0; i < 4 * ST; ++i) vm = fmaxf(vm, vq[i] < INFINITY ? vq[i] : 0.0f);
+        vm = fmaxf(vm, xor16_f(vm));
+        vm = fmaxf(vm, xor32_f(vm));
+        over |= vm > 4.0f * vref[0];
       }
+      if (__ballot(over) != 0) break;
       VPair v[NPAIR];
 #pragma unroll
       for (int b = 0; b < NPAIR; ++b) v[b] = vread(at, 0, b);
-      values(at, v, eh, el);
-    }
-    next();
-    // ---- the chunks of the prefix: every column sees every slot.  A chunk whose
-    // scores (or value scales) have left the columns' references behind is begun
-    // again after a rescale, which leaves the columns that it does not move as they
-    // were.  (A column that a NaN or +inf has reached asks for none: its queries may
-    // be those of rows past the drafts, which hold anything.)
-    int settled = -1;
-    while (j < j_prefix) {
-      float mx[NT], vm = 0.0f;
-      bool over = false;
-      for (;;) {
-        const uint32_t at = lds0 + stage * SB;
-        f32x4 sc[NT][ST];
-        float vq[Q8 ? 4 * ST : 1];
-        scores(at, sc, vq);
-        over = false;
+      float w8[Q8 ? 4 * ST : 1];
+      if constexpr (Q8) {
+        const float inv = inverse(vref[0]);  // (alike in every column)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mx[nt] = largest(sc[nt]);
-          over |= !(fmaf(mx[nt], s2[nt], -m[nt]) <= kLag) && m[nt] < INFINITY;
-        }
-        if constexpr (Q8) {
-          vm = 0.0f;  // the largest finite scale
-#pragma unroll
-          for (int i = 0; i < 4 * ST; ++i) vm = fmaxf(vm, vq[i] < INFINITY ? vq[i] : 0.0f);
-          vm = fmaxf(vm, xor16_f(vm));
-          vm = fmaxf(vm, xor32_f(vm));
-          over |= vm > 4.0f * vref[0];
-        }
-        if (j != settled && __ballot(over) != 0) break;
-        VPair v[NPAIR];
-#pragma unroll
-        for (int b = 0; b < NPAIR; ++b) v[b] = vread(at, 0, b);
-        float w8[Q8 ? 4 * ST : 1];
-        if constexpr (Q8) {
-          const float inv = inverse(vref[0]);  // (alike in every column)
-#pragma unroll
-          for (int i = 0; i < 4 * ST; ++i) w8[i] = vq[i] * inv;
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        h16x8 eh[NT][NE], el[NT][NE];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) l[nt] += weights(sc[nt], s2[nt], m[nt], w8, eh[nt], el[nt]);
-        __builtin_amdgcn_sched_barrier(0);
-        values(at, v, eh, el);
-        next();
-        if (j >= j_prefix) break;
+        for (int i = 0; i < 4 * ST; ++i) w8[i] = vq[i] * inv;
       }
-      if (j >= j_prefix) break;
-      settled = j;
+      __builtin_amdgcn_sched_barrier(0);
+      h16x8 eh[NT][NE], el[NT][NE];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float alpha = moved(nt, mx[nt]);
-        l[nt] *= alpha;
-        if constexpr (Q8) {
-          const float ref = vm > 4.0f * vref[nt] ? vref_of(vm) : vref[nt];
-          alpha *= vref[nt] * inverse(ref);
-          vref[nt] = ref;
-        }
-        rescale(nt, alpha);
+        float w[4 * ST];
+        l[nt] += weights(sc[nt], s2[nt], m[nt], w8, w);
+        operand(w, eh[nt], el[nt]);
       }
+      __builtin_amdgcn_sched_barrier(0);
+      values(at, v, eh, el);
+      next();
     }
   }
 

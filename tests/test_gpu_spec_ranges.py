@@ -75,3 +75,87 @@ def test_rows_that_are_not_drafts(device, t, fmt, nh, T):
             with np.errstate(invalid="ignore"):
                 got, _ = S.run_tree(c, t, other, T, prefixes, counts, sees, nh)
             assert np.array_equal(got[:, [0, 2]], clean[:, [0, 2]]), what
+
+
+def tree64p(q, kv, amax, prefix, sees, scale, t):
+    """Attention of full sets of drafts in float64, with a bound that weighs each slot's
+    error by its own share: a weight is off by 32 U |q||k| scale + 64 U of itself, and
+    by 2^-25 of the largest product of a share p and its row's largest magnitude
+    (`amax`), at random over the slots: six standard deviations."""
+    n, T, nh, D = q.shape
+    nk = kv[0].shape[1]
+    out, bound = np.empty(q.shape), np.empty(q.shape)
+    for s in range(n):
+        for h in range(nh):
+            kh = h * nk // nh
+            for i in range(T):
+                slots = np.concatenate([np.arange(prefix[s]), prefix[s] + np.nonzero(sees[s, i])[0]]).astype(int)
+                ks, vs = kv[0][s, kh][slots], kv[1][s, kh][slots]
+                x = scale * (ks @ q[s, i, h])
+                p = np.exp(x - x.max())
+                p /= p.sum()
+                o = p @ vs
+                off = p * (32 * U * scale * (np.abs(ks) @ np.abs(q[s, i, h])) + 64 * U)
+                out[s, i, h] = o
+                bound[s, i, h] = off @ np.abs(vs) + off.sum() * np.abs(o) + 6 * 2.0 ** -25 * np.sqrt(slots.size) * (p * amax[s, kh][slots]).max() \
+                    + HALF[t] * np.abs(o) + (2.0 ** -25 if t == F16 else 2.0 ** -126)
+    return out, bound
+
+
+def steered(rng, q, nk, P, nats, sizes, noise=0.3):
+    """Keys and values [1][P][nk][D] of P slots whose scores against every row of q are about
+    `nats` (before the 1/sqrt(D) is taken out) and whose values are about `sizes`."""
+    D = q.shape[-1]
+    u = q.mean((0, 1)).reshape(nk, -1, D).mean(1)
+    u /= (u * u).sum(-1, keepdims=True)
+    k = D ** 0.5 * np.asarray(nats)[None, :, None, None] * u + noise * rng.normal(size=(1, P, nk, D))
+    return k, rng.normal(size=(1, P, nk, D)) * np.asarray(sizes)[None, :, None, None]
+
+
+LN2 = float(np.log(2.0))
+# per slot of P: scores in nats and sizes of the values
+UNITS = {
+    "one slot of 2^16": lambda P, at: (np.where(np.arange(P) == at, -30.0, 0.0), np.where(np.arange(P) == at, 2.0 ** 16, 1.0)),
+    "one slot of 2^28": lambda P, at: (np.where(np.arange(P) == at, -40.0, 0.0), np.where(np.arange(P) == at, 2.0 ** 28, 1.0)),
+    "one slot of 2^40": lambda P, at: (np.where(np.arange(P) == at, -60.0, 0.0), np.where(np.arange(P) == at, 2.0 ** 40, 1.0)),
+    "one slot of 2^40, no weight": lambda P, at: (np.where(np.arange(P) == at, -300.0, 0.0), np.where(np.arange(P) == at, 2.0 ** 40, 1.0)),
+    "one heavy slot of 2^-30": lambda P, at: (np.where(np.arange(P) == at, 24.0, 0.0), np.where(np.arange(P) == at, 2.0 ** -30, 1.0)),
+    "shares and sizes opposed": lambda P, at: (-40 * LN2 * np.arange(P) / P, 2.0 ** (40 * np.arange(P) / P)),
+    "sizes fall twice as fast": lambda P, at: (20 * LN2 * np.arange(P) / P, 2.0 ** (-40 * np.arange(P) / P)),
+    "sizes fall, scores rise": lambda P, at: (40 * LN2 * np.arange(P) / P, 2.0 ** (-20 * np.arange(P) / P)),
+    "waves": lambda P, at: (20 * np.sin(np.arange(P) / 40), 2.0 ** (20 * np.cos(np.arange(P) / 70))),
+}
+
+
+@pytest.mark.parametrize("fmt", [K.KV_F8, K.KV_I8])
+@pytest.mark.parametrize("tile", range(len(TILES)))
+@pytest.mark.parametrize("units", list(UNITS))
+def test_units_of_values(device, fmt, tile, units):
+    """8-bit values whose scales lie far apart: what an output is made of keeps its bits
+    whatever slots of next to no weight hold, wherever they lie (the activations' types
+    in turn)."""
+    t, (nh, T, bound_p) = TYPES[(list(UNITS).index(units) + fmt + tile) % 3], TILES[tile]
+    print(f"units '{units}' type {t} format {fmt} heads {nh} drafts {T}", flush=True)
+    rng = np.random.default_rng([t, fmt, nh, T])
+    D, P = 64, 900
+    c = K.KvCache.allocate(fmt, 1, 1, max(bound_p, P) + T, D)
+    q = S.decode(S.encode(2 * rng.normal(size=D) + 0.1 * rng.normal(size=(1, T, nh, D)), t), t)
+    sees = S.tree_bits(rng, T)[None]
+    for at in (3, 200, 700, P - 1, P + T - 1) if "slot" in units else (0,):
+        nats, sizes = UNITS[units](P + T, at)
+        k, v = steered(rng, q, 1, P + T, nats, sizes)
+        kv = S.store_prefix(c, [k, v], P + T)
+        amax = np.abs(v).max(-1).transpose(0, 2, 1)
+        with np.errstate(over="ignore"):
+            got, _ = S.run_tree(c, t, q, T, [P], None, sees, nh, max_prefix=max(bound_p, P))
+            want, bound = tree64p(q, kv, amax, [P], sees, D ** -0.5, t)
+        if t == F16:
+            assert np.abs(want).max() < 65000
+        S.close(got, want, bound, f"outlier at {at}")
+        # the bits of a draft hang on nothing that its neighbours hold
+        if T > 3:
+            other = q.copy()
+            other[:, T - 1] = np.nan
+            with np.errstate(invalid="ignore"):
+                again, _ = S.run_tree(c, t, other, T, [P], None, sees, nh, max_prefix=max(bound_p, P))
+            assert np.array_equal(again[:, :T - 1], got[:, :T - 1])
