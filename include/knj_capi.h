@@ -244,6 +244,8 @@ int knj_kv_load(const knj_kv_cache* cache, int type, const int32_t* slots, int n
  *   prefix[s] is held to [0, max_prefix] and counts[s] to [0, n_rows]; max_prefix +
  *   n_rows <= n_ctx, n_rows <= 1024, scale in [1e-6, 1e6], n_head a multiple of n_head_kv
  *   and at most 1024.
+ *   Queries may be of any size that leaves the scores, scale q.k, below 2^25 in magnitude,
+ *   with scale |q| below 2^126 and 8-bit keys below 2^100.
  *   out may be q (with out_stride = q_stride).  On the matrix cores f32 queries, and the softmax's weights
  *   with any activations, keep 22 bits: with an 8-bit cache of the largest product of a
  *   weight and a value scale, down to 2^-80 of the largest weight times the largest scale.

@@ -325,9 +325,10 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
     }
     am = fmaxf(am, xor16_f(am));
     am = fmaxf(am, xor32_f(am));
-    const int e = min(max((int)(__float_as_uint(am) >> 23) - 127, -100), 100);
+    // (2^e and 2^-e both normal numbers; a factor beyond f32 is held to its largest)
+    const int e = min(max((int)(__float_as_uint(am) >> 23) - 127, -126), 126);
     const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-    s2[nt] = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + e) << 23);
+    s2[nt] = fminf(a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + e) << 23), 0x1.fffffep127f);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
       const float4 u = make_float4(x[c].x * down, x[c].y * down, x[c].z * down, x[c].w * down);

@@ -159,3 +159,26 @@ def test_units_of_values(device, fmt, tile, units):
             with np.errstate(invalid="ignore"):
                 again, _ = S.run_tree(c, t, other, T, [P], None, sees, nh, max_prefix=max(bound_p, P))
             assert np.array_equal(again[:, :T - 1], got[:, :T - 1])
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("fmt,size", [(f, z) for f in FORMATS for z in (-140, -112, -101, 30, 112, 117, 126) if f != K.KV_F16 or z <= 30])
+@pytest.mark.parametrize("nh,T,bound_p", TILES)
+def test_queries_of_any_size(device, t, fmt, nh, T, bound_p, size):
+    """Queries up to the ends of f32's range, 2^size, against keys and a scale that keep
+    the scores ordinary (of the smallest: next to nothing, every slot the same; no f16
+    keys suit the largest)."""
+    ksize = 2.0 ** (-10 if size > 0 else 0) if fmt == K.KV_F16 else 2.0 ** min(95, max(-114, -size))
+    scale = float(np.float32(min(1e6, max(1e-6, 2.0 ** -size / ksize / 8))))
+    print(f"queries of 2^{size} type {t} format {fmt} heads {nh} drafts {T}", flush=True)
+    rng = np.random.default_rng([t, fmt, nh, T, size + 200])
+    D, P = 64, 300
+    c = K.KvCache.allocate(fmt, 1, 1, max(bound_p, P) + T, D)
+    k, v = rng.normal(size=(2, 1, P + T, 1, D))
+    kv = S.store_prefix(c, [ksize * k, v], P + T)
+    q = S.decode(S.encode(np.clip(rng.normal(size=(1, T, nh, D)), -3.9, 3.9) * 2.0 ** size, t), t)
+    assert np.isfinite(q).all()
+    sees = S.tree_bits(rng, T)[None]
+    got, _ = S.run_tree(c, t, q, T, [P], None, sees, nh, max_prefix=max(bound_p, P), scale=scale)
+    want, bound = S.tree64(q, kv, [P], [T], sees, scale, F32)
+    S.close(got, want, bound + HALF[t] * np.abs(want), "queries")
