@@ -210,8 +210,8 @@ int knj_rope(int type, int layout, int n_rot, const double* inv_freq, float msca
  * knj_kv_load: slots[s][t] (NULL: slot t) of the cache into rows k and v of the
  *   same form, as code * scale rounded to `type`; rows whose slot is outside
  *   [0, n_ctx) are left as they were.  Loaded as f32 and stored again, a row keeps
- *   its codes, and its scale to a rounding: how an accepted path of drafts moves
- *   to the end of the prefix. */
+ *   its codes, and its scale to a rounding (one within a rounding of 2^-119 may come
+ *   out as zeros): how an accepted path of drafts moves to the end of the prefix. */
 #define KNJ_KV_F16 0
 #define KNJ_KV_F8 1
 #define KNJ_KV_I8 2

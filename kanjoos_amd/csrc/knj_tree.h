@@ -527,10 +527,11 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
     }
   };
   // a value scale's reference: the power of two above the largest, which a later
-  // scale may pass fourfold before it moves (weights stay up to 2^15)
+  // scale may pass fourfold before it moves (weights stay up to 2^15); 2^-126 above
+  // subnormal scales, and at most 2^126, so that its inverse is a normal number too
   auto vref_of = [](float vm) {
     const uint32_t e = __float_as_uint(vm) & 0x7F800000u;
-    return __uint_as_float(e ? e + 0x00800000u : 0u);
+    return __uint_as_float(vm > 0.0f ? min(e + 0x00800000u, 0x7E800000u) : 0u);
   };
   auto inverse = [](float ref) { return ref > 0.0f ? __uint_as_float((254u << 23) - __float_as_uint(ref)) : 0.0f; };
   // column nt's reference moved if the largest score has passed it; the factor of what
@@ -766,10 +767,12 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
     l[nt] += xor32_f(l[nt]);
     if (spoilt[nt]) l[nt] = NAN;
     if constexpr (Q8) {
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[nt][dt][i] *= vref[nt];
+      // (a scale above 1 goes into the sum's unit, 2^-k of it against a reference k
+      // higher: times the values it could pass f32)
+      const float up = fmaxf(vref[nt], 1.0f);
+      m[nt] += (float)((int)(__float_as_uint(up) >> 23) - 127);
+      l[nt] *= inverse(up);
+      rescale(nt, fminf(vref[nt], 1.0f));
     }
   }
   __builtin_amdgcn_s_waitcnt(0);  // the fetches past the range land before LDS is reused or given back

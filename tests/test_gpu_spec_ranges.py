@@ -182,3 +182,26 @@ def test_queries_of_any_size(device, t, fmt, nh, T, bound_p, size):
     got, _ = S.run_tree(c, t, q, T, [P], None, sees, nh, max_prefix=max(bound_p, P), scale=scale)
     want, bound = S.tree64(q, kv, [P], [T], sees, scale, F32)
     S.close(got, want, bound + HALF[t] * np.abs(want), "queries")
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("fmt", [K.KV_F8, K.KV_I8])
+@pytest.mark.parametrize("nh,T,bound_p", TILES + [(4, 3, 12000)])
+@pytest.mark.parametrize("low,high", [(-118.95, -117.3), (-119.0, -110.0), (90.0, 100.0), (119.0, 127.9), (-118.9, 127.9)])
+def test_values_of_any_size(device, t, fmt, nh, T, bound_p, low, high):
+    """8-bit value rows whose largest magnitudes lie between 2^low and 2^high, to both
+    ends of what a cache holds (e4m3 scales below f32's normal numbers among them)."""
+    print(f"values of 2^{low} to 2^{high} type {t} format {fmt} heads {nh} drafts {T}", flush=True)
+    rng = np.random.default_rng([t, fmt, nh, T, int(low) + 200])
+    D, P = 64, 300
+    c = K.KvCache.allocate(fmt, 1, 1, max(bound_p, P) + T, D)
+    k, v = rng.normal(size=(2, 1, P + T, 1, D))
+    v *= 2.0 ** rng.uniform(low, high, size=(1, P + T, 1, 1)) / np.abs(v).max(-1, keepdims=True)
+    v[:, 7::40] = 0
+    kv = S.store_prefix(c, [k, v], P + T)
+    assert np.all(np.abs(kv[1]).max(-1)[..., [0, 100, P]] > 0)
+    q = S.decode(S.encode(rng.normal(size=(1, T, nh, D)), t), t)
+    sees = S.tree_bits(rng, T)[None]
+    got, _ = S.run_tree(c, t, q, T, [P], None, sees, nh, max_prefix=max(bound_p, P))
+    want, bound = S.tree64(q, kv, [P], [T], sees, D ** -0.5, F32)
+    S.close(got, want, bound - 1e-37 + HALF[t] * np.abs(want) + 2.0 ** (-148 if t == F32 else -134), "values")
