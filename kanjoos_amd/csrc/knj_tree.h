@@ -212,13 +212,12 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
   constexpr int NW = WC * WS, NTH = 64 * NW, C = WS * SW, COLS = WC * NT * 16, ST = SW / 16;
   constexpr int RB = Q8 ? D : 2 * D;                     // bytes of a cache row
   constexpr int RPB = 256 / RB, NSLOT = RB / 16, NPAIR = RB / 32, CB = C * RB;
-  constexpr bool HALVES = CB / 1024 < NW;                // half of the waves fetch K, half V
-  constexpr int NI = HALVES ? 1 : CB / 1024 / NW;        // 1 KB DMA instructions per wave and matrix
+  constexpr int NI = CB / 1024 / NW;                     // 1 KB DMA instructions per wave and matrix
   constexpr int SB = 2 * CB + (Q8 ? 8 * C : 0);          // bytes of a stage: K, V, scales of both
   constexpr int DT = D / 16;                             // accumulator tiles per column tile
   constexpr int JOIN = WS > 1 ? WS / 2 * WC * NT * (DT * 1024 + 512) : 0;
   constexpr int LDS = 2 * SB > JOIN ? 2 * SB : JOIN;
-  static_assert(HALVES ? 2 * CB == 1024 * NW : CB % (1024 * NW) == 0, "whole DMA instructions");
+  static_assert(CB % (1024 * NW) == 0, "whole DMA instructions");
   static_assert(C % 32 == 0 && NW % (C / 32) == 0, "whole DMA instructions of scales");
   static_assert(SB % 256 == 0, "stages on whole rows");
   static_assert(SW == 16 || SW % 32 == 0, "16 slots, or steps of 32");
@@ -242,27 +241,25 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
   // ---- chunk j's bytes into stage `st`: wave w's instruction i fills KB i NW + w
   // of the chunk's K and of its V, whose rows share row 1024 w / RB + lane RB/16's
   // permutation (rows past the cache are its last row); with 8 bits, 64 of the scales
-  const int dw = HALVES ? wave % (NW / 2) : wave;
-  const bool dv = HALVES && wave >= NW / 2;
-  const int dq = (dw * 1024 + 16 * lane) / RB, dsl = lane % NSLOT;
+  const int dq = (wave * 1024 + 16 * lane) / RB, dsl = lane % NSLOT;
   const uint32_t koff = 16 * (dsl ^ ((dq / RPB) & (NSLOT - 1)));
   const uint32_t voff = 16 * (dsl ^ (((dq / RPB) & (NPAIR - 1)) << 1));
   auto dma = [&](int j, int st) {
     const int p0 = j * C;
-    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(lds + st * SB + dw * 1024));
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(lds + st * SB + wave * 1024));
     if (__builtin_expect(p0 + C <= n_ctx, 1)) {  // uniform
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const uint64_t at = (uint64_t)p0 * RB + i * NW * 1024;
-        if (!dv) dma16_at(kc + at, dq * RB + koff, to + i * NW * 1024);
-        if (!HALVES || dv) dma16_at(vc + at, dq * RB + voff, to + CB + i * NW * 1024);
+        dma16_at(kc + at, dq * RB + koff, to + i * NW * 1024);
+        dma16_at(vc + at, dq * RB + voff, to + CB + i * NW * 1024);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const uint64_t row = (uint64_t)min(p0 + i * (NW * 1024 / RB) + dq, n_ctx - 1) * RB;
-        if (!dv) dma16(kc + row + koff, to + i * NW * 1024);
-        if (!HALVES || dv) dma16(vc + row + voff, to + CB + i * NW * 1024);
+        dma16(kc + row + koff, to + i * NW * 1024);
+        dma16(vc + row + voff, to + CB + i * NW * 1024);
       }
     }
     if constexpr (Q8) {
