@@ -28,7 +28,9 @@ constexpr int kCand = kMaxTop * (kMaxTop + 1) / 2;  // candidates of the largest
 // going.  Calls over rows of 151,936 f32 with the 5 and the 20 largest, sixteen
 // against four: 1 row 9.9 and 11.5 against 11.6 and 16.2 us, 256 rows 37.9 and 42.2
 // against 38.5 and 44.4, 400 rows 57.4 and 63.0 against 53.3 and 59.2 (eight were
-// between the two at every count).
+// between the two at every count).  With fewer pieces than n, which only sixteen hold
+// all of for a threshold, sixteen: 1 and 500 rows of 32,000 f32 with the 20 largest 11.7
+// and 35.6 us, where taking them out of the pieces one by one was 39.4 and 108.
 constexpr int kJoinRows = 256;
 
 struct Record {
@@ -189,6 +191,7 @@ __device__ __forceinline__ void rank_keys(const unsigned long long* keys, int n,
 template <int TYPE, int W>
 __global__ __launch_bounds__(64 * W) void k_logprob_join(LogprobArgs a, int n_pieces, double c) {
   constexpr int NT = 64 * W, R = kMaxPieces > NT ? kMaxPieces / NT : 1;  // records a thread
+  constexpr bool kHoldAll = 2 * W >= kMaxTop;  // pieces, where there are fewer than n
   __shared__ __align__(16) unsigned long long keys[kMaxPieces];
   __shared__ __align__(16) unsigned long long cand[kCand];
   __shared__ unsigned long long red_key[W];
@@ -291,10 +294,39 @@ __global__ __launch_bounds__(64 * W) void k_logprob_join(LogprobArgs a, int n_pi
     if (a.logprob) a.logprob[row] = tok < 0 ? 0.0f : tok >= a.n_vocab ? NAN : logp(x_tok);
   }
   if (n == 0) return;
-  // Every one of the n largest logits is at least the n-th piece's largest: the
-  // logits that are (few more than n, as a rule) become candidates, in any order.
-  const unsigned long long least = n_pieces >= n ? keys[chosen[n - 1]] : 1ull;
-  const float least_value = n_pieces >= n ? order_value((uint32_t)(least >> 32)) : -INFINITY;
+  // Every one of the n largest logits is at least the n-th piece's largest, or with
+  // fewer pieces than n the n-th largest of the maxima of groups of lanes, 2 n to 4 n of
+  // them (the waves then hold all pieces): the logits that are (few more than n, as a
+  // rule) become candidates, in any order.
+  unsigned long long least;
+  if constexpr (kHoldAll) {
+    if (n_pieces < n) {
+      int g = 64;  // lanes of a group
+      while (g > 1 && n_pieces * (64 / g) < 2 * n) g >>= 1;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int q = h * W + wave;
+        if (q >= n_sel) break;
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) m = fmaxf(m, v[h][i]);
+        for (int o = 1; o < g; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+        const int at = (q * 64 + lane) / g;
+        if (lane % g == 0) keys[at] = ((unsigned long long)order_key(m) << 32) | (0xFFFFFFFFu - (uint32_t)at);
+      }
+      __syncthreads();
+      rank_keys<NT>(keys, n_pieces * (64 / g), [&](int i, int rank) {
+        if (rank == n - 1) red_key[0] = keys[i] >> 32 << 32;
+      });
+      __syncthreads();
+      least = red_key[0];
+    } else {
+      least = keys[chosen[n - 1]];
+    }
+  } else {
+    least = keys[chosen[n - 1]];
+  }
+  const float least_value = order_value((uint32_t)(least >> 32));
   for (int q0 = 0; q0 < n_sel; q0 += 2 * W) {
     if (q0) fetch(q0);
 #pragma unroll
@@ -365,7 +397,7 @@ hipError_t launch_token_logprobs(int type, const LogprobArgs& a, hipStream_t s) 
 #define KNJ_LOGPROBS(TYPE)                                                                            \
   do {                                                                                                \
     KNJ_LAUNCH(k_logprob_pieces<TYPE>, grid, dim3(kBlock), 0, s, a, n_pieces, c_hi, c_lo);            \
-    if (a.n_rows <= kJoinRows)                                                                        \
+    if (a.n_rows <= kJoinRows || n_pieces < a.n_top)                                                  \
       KNJ_LAUNCH((k_logprob_join<TYPE, 16>), dim3(a.n_rows), dim3(1024), 0, s, a, n_pieces, c);       \
     else                                                                                              \
       KNJ_LAUNCH((k_logprob_join<TYPE, 4>), dim3(a.n_rows), dim3(256), 0, s, a, n_pieces, c);         \

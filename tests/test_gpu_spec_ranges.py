@@ -205,3 +205,28 @@ def test_values_of_any_size(device, t, fmt, nh, T, bound_p, low, high):
     got, _ = S.run_tree(c, t, q, T, [P], None, sees, nh, max_prefix=max(bound_p, P))
     want, bound = S.tree64(q, kv, [P], [T], sees, D ** -0.5, F32)
     S.close(got, want, bound - 1e-37 + HALF[t] * np.abs(want) + 2.0 ** (-148 if t == F32 else -134), "values")
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("V,n_top", [(33, 32), (300, 2), (300, 32), (2048, 20), (2049, 3), (4097, 4), (8000, 20), (32000, 17), (32000, 32),
+                                     (2048 * 19 - 5, 20)])
+def test_largest_of_small_vocabularies(device, t, V, n_top):
+    """Fewer pieces of 2048 logits than alternatives asked for: rows in any order, with
+    ties across the threshold, with few or no tokens left, with NaN; few rows and many."""
+    print(f"small vocabulary type {t} vocab {V} top {n_top}", flush=True)
+    rng = np.random.default_rng([t, V, n_top])
+    few = np.full(V, -np.inf)
+    few[rng.permutation(V)[:n_top // 2]] = rng.normal(size=n_top // 2)
+    crowd = rng.normal(size=V)
+    crowd[V // 2:V // 2 + 2 * n_top] += 20  # next to one another
+    nan = rng.normal(size=V)
+    nan[rng.permutation(V)[:V // 3]] = np.nan
+    rows = np.stack([3 * rng.normal(size=V), np.sort(rng.normal(size=V)), np.sort(rng.normal(size=V))[::-1], np.zeros(V),
+                     rng.integers(0, 4, V), few, crowd, nan, np.full(V, -np.inf), np.sort(rng.integers(0, 2, V))])
+    raw = S.encode(rows, t)
+    tokens = rng.integers(0, V, len(rows))
+    S.check_logprobs(S.decode(raw, t), raw, t, tokens, n_top, 1.0)
+    pick = rng.integers(0, len(rows), 300)
+    a, b = S.run_logprobs(raw, t, V, tokens, n_top, 1.0), S.run_logprobs(raw[pick], t, V, tokens[pick], n_top, 1.0)
+    for x, y in zip(a, b):
+        np.testing.assert_array_equal(y, x[pick])
