@@ -48,7 +48,8 @@ __device__ __forceinline__ void st4(void* p, uint64_t i, float4 v) {
 // and sin of the row's angles are formed once per workgroup: the product
 // pos * f and its reduction to [-pi, pi] in f64 (an f32 product is off by
 // pos * 2^-24 radians, 0.06 at a million), the functions in f32 on the reduced
-// angle.
+// angle's f32 part a, with its remainder d (up to 2^-23, which alone would cost an
+// angle near pi a bit) by cos(a + d) = cos a - d sin a, sin(a + d) = sin a + d cos a.
 //
 // Bound by memory: 4000 rows of 36 f32 heads of 128 (147 MB in and out) 30.9 us a call,
 // 4.8 TB/s, where a large copy reaches 5.1.  One row is a launch: 2.1 us on the chip.
@@ -80,10 +81,11 @@ __global__ __launch_bounds__(kBlock) void k_rope(RopeArgs a) {
     const double n = rint(t * 0.15915494309189535);            // turns
     double r = fma(-n, 6.283185307179586, t);                   // 2 pi in two parts
     r = fma(-n, 2.4492935982947064e-16, r);
+    const float near = (float)r, d = (float)(r - (double)near);
     float s, co;
-    sincosf((float)r, &s, &co);
-    cs[threadIdx.x] = co * a.mscale;
-    sn[threadIdx.x] = s * a.mscale;
+    sincosf(near, &s, &co);
+    cs[threadIdx.x] = fmaf(-d, s, co) * a.mscale;
+    sn[threadIdx.x] = fmaf(d, co, s) * a.mscale;
   }
   float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w;
   ss = group_sum<T>(ss);

@@ -230,3 +230,30 @@ def test_largest_of_small_vocabularies(device, t, V, n_top):
     a, b = S.run_logprobs(raw, t, V, tokens, n_top, 1.0), S.run_logprobs(raw[pick], t, V, tokens[pick], n_top, 1.0)
     for x, y in zip(a, b):
         np.testing.assert_array_equal(y, x[pick])
+
+
+@pytest.mark.parametrize("layout", [K.ROPE_HALF, K.ROPE_INTERLEAVED])
+def test_rotation_near_the_axes(device, layout):
+    """Angles next to multiples of pi/2, where one of cos and sin is all remainder: the
+    pair (1, 0) turned by angles that no f32 holds comes out with the f32 functions'
+    own error (2 U relative, a step) and the remainder's two roundings (2 U more),
+    not with the angle's rounding (up to 2^-23 whatever the result)."""
+    D = 128
+    rng = np.random.default_rng(layout)
+    pos = np.array([1, 3, 1000, 77777, 1 << 20])
+    k = rng.integers(1, 9, D // 2)
+    for p in pos:
+        angle = k * (np.pi / 2) + rng.uniform(-1, 1, D // 2) * 10.0 ** rng.uniform(-6, -0.5, D // 2)
+        inv = angle / p  # (f64: p * inv is the angle to 2^-52)
+        x = np.zeros((1, 1, D), np.float32)
+        if layout == K.ROPE_HALF:
+            x[..., :D // 2] = 1
+        else:
+            x[..., 0::2] = 1
+        out = K.DeviceBuffer(x.nbytes)
+        K.rope(F32, S.put(x), None, S.i32([p]), S.put(inv), 1, 1, 0, D, q_out=out, layout=layout)
+        y = out.download(np.float32).astype(np.float64)
+        c, s = (y[:D // 2], y[D // 2:]) if layout == K.ROPE_HALF else (y[0::2], y[1::2])
+        th = p * inv
+        for got, want, what in ((c, np.cos(th), "cos"), (s, np.sin(th), "sin")):
+            S.close(got, want, 4 * U * np.abs(want) + 1e-14, f"{what} at {p}")
