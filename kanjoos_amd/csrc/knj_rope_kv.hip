@@ -90,7 +90,21 @@ __global__ __launch_bounds__(kBlock) void k_rope(RopeArgs a) {
   float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w;
   ss = group_sum<T>(ss);
   if (nw) {
-    const float g = 1.0f / sqrtf(ss / (float)D + a.eps);
+    float g = 1.0f / sqrtf(ss / (float)D + a.eps);
+    // (squares beyond f32, or lost below it: again with the head's largest near 1)
+    const bool far = !(ss <= 0x1p100f) || ss < 0x1p-60f;
+    if (__builtin_expect(__ballot(far) != 0, 0)) {
+      float am = fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))),
+                       fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+      am = group_max<T>(am);
+      const int e = far ? min(max((int)(__float_as_uint(am) >> 23) - 127, -126), 126) : 0;
+      const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+      x = make_float4(x.x * down, x.y * down, x.z * down, x.w * down);
+      y = make_float4(y.x * down, y.y * down, y.z * down, y.w * down);
+      ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w;
+      ss = group_sum<T>(ss);
+      if (far) g = (float)(1.0 / sqrt((double)ss / D + ldexp((double)a.eps, -2 * e)));
+    }
     x = make_float4(x.x * g * wx.x, x.y * g * wx.y, x.z * g * wx.z, x.w * g * wx.w);
     y = make_float4(y.x * g * wy.x, y.y * g * wy.y, y.z * g * wy.z, y.w * g * wy.w);
   }

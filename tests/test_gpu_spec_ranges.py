@@ -257,3 +257,28 @@ def test_rotation_near_the_axes(device, layout):
         th = p * inv
         for got, want, what in ((c, np.cos(th), "cos"), (s, np.sin(th), "sin")):
             S.close(got, want, 4 * U * np.abs(want) + 1e-14, f"{what} at {p}")
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("D,n_rot", [(128, 128), (64, 24)])
+@pytest.mark.parametrize("eps", [1e-6, 0.0])
+def test_norms_of_any_size(device, t, D, n_rot, eps):
+    """Heads whose squares f32 does not hold, beside ordinary ones: normalised all the same."""
+    rng = np.random.default_rng([t, D, n_rot])
+    sizes = [0, 66, 100, 125, -20, 0, -66, -100, -130]
+    rows, nh, nk = len(sizes), 9, 3
+    x = np.clip(rng.normal(size=(rows, nh + nk, D)), -3.9, 3.9) * 2.0 ** np.array(sizes)[:, None, None]
+    x[:, 1::4] = np.clip(rng.normal(size=x[:, 1::4].shape), -3.9, 3.9)
+    raw = S.encode(x.reshape(rows, -1), t)
+    x = S.decode(raw, t).reshape(x.shape)
+    w = [(1 + 0.1 * rng.normal(size=D)).astype(np.float32) for _ in range(2)]
+    inv, ms = K.rope_freqs(n_rot, 1e6)
+    pos = rng.integers(0, 40000, rows)
+    buf, stride = S.put(raw), (nh + nk) * D
+    K.rope(t, buf.ptr, buf.ptr + nh * D * raw.itemsize, S.i32(pos), S.put(inv), rows, nh, nk, D, n_rot=n_rot, q_norm=S.put(w[0]),
+           k_norm=S.put(w[1]), eps=eps, q_stride=stride, k_stride=stride)
+    got = S.decode(buf.download(S.np_type(t), raw.size), t).reshape(x.shape)
+    eps = float(np.float32(eps))
+    for part, wt in ((slice(0, nh), w[0].astype(np.float64)), (slice(nh, None), w[1].astype(np.float64))):
+        want = S.rope64(x[:, part], wt, pos, inv, ms, n_rot, K.ROPE_HALF, eps)
+        S.close(got[:, part], want, S.rope_bound(want, x[:, part], wt, ms, t, eps), "norms")
