@@ -164,7 +164,7 @@ int knj_attention_step(const float* q, const float* k, const float* v, const flo
 
 /* knj_rope: every head of rows q [n_rows][n_head][head_dim] (and k
  *   [n_rows][n_head_kv][head_dim]; n_head_kv 0: none) RMS-normalised with its
- *   norm weight (NULL: not) and rotated at position pos[row]: the first n_rot
+ *   norm weight (NULL: not; eps at least 0) and rotated at position pos[row]: the first n_rot
  *   dims (a multiple of 8) in pairs (i, i + n_rot/2) (KNJ_ROPE_HALF) or
  *   (2i, 2i + 1) (KNJ_ROPE_INTERLEAVED) by the angle pos * inv_freq[i], cos and
  *   sin times mscale; the other dims pass.  Angles are formed in f64 (the decode

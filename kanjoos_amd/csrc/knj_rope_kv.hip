@@ -432,6 +432,7 @@ int knj_rope(int type, int layout, int n_rot, const double* inv_freq, float msca
                     (n_head_kv == 0 || (rows_aligned(k, k_stride, eb) && rows_aligned(k_out, k_out_stride, eb))),
                 "rows must start on 16-byte boundaries");
   KNJ_CHECK_ARG(mscale > 0.0f && std::isfinite(mscale), "mscale must be finite and positive");
+  KNJ_CHECK_ARG((!q_norm && !k_norm) || (eps >= 0.0f && std::isfinite(eps)), "eps must be finite and not negative");
   const int rc = require_device();
   if (rc || n_rows == 0) return rc;
   RopeArgs a{q, k, q_out, k_out, q_stride, k_stride, q_out_stride, k_out_stride, q_norm, k_norm,
