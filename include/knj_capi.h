@@ -169,7 +169,8 @@ int knj_attention_step(const float* q, const float* k, const float* v, const flo
  *   (2i, 2i + 1) (KNJ_ROPE_INTERLEAVED) by the angle pos * inv_freq[i], cos and
  *   sin times mscale; the other dims pass.  Angles are formed in f64 (the decode
  *   step's own tables hold f32 angles: they part by up to pos * 2^-24 radians).
- *   An output may be its own input (the same pointer and stride).  n_rows < 2^24.
+ *   An output may be its own input (the same pointer and stride; another stride is
+ *   refused) and overlaps no other row.  n_rows < 2^24.
  * knj_rope_freqs (host only): the n_rot/2 frequencies base^(-2i/n_rot) under a
  *   scaling for contexts `factor` (>= 1) times orig_ctx, to be copied to the
  *   device, and mscale.  KNJ_ROPE_LINEAR: / factor.  KNJ_ROPE_NTK: base times
@@ -246,9 +247,10 @@ int knj_kv_load(const knj_kv_cache* cache, int type, const int32_t* slots, int n
  *   and at most 1024.
  *   Queries may be of any size that leaves the scores, scale q.k, below 2^25 in magnitude,
  *   with scale |q| below 2^126 and 8-bit keys below 2^100.
- *   out may be q (with out_stride = q_stride).  On the matrix cores f32 queries, and the softmax's weights
- *   with any activations, keep 22 bits: with an 8-bit cache of the largest product of a
- *   weight and a value scale, down to 2^-80 of the largest weight times the largest scale.
+ *   out may be q (with out_stride = q_stride; another is refused) and overlaps nothing
+ *   else.  On the matrix cores f32 queries, and the softmax's weights with any
+ *   activations, keep 22 bits: with an 8-bit cache of the largest product of a weight and
+ *   a value scale, down to 2^-80 of the largest weight times the largest scale.
  * knj_attention_tree_workspace: bytes its workspace needs for these sizes (0: none,
  *   or arguments that it refuses); any contents.  Smaller sizes can need more (their
  *   slots are split further), but none more than 262144 * (head_dim + 4). */

@@ -431,6 +431,9 @@ int knj_rope(int type, int layout, int n_rot, const double* inv_freq, float msca
   KNJ_CHECK_ARG(rows_aligned(q, q_stride, eb) && rows_aligned(q_out, q_out_stride, eb) &&
                     (n_head_kv == 0 || (rows_aligned(k, k_stride, eb) && rows_aligned(k_out, k_out_stride, eb))),
                 "rows must start on 16-byte boundaries");
+  KNJ_CHECK_ARG(n_rows <= 1 || ((q != q_out || q_stride == q_out_stride) &&
+                                (n_head_kv == 0 || k != k_out || k_stride == k_out_stride)),
+                "an output in place takes its input's stride");
   KNJ_CHECK_ARG(mscale > 0.0f && std::isfinite(mscale), "mscale must be finite and positive");
   KNJ_CHECK_ARG((!q_norm && !k_norm) || (eps >= 0.0f && std::isfinite(eps)), "eps must be finite and not negative");
   const int rc = require_device();
@@ -501,6 +504,8 @@ int knj_attention_tree(const knj_kv_cache* cache, int type, const void* q, uint6
   KNJ_CHECK_ARG(q_stride >= width && out_stride >= width, "a row stride is below the row's width");
   KNJ_CHECK_ARG(rows_aligned(q, q_stride, eb) && rows_aligned(out, out_stride, eb),
                 "rows must start on 16-byte boundaries");
+  KNJ_CHECK_ARG(q != out || q_stride == out_stride || (uint64_t)cache->n_seq * n_rows <= 1,
+                "an output in place takes its input's stride");
   const uint64_t need = n_rows ? tree_partial_bytes(*cache, type, n_head, n_rows, max_prefix) : 0;
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) {
     set_error("knj_attention_tree: these sizes need a 16-byte aligned workspace of " + std::to_string(need) + " bytes");

@@ -15,3 +15,16 @@ def test_rope_eps(eps):
         refused(lambda: K.rope(F32, A, A, A, A, 4, 8, 1, 128, eps=eps, **norms), "eps")
     if K.lib().knj_synchronize() != K.KNJ_OK:  # (no GPU: the next check is the device's)
         refused(lambda: K.rope(F32, A, A, A, A, 4, 8, 1, 128, eps=eps), "not open", K.KNJ_E_STATE)
+
+
+def test_in_place_with_another_stride():
+    """Rows written over rows that are still to be read."""
+    a = dict(type_id=F32, q=A, k=2 * A, pos=A, inv_freq=A, n_rows=4, n_head=8, n_head_kv=1, head_dim=128)
+    refused(lambda: K.rope(**{**a, "q_out": A, "q_stride": 1536}), "in place")  # (q_out_stride defaults to packed rows)
+    refused(lambda: K.rope(**{**a, "k_out": 2 * A, "k_stride": 1536, "k_out_stride": 256}), "in place")
+    c = cache(n_ctx=200)
+    for n_seq, n_rows in ((2, 1), (1, 3)):
+        c = cache(n_ctx=200, n_seq=n_seq)
+        refused(lambda: K.attention_tree(c, F32, A, A, 32, n_rows, A, 100, q_stride=5120), "in place")
+    if K.lib().knj_synchronize() != K.KNJ_OK:  # one row has no other to overwrite
+        refused(lambda: K.rope(**{**a, "q_out": A, "q_stride": 1536, "n_rows": 1}), "not open", K.KNJ_E_STATE)
