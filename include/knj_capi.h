@@ -243,7 +243,7 @@ int knj_kv_load(const knj_kv_cache* cache, int type, const int32_t* slots, int n
  *   gives zeros; rows past counts[s] are left as they were.  A draft that sees a
  *   draft whose value row holds an infinity or a NaN gives NaN (all of its dims).
  *   prefix[s] is held to [0, max_prefix] and counts[s] to [0, n_rows]; max_prefix +
- *   n_rows <= n_ctx, n_rows <= 1024, scale in [1e-6, 1e6], n_head a multiple of n_head_kv
+ *   n_rows <= n_ctx and below 2^31 - 256, n_rows <= 1024, scale in [1e-6, 1e6], n_head a multiple of n_head_kv
  *   and at most 1024.
  *   Queries may be of any size that leaves the scores, scale q.k, below 2^25 in magnitude,
  *   with scale |q| below 2^126 and 8-bit keys below 2^100.

@@ -483,6 +483,10 @@ int knj_kv_load(const knj_kv_cache* cache, int type, const int32_t* slots, int n
   return KNJ_OK;
 }
 
+// Slots of a sequence that the attention numbers in 32 bits, with the chunk that is
+// fetched past the last one.
+static constexpr int64_t kMaxSlots = 0x7FFFFFFF - 256;
+
 int knj_attention_tree(const knj_kv_cache* cache, int type, const void* q, uint64_t q_stride,
                        int n_head, int n_rows, const int32_t* prefix, int max_prefix,
                        const int32_t* counts, const uint64_t* mask, int mask_shared, float scale,
@@ -498,6 +502,7 @@ int knj_attention_tree(const knj_kv_cache* cache, int type, const void* q, uint6
                 "n_head must be a positive multiple of n_head_kv, at most 1024");
   KNJ_CHECK_ARG(max_prefix >= 0 && (int64_t)max_prefix + n_rows <= cache->n_ctx,
                 "max_prefix and the drafts must fit into n_ctx");
+  KNJ_CHECK_ARG((int64_t)max_prefix + n_rows <= kMaxSlots, "max_prefix and the drafts must stay below 2^31 - 256");
   KNJ_CHECK_ARG(scale >= 1e-6f && scale <= 1e6f, "the scale must be in [1e-6, 1e6]");
   KNJ_CHECK_ARG((uint64_t)cache->n_seq * n_rows * n_head < (1ull << 31), "too many rows for one call");
   const uint64_t width = (uint64_t)n_head * cache->head_dim;
@@ -521,7 +526,7 @@ int knj_attention_tree(const knj_kv_cache* cache, int type, const void* q, uint6
 
 uint64_t knj_attention_tree_workspace(const knj_kv_cache* cache, int n_head, int n_rows, int max_prefix) {
   if (check_kv_cache(cache) || n_head <= 0 || n_head > 1024 || n_head % cache->n_head_kv || n_rows <= 0 ||
-      n_rows > 1024 || max_prefix < 0 || (int64_t)max_prefix + n_rows > cache->n_ctx)
+      n_rows > 1024 || max_prefix < 0 || (int64_t)max_prefix + n_rows > std::min<int64_t>(cache->n_ctx, kMaxSlots))
     return 0;
   // (enough for every type)
   return std::max(tree_partial_bytes(*cache, KNJ_TYPE_F32, n_head, n_rows, max_prefix),

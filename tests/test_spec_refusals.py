@@ -28,3 +28,14 @@ def test_in_place_with_another_stride():
         refused(lambda: K.attention_tree(c, F32, A, A, 32, n_rows, A, 100, q_stride=5120), "in place")
     if K.lib().knj_synchronize() != K.KNJ_OK:  # one row has no other to overwrite
         refused(lambda: K.rope(**{**a, "q_out": A, "q_stride": 1536, "n_rows": 1}), "not open", K.KNJ_E_STATE)
+
+
+def test_attention_tree_slot_limit():
+    """Slots are numbered in 32 bits, with a chunk that is fetched past the last one."""
+    c = cache(n_ctx=2 ** 31 - 1, n_seq=1, n_head_kv=1, head_dim=64)
+    most = 2 ** 31 - 1 - 256
+    for n_rows in (1, 1000):
+        assert 0 < K.attention_tree_workspace(c, 8, n_rows, most - n_rows) <= 262144 * 68
+        for over in (1, 200, 256):
+            assert K.attention_tree_workspace(c, 8, n_rows, most - n_rows + over) == 0
+            refused(lambda: K.attention_tree(c, F32, A, A, 8, n_rows, A, most - n_rows + over), "2\\^31")
