@@ -160,7 +160,7 @@ int knj_attention_step(const float* q, const float* k, const float* v, const flo
  * one (KNJ_E_STATE otherwise).  `type` is that of the activations: KNJ_TYPE_F32,
  * KNJ_TYPE_F16 or KNJ_TYPE_BF16; arithmetic is f32 (angles f64), rounded once.
  * Rows of activations and caches start on 16-byte boundaries, their strides
- * count elements; anything else is refused.  head_dim is 64 or 128. */
+ * count elements, other arrays are aligned to their types; anything else is refused.  head_dim is 64 or 128. */
 
 /* knj_rope: every head of rows q [n_rows][n_head][head_dim] (and k
  *   [n_rows][n_head_kv][head_dim]; n_head_kv 0: none) RMS-normalised with its

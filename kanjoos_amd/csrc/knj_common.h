@@ -49,6 +49,11 @@ inline int act_bytes(int type) {
 inline bool rows_aligned(const void* p, uint64_t stride, int elem_bytes) {
   return ((uintptr_t)p & 15) == 0 && (stride * (uint64_t)elem_bytes & 15) == 0;
 }
+// Arrays of 32-bit values that a kernel reads or writes one by one.
+template <class... P>
+inline bool words_aligned(const P*... p) {
+  return (((uintptr_t)p | ...) & 3) == 0;
+}
 // KNJ_E_ARG, with the reason, for a cache description that is not one.
 int check_kv_cache(const knj_kv_cache* c);
 

@@ -419,6 +419,7 @@ int knj_rope(int type, int layout, int n_rot, const double* inv_freq, float msca
   KNJ_CHECK_ARG(inv_freq && pos && q && q_out, "null pointer");
   KNJ_CHECK_ARG(((uintptr_t)inv_freq & 7) == 0 && (((uintptr_t)q_norm | (uintptr_t)k_norm) & 15) == 0,
                 "inv_freq must be 8-byte and the norm weights 16-byte aligned");
+  KNJ_CHECK_ARG(words_aligned(pos), "pos must be aligned to its type");
   KNJ_CHECK_ARG(n_rows >= 0, "negative row count");
   KNJ_CHECK_ARG(n_rows < (1 << 24), "too many rows for one call");  // (a grid holds 2^32 threads a dim)
   KNJ_CHECK_ARG(n_head > 0 && n_head <= 4096 && n_head_kv >= 0 && n_head_kv <= 4096,
@@ -465,6 +466,7 @@ int knj_kv_store(const knj_kv_cache* cache, int type, const void* k, const void*
   int rc = check_kv_rows(cache, type, k, v, row_stride, n_rows);
   if (rc) return rc;
   KNJ_CHECK_ARG(start, "null start");
+  KNJ_CHECK_ARG(words_aligned(start, counts), "start and counts must be aligned to their type");
   rc = require_device();
   if (rc || n_rows == 0) return rc;
   KvRowsArgs a{with_stride(*cache), const_cast<void*>(k), const_cast<void*>(v), row_stride, start, counts, n_rows};
@@ -476,6 +478,7 @@ int knj_kv_load(const knj_kv_cache* cache, int type, const int32_t* slots, int n
                 void* v, uint64_t row_stride, void* stream) {
   int rc = check_kv_rows(cache, type, k, v, row_stride, n_rows);
   if (rc) return rc;
+  KNJ_CHECK_ARG(words_aligned(slots), "slots must be aligned to their type");
   rc = require_device();
   if (rc || n_rows == 0) return rc;
   KvRowsArgs a{with_stride(*cache), k, v, row_stride, slots, nullptr, n_rows};
@@ -497,6 +500,7 @@ int knj_attention_tree(const knj_kv_cache* cache, int type, const void* q, uint6
   const int eb = act_bytes(type);
   KNJ_CHECK_ARG(eb, "activations must be F32, F16 or BF16");
   KNJ_CHECK_ARG(q && out && prefix, "null pointer");
+  KNJ_CHECK_ARG(words_aligned(prefix, counts) && ((uintptr_t)mask & 7) == 0, "prefix, counts and mask must be aligned to their types");
   KNJ_CHECK_ARG(n_rows >= 0 && n_rows <= 1024, "n_rows must be in [0, 1024]");
   KNJ_CHECK_ARG(n_head > 0 && n_head <= 1024 && n_head % cache->n_head_kv == 0,
                 "n_head must be a positive multiple of n_head_kv, at most 1024");

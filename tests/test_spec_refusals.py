@@ -39,3 +39,20 @@ def test_attention_tree_slot_limit():
         for over in (1, 200, 256):
             assert K.attention_tree_workspace(c, 8, n_rows, most - n_rows + over) == 0
             refused(lambda: K.attention_tree(c, F32, A, A, 8, n_rows, A, most - n_rows + over), "2\\^31")
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_misaligned_arrays(off):
+    """Lengths, slots, masks and outputs off their types' boundaries (a scalar load
+    would drop the address's low bits)."""
+    bad, c = A + off, cache(n_ctx=200)
+    refused(lambda: K.rope(F32, A, A, bad, A, 4, 8, 1, 128), "pos must")
+    refused(lambda: K.kv_store(c, F32, A, A, bad, 1), "start")
+    refused(lambda: K.kv_store(c, F32, A, A, A, 1, counts=bad), "counts")
+    refused(lambda: K.kv_load(c, F32, A, A, 1, slots=bad), "slots")
+    refused(lambda: K.attention_tree(c, F32, A, 2 * A, 32, 1, bad, 100), "prefix")
+    refused(lambda: K.attention_tree(c, F32, A, 2 * A, 32, 1, A, 100, counts=bad), "counts")
+    refused(lambda: K.attention_tree(c, F32, A, 2 * A, 32, 1, A, 100, mask=A + 4), "mask")
+    for kw in (dict(tokens=bad, logprob=A), dict(tokens=A, logprob=bad), dict(entropy=bad), dict(n_top=2, top_idx=bad, top_logprob=A),
+               dict(n_top=2, top_idx=A, top_logprob=bad)):
+        refused(lambda: K.token_logprobs(F32, A, 7, 1000, None, **kw), "aligned")
