@@ -110,21 +110,28 @@ struct Planned {
   int cols;  // columns of a tile
 };
 
-// Tiles of 32 columns (16 where there are no more) finish a chunk soonest; wider
-// ones read and decode the cache for more columns at once and win when there is
-// work enough for every wave (64 drafts x 8 heads at 32K slots: 64 us with 128
-// columns, 81 with 32; at 4K slots 30 and 25; 25 drafts over 4K 25.7 and 21.5).
-// Two workgroups a CU where each then has several chunks, else one, with fewer
-// records to merge (16 drafts x 8 heads over 16K slots 22.3 against 25.0 us, over
-// 4K 15.0 against 14.2).
-constexpr int64_t kWideWork = 10000, kTwoWork = 2500;  // chunks of 32-column tiles, chunks of tiles
+// Tiles of 32 columns (16 where there are no more) finish a chunk soonest; wider ones
+// read and decode the cache for more columns at once and win when there is work enough
+// for every wave, counted in chunks of 32-column tiles.  Wide against narrow over e4m3,
+// 16-bit queries: 64 drafts x 8 heads a kv head at 8,064, 12,096 and 16,064 chunks 40.0,
+// 46.9 and 54.8 against 36.4, 48.8 and 59.5 us, 32 sequences of 8 drafts at 8,448 and
+// 12,032 40.3 and 48.0 against 39.0 and 49.4 (int8 with f32 queries crosses there too);
+// over f16, where nothing is decoded, 64 drafts at 12,096 and 16,064 38.8 and 44.4
+// against 37.4 and 45.1, 25 at 14,028 and 28,028 43.5 and 69.0 against 40.9 and 72.3
+// (with f32 queries between 12,000, for many sequences, and 30,000, for one).
+// Two workgroups a CU where each then has several chunks, else one, with fewer records
+// to merge: two against one for 16 drafts x 8 heads over 8,000, 12,000 and 16,000 f16
+// slots (2,016, 3,008 and 4,016 chunks of tiles) 16.0, 18.3 and 20.6 against 15.6, 19.1
+// and 22.2 us, over int8 with f32 queries 21.8, 25.4 and 29.5 against 22.5, 28.2 and 34.0;
+// 4 drafts over 8,000 f16 slots (504) 16.8 against 12.5.
+constexpr int64_t kWideWork = 10000, kWideWorkF16 = 16000, kTwoWork = 2500;  // chunks of 32-column tiles, chunks of tiles
 
 Planned plan(const knj_kv_cache& c, int type, int n_head, int n_rows, int max_prefix) {
   const int group = n_head / c.n_head_kv, n_cols = n_rows * group;
   const int chunks = (max_prefix + n_rows + kTreeChunk - 1) / kTreeChunk;
   const int64_t units = (int64_t)c.n_seq * c.n_head_kv;
   int cols = n_cols <= 16 ? 16 : 32;
-  if (n_cols > 32 && units * ((n_cols + 31) / 32) * chunks >= kWideWork)
+  if (n_cols > 32 && units * ((n_cols + 31) / 32) * chunks >= (c.format == KNJ_KV_F16 ? kWideWorkF16 : kWideWork))
     cols = n_cols <= 64 || type == KNJ_TYPE_F32 ? 64 : 128;
   const int tiles = (n_cols + cols - 1) / cols;
   const int64_t wgs = units * tiles * chunks >= kTwoWork ? 512 : 256;

@@ -15,7 +15,7 @@ U, HALF, TYPES, FORMATS = S.U, S.HALF, S.TYPES, S.FORMATS
 
 
 # (query heads of the one kv head, drafts, bound on the prefix): tiles of 16, 32, 64 and 128 columns
-TILES = [(4, 3, 300), (8, 4, 300), (16, 4, 320000), (16, 8, 320000)]
+TILES = [(4, 3, 300), (8, 4, 300), (16, 4, 640000), (16, 8, 640000)]
 
 
 @pytest.mark.parametrize("t", [F16, BF16])
