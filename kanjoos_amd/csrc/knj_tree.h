@@ -634,6 +634,11 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
     h16x8 eh[NT][NE], el[NT][NE];
     float w[NT][4 * ST], es[NT], alpha[NT], t[Q8 ? NT : 1];
     bool out[Q8 ? NT : 1];
+    auto add = [&](int nt) {
+      l[nt] += es[nt];
+      operand(w[nt], eh[nt], el[nt]);
+      rescale(nt, alpha[nt]);
+    };
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       // the slots that the column sees: four bits per lane and slot tile
@@ -672,9 +677,8 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
         for (int i = 0; i < 4 * ST; ++i) w8[i] = vin[i] * inv;
       }
       es[nt] = weights(sc[nt], s2[nt], m[nt], w8, w[nt]);
-      if constexpr (Q8) {
-        out[nt] = low_or_beyond(top[nt] * alpha[nt], largest_product(w[nt]), !same, t[nt]);
-      }
+      if constexpr (Q8) out[nt] = low_or_beyond(top[nt] * alpha[nt], largest_product(w[nt]), !same, t[nt]);
+      else add(nt);
     }
     if constexpr (Q8) {
       bool any = false, any_lift = false;
@@ -698,12 +702,8 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
         any_lift |= lag[nt] > kLag;
       }
       lifted = __ballot(any_lift) != 0;
-    }
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      l[nt] += es[nt];
-      operand(w[nt], eh[nt], el[nt]);
-      rescale(nt, alpha[nt]);
+      for (int nt = 0; nt < NT; ++nt) add(nt);
     }
     VPair v[NPAIR];
 #pragma unroll
@@ -711,49 +711,65 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
     values(at, v, eh, el);
     next();
     // ---- the chunks of the prefix: every column sees every slot.  A chunk whose
-    // scores or value scales have left the columns' references behind is done above,
-    // which leaves the columns that it does not move as they were, and so is every
-    // chunk while a column is lifted and its products have to be watched.  (A column
-    // that a NaN or +inf has reached asks for none of it: its queries may be those of
-    // rows past the drafts, which hold anything.)
+    // scores or value scales have left the columns' references behind is with 8 bits
+    // done above, as is every chunk while a column is lifted and its products have to
+    // be watched; over f16 it is begun again after a rescale.  Either leaves the columns
+    // that it does not move as they were.  (A column that a NaN or +inf has reached
+    // asks for none of it: its queries may be those of rows past the drafts, which
+    // hold anything.)
+    int settled = -1;
     while (j < j_prefix && !lifted) {
-      const uint32_t at = lds0 + stage * SB;
-      f32x4 sc[NT][ST];
-      float vq[Q8 ? 4 * ST : 1];
-      scores(at, sc, vq);
-      bool over = false;
+      float mx[NT];
+      for (;;) {
+        const uint32_t at = lds0 + stage * SB;
+        f32x4 sc[NT][ST];
+        float vq[Q8 ? 4 * ST : 1];
+        scores(at, sc, vq);
+        bool over = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        over |= !(fmaf(largest(sc[nt]), s2[nt], -m[nt]) <= kLag) && m[nt] < INFINITY;
-      if constexpr (Q8) {
-        float vm = 0.0f;  // the largest finite scale
+        for (int nt = 0; nt < NT; ++nt) {
+          mx[nt] = largest(sc[nt]);
+          over |= !(fmaf(mx[nt], s2[nt], -m[nt]) <= kLag) && m[nt] < INFINITY;
+        }
+        if constexpr (Q8) {
+          float vm = 0.0f;  // the largest finite scale
 #pragma unroll
-        for (int i = 0; i < 4 * ST; ++i) vm = fmaxf(vm, vq[i] < INFINITY ? vq[i] : 0.0f);
-        vm = fmaxf(vm, xor16_f(vm));
-        vm = fmaxf(vm, xor32_f(vm));
-        over |= vm > 4.0f * vref[0];
+          for (int i = 0; i < 4 * ST; ++i) vm = fmaxf(vm, vq[i] < INFINITY ? vq[i] : 0.0f);
+          vm = fmaxf(vm, xor16_f(vm));
+          vm = fmaxf(vm, xor32_f(vm));
+          over |= vm > 4.0f * vref[0];
+        }
+        if ((Q8 || j != settled) && __ballot(over) != 0) break;
+        VPair v[NPAIR];
+#pragma unroll
+        for (int b = 0; b < NPAIR; ++b) v[b] = vread(at, 0, b);
+        float w8[Q8 ? 4 * ST : 1];
+        if constexpr (Q8) {
+          const float inv = inverse(vref[0]);  // (alike in every column)
+#pragma unroll
+          for (int i = 0; i < 4 * ST; ++i) w8[i] = vq[i] * inv;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        h16x8 eh[NT][NE], el[NT][NE];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float w[4 * ST];
+          l[nt] += weights(sc[nt], s2[nt], m[nt], w8, w);
+          operand(w, eh[nt], el[nt]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        values(at, v, eh, el);
+        next();
+        if (j >= j_prefix) break;
       }
-      if (__ballot(over) != 0) break;
-      VPair v[NPAIR];
-#pragma unroll
-      for (int b = 0; b < NPAIR; ++b) v[b] = vread(at, 0, b);
-      float w8[Q8 ? 4 * ST : 1];
-      if constexpr (Q8) {
-        const float inv = inverse(vref[0]);  // (alike in every column)
-#pragma unroll
-        for (int i = 0; i < 4 * ST; ++i) w8[i] = vq[i] * inv;
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      h16x8 eh[NT][NE], el[NT][NE];
+      if (Q8 || j >= j_prefix) break;
+      settled = j;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float w[4 * ST];
-        l[nt] += weights(sc[nt], s2[nt], m[nt], w8, w);
-        operand(w, eh[nt], el[nt]);
+        const float alpha = moved(nt, mx[nt]);
+        l[nt] *= alpha;
+        rescale(nt, alpha);
       }
-      __builtin_amdgcn_sched_barrier(0);
-      values(at, v, eh, el);
-      next();
     }
   }
 
