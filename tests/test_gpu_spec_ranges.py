@@ -123,6 +123,7 @@ UNITS = {
     "shares and sizes opposed": lambda P, at: (-40 * LN2 * np.arange(P) / P, 2.0 ** (40 * np.arange(P) / P)),
     "sizes fall twice as fast": lambda P, at: (20 * LN2 * np.arange(P) / P, 2.0 ** (-40 * np.arange(P) / P)),
     "sizes fall, scores rise": lambda P, at: (40 * LN2 * np.arange(P) / P, 2.0 ** (-20 * np.arange(P) / P)),
+    "heavy tails": lambda P, at: tuple(f(np.random.default_rng(5).normal(size=(2, P))[i]) for i, f in enumerate((lambda z: 8 * z, lambda z: 2.0 ** (8 * z)))),
     "waves": lambda P, at: (20 * np.sin(np.arange(P) / 40), 2.0 ** (20 * np.cos(np.arange(P) / 70))),
 }
 
@@ -159,6 +160,28 @@ def test_units_of_values(device, fmt, tile, units):
             with np.errstate(invalid="ignore"):
                 again, _ = S.run_tree(c, t, other, T, [P], None, sees, nh, max_prefix=max(bound_p, P))
             assert np.array_equal(again[:, :T - 1], got[:, :T - 1])
+
+
+@pytest.mark.parametrize("fmt", [K.KV_F8, K.KV_I8])
+@pytest.mark.parametrize("nh,T,t", [(4, 3, F32), (16, 6, BF16)])
+@pytest.mark.parametrize("units", list(UNITS))
+def test_units_over_splits(device, fmt, nh, T, t, units):
+    """The same over sequences whose slots are split over workgroups of many chunks each."""
+    print(f"units '{units}' over splits type {t} format {fmt} heads {nh} drafts {T}", flush=True)
+    rng = np.random.default_rng([fmt, nh, T])
+    n, nk, D, P = 32, 2, 64, 2000
+    c = K.KvCache.allocate(fmt, n, nk, P + T, D)
+    q = S.decode(S.encode(2 * rng.normal(size=D) + 0.1 * rng.normal(size=(n, T, nh, D)), t), t)
+    nats, sizes = UNITS[units](P + T, 1234)
+    parts = [steered(rng, q[s:s + 1], nk, P + T, nats, sizes) for s in range(n)]
+    k, v = (np.concatenate([p[i] for p in parts]) for i in range(2))
+    kv = S.store_prefix(c, [k, v], P + T)
+    sees = np.stack([S.tree_bits(rng, T)] * n)
+    got, _ = S.run_tree(c, t, q, T, [P] * n, None, sees, nh)
+    assert np.isfinite(got).all()
+    some = [0, 13, 31]
+    want, bound = tree64p(q[some], [a[some] for a in kv], np.abs(v).max(-1).transpose(0, 2, 1)[some], [P] * 3, sees[some], D ** -0.5, t)
+    S.close(got[some], want, bound, "split")
 
 
 @pytest.mark.parametrize("t", [F32, BF16])
@@ -274,11 +297,13 @@ def test_norms_of_any_size(device, t, D, n_rot, eps):
     w = [(1 + 0.1 * rng.normal(size=D)).astype(np.float32) for _ in range(2)]
     inv, ms = K.rope_freqs(n_rot, 1e6)
     pos = rng.integers(0, 40000, rows)
-    buf, stride = S.put(raw), (nh + nk) * D
-    K.rope(t, buf.ptr, buf.ptr + nh * D * raw.itemsize, S.i32(pos), S.put(inv), rows, nh, nk, D, n_rot=n_rot, q_norm=S.put(w[0]),
-           k_norm=S.put(w[1]), eps=eps, q_stride=stride, k_stride=stride)
-    got = S.decode(buf.download(S.np_type(t), raw.size), t).reshape(x.shape)
-    eps = float(np.float32(eps))
-    for part, wt in ((slice(0, nh), w[0].astype(np.float64)), (slice(nh, None), w[1].astype(np.float64))):
-        want = S.rope64(x[:, part], wt, pos, inv, ms, n_rot, K.ROPE_HALF, eps)
-        S.close(got[:, part], want, S.rope_bound(want, x[:, part], wt, ms, t, eps), "norms")
+    stride, eps32 = (nh + nk) * D, float(np.float32(eps))
+    for norms in ((True, True), (True, False), (False, True)):
+        buf = S.put(raw)
+        K.rope(t, buf.ptr, buf.ptr + nh * D * raw.itemsize, S.i32(pos), S.put(inv), rows, nh, nk, D, n_rot=n_rot,
+               q_norm=S.put(w[0]) if norms[0] else None, k_norm=S.put(w[1]) if norms[1] else None, eps=eps, q_stride=stride, k_stride=stride)
+        got = S.decode(buf.download(S.np_type(t), raw.size), t).reshape(x.shape)
+        for part, wt, on in ((slice(0, nh), w[0], norms[0]), (slice(nh, None), w[1], norms[1])):
+            wt = wt.astype(np.float64) if on else None
+            want = S.rope64(x[:, part], wt, pos, inv, ms, n_rot, K.ROPE_HALF, eps32)
+            S.close(got[:, part], want, S.rope_bound(want, x[:, part], wt, ms, t, eps32), f"norms {norms}")
