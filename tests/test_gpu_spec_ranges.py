@@ -207,6 +207,32 @@ def test_queries_of_any_size(device, t, fmt, nh, T, bound_p, size):
     S.close(got, want, bound + HALF[t] * np.abs(want), "queries")
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("nh,T,bound_p", TILES)
+def test_largest_scores(device, t, fmt, nh, T, bound_p):
+    """Scores to 2^25, far from one another: the largest slot's value row is the output."""
+    rng = np.random.default_rng([t, fmt, nh, T])
+    D, P = 64, 700
+    c = K.KvCache.allocate(fmt, 1, 1, max(bound_p, P) + T, D)
+    k, v = rng.normal(size=(2, 1, P + T, 1, D))
+    kv = S.store_prefix(c, [1000 * k, v], P + T)
+    q = S.decode(S.encode(700 * rng.normal(size=(1, T, nh, D)), t), t)
+    sees = np.eye(T, dtype=bool)[None]
+    got, _ = S.run_tree(c, t, q, T, [P], None, sees, nh, max_prefix=max(bound_p, P), scale=1.0)
+    for i in range(T):
+        slots = np.append(np.arange(P), P + i)
+        sc = q[0, i] @ kv[0][0, 0][slots].T
+        order = np.sort(sc, axis=-1)
+        assert 2.0 ** 22 < np.abs(sc).max() < 2.0 ** 25
+        clear = order[:, -1] - order[:, -2] > 300  # (a score is off by 2^-20 of |q||k|, 2^27)
+        want = kv[1][0, 0][slots[sc.argmax(-1)]]
+        # of the one weight: times its scale U, as two parts of 11 bits 2 U, their products' sum U, joined with
+        # other splits' zeros 2 U, over the sum of weights 2 U; then the output's rounding
+        S.close(got[0, i][clear], want[clear], (8 * U + HALF[t]) * np.abs(want[clear]) + (2.0 ** -25 if t == F16 else 0.0), "largest")
+        assert clear.any()
+
+
 @pytest.mark.parametrize("t", [F32, BF16])
 @pytest.mark.parametrize("fmt", [K.KV_F8, K.KV_I8])
 @pytest.mark.parametrize("nh,T,bound_p", TILES + [(4, 3, 12000)])
