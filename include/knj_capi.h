@@ -158,9 +158,11 @@ int knj_attention_step(const float* q, const float* k, const float* v, const flo
  * that may run at once need a workspace each.  All pointers are memory of the
  * device opened by knj_device_open, which must be the calling thread's current
  * one (KNJ_E_STATE otherwise).  `type` is that of the activations: KNJ_TYPE_F32,
- * KNJ_TYPE_F16 or KNJ_TYPE_BF16; arithmetic is f32 (angles f64), rounded once.
+ * KNJ_TYPE_F16 or KNJ_TYPE_BF16; arithmetic is f32 (angles f64; the attention's operands
+ * as knj_attention_tree says), results are rounded once.
  * Rows of activations and caches start on 16-byte boundaries, their strides
- * count elements, other arrays are aligned to their types; anything else is refused.  head_dim is 64 or 128. */
+ * count elements, other arrays are aligned to their types; anything else is refused.
+ * head_dim is 64 or 128. */
 
 /* knj_rope: every head of rows q [n_rows][n_head][head_dim] (and k
  *   [n_rows][n_head_kv][head_dim]; n_head_kv 0: none) RMS-normalised with its
@@ -206,7 +208,8 @@ int knj_rope(int type, int layout, int n_rot, const double* inv_freq, float msca
  *   a NaN reads back as NaN (KNJ_KV_F16 keeps them as they are).
  * knj_kv_store: rows t < counts[s] (NULL: n_rows) of sequence s, k and v
  *   [n_seq][n_rows][n_head_kv][head_dim] with row_stride elements from a row to
- *   the next (of both), go to slots start[s] + t.  Rows that would fall outside
+ *   the next (of both: keys rotated in place in their projections' rows keep the
+ *   values' stride), go to slots start[s] + t.  Rows that would fall outside
  *   [0, n_ctx) are not stored.  n_rows * n_head_kv < 2^27, here and in knj_kv_load.
  * knj_kv_load: slots[s][t] (NULL: slot t) of the cache into rows k and v of the
  *   same form, as code * scale rounded to `type`; rows whose slot is outside
@@ -241,10 +244,11 @@ int knj_kv_load(const knj_kv_cache* cache, int type, const int32_t* slots, int n
  *   elements per row; out = softmax(scale * q.k) v over the slots seen.  Whatever
  *   unseen slots hold counts for nothing, NaN included; a draft that sees nothing
  *   gives zeros; rows past counts[s] are left as they were.  A draft that sees a
- *   draft whose value row holds an infinity or a NaN gives NaN (all of its dims).
+ *   draft whose value row holds an infinity or a NaN gives NaN (all of its dims); one
+ *   that sees a key row with either may give NaN.
  *   prefix[s] is held to [0, max_prefix] and counts[s] to [0, n_rows]; max_prefix +
- *   n_rows <= n_ctx and below 2^31 - 256, n_rows <= 1024, scale in [1e-6, 1e6], n_head a multiple of n_head_kv
- *   and at most 1024.
+ *   n_rows <= n_ctx and below 2^31 - 256, n_rows <= 1024, scale in [1e-6, 1e6], n_head a
+ *   multiple of n_head_kv and at most 1024.
  *   Queries may be of any size that leaves the scores, scale q.k, below 2^25 in magnitude,
  *   with scale |q| below 2^126 and 8-bit keys below 2^100.
  *   out may be q (with out_stride = q_stride; another is refused) and overlaps nothing

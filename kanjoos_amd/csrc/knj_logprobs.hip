@@ -109,7 +109,8 @@ __device__ __forceinline__ unsigned long long piece_key(float v, uint32_t idx, i
 // Bound by the read of the logits: 32 values a lane are eight (f32) or four loads in
 // flight a wave, then kept in registers, so that the largest is known before the
 // exponentials and no running rescale is needed.  500 rows of 151,936 f32 (304 MB):
-// 52.9 us, 5.7 TB/s (a copy reads and writes 5.1); one row 4.2 us, the latency of a
+// 55.2 us, 5.5 TB/s (a copy reads and writes 5.1); of f16 50.0, the exponentials and
+// the entropy's products of 76 million logits then count; one row 4.2 us, the latency of a
 // launch, one load and the two reductions.
 template <int TYPE>
 __global__ __launch_bounds__(kBlock) void k_logprob_pieces(LogprobArgs a, int n_pieces, float c_hi, float c_lo) {
@@ -184,10 +185,11 @@ __device__ __forceinline__ void rank_keys(const unsigned long long* keys, int n,
 // that the sums are formed while they are on their way.  W waves a row.
 //
 // Bound by its own chain of steps (records, maximum, ranks, pieces, candidates, ranks
-// again): 7.5 us for one row and its 20 largest, of which 3.7 are the top's; 10.6 us
-// for 500 rows and 5.  Sums over few records cost nothing in f64, and ranks counted
-// by comparison need no passes over the keys: eight lanes a key took 2 us off a lane
-// a key.
+// again): 7.1 us for one row and its 20 largest, of which 3.7 are the top's (the f32
+// kernel of sixteen waves leaves three of its registers in scratch, at its limit of
+// 128); 11.8 us for 500 rows and 5.  Sums over few records cost nothing in f64, and
+// ranks counted by comparison need no passes over the keys: eight lanes a key took 2 us
+// off a lane a key.
 template <int TYPE, int W>
 __global__ __launch_bounds__(64 * W) void k_logprob_join(LogprobArgs a, int n_pieces, double c) {
   constexpr int NT = 64 * W, R = kMaxPieces > NT ? kMaxPieces / NT : 1;  // records a thread
@@ -347,7 +349,8 @@ __global__ __launch_bounds__(64 * W) void k_logprob_join(LogprobArgs a, int n_pi
   __syncthreads();
   int nc = n_cand;
   if (nc > kCand) {
-    // Rows whose largest logits crowd into few pieces (sorted ones, equal ones): the
+    // Rows whose largest logits crowd into few pieces (sorted ones, equal ones; a row of
+    // 151,936 and its 20 largest then take 44 us, of 32,000 33 to 40): the
     // chosen piece of rank q holds at most n - q of the n largest, taken out one
     // after the other.
     __syncthreads();

@@ -51,8 +51,9 @@ __device__ __forceinline__ void st4(void* p, uint64_t i, float4 v) {
 // angle's f32 part a, with its remainder d (up to 2^-23, which alone would cost an
 // angle near pi a bit) by cos(a + d) = cos a - d sin a, sin(a + d) = sin a + d cos a.
 //
-// Bound by memory: 4000 rows of 36 f32 heads of 128 (147 MB in and out) 30.9 us a call,
-// 4.8 TB/s, where a large copy reaches 5.1.  One row is a launch: 2.1 us on the chip.
+// Bound by memory: 4000 rows of 36 f32 heads of 128 (147 MB in and out) 30.8 us a call,
+// 4.8 TB/s, where a large copy reaches 5.1; of bf16 (74 MB) 18.1, 4.1 TB/s: a row's three
+// workgroups form the same angles.  One row is a launch: 2.3 us on the chip.
 template <int TYPE, int LAYOUT, int D>
 __global__ __launch_bounds__(kBlock) void k_rope(RopeArgs a) {
   constexpr int T = D / 8, HPB = kBlock / T;
@@ -202,8 +203,8 @@ __device__ __forceinline__ uint2 quantise8(const float (&x)[8], float& scale) {
 
 // Rows of `FORMAT` from rows of activations; blockIdx.y is the sequence.  The same
 // lanes take a head's key and its value, so that the two reductions and divisions
-// run side by side (4096 rows of 4 f32 heads of 128 as e4m3 with a group for each
-// matrix: 8.9 us, so 8.2).  That is 21 MB, 4.1 us at a copy's rate: the rest is one
+// run side by side (a group for each matrix was 9 % slower): 4096 rows of 4 f32 heads
+// of 128 as e4m3 7.0 us.  That is 21 MB, 4.1 us at a copy's rate: the rest is one
 // pass of latency (loads, two maxima over 16 lanes, a division, stores) of 1024
 // workgroups that are all resident at once; 32 sequences' one row 3.3 us.
 template <int TYPE, int FORMAT, int D>
@@ -258,8 +259,8 @@ __device__ __forceinline__ void values8(uint2 w, float scale, float4& a, float4&
 }
 
 // The reverse: rows of activations from cache slots.  Bound by memory: 32,000 rows of
-// 4 int8 heads of 128 to f16 (99 MB) 22.0 us, 4.5 TB/s, with keys and values by the
-// same lanes (28 with a group for each); gathered rows of 32 sequences 2.6 us.
+// 4 int8 heads of 128 to f16 (99 MB) 21.8 us, 4.5 TB/s, with keys and values by the
+// same lanes (28 with a group for each); gathered rows of 32 sequences 2.7 us.
 template <int TYPE, int FORMAT, int D>
 __global__ __launch_bounds__(kBlock) void k_kv_load(KvRowsArgs a) {
   const knj_kv_cache& c = a.c;

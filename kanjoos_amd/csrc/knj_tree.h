@@ -194,15 +194,14 @@ typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 // there, and the chunks that reach the drafts are cleaned before use (below).
 //
 // What bounds it (f16, 64 drafts x 32 heads over 32,764 slots of 4 kv heads, 34 GFLOP:
-// 58.5 us a call, 0.59 PFLOP/s; 49 us here, 9 in the merge): of a wave's life the
-// matrix cores are busy for 42 %, vector instructions issue for 25 % (two waves share
-// a SIMD, so 51 % of it) and LDS delivers for 45 % of the CU's; the two waves that
-// the accumulators leave room for do not cover one another's waits.  Taken out one
-// at a time, in a copy: the exponentials change nothing, a chunk that is always in L2
-// saves 6 us, 24 of a chunk's 64 products with their reads 10.  Calls of few drafts
-// are one wave's path through a chunk, 1.7 us of conversions, reductions and waits,
-// and two launches: 9.5 us for 4 drafts over 1000 f16 slots.
-// Tried and no faster: eight waves to a tile (of 128 columns within 3 %, of 32
+// 69.6 us a call, 0.49 PFLOP/s; profiled, 73 us here, 65 at least, and 9 in the merge):
+// of a wave's life the matrix cores are busy for 49 % (96 products a wave and chunk,
+// a third of them the weights' remainders, without which the call took 57.7 us), vector
+// instructions issue for 29 % (two waves share a SIMD, so 57 % of it); the two waves
+// that the accumulators leave room for do not cover one another's waits.  Calls of few
+// drafts are one wave's path through a chunk, 1.7 us of conversions, reductions and
+// waits, and two launches: 9.5 us for 4 drafts over 1000 f16 slots.
+// Tried before the remainders and no faster: eight waves to a tile (of 128 columns within 3 %, of 32
 // slower), a raised wave priority around the products, 768 or 1024 workgroups,
 // chunks of 128 slots, chunks through registers instead of DMA, the next chunk's DMA
 // behind this one's reads (1 to 5 % slower).
@@ -581,7 +580,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
   // chunk j's stage ready: this wave's DMA of it has landed; the barrier hands every
   // wave's part over and ends the reads of chunk j - 1, whose stage the next chunk
   // then refills (past the range: fetched and not used).  A third stage, a chunk more
-  // ahead, gained nothing (int8 at 32K slots 18.6 us against 17.9).
+  // ahead, was 4 % slower (one draft over 32K int8 slots).
   int j = c0, stage = 0;
   auto ready = [&]() {
     KNJ_BARRIER_AFTER(vm_lds_imm(0));

@@ -20,7 +20,7 @@ hipError_t launch_format<KNJ_KV_I8>(const TreeArgs&, const TreePlan&, int, hipSt
 // split has its place, and those that the sequence does not reach, which hold no
 // record, are dropped afterwards.
 // Bound by the records: 64 drafts x 32 heads of 32 splits (35 MB, written just before)
-// 8.9 us, 3.9 TB/s; 4 drafts 3.3 us, a launch and one batch of loads.
+// 9.2 us, 3.8 TB/s; 4 drafts 3.3 us, a launch and one batch of loads.
 template <int D, int NP>
 __global__ __launch_bounds__(kBlock) void k_tree_merge(TreeArgs a, TreePlan p, int chunk, int n_cols, uint32_t n_out) {
   constexpr int ND = D / 4, B = 8, PER = kBlock / (ND * NP);
@@ -160,9 +160,9 @@ hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t s) {
   else e = tree::launch_format<KNJ_KV_I8>(a, q.p, q.cols, s);
   if (e != hipSuccess || q.p.n_split == 1) return e;
   // Few outputs or many splits: the splits over a workgroup's parts, for latency (one
-  // draft over 4000 f16 slots 10.8 us a call, 17.4 with one part; 8 over 32K int8 26.6
-  // and 32.3).  Many outputs of up to eight splits, one batch of loads: one part (32 x 8
-  // drafts at 2K 34.2 us, 43.9 with eight).
+  // draft over 4000 f16 slots 10.4 us a call, 16.8 with one part; 8 over 32K int8 28.9
+  // and 34.8).  Many outputs of up to eight splits, one batch of loads: one part (32 x 8
+  // drafts at 2K 37.1 us, 46.6 with eight).
   const uint32_t n_out = (uint32_t)a.c.n_seq * a.n_rows * a.n_head;
   const int n_cols = q.p.n_tiles * q.cols;
   const bool wide = n_out <= 512 || q.p.n_split > 8;
