@@ -200,7 +200,8 @@ __global__ __launch_bounds__(64 * W) void k_logprob_join(LogprobArgs a, int n_pi
   __shared__ double red_rest[W], red_ent[W];
   __shared__ int red_bad[W], chosen[kMaxTop];
   __shared__ int n_cand;
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int row = blockIdx.y * gridDim.x + blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (row >= a.n_rows) return;
   const Record* rec = (const Record*)a.records + (uint64_t)row * n_pieces;
   const uint64_t row_at = (uint64_t)row * a.row_stride;
   const int n = a.n_top, n_sel = min(n, n_pieces);
@@ -395,15 +396,18 @@ hipError_t launch_token_logprobs(int type, const LogprobArgs& a, hipStream_t s) 
   const int n_pieces = pieces_of(a.n_vocab);
   const uint64_t waves = (uint64_t)a.n_rows * n_pieces;
   const dim3 grid((unsigned)((waves + kBlock / 64 - 1) / (kBlock / 64)));
+  // (a grid holds 2^32 threads a dim: 2^21 workgroups of 1024 are half of it)
+  const unsigned across = a.n_rows < (1 << 21) ? a.n_rows : 1u << 21;
+  const dim3 join(across, (a.n_rows + across - 1) / across);
   const double c = 1.4426950408889634 * a.inv_temp;
   const float c_hi = (float)c, c_lo = (float)(c - (double)c_hi);
 #define KNJ_LOGPROBS(TYPE)                                                                            \
   do {                                                                                                \
     KNJ_LAUNCH(k_logprob_pieces<TYPE>, grid, dim3(kBlock), 0, s, a, n_pieces, c_hi, c_lo);            \
     if (a.n_rows <= kJoinRows || n_pieces < a.n_top)                                                  \
-      KNJ_LAUNCH((k_logprob_join<TYPE, 16>), dim3(a.n_rows), dim3(1024), 0, s, a, n_pieces, c);       \
+      KNJ_LAUNCH((k_logprob_join<TYPE, 16>), join, dim3(1024), 0, s, a, n_pieces, c);                 \
     else                                                                                              \
-      KNJ_LAUNCH((k_logprob_join<TYPE, 4>), dim3(a.n_rows), dim3(256), 0, s, a, n_pieces, c);         \
+      KNJ_LAUNCH((k_logprob_join<TYPE, 4>), join, dim3(256), 0, s, a, n_pieces, c);                   \
   } while (0)
   if (type == KNJ_TYPE_F32) KNJ_LOGPROBS(KNJ_TYPE_F32);
   else if (type == KNJ_TYPE_F16) KNJ_LOGPROBS(KNJ_TYPE_F16);

@@ -281,6 +281,18 @@ def test_largest_of_small_vocabularies(device, t, V, n_top):
         np.testing.assert_array_equal(y, x[pick])
 
 
+def test_largest_of_more_rows_than_a_grid_line(device):
+    """Rows past what one dimension of a grid holds in workgroups of sixteen waves."""
+    rng = np.random.default_rng(3)
+    rows, V, n_top = (1 << 22) + 3, 5, 2
+    x = rng.permuted(np.broadcast_to(np.arange(V, dtype=np.float16), (rows, V)), axis=1)
+    lp, ent, idx, top = S.run_logprobs(x, F16, V, np.zeros(rows), n_top, 1.0)
+    lse = np.log(np.exp(np.arange(V) - (V - 1.0)).sum())
+    assert np.array_equal(idx, np.argsort(-x.astype(np.float32), axis=1, kind="stable")[:, :n_top])
+    np.testing.assert_allclose(top, np.broadcast_to([-lse, -lse - 1], (rows, 2)), rtol=48 * U)
+    np.testing.assert_allclose(lp, x[:, 0].astype(np.float64) - (V - 1) - lse, rtol=48 * U)
+
+
 @pytest.mark.parametrize("layout", [K.ROPE_HALF, K.ROPE_INTERLEAVED])
 def test_rotation_near_the_axes(device, layout):
     """Angles next to multiples of pi/2, where one of cos and sin is all remainder: the
