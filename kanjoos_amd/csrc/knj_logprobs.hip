@@ -439,7 +439,8 @@ int knj_token_logprobs(int type, const void* logits, uint64_t row_stride, int n_
   KNJ_CHECK_ARG(!tokens == !logprob, "tokens and logprob go together");
   KNJ_CHECK_ARG(n_top >= 0 && n_top <= kMaxTop && n_top <= n_vocab, "n_top must be in [0, min(32, n_vocab)]");
   KNJ_CHECK_ARG(n_top == 0 || (top_idx && top_logprob), "null top_idx or top_logprob");
-  KNJ_CHECK_ARG(words_aligned(tokens, logprob, entropy, top_idx, top_logprob), "tokens and outputs must be aligned to their types");
+  KNJ_CHECK_ARG(words_aligned(tokens, logprob, entropy, top_idx, top_logprob),
+                "tokens and outputs must be aligned to their types");
   const uint64_t need = logprob_record_bytes(n_rows, n_vocab);
   if (n_rows && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) {
     set_error("knj_token_logprobs: these sizes need a 16-byte aligned workspace of " + std::to_string(need) + " bytes");

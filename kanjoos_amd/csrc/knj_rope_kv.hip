@@ -501,7 +501,8 @@ int knj_attention_tree(const knj_kv_cache* cache, int type, const void* q, uint6
   const int eb = act_bytes(type);
   KNJ_CHECK_ARG(eb, "activations must be F32, F16 or BF16");
   KNJ_CHECK_ARG(q && out && prefix, "null pointer");
-  KNJ_CHECK_ARG(words_aligned(prefix, counts) && ((uintptr_t)mask & 7) == 0, "prefix, counts and mask must be aligned to their types");
+  KNJ_CHECK_ARG(words_aligned(prefix, counts) && ((uintptr_t)mask & 7) == 0,
+                "prefix, counts and mask must be aligned to their types");
   KNJ_CHECK_ARG(n_rows >= 0 && n_rows <= 1024, "n_rows must be in [0, 1024]");
   KNJ_CHECK_ARG(n_head > 0 && n_head <= 1024 && n_head % cache->n_head_kv == 0,
                 "n_head must be a positive multiple of n_head_kv, at most 1024");

@@ -184,10 +184,11 @@ typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 // 8-bit codes become f16 (exactly) as operands.  Their scales stay out of the
 // products: a score is multiplied by its slot's, a weight by its slot's over the
 // running largest of the scales its column has seen (a power of two, so a weight
-// stays in f16's range whatever the cache's units; kMostLift has the other end).  Queries are scaled by a
-// power of two per row, so that f16 holds any of them.  Weights are f16 high parts and
-// remainders (22 bits) whatever the activations: 11 bits of a weight leave errors of
-// the size of an f16 output's own rounding.  SPLIT keeps f32 queries so too.
+// stays in f16's range whatever the cache's units; kMostLift has the other end).
+// Queries are scaled by a power of two per row, so that f16 holds any of them.  Weights
+// are f16 high parts and remainders (22 bits) whatever the activations: 11 bits of a
+// weight leave errors of the size of an f16 output's own rounding.  SPLIT keeps f32
+// queries so too.
 //
 // The loads that need no sequence length (a chunk's rows, the queries) come
 // first; rows of a chunk past the sequence's slots hold whatever the cache does
@@ -201,10 +202,10 @@ typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 // that the accumulators leave room for do not cover one another's waits.  Calls of few
 // drafts are one wave's path through a chunk, 1.7 us of conversions, reductions and
 // waits, and two launches: 9.5 us for 4 drafts over 1000 f16 slots.
-// Tried before the remainders and no faster: eight waves to a tile (of 128 columns within 3 %, of 32
-// slower), a raised wave priority around the products, 768 or 1024 workgroups,
-// chunks of 128 slots, chunks through registers instead of DMA, the next chunk's DMA
-// behind this one's reads (1 to 5 % slower).
+// Tried before the remainders and no faster: eight waves to a tile (of 128 columns
+// within 3 %, of 32 slower), a raised wave priority around the products, 768 or 1024
+// workgroups, chunks of 128 slots, chunks through registers instead of DMA, the next
+// chunk's DMA behind this one's reads (1 to 5 % slower).
 template <int D, int FORMAT, bool SPLIT, int NT, int WC, int WS, int SW>
 __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p) {
   constexpr bool Q8 = FORMAT != KNJ_KV_F16;
@@ -780,11 +781,15 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
     if (spoilt[nt]) l[nt] = NAN;
     if constexpr (Q8) {
       // (a scale above 1 goes into the sum's unit, 2^-k of it against a reference k
-      // higher: times the values it could pass f32)
-      const float up = fmaxf(vref[nt], 1.0f);
-      m[nt] += (float)((int)(__float_as_uint(up) >> 23) - 127);
-      l[nt] *= inverse(up);
-      rescale(nt, fminf(vref[nt], 1.0f));
+      // higher: times the values it could pass f32; what the sum r + k is rounded by
+      // goes into the factors)
+      const float up = fmaxf(vref[nt], 1.0f), k = (float)((int)(__float_as_uint(up) >> 23) - 127);
+      const float old = m[nt];
+      m[nt] += k;
+      const float part = m[nt] - old;
+      const float f = fabsf(old) < INFINITY ? __builtin_amdgcn_exp2f((old - (m[nt] - part)) + (k - part)) : 1.0f;
+      l[nt] *= inverse(up) * f;
+      rescale(nt, fminf(vref[nt], 1.0f) * f);
     }
   }
   __builtin_amdgcn_s_waitcnt(0);  // the fetches past the range land before LDS is reused or given back

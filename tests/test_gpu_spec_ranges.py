@@ -345,3 +345,23 @@ def test_norms_of_any_size(device, t, D, n_rot, eps):
             wt = wt.astype(np.float64) if on else None
             want = S.rope64(x[:, part], wt, pos, inv, ms, n_rot, K.ROPE_HALF, eps32)
             S.close(got[:, part], want, S.rope_bound(want, x[:, part], wt, ms, t, eps32), f"norms {norms}")
+
+
+@pytest.mark.parametrize("fmt", [K.KV_F8, K.KV_I8])
+@pytest.mark.parametrize("nh,T,bound_p", TILES + [(4, 3, 12000)])
+@pytest.mark.parametrize("power", [-20, 8, 45, 90])
+def test_unit_of_values_leaves_the_result(device, fmt, nh, T, bound_p, power):
+    """Values times a power of two: the same codes, and the result times it to the last
+    roundings (each of a wave's and a split's two factors 2 U at most, of 16 joined)."""
+    rng = np.random.default_rng([fmt, nh, T])
+    D, P = 64, 900
+    k, v = rng.normal(size=(2, 1, P + T, 1, D))
+    q = rng.normal(size=(1, T, nh, D)).astype(np.float32).astype(np.float64)
+    sees = S.tree_bits(rng, T)[None]
+    out = []
+    for z in (0, power):
+        c = K.KvCache.allocate(fmt, 1, 1, max(bound_p, P) + T, D)
+        kv = S.store_prefix(c, [k, v * 2.0 ** z], P + T)
+        out.append(S.run_tree(c, F32, q, T, [P], None, sees, nh, max_prefix=max(bound_p, P))[0] * 2.0 ** -z)
+    p = S.tree64(q, [kv[0], np.abs(kv[1]) * 2.0 ** -power], [P], [T], sees, D ** -0.5, F32)[0]  # sum of shares times |values|
+    S.close(out[1], out[0], 8 * U * p, "unit")
