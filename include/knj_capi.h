@@ -286,6 +286,101 @@ int knj_token_logprobs(int type, const void* logits, uint64_t row_stride, int n_
                        uint64_t workspace_bytes, void* stream);
 uint64_t knj_token_logprobs_workspace(int n_rows, int n_vocab);
 
+/* ------------------------------------------------------------ a 4-bit cache in pages
+ * A cache of n_layer layers in 4 bits whose slots lie in pages that sequences share: a
+ * prompt's pages serve every answer to it, beams take over their parents' pages, and what
+ * is written is copied first.  No counterpart in the reference.  The rules of the
+ * speculative step's calls hold (stream, no allocation, device, types, alignment); calls
+ * that change the table, the counts or a page are ordered by the caller (one stream).
+ *
+ * Keys and values are held in groups of 32 dims as code * step + low rounded to f16 (one
+ *   rounding), step and low f16, code 0 to 15: low is the group's smallest element rounded
+ *   to f16, step the largest f16 not above (largest - low) / 15 (0 if that is negative),
+ *   code = (x - low) / step in f64, rounded to nearest even and held to [0, 15] (0 where step
+ *   is 0).  A group that holds an infinity, a NaN or a magnitude above 65504 reads back as
+ *   NaN.
+ * data [n_layer][n_page] pages of n_head_kv * page_size * head_dim * 5 / 4 bytes: per kv
+ *   head the page's key codes [page_size][head_dim / 2] bytes, its value codes, then a word
+ *   a group [page_size][head_dim / 32] for keys and for values (step the low half, low the
+ *   high one).  Of eight dims from 8 w on, word w of a row's codes holds dim 8 w + i in bits
+ *   4 (i / 2) + 16 (i % 2) and up.
+ * table [n_seq][n_table]: the page of a sequence's slots e * page_size to (e + 1) *
+ *   page_size - 1; an entry outside [0, n_page) is none.  refs [n_page]: how many entries
+ *   hold a page; a page with none is free (a caller who wants a page to outlive its entries
+ *   adds a count of its own).  Calls that do not name the table (knj_pages_copy) or the counts
+ *   (all but reserve, fork and free) take NULL there.
+ * page_size: a power of two from 16 to 256.  n_layer at most 1024, n_seq at most 4096, n_head_kv
+ *   at most 64, n_page below 2^26, n_table * page_size below 2^31 - 256, n_seq * n_table below
+ *   2^31.  data is 16-byte aligned.
+ * knj_pages_bytes: bytes of data (0: sizes that are refused); pointers are not looked at. */
+typedef struct knj_kv_pages {
+  void* data;
+  int32_t* table;
+  int32_t* refs;
+  int32_t n_layer, n_page, page_size, n_head_kv, head_dim;
+  int32_t n_seq, n_table;
+} knj_kv_pages;
+uint64_t knj_pages_bytes(const knj_kv_pages* pages);
+
+/* knj_pages_store, knj_pages_load: as knj_kv_store and knj_kv_load, of one layer.  Rows
+ *   whose slot has no page are not stored, and left as they were when loaded.  Rows stored
+ *   into a page that has other holders are theirs too (knj_pages_reserve gives a
+ *   sequence pages of its own). */
+int knj_pages_store(const knj_kv_pages* pages, int layer, int type, const void* k, const void* v,
+                    uint64_t row_stride, const int32_t* start, const int32_t* counts, int n_rows,
+                    void* stream);
+int knj_pages_load(const knj_kv_pages* pages, int layer, int type, const int32_t* slots,
+                   int n_rows, void* k, void* v, uint64_t row_stride, void* stream);
+
+/* knj_attention_pages: knj_attention_tree over one layer of pages: its arguments, masks and
+ *   limits (n_ctx is n_table * page_size; a decode step is n_rows 1 with its own key stored, a
+ *   piece of a prompt n_rows up to 1024 without a mask).  A slot without a page holds NaN.
+ *   f32 queries keep 22 bits; weights keep 22 bits with any activations, and queries are of
+ *   any size that leaves the scores, scale q.k, below 2^25 in magnitude with scale |q| below
+ *   2^126. */
+int knj_attention_pages(const knj_kv_pages* pages, int layer, int type, const void* q,
+                        uint64_t q_stride, int n_head, int n_rows, const int32_t* prefix,
+                        int max_prefix, const int32_t* counts, const uint64_t* mask,
+                        int mask_shared, float scale, void* out, uint64_t out_stride,
+                        void* workspace, uint64_t workspace_bytes, void* stream);
+uint64_t knj_attention_pages_workspace(const knj_kv_pages* pages, int n_head, int n_rows,
+                                       int max_prefix);
+
+/* knj_pages_reserve: sequence s, which holds length[s] slots, gets a page of its own for every
+ *   slot from start[s] (NULL: length[s]) to want[s] - 1: entries that are none, and those
+ *   whose page has other holders, take the lowest-numbered free pages, in order of sequence
+ *   and entry.  Of a page that is replaced the slots below length[s] are copied, in all
+ *   layers; a page that all its holders would replace stays with the last of them.  If there
+ *   are not enough free pages nothing changes.  *missing: how many were short (0: done).
+ *   Slots past the table's n_table * page_size get none.
+ * knj_pages_fork: sequence s becomes the first keep[s] slots (NULL: all) of sequence parent[s]
+ *   as it was before the call, for all s at once (parent[s] = s keeps a sequence, one outside
+ *   [0, n_seq) empties it).  Pages are shared, not copied.
+ * knj_pages_free: sequence s keeps its first keep[s] slots (a negative keep[s]: all) and gives
+ *   the pages behind them back.
+ * knj_pages_compact: in every layer, the key and value of slot rows[s][i] move to slot
+ *   start[s] + i, i < counts[s] (NULL: n_rows); rows [n_seq][n_rows] ascend and rows[s][i] is
+ *   at least start[s] + i.  How the accepted path of a tree of drafts moves behind the
+ *   prefix, or what is kept of a long context together.  Codes move as they are.  The pages
+ *   written to are to be the sequence's own (knj_pages_reserve from start[s] on).  A row
+ *   whose slot, old or new, has no page stays.
+ * knj_pages_copy: pages src[i] of one pool into pages dst[i] of another of the same n_layer,
+ *   page_size, n_head_kv and head_dim, or of the same pool, i < n < 2^24, in all layers.  Pairs with a
+ *   number outside its pool are left out; no page that is written may be read or written
+ *   by another pair.
+ * knj_pages_workspace: bytes of the workspace of reserve and fork; any contents. */
+int knj_pages_reserve(const knj_kv_pages* pages, const int32_t* start, const int32_t* length,
+                      const int32_t* want, int32_t* missing, void* workspace,
+                      uint64_t workspace_bytes, void* stream);
+int knj_pages_fork(const knj_kv_pages* pages, const int32_t* parent, const int32_t* keep,
+                   void* workspace, uint64_t workspace_bytes, void* stream);
+int knj_pages_free(const knj_kv_pages* pages, const int32_t* keep, void* stream);
+int knj_pages_compact(const knj_kv_pages* pages, const int32_t* start, const int32_t* rows,
+                      const int32_t* counts, int n_rows, void* stream);
+int knj_pages_copy(const knj_kv_pages* to, const knj_kv_pages* from, const int32_t* dst,
+                   const int32_t* src, int n, void* stream);
+uint64_t knj_pages_workspace(const knj_kv_pages* pages);
+
 /* ------------------------------------------------------------ model step
  * The device counterpart of knj::Model (/root/reference/src/model/model.h:55-80):
  * open -> forward(tokens, n) -> logits of the last token, reset(), pos().

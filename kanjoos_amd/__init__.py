@@ -36,7 +36,10 @@ EXPORTS = (
     "knj_built_arch", "knj_last_error", "knj_malloc", "knj_free", "knj_memcpy_h2d",
     "knj_memcpy_d2h", "knj_memset_zero", "knj_synchronize", "knj_dequant", "knj_gemv",
     "knj_rmsnorm", "knj_rope_freqs", "knj_rope", "knj_kv_store", "knj_kv_load", "knj_attention_tree",
-    "knj_attention_tree_workspace", "knj_token_logprobs", "knj_token_logprobs_workspace", "knj_moe_router", "knj_moe_decode_layer", "knj_moe_decode_layer_noalloc", "knj_moe_batch_layer", "knj_attention_step", "knj_model_create_synthetic", "knj_model_create_from_image",
+    "knj_attention_tree_workspace", "knj_token_logprobs", "knj_token_logprobs_workspace",
+    "knj_pages_bytes", "knj_pages_store", "knj_pages_load", "knj_attention_pages", "knj_attention_pages_workspace",
+    "knj_pages_reserve", "knj_pages_fork", "knj_pages_free", "knj_pages_compact", "knj_pages_copy", "knj_pages_workspace",
+    "knj_moe_router", "knj_moe_decode_layer", "knj_moe_decode_layer_noalloc", "knj_moe_batch_layer", "knj_attention_step", "knj_model_create_synthetic", "knj_model_create_from_image",
     "knj_model_free", "knj_model_image_bytes", "knj_model_image_device", "knj_model_layer_offsets", "knj_model_fill_kv", "knj_gguf_probe",
     "knj_model_create_from_gguf", "knj_model_config_get",
     "knj_model_download_image", "knj_model_reset", "knj_model_pos", "knj_model_set_pos",
@@ -104,6 +107,13 @@ class KvCacheDesc(C.Structure):
                 ("n_ctx", C.c_int32), ("head_dim", C.c_int32)]
 
 
+class KvPagesDesc(C.Structure):
+    """``knj_kv_pages`` (include/knj_capi.h)."""
+    _fields_ = [("data", C.c_void_p), ("table", C.c_void_p), ("refs", C.c_void_p), ("n_layer", C.c_int32),
+                ("n_page", C.c_int32), ("page_size", C.c_int32), ("n_head_kv", C.c_int32), ("head_dim", C.c_int32),
+                ("n_seq", C.c_int32), ("n_table", C.c_int32)]
+
+
 class DeviceCaps(C.Structure):
     _fields_ = [
         ("gcn_arch", C.c_char * 32), ("name", C.c_char * 64), ("wave_size", C.c_int32),
@@ -151,6 +161,17 @@ _SIGS = {
     "knj_attention_tree_workspace": (_u64, [_P, _i, _i, _i]),
     "knj_token_logprobs": (_i, [_i, _P, _u64, _i, _i, _f, _P, _P, _P, _i, _P, _P, _P, _u64, _P]),
     "knj_token_logprobs_workspace": (_u64, [_i, _i]),
+    "knj_pages_bytes": (_u64, [_P]),
+    "knj_pages_store": (_i, [_P, _i, _i, _P, _P, _u64, _P, _P, _i, _P]),
+    "knj_pages_load": (_i, [_P, _i, _i, _P, _i, _P, _P, _u64, _P]),
+    "knj_attention_pages": (_i, [_P, _i, _i, _P, _u64, _i, _i, _P, _i, _P, _P, _i, _f, _P, _u64, _P, _u64, _P]),
+    "knj_attention_pages_workspace": (_u64, [_P, _i, _i, _i]),
+    "knj_pages_reserve": (_i, [_P, _P, _P, _P, _P, _P, _u64, _P]),
+    "knj_pages_fork": (_i, [_P, _P, _P, _P, _u64, _P]),
+    "knj_pages_free": (_i, [_P, _P, _P]),
+    "knj_pages_compact": (_i, [_P, _P, _P, _P, _i, _P]),
+    "knj_pages_copy": (_i, [_P, _P, _P, _P, _i, _P]),
+    "knj_pages_workspace": (_u64, [_P]),
     "knj_model_create_synthetic": (_i, [C.POINTER(ModelConfig), _u64, C.POINTER(_P)]),
     "knj_model_create_from_image": (_i, [C.POINTER(ModelConfig), _P, _u64, C.POINTER(_P)]),
     "knj_model_free": (_i, [_P]),
@@ -471,6 +492,106 @@ def token_logprobs(type_id: int, logits, n_rows: int, n_vocab: int, workspace: D
                                    temperature, _p(tokens), _p(logprob), _p(entropy), n_top, _p(top_idx),
                                    _p(top_logprob), _p(workspace), workspace.nbytes if workspace is not None else 0,
                                    stream))
+
+
+# ------------------------------------------------------------------ a 4-bit cache in pages
+#
+# Pages that sequences share through a table (include/knj_capi.h, "a 4-bit cache in pages").  They queue on
+# `stream` and return; buffers must live until the stream has passed them.
+
+class KvPages:
+    """A 4-bit cache of several layers in pages (knj_kv_pages) over given buffers, or with :meth:`allocate` over its
+    own, without pages in its table."""
+
+    def __init__(self, n_layer: int, n_page: int, page_size: int, n_head_kv: int, head_dim: int, n_seq: int,
+                 n_table: int, data, table=None, refs=None):
+        self.data, self.table, self.refs = data, table, refs
+        self.desc = KvPagesDesc(_p(data), _p(table), _p(refs), n_layer, n_page, page_size, n_head_kv, head_dim, n_seq,
+                                n_table)
+        self.ref = C.addressof(self.desc)
+
+    @classmethod
+    def allocate(cls, n_layer: int, n_page: int, page_size: int, n_head_kv: int, head_dim: int, n_seq: int,
+                 n_table: int) -> "KvPages":
+        desc = KvPagesDesc(None, None, None, n_layer, n_page, page_size, n_head_kv, head_dim, n_seq, n_table)
+        nbytes = lib().knj_pages_bytes(C.addressof(desc))
+        if not nbytes:
+            raise KnjError(KNJ_E_ARG, lib().knj_last_error().decode(errors="replace"))
+        data, refs = DeviceBuffer(nbytes), DeviceBuffer(4 * n_page)
+        for b in (data, refs):
+            b.zero()
+        table = DeviceBuffer.from_array(np.full((n_seq, n_table), -1, np.int32))
+        return cls(n_layer, n_page, page_size, n_head_kv, head_dim, n_seq, n_table, data, table, refs)
+
+
+def pages_store(pages: KvPages, layer: int, type_id: int, k, v, start, n_rows: int, counts=None,
+                row_stride: int | None = None, stream=None) -> None:
+    """Rows t < counts[s] of every sequence into slots start[s] + t of a layer (knj_pages_store)."""
+    d = pages.desc
+    check(lib().knj_pages_store(pages.ref, layer, type_id, _p(k), _p(v),
+                                d.n_head_kv * d.head_dim if row_stride is None else row_stride, _p(start), _p(counts),
+                                n_rows, stream))
+
+
+def pages_load(pages: KvPages, layer: int, type_id: int, k, v, n_rows: int, slots=None, row_stride: int | None = None,
+               stream=None) -> None:
+    """Slots of every sequence (slots [n_seq][n_rows]; None: slot t) read back into rows k and v (knj_pages_load)."""
+    d = pages.desc
+    check(lib().knj_pages_load(pages.ref, layer, type_id, _p(slots), n_rows, _p(k), _p(v),
+                               d.n_head_kv * d.head_dim if row_stride is None else row_stride, stream))
+
+
+def attention_pages_workspace(pages: KvPages, n_head: int, n_rows: int, max_prefix: int) -> int:
+    """Bytes of workspace that attention_pages needs for these sizes (0: none)."""
+    return lib().knj_attention_pages_workspace(pages.ref, n_head, n_rows, max_prefix)
+
+
+def attention_pages(pages: KvPages, layer: int, type_id: int, q, out, n_head: int, n_rows: int, prefix, max_prefix: int,
+                    workspace: DeviceBuffer | None = None, counts=None, mask=None, mask_shared: bool = False,
+                    scale: float | None = None, q_stride: int | None = None, out_stride: int | None = None,
+                    stream=None) -> None:
+    """Attention of rows of queries per sequence over a layer of the pages (knj_attention_pages); scale defaults to
+    1 / sqrt(head_dim)."""
+    d = pages.desc
+    width = n_head * d.head_dim
+    check(lib().knj_attention_pages(pages.ref, layer, type_id, _p(q), width if q_stride is None else q_stride, n_head,
+                                    n_rows, _p(prefix), max_prefix, _p(counts), _p(mask), int(mask_shared),
+                                    d.head_dim ** -0.5 if scale is None else scale, _p(out),
+                                    width if out_stride is None else out_stride, _p(workspace),
+                                    workspace.nbytes if workspace is not None else 0, stream))
+
+
+def pages_workspace(pages: KvPages) -> int:
+    """Bytes of workspace that pages_reserve and pages_fork need."""
+    return lib().knj_pages_workspace(pages.ref)
+
+
+def pages_reserve(pages: KvPages, length, want, missing, workspace: DeviceBuffer, start=None, stream=None) -> None:
+    """Pages of its own for every sequence's slots from start[s] (None: length[s]) to want[s] - 1
+    (knj_pages_reserve); missing: int32, the number of pages that were short."""
+    check(lib().knj_pages_reserve(pages.ref, _p(start), _p(length), _p(want), _p(missing), _p(workspace),
+                                  workspace.nbytes if workspace is not None else 0, stream))
+
+
+def pages_fork(pages: KvPages, parent, workspace: DeviceBuffer, keep=None, stream=None) -> None:
+    """Every sequence becomes the first keep[s] slots (None: all) of sequence parent[s] (knj_pages_fork)."""
+    check(lib().knj_pages_fork(pages.ref, _p(parent), _p(keep), _p(workspace),
+                               workspace.nbytes if workspace is not None else 0, stream))
+
+
+def pages_free(pages: KvPages, keep, stream=None) -> None:
+    """The pages behind every sequence's first keep[s] slots given back (knj_pages_free)."""
+    check(lib().knj_pages_free(pages.ref, _p(keep), stream))
+
+
+def pages_compact(pages: KvPages, start, rows, n_rows: int, counts=None, stream=None) -> None:
+    """Slots rows[s][i] (i < counts[s]) of every sequence moved to start[s] + i in all layers (knj_pages_compact)."""
+    check(lib().knj_pages_compact(pages.ref, _p(start), _p(rows), _p(counts), n_rows, stream))
+
+
+def pages_copy(to: KvPages, pages: KvPages, dst, src, n: int, stream=None) -> None:
+    """Pages src[i] of one pool into pages dst[i] of another, or of the same (knj_pages_copy)."""
+    check(lib().knj_pages_copy(to.ref, pages.ref, _p(dst), _p(src), n, stream))
 
 
 # ------------------------------------------------------------------ model

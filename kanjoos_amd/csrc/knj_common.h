@@ -322,9 +322,55 @@ struct TreeArgs {
   float scale;
   int n_head, n_rows, max_prefix, mask_shared;
   int type;                   // of q and out
+  const uint8_t* pages;       // a layer of 4-bit pages, in place of c's pointers
+  const int32_t* table;       // [n_seq][n_table]
+  int n_page, n_table, page_shift;
 };
+// Slots of a sequence that the attention numbers in 32 bits, with the chunk that is
+// fetched past the last one.
+constexpr int64_t kMaxSlots = 0x7FFFFFFF - 256;
+// Beside the formats of knj_kv_cache: 4-bit pages (TreeArgs::pages).
+constexpr int kFormatPages = 16;
 uint64_t tree_partial_bytes(const knj_kv_cache& c, int type, int n_head, int n_rows, int max_prefix);
+// The same, enough for every type; 0 for sizes that are refused.
+uint64_t tree_workspace(const knj_kv_cache& c, int n_head, int n_rows, int max_prefix);
+// KNJ_E_ARG, with the reason, for arguments that `what` does not take (a.c has been checked).
+int check_tree(const TreeArgs& a, uint64_t workspace_bytes, const char* what);
 hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t s);
+
+// A 4-bit cache in pages: checked, with its sizes in bytes.
+struct PageGeom {
+  uint8_t* data;
+  int32_t *table, *refs;
+  int n_layer, n_page, shift, n_head_kv, head_dim, n_seq, n_table;  // page_size 1 << shift
+  __host__ __device__ int size() const { return 1 << shift; }
+  __host__ __device__ uint32_t head_bytes() const { return (uint32_t)(head_dim * 5 / 4) << shift; }
+  __host__ __device__ uint32_t page_bytes() const { return n_head_kv * head_bytes(); }
+};
+struct PageRowsArgs {
+  PageGeom g;
+  uint64_t layer;             // its bytes from data
+  void *k, *v;                // as KvRowsArgs
+  uint64_t row_stride;
+  const int32_t *index, *counts;
+  int n_rows;
+};
+hipError_t launch_pages_store(int type, const PageRowsArgs& a, hipStream_t s);
+hipError_t launch_pages_load(int type, const PageRowsArgs& a, hipStream_t s);
+struct PageReserveArgs {
+  PageGeom g;
+  const int32_t *start, *length, *want;
+  int32_t* missing;
+  int32_t* ws;                // page_workspace_ints
+};
+uint64_t page_workspace_ints(const PageGeom& g);
+hipError_t launch_pages_reserve(const PageReserveArgs& a, hipStream_t s);
+hipError_t launch_pages_fork(const PageGeom& g, const int32_t* parent, const int32_t* keep, int32_t* ws, hipStream_t s);
+hipError_t launch_pages_free(const PageGeom& g, const int32_t* keep, hipStream_t s);
+hipError_t launch_pages_compact(const PageGeom& g, const int32_t* start, const int32_t* rows, const int32_t* counts,
+                                int n_rows, hipStream_t s);
+hipError_t launch_pages_copy(const PageGeom& to, const PageGeom& from, const int32_t* dst, const int32_t* src, int n,
+                             hipStream_t s);
 
 struct LogprobArgs {
   const void* logits;

@@ -67,6 +67,29 @@ __device__ __forceinline__ uint32_t pack_act(float a, float b) {
            ((uint32_t)__builtin_bit_cast(unsigned short, (__bf16)b) << 16);
 }
 
+// Four consecutive activations as f32, and back.
+template <int TYPE>
+__device__ __forceinline__ float4 ld4(const void* p, uint64_t i) {
+  if constexpr (TYPE == KNJ_TYPE_F32) {
+    return *reinterpret_cast<const float4*>((const float*)p + i);
+  } else {
+    const uint2 u = *reinterpret_cast<const uint2*>((const uint16_t*)p + i);
+    if constexpr (TYPE == KNJ_TYPE_F16)
+      return make_float4(h2f(u.x), h2f(u.x >> 16), h2f(u.y), h2f(u.y >> 16));
+    else
+      return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
+                         __uint_as_float(u.y & 0xFFFF0000u));
+  }
+}
+
+template <int TYPE>
+__device__ __forceinline__ void st4(void* p, uint64_t i, float4 v) {
+  if constexpr (TYPE == KNJ_TYPE_F32)
+    *reinterpret_cast<float4*>((float*)p + i) = v;
+  else
+    *reinterpret_cast<uint2*>((uint16_t*)p + i) = make_uint2(pack_act<TYPE>(v.x, v.y), pack_act<TYPE>(v.z, v.w));
+}
+
 // ---- cross-lane moves without the LDS crossbar.  Rows of 16 lanes exchange
 // through DPP (quad permutes, the 8- and 16-lane mirrors, row rotation); rows
 // and half-waves through the gfx950 permlane swaps.  Every lane of the group

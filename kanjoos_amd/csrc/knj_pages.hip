@@ -1,0 +1,734 @@
+// kanjoos_amd/csrc/knj_pages.hip -- a 4-bit cache in pages: rows stored and read back, pages
+// reserved, shared, given back, moved together and copied.
+#include "knj_pages.h"
+
+#include <algorithm>
+#include <string>
+
+#include "knj_common.h"
+#include "knj_dev.h"
+
+namespace knj {
+namespace {
+
+using namespace dev;
+
+// ---------------------------------------------------------------- rows
+// A row's kv head is D/8 lanes of eight dims, four lanes a group of 32; the same lanes
+// take its key and its value.  blockIdx.y is the sequence.
+template <int D>
+struct PageUnit {
+  static constexpr int T = D / 8;
+  uint32_t t;  // row
+  int h, lane;
+  bool in;  // (the lanes past the last unit repeat it and store nothing)
+  __device__ __forceinline__ PageUnit(const PageRowsArgs& a) {
+    const uint32_t nk = a.g.n_head_kv, total = (uint32_t)a.n_rows * nk;
+    const uint32_t u = blockIdx.x * (kBlock / T) + threadIdx.x / T;
+    in = u < total;
+    const uint32_t v = in ? u : total - 1;
+    t = v / nk;
+    h = (int)(v - t * nk);
+    lane = threadIdx.x % T;
+  }
+};
+
+// Page of a sequence's slot, -1 if it has none.
+__device__ __forceinline__ int page_of(const PageGeom& g, uint32_t s, int64_t slot) {
+  if (slot < 0 || slot >= ((int64_t)g.n_table << g.shift)) return -1;
+  const int p = g.table[(uint64_t)s * g.n_table + (slot >> g.shift)];
+  return p >= 0 && p < g.n_page ? p : -1;
+}
+
+// Eight dims of a group held by four lanes as codes, and the group's word.
+// The f32 quotient is off by at most 16 * 2^-22 (x - low is rounded only where the two
+// are far apart, and then to 2^-24 of itself), which decides a rounding only next to a
+// tie: there it is formed in f64.
+__device__ __forceinline__ uint32_t quantise4(const float (&x)[8], uint32_t& word) {
+  float mn = x[0], mx = x[0];
+  bool bad = false;  // (of a NaN or what f16 does not hold)
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    mn = fminf(mn, x[i]);
+    mx = fmaxf(mx, x[i]);
+    bad |= !(fabsf(x[i]) <= 65504.0f);
+  }
+  mn = -group_max<4>(-mn);
+  mx = group_max<4>(mx);
+  bad = group_max<4>(bad ? 1.0f : 0.0f) != 0.0f;
+  const uint32_t low16 = f2h(mn + 0.0f);
+  const float low = h2f(low16);
+  // the quotient towards zero: to f32, then to f16
+  const double room = fmax(((double)mx - (double)low) / 15.0, 0.0);
+  float r = (float)room;
+  if ((double)r > room) r = __uint_as_float(__float_as_uint(r) - 1);
+  const uint32_t step16 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r, 0.0f)) & 0xFFFFu;
+  const float step = h2f(step16);
+  const bool live = !bad && step > 0.0f;
+  const float inv = live ? 1.0f / step : 0.0f;
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y = live ? (x[i] - low) * inv : 0.0f;
+    float t = rintf(y);
+    if (fabsf(fabsf(y - t) - 0.5f) < 1e-4f) t = (float)rint(((double)x[i] - (double)low) / (double)step);
+    w |= (uint32_t)fminf(fmaxf(t, 0.0f), 15.0f) << (4 * (i >> 1) + 16 * (i & 1));
+  }
+  word = bad ? kNanGroup : (low16 << 16) | step16;
+  return w;
+}
+
+template <int TYPE, int D>
+__global__ __launch_bounds__(kBlock) void k_pages_store(PageRowsArgs a) {
+  const PageGeom& g = a.g;
+  const PageUnit<D> u(a);
+  const uint32_t s = blockIdx.y;
+  const int64_t slot = (int64_t)a.index[s] + u.t;
+  const uint64_t at = ((uint64_t)s * a.n_rows + u.t) * a.row_stride + (uint64_t)u.h * D + 8 * u.lane;
+  const float4 k0 = ld4<TYPE>(a.k, at), k1 = ld4<TYPE>(a.k, at + 4);
+  const float4 v0 = ld4<TYPE>(a.v, at), v1 = ld4<TYPE>(a.v, at + 4);
+  const int page = u.in && (!a.counts || (int64_t)u.t < a.counts[s]) ? page_of(g, s, slot) : -1;
+  const float k[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
+  const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+  uint32_t km, vm;
+  const uint32_t kw = quantise4(k, km), vw = quantise4(v, vm);
+  if (page < 0) return;
+  using H = PageHead<D>;
+  uint8_t* to = g.data + a.layer + (uint64_t)page * g.page_bytes() + (uint64_t)u.h * g.head_bytes();
+  const uint32_t r = (uint32_t)slot & (g.size() - 1), c = r * H::kCode + 4 * u.lane, m = r * H::kMeta + u.lane;
+  *reinterpret_cast<uint32_t*>(to + H::codes(0, g.shift) + c) = kw;
+  *reinterpret_cast<uint32_t*>(to + H::codes(1, g.shift) + c) = vw;
+  if ((u.lane & 3) == 0) {
+    *reinterpret_cast<uint32_t*>(to + H::meta(0, g.shift) + m) = km;
+    *reinterpret_cast<uint32_t*>(to + H::meta(1, g.shift) + m) = vm;
+  }
+}
+
+template <int TYPE, int D>
+__global__ __launch_bounds__(kBlock) void k_pages_load(PageRowsArgs a) {
+  const PageGeom& g = a.g;
+  const PageUnit<D> u(a);
+  const uint32_t s = blockIdx.y;
+  const uint64_t out = (uint64_t)s * a.n_rows + u.t;
+  const int slot = a.index ? a.index[out] : (int)u.t;
+  const int page = u.in ? page_of(g, s, slot) : -1;
+  if (page < 0) return;
+  using H = PageHead<D>;
+  const uint8_t* from = g.data + a.layer + (uint64_t)page * g.page_bytes() + (uint64_t)u.h * g.head_bytes();
+  const uint32_t r = (uint32_t)slot & (g.size() - 1), c = r * H::kCode + 4 * u.lane, m = r * H::kMeta + (u.lane & ~3);
+  const uint64_t to = out * a.row_stride + (uint64_t)u.h * D + 8 * u.lane;
+  uint32_t w[2], meta[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    w[i] = *reinterpret_cast<const uint32_t*>(from + H::codes(i, g.shift) + c);
+    meta[i] = *reinterpret_cast<const uint32_t*>(from + H::meta(i, g.shift) + m);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    hx2 step, low;
+    group_word(meta[i], step, low);
+    const uint4 x = decode8(w[i], step, low);
+    st4<TYPE>(i ? a.v : a.k, to, make_float4(h2f(x.x), h2f(x.x >> 16), h2f(x.y), h2f(x.y >> 16)));
+    st4<TYPE>(i ? a.v : a.k, to + 4, make_float4(h2f(x.z), h2f(x.z >> 16), h2f(x.w), h2f(x.w >> 16)));
+  }
+}
+
+// ---------------------------------------------------------------- the table
+// Entries that slots below `slots` need.
+__device__ __forceinline__ int entries_of(const PageGeom& g, int slots) {
+  return (int)(((int64_t)max(slots, 0) + g.size() - 1) >> g.shift);
+}
+
+// Entry (s, e) of the forked table into the workspace, its holder counted.
+__global__ __launch_bounds__(kBlock) void k_pages_fork_read(PageGeom g, const int32_t* parent, const int32_t* keep,
+                                                            int32_t* ws) {
+  const uint32_t s = blockIdx.y, e = blockIdx.x * kBlock + threadIdx.x;
+  if (e >= (uint32_t)g.n_table) return;
+  const int p = parent[s];
+  int page = -1;
+  if (p >= 0 && p < g.n_seq && (!keep || (int)e < entries_of(g, keep[s]))) page = g.table[(uint64_t)p * g.n_table + e];
+  if (page < 0 || page >= g.n_page) page = -1;
+  ws[(uint64_t)s * g.n_table + e] = page;
+  if (page >= 0) atomicAdd(&g.refs[page], 1);
+}
+
+__global__ __launch_bounds__(kBlock) void k_pages_fork_write(PageGeom g, const int32_t* ws) {
+  const uint32_t s = blockIdx.y, e = blockIdx.x * kBlock + threadIdx.x;
+  if (e >= (uint32_t)g.n_table) return;
+  const uint64_t i = (uint64_t)s * g.n_table + e;
+  const int old = g.table[i];
+  if (old >= 0 && old < g.n_page) atomicSub(&g.refs[old], 1);
+  g.table[i] = ws[i];
+}
+
+__global__ __launch_bounds__(kBlock) void k_pages_free(PageGeom g, const int32_t* keep) {
+  const uint32_t s = blockIdx.y, e = blockIdx.x * kBlock + threadIdx.x;
+  const int n = keep[s];
+  if (e >= (uint32_t)g.n_table || n < 0 || (int)e < entries_of(g, n)) return;
+  const uint64_t i = (uint64_t)s * g.n_table + e;
+  const int old = g.table[i];
+  if (old >= 0 && old < g.n_page) atomicSub(&g.refs[old], 1);
+  g.table[i] = -1;
+}
+
+// Workspace of a reservation, in words: the copies' count and their (source,
+// destination, rows); of each page how many entries ask to replace it and the last of
+// them; the entries that get a free page, and the free pages, in order.
+struct ReserveWs {
+  int32_t *count, *copies, *asked, *last, *fresh, *unused;
+  __host__ __device__ ReserveWs(int32_t* p, int n_page)
+      : count(p), copies(p + 4), asked(copies + 3 * (uint64_t)n_page), last(asked + n_page), fresh(last + n_page),
+        unused(fresh + n_page) {}
+};
+
+constexpr int kMaxSeq = 4096, kPlan = 1024, kPlanWaves = kPlan / 64;
+
+// How many of the workgroup's flags are set before this thread's, and in all.
+__device__ __forceinline__ int flags_before(bool f, int* waves, int& total) {
+  const uint64_t b = __ballot(f);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __syncthreads();
+  if (lane == 0) waves[wave] = __popcll(b);
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < kPlanWaves; ++i) {
+    if (i < wave) before += waves[i];
+    total += waves[i];
+  }
+  return before + __popcll(b & ((1ull << lane) - 1));
+}
+
+__device__ __forceinline__ int ld_agent(const int32_t* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Which entries get which page, by one workgroup: the answer hangs on an order over all
+// sequences (lowest page first, all or none), and the entries of a step are few.  The
+// asked entries of all sequences are numbered through, and each thread takes every
+// 1024th.
+__global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
+  const PageGeom& g = a.g;
+  const ReserveWs ws(a.ws, g.n_page);
+  __shared__ int first[kMaxSeq + 1];  // asked entries of the sequences before
+  __shared__ int lowest[kMaxSeq];     // a sequence's first asked entry
+  __shared__ int waves[kPlanWaves], counts[64], n_copies;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+
+  int n_asked = 0;
+  for (int s0 = 0; s0 < g.n_seq; s0 += kPlan) {
+    const int s = s0 + tid;
+    int lo = 0, n = 0;
+    if (s < g.n_seq) {
+      const int want = a.want[s], from = max((a.start ? a.start : a.length)[s], 0);
+      lo = from >> g.shift;
+      n = want > from ? max(min(entries_of(g, want), g.n_table) - lo, 0) : 0;
+      lowest[s] = lo;
+    }
+    int sum = n;  // up to this lane
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int v = __shfl_up(sum, d);
+      if (lane >= d) sum += v;
+    }
+    __syncthreads();
+    if (lane == 63) waves[wave] = sum;
+    __syncthreads();
+    int before = n_asked;
+#pragma unroll
+    for (int i = 0; i < kPlanWaves; ++i) {
+      if (i < wave) before += waves[i];
+      n_asked += waves[i];
+    }
+    if (s < g.n_seq) first[s] = before + sum - n;
+  }
+  if (tid == 0) {
+    first[g.n_seq] = n_asked;
+    n_copies = 0;
+  }
+  __syncthreads();
+
+  // entry number f: its place in the table, and the page that it holds (-1: none)
+  auto entry = [&](int f, int& s, int& e) {
+    int lo = 0, hi = g.n_seq;  // first[lo] <= f < first[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (first[mid] <= f) lo = mid;
+      else hi = mid;
+    }
+    s = lo;
+    e = lowest[lo] + (f - first[lo]);
+    return s * g.n_table + e;
+  };
+  auto held = [&](int at) {
+    const int p = g.table[at];
+    return p >= 0 && p < g.n_page ? p : -1;
+  };
+  auto each_shared = [&](auto&& fn) {
+    for (int f = tid; f < n_asked; f += kPlan) {
+      int s, e;
+      const int at = entry(f, s, e), p = held(at);
+      if (p >= 0 && g.refs[p] > 1) fn(at, p);
+    }
+    __builtin_amdgcn_s_waitcnt(0);  // (stores, then atomics, of one page by several waves)
+    __syncthreads();
+  };
+  each_shared([&](int, int p) {
+    ws.asked[p] = 0;
+    ws.last[p] = -1;
+  });
+  each_shared([&](int at, int p) {
+    atomicAdd(&ws.asked[p], 1);
+    atomicMax(&ws.last[p], at);
+  });
+  int n_fresh = 0;
+  for (int f0 = 0; f0 < n_asked; f0 += kPlan) {
+    const int f = f0 + tid;
+    bool fresh = false;
+    int at = 0;
+    if (f < n_asked) {
+      int s, e;
+      at = entry(f, s, e);
+      const int p = held(at);
+      fresh = p < 0;
+      if (p >= 0 && g.refs[p] > 1) fresh = ld_agent(&ws.asked[p]) != g.refs[p] || ld_agent(&ws.last[p]) != at;
+    }
+    int n;
+    const int i = n_fresh + flags_before(fresh, waves, n);
+    if (fresh && i < g.n_page) ws.fresh[i] = f;
+    n_fresh += n;
+  }
+  // the free pages, in order, until there are enough: four in a row of 64 lanes at a time
+  int found = 0;
+  for (int p0 = 0; p0 < g.n_page && found < n_fresh; p0 += 4 * kPlan) {
+    uint64_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = p0 + wave * 256 + 64 * i + lane;
+      b[i] = __ballot(p < g.n_page && g.refs[p] <= 0);
+    }
+    __syncthreads();
+    if (lane < 4) counts[4 * wave + lane] = __popcll(lane == 0 ? b[0] : lane == 1 ? b[1] : lane == 2 ? b[2] : b[3]);
+    __syncthreads();
+    int sum = counts[lane];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int v = __shfl_up(sum, d);
+      if (lane >= d) sum += v;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = found + __shfl(sum, 4 * wave + i) - __popcll(b[i]) + __popcll(b[i] & ((1ull << lane) - 1));
+      if ((b[i] >> lane) & 1) ws.unused[at] = p0 + wave * 256 + 64 * i + lane;
+    }
+    found += __shfl(sum, 63);
+  }
+  __syncthreads();
+  if (found < n_fresh) {
+    if (tid == 0) {
+      *a.missing = n_fresh - found;
+      *ws.count = 0;
+    }
+    return;
+  }
+  for (int i = tid; i < n_fresh; i += kPlan) {
+    int s, e;
+    const int at = entry(ws.fresh[i], s, e), old = held(at), page = ws.unused[i];
+    g.table[at] = page;
+    g.refs[page] = 1;
+    if (old < 0) continue;
+    atomicSub(&g.refs[old], 1);
+    const int64_t rows = min((int64_t)a.length[s] - ((int64_t)e << g.shift), (int64_t)g.size());
+    if (rows <= 0) continue;
+    int32_t* c = ws.copies + 3 * (uint64_t)atomicAdd(&n_copies, 1);
+    c[0] = old;
+    c[1] = page;
+    c[2] = (int)rows;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    *a.missing = 0;
+    *ws.count = n_copies;
+  }
+}
+
+// The first rows of pages copied, a layer per blockIdx.y, kBlock units of a page a
+// workgroup: units of D/8 bytes, of a row four of key codes, four of value codes and one
+// of either's words.
+template <int D>
+__global__ __launch_bounds__(kBlock) void k_pages_cow(PageGeom g, int32_t* words, uint32_t pieces) {
+  using Piece = std::conditional_t<D == 128, uint4, uint2>;
+  const ReserveWs ws(words, g.n_page);
+  const uint64_t n = (uint64_t)*ws.count * pieces;
+  uint8_t* layer = g.data + (uint64_t)blockIdx.y * g.n_page * g.page_bytes();
+  for (uint64_t w = blockIdx.x; w < n; w += gridDim.x) {
+    const uint32_t i = (uint32_t)(w / pieces);
+    const uint32_t rows = ws.copies[3 * (uint64_t)i + 2], units = 10 * rows;
+    const uint32_t u = (uint32_t)(w - (uint64_t)i * pieces) * kBlock + threadIdx.x;
+    if (u >= units * g.n_head_kv) continue;
+    const Piece* from = reinterpret_cast<const Piece*>(layer + (uint64_t)ws.copies[3 * (uint64_t)i] * g.page_bytes());
+    Piece* to = reinterpret_cast<Piece*>(layer + (uint64_t)ws.copies[3 * (uint64_t)i + 1] * g.page_bytes());
+    const uint32_t h = u / units, r = u - h * units;
+    const uint32_t at = r < 4 * rows   ? r
+                        : r < 8 * rows ? (4u << g.shift) + r - 4 * rows
+                        : r < 9 * rows ? (8u << g.shift) + r - 8 * rows
+                                       : (9u << g.shift) + r - 9 * rows;
+    const uint32_t o = h * (10u << g.shift) + at;
+    to[o] = from[o];
+  }
+}
+
+// Rows moved together in place: a workgroup has one matrix of a layer's kv head of a
+// sequence and takes its rows in order, B at a time, which are read before any is written:
+// a row's new slot is at or below its old one, so that no row is overwritten before it
+// has been read.
+template <int D, int B>
+__global__ __launch_bounds__(B) void k_pages_compact(PageGeom g, const int32_t* start, const int32_t* rows,
+                                                     const int32_t* counts, int n_rows) {
+  using H = PageHead<D>;
+  using Piece = std::conditional_t<D == 128, uint4, uint2>;  // a quarter of a row's codes, or its words
+  const uint32_t s = blockIdx.z, h = blockIdx.x >> 1, v = blockIdx.x & 1;
+  const int n = counts ? min(max(counts[s], 0), n_rows) : n_rows;
+  const int64_t to0 = start[s];
+  const int tid = threadIdx.x;
+  uint8_t* head = g.data + (uint64_t)blockIdx.y * g.n_page * g.page_bytes() + (uint64_t)h * g.head_bytes();
+  __shared__ uint64_t src[B], dst[B];  // a row's piece numbers, all ones if it stays
+  constexpr uint64_t kStays = ~0ull;
+  for (int i0 = 0; i0 < n; i0 += B) {
+    const int i = i0 + tid;
+    uint64_t a = kStays, b = kStays;
+    if (i < n) {
+      const int from = rows[(uint64_t)s * n_rows + i];
+      const int64_t to = to0 + i;
+      const int p = page_of(g, s, from), q = page_of(g, s, to);
+      if (p >= 0 && q >= 0 && from != to) {
+        a = (uint64_t)p * g.page_bytes() / sizeof(Piece) + (from & (g.size() - 1));
+        b = (uint64_t)q * g.page_bytes() / sizeof(Piece) + (to & (g.size() - 1));
+      }
+    }
+    src[tid] = a;
+    dst[tid] = b;
+    __syncthreads();
+    const uint32_t codes = H::codes(v, g.shift) / sizeof(Piece), meta = H::meta(v, g.shift) / sizeof(Piece);
+    Piece* base = reinterpret_cast<Piece*>(head);
+    Piece x[4], m;
+    uint64_t to[4];
+    // (piece number of row r's codes: the page's, the block's and 4 r, of which a and b hold r)
+    auto code = [&](uint64_t at) { return (at & ~(uint64_t)(g.size() - 1)) + codes + 4 * (at & (g.size() - 1)); };
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = (tid + B * k) >> 2;
+      const uint64_t f = src[r];
+      to[k] = dst[r];
+      if (f != kStays) x[k] = base[code(f) + (tid & 3)];
+    }
+    if (a != kStays) m = base[a + meta];
+    __builtin_amdgcn_s_waitcnt(0);  // every row of the B has been read
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (to[k] != kStays) base[code(to[k]) + (tid & 3)] = x[k];
+    if (b != kStays) base[b + meta] = m;
+  }
+}
+
+// Whole pages, a layer per blockIdx.y: 16 KB a workgroup, four 16-byte loads a thread.
+constexpr int kCopyPiece = 4 * kBlock;  // of 16 bytes
+__global__ __launch_bounds__(kBlock) void k_pages_copy(PageGeom to, PageGeom from, const int32_t* dst, const int32_t* src,
+                                                       uint32_t pieces, uint64_t n) {
+  const uint32_t units = to.page_bytes() / 16;
+  for (uint64_t w = blockIdx.x; w < n; w += gridDim.x) {
+    const uint32_t i = (uint32_t)(w / pieces);
+    const int p = src[i], q = dst[i];
+    if (p < 0 || p >= from.n_page || q < 0 || q >= to.n_page) continue;
+    const uint4* f = reinterpret_cast<const uint4*>(from.data + ((uint64_t)blockIdx.y * from.n_page + p) * from.page_bytes());
+    uint4* t = reinterpret_cast<uint4*>(to.data + ((uint64_t)blockIdx.y * to.n_page + q) * to.page_bytes());
+    const uint32_t u0 = (uint32_t)(w - (uint64_t)i * pieces) * kCopyPiece + threadIdx.x;
+    uint4 x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (u0 + k * kBlock < units) x[k] = f[u0 + k * kBlock];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (u0 + k * kBlock < units) t[u0 + k * kBlock] = x[k];
+  }
+}
+
+dim3 page_rows_grid(const PageRowsArgs& a) {
+  const uint32_t units = (uint32_t)a.n_rows * a.g.n_head_kv, per = kBlock / (a.g.head_dim / 8);
+  return dim3((units + per - 1) / per, a.g.n_seq);
+}
+dim3 table_grid(const PageGeom& g) { return dim3((g.n_table + kBlock - 1) / kBlock, g.n_seq); }
+
+}  // namespace
+
+#define KNJ_PAGE_ROWS(KERNEL)                                                                       \
+  do {                                                                                              \
+    const dim3 grid = page_rows_grid(a);                                                            \
+    if (type == KNJ_TYPE_F32) KNJ_PAGE_DIM(KERNEL, KNJ_TYPE_F32);                                   \
+    else if (type == KNJ_TYPE_F16) KNJ_PAGE_DIM(KERNEL, KNJ_TYPE_F16);                              \
+    else KNJ_PAGE_DIM(KERNEL, KNJ_TYPE_BF16);                                                       \
+    return hipGetLastError();                                                                       \
+  } while (0)
+#define KNJ_PAGE_DIM(KERNEL, TYPE)                                                                  \
+  do {                                                                                              \
+    if (a.g.head_dim == 128) KNJ_LAUNCH((KERNEL<TYPE, 128>), grid, dim3(kBlock), 0, s, a);          \
+    else KNJ_LAUNCH((KERNEL<TYPE, 64>), grid, dim3(kBlock), 0, s, a);                               \
+  } while (0)
+
+hipError_t launch_pages_store(int type, const PageRowsArgs& a, hipStream_t s) { KNJ_PAGE_ROWS(k_pages_store); }
+hipError_t launch_pages_load(int type, const PageRowsArgs& a, hipStream_t s) { KNJ_PAGE_ROWS(k_pages_load); }
+
+uint64_t page_workspace_ints(const PageGeom& g) {
+  return std::max<uint64_t>(4 + 7 * (uint64_t)g.n_page, (uint64_t)g.n_seq * g.n_table);
+}
+
+hipError_t launch_pages_reserve(const PageReserveArgs& a, hipStream_t s) {
+  KNJ_LAUNCH(k_pages_plan, dim3(1), dim3(kPlan), 0, s, a);
+  // (how many pages are copied is known on the device only: as many workgroups as a page
+  // of each sequence needs, to a chipful)
+  const uint32_t pieces = (a.g.page_bytes() / (a.g.head_dim / 8) + kBlock - 1) / kBlock;
+  const uint64_t want = std::min<uint64_t>((uint64_t)pieces * a.g.n_seq, 8192 / a.g.n_layer);
+  const dim3 grid((uint32_t)std::max<uint64_t>(want, 1), a.g.n_layer);
+  if (a.g.head_dim == 128) KNJ_LAUNCH(k_pages_cow<128>, grid, dim3(kBlock), 0, s, a.g, a.ws, pieces);
+  else KNJ_LAUNCH(k_pages_cow<64>, grid, dim3(kBlock), 0, s, a.g, a.ws, pieces);
+  return hipGetLastError();
+}
+
+hipError_t launch_pages_fork(const PageGeom& g, const int32_t* parent, const int32_t* keep, int32_t* ws, hipStream_t s) {
+  KNJ_LAUNCH(k_pages_fork_read, table_grid(g), dim3(kBlock), 0, s, g, parent, keep, ws);
+  KNJ_LAUNCH(k_pages_fork_write, table_grid(g), dim3(kBlock), 0, s, g, ws);
+  return hipGetLastError();
+}
+
+hipError_t launch_pages_free(const PageGeom& g, const int32_t* keep, hipStream_t s) {
+  KNJ_LAUNCH(k_pages_free, table_grid(g), dim3(kBlock), 0, s, g, keep);
+  return hipGetLastError();
+}
+
+hipError_t launch_pages_compact(const PageGeom& g, const int32_t* start, const int32_t* rows, const int32_t* counts,
+                                int n_rows, hipStream_t s) {
+  const dim3 grid(2 * g.n_head_kv, g.n_layer, g.n_seq);
+#define KNJ_PAGE_COMPACT(D, B) \
+  KNJ_LAUNCH((k_pages_compact<D, B>), grid, dim3(B), 0, s, g, start, rows, counts, n_rows)
+  if (g.head_dim == 128) {
+    if (n_rows <= 64) KNJ_PAGE_COMPACT(128, 64);
+    else KNJ_PAGE_COMPACT(128, 256);
+  } else {
+    if (n_rows <= 64) KNJ_PAGE_COMPACT(64, 64);
+    else KNJ_PAGE_COMPACT(64, 256);
+  }
+#undef KNJ_PAGE_COMPACT
+  return hipGetLastError();
+}
+
+hipError_t launch_pages_copy(const PageGeom& to, const PageGeom& from, const int32_t* dst, const int32_t* src, int n,
+                             hipStream_t s) {
+  const uint32_t pieces = (to.page_bytes() / 16 + kCopyPiece - 1) / kCopyPiece;
+  const uint64_t work = (uint64_t)pieces * n;
+  KNJ_LAUNCH(k_pages_copy, dim3((uint32_t)std::min<uint64_t>(work, 1 << 20), to.n_layer), dim3(kBlock), 0, s, to, from,
+             dst, src, pieces, work);
+  return hipGetLastError();
+}
+
+}  // namespace knj
+
+using namespace knj;
+
+// The cache that the attention's sizes are taken from.
+static knj_kv_cache page_cache(const PageGeom& g) {
+  return {nullptr, nullptr, nullptr, nullptr, 0, kFormatPages, g.n_seq, g.n_head_kv, g.n_table << g.shift, g.head_dim};
+}
+
+// KNJ_E_ARG, with the reason, for sizes that are not a pool's; pointers are not looked at.
+static int check_page_sizes(const knj_kv_pages* p) {
+  KNJ_CHECK_ARG(p, "null pages");
+  KNJ_CHECK_ARG(p->head_dim == 64 || p->head_dim == 128, "head_dim must be 64 or 128");
+  KNJ_CHECK_ARG(p->page_size >= 16 && p->page_size <= 256 && (p->page_size & (p->page_size - 1)) == 0,
+                "page_size must be a power of two from 16 to 256");
+  KNJ_CHECK_ARG(p->n_head_kv > 0 && p->n_head_kv <= 64, "n_head_kv must be in [1, 64]");
+  KNJ_CHECK_ARG(p->n_layer > 0 && p->n_layer <= 1024, "n_layer must be in [1, 1024]");
+  KNJ_CHECK_ARG(p->n_page > 0 && p->n_page < (1 << 26), "n_page must be in [1, 2^26)");
+  KNJ_CHECK_ARG(p->n_seq > 0 && p->n_seq <= kMaxSeq, "n_seq must be in [1, 4096]");
+  KNJ_CHECK_ARG(p->n_table > 0 && (int64_t)p->n_table * p->page_size < kMaxSlots,
+                "n_table must be positive and its slots fewer than 2^31 - 256");
+  KNJ_CHECK_ARG((int64_t)p->n_seq * p->n_table < (1ll << 31), "the table must have fewer than 2^31 entries");
+  return KNJ_OK;
+}
+
+static int check_pages(const knj_kv_pages* p, bool table, bool refs) {
+  const int rc = check_page_sizes(p);
+  if (rc) return rc;
+  KNJ_CHECK_ARG(p->data && (!table || p->table) && (!refs || p->refs), "null pointer in the pages");
+  KNJ_CHECK_ARG(((uintptr_t)p->data & 15) == 0, "page data must be 16-byte aligned");
+  KNJ_CHECK_ARG(words_aligned(p->table, p->refs), "table and refs must be aligned to their type");
+  return KNJ_OK;
+}
+
+static PageGeom geom(const knj_kv_pages& p) {
+  int shift = 4;
+  while ((1 << shift) < p.page_size) ++shift;
+  return {(uint8_t*)p.data, p.table, p.refs, p.n_layer, p.n_page, shift, p.n_head_kv, p.head_dim, p.n_seq, p.n_table};
+}
+
+static uint64_t layer_at(const PageGeom& g, int layer) { return (uint64_t)layer * g.n_page * g.page_bytes(); }
+
+static int check_page_rows(const knj_kv_pages* pages, int layer, int type, const void* k, const void* v,
+                           uint64_t row_stride, int n_rows) {
+  const int rc = check_pages(pages, true, false);
+  if (rc) return rc;
+  const int eb = act_bytes(type);
+  KNJ_CHECK_ARG(layer >= 0 && layer < pages->n_layer, "the layer must be in [0, n_layer)");
+  KNJ_CHECK_ARG(eb, "activations must be F32, F16 or BF16");
+  KNJ_CHECK_ARG(k && v, "null pointer");
+  KNJ_CHECK_ARG(n_rows >= 0, "negative row count");
+  KNJ_CHECK_ARG(row_stride >= (uint64_t)pages->n_head_kv * pages->head_dim, "the row stride is below the row's width");
+  KNJ_CHECK_ARG(rows_aligned(k, row_stride, eb) && rows_aligned(v, row_stride, eb),
+                "rows must start on 16-byte boundaries");
+  KNJ_CHECK_ARG((uint64_t)n_rows * pages->n_head_kv < (1ull << 27), "too many rows for one call");
+  return KNJ_OK;
+}
+
+static int check_page_workspace(const knj_kv_pages* pages, const void* workspace, uint64_t bytes, const char* what) {
+  const uint64_t need = page_workspace_ints(geom(*pages)) * sizeof(int32_t);
+  if (workspace && bytes >= need && words_aligned((const char*)workspace)) return KNJ_OK;
+  set_error(std::string(what) + ": these sizes need a 4-byte aligned workspace of " + std::to_string(need) + " bytes");
+  return KNJ_E_ARG;
+}
+
+extern "C" {
+
+uint64_t knj_pages_bytes(const knj_kv_pages* pages) {
+  if (check_page_sizes(pages)) return 0;
+  const PageGeom g = geom(*pages);
+  return layer_at(g, g.n_layer);
+}
+
+uint64_t knj_pages_workspace(const knj_kv_pages* pages) {
+  return check_page_sizes(pages) ? 0 : page_workspace_ints(geom(*pages)) * sizeof(int32_t);
+}
+
+int knj_pages_store(const knj_kv_pages* pages, int layer, int type, const void* k, const void* v,
+                    uint64_t row_stride, const int32_t* start, const int32_t* counts, int n_rows,
+                    void* stream) {
+  int rc = check_page_rows(pages, layer, type, k, v, row_stride, n_rows);
+  if (rc) return rc;
+  KNJ_CHECK_ARG(start, "null start");
+  KNJ_CHECK_ARG(words_aligned(start, counts), "start and counts must be aligned to their type");
+  rc = require_device();
+  if (rc || n_rows == 0) return rc;
+  const PageGeom g = geom(*pages);
+  KNJ_HIP(launch_pages_store(type, {g, layer_at(g, layer), const_cast<void*>(k), const_cast<void*>(v), row_stride, start,
+                                    counts, n_rows}, (hipStream_t)stream));
+  return KNJ_OK;
+}
+
+int knj_pages_load(const knj_kv_pages* pages, int layer, int type, const int32_t* slots,
+                   int n_rows, void* k, void* v, uint64_t row_stride, void* stream) {
+  int rc = check_page_rows(pages, layer, type, k, v, row_stride, n_rows);
+  if (rc) return rc;
+  KNJ_CHECK_ARG(words_aligned(slots), "slots must be aligned to their type");
+  rc = require_device();
+  if (rc || n_rows == 0) return rc;
+  const PageGeom g = geom(*pages);
+  KNJ_HIP(launch_pages_load(type, {g, layer_at(g, layer), k, v, row_stride, slots, nullptr, n_rows},
+                            (hipStream_t)stream));
+  return KNJ_OK;
+}
+
+int knj_pages_reserve(const knj_kv_pages* pages, const int32_t* start, const int32_t* length,
+                      const int32_t* want, int32_t* missing, void* workspace,
+                      uint64_t workspace_bytes, void* stream) {
+  int rc = check_pages(pages, true, true);
+  if (rc) return rc;
+  KNJ_CHECK_ARG(length && want && missing, "null pointer");
+  KNJ_CHECK_ARG(words_aligned(start, length, want, missing), "start, length, want and missing must be aligned to their type");
+  rc = check_page_workspace(pages, workspace, workspace_bytes, "knj_pages_reserve");
+  if (rc) return rc;
+  rc = require_device();
+  if (rc) return rc;
+  KNJ_HIP(launch_pages_reserve({geom(*pages), start, length, want, missing, (int32_t*)workspace}, (hipStream_t)stream));
+  return KNJ_OK;
+}
+
+int knj_pages_fork(const knj_kv_pages* pages, const int32_t* parent, const int32_t* keep,
+                   void* workspace, uint64_t workspace_bytes, void* stream) {
+  int rc = check_pages(pages, true, true);
+  if (rc) return rc;
+  KNJ_CHECK_ARG(parent, "null pointer");
+  KNJ_CHECK_ARG(words_aligned(parent, keep), "parent and keep must be aligned to their type");
+  rc = check_page_workspace(pages, workspace, workspace_bytes, "knj_pages_fork");
+  if (rc) return rc;
+  rc = require_device();
+  if (rc) return rc;
+  KNJ_HIP(launch_pages_fork(geom(*pages), parent, keep, (int32_t*)workspace, (hipStream_t)stream));
+  return KNJ_OK;
+}
+
+int knj_pages_free(const knj_kv_pages* pages, const int32_t* keep, void* stream) {
+  int rc = check_pages(pages, true, true);
+  if (rc) return rc;
+  KNJ_CHECK_ARG(keep, "null pointer");
+  KNJ_CHECK_ARG(words_aligned(keep), "keep must be aligned to its type");
+  rc = require_device();
+  if (rc) return rc;
+  KNJ_HIP(launch_pages_free(geom(*pages), keep, (hipStream_t)stream));
+  return KNJ_OK;
+}
+
+int knj_pages_compact(const knj_kv_pages* pages, const int32_t* start, const int32_t* rows,
+                      const int32_t* counts, int n_rows, void* stream) {
+  int rc = check_pages(pages, true, false);
+  if (rc) return rc;
+  KNJ_CHECK_ARG(start && rows, "null pointer");
+  KNJ_CHECK_ARG(words_aligned(start, rows, counts), "start, rows and counts must be aligned to their type");
+  KNJ_CHECK_ARG(n_rows >= 0 && n_rows < kMaxSlots, "n_rows must be in [0, 2^31 - 256)");
+  rc = require_device();
+  if (rc || n_rows == 0) return rc;
+  KNJ_HIP(launch_pages_compact(geom(*pages), start, rows, counts, n_rows, (hipStream_t)stream));
+  return KNJ_OK;
+}
+
+int knj_pages_copy(const knj_kv_pages* to, const knj_kv_pages* from, const int32_t* dst,
+                   const int32_t* src, int n, void* stream) {
+  int rc = check_pages(to, false, false);
+  if (!rc) rc = check_pages(from, false, false);
+  if (rc) return rc;
+  KNJ_CHECK_ARG(to->n_layer == from->n_layer && to->page_size == from->page_size && to->n_head_kv == from->n_head_kv &&
+                    to->head_dim == from->head_dim,
+                "the pools must have the same n_layer, page_size, n_head_kv and head_dim");
+  KNJ_CHECK_ARG(dst && src, "null pointer");
+  KNJ_CHECK_ARG(words_aligned(dst, src), "dst and src must be aligned to their type");
+  KNJ_CHECK_ARG(n >= 0 && n < (1 << 24), "n must be in [0, 2^24)");
+  rc = require_device();
+  if (rc || n == 0) return rc;
+  KNJ_HIP(launch_pages_copy(geom(*to), geom(*from), dst, src, n, (hipStream_t)stream));
+  return KNJ_OK;
+}
+
+int knj_attention_pages(const knj_kv_pages* pages, int layer, int type, const void* q,
+                        uint64_t q_stride, int n_head, int n_rows, const int32_t* prefix,
+                        int max_prefix, const int32_t* counts, const uint64_t* mask,
+                        int mask_shared, float scale, void* out, uint64_t out_stride,
+                        void* workspace, uint64_t workspace_bytes, void* stream) {
+  int rc = check_pages(pages, true, false);
+  if (rc) return rc;
+  KNJ_CHECK_ARG(layer >= 0 && layer < pages->n_layer, "the layer must be in [0, n_layer)");
+  const PageGeom g = geom(*pages);
+  TreeArgs a{page_cache(g), q, out, q_stride, out_stride, prefix, counts, mask, (float*)workspace, scale,
+             n_head, n_rows, max_prefix, mask_shared, type, g.data + layer_at(g, layer), g.table, g.n_page, g.n_table,
+             g.shift};
+  rc = check_tree(a, workspace_bytes, "knj_attention_pages");
+  if (rc) return rc;
+  rc = require_device();
+  if (rc || n_rows == 0) return rc;
+  KNJ_HIP(launch_attention_tree(a, (hipStream_t)stream));
+  return KNJ_OK;
+}
+
+uint64_t knj_attention_pages_workspace(const knj_kv_pages* pages, int n_head, int n_rows, int max_prefix) {
+  return check_page_sizes(pages) ? 0 : tree_workspace(page_cache(geom(*pages)), n_head, n_rows, max_prefix);
+}
+
+}  // extern "C"

@@ -17,30 +17,6 @@ namespace {
 
 using namespace dev;
 
-// Eight consecutive activations as f32 (16-byte aligned rows; 4 at a time for
-// the halves of a rotation).
-template <int TYPE>
-__device__ __forceinline__ float4 ld4(const void* p, uint64_t i) {
-  if constexpr (TYPE == KNJ_TYPE_F32) {
-    return *reinterpret_cast<const float4*>((const float*)p + i);
-  } else {
-    const uint2 u = *reinterpret_cast<const uint2*>((const uint16_t*)p + i);
-    if constexpr (TYPE == KNJ_TYPE_F16)
-      return make_float4(h2f(u.x), h2f(u.x >> 16), h2f(u.y), h2f(u.y >> 16));
-    else
-      return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
-                         __uint_as_float(u.y & 0xFFFF0000u));
-  }
-}
-
-template <int TYPE>
-__device__ __forceinline__ void st4(void* p, uint64_t i, float4 v) {
-  if constexpr (TYPE == KNJ_TYPE_F32)
-    *reinterpret_cast<float4*>((float*)p + i) = v;
-  else
-    *reinterpret_cast<uint2*>((uint16_t*)p + i) = make_uint2(pack_act<TYPE>(v.x, v.y), pack_act<TYPE>(v.z, v.w));
-}
-
 // ---------------------------------------------------------------- rotary positions
 // y = R(pos) (x / sqrt(mean x^2 + eps) * w).  A lane holds both elements of its
 // four pairs: elements 4c.. of the rotated part's two halves (HALF) or eight
@@ -487,10 +463,6 @@ int knj_kv_load(const knj_kv_cache* cache, int type, const int32_t* slots, int n
   return KNJ_OK;
 }
 
-// Slots of a sequence that the attention numbers in 32 bits, with the chunk that is
-// fetched past the last one.
-static constexpr int64_t kMaxSlots = 0x7FFFFFFF - 256;
-
 int knj_attention_tree(const knj_kv_cache* cache, int type, const void* q, uint64_t q_stride,
                        int n_head, int n_rows, const int32_t* prefix, int max_prefix,
                        const int32_t* counts, const uint64_t* mask, int mask_shared, float scale,
@@ -498,45 +470,18 @@ int knj_attention_tree(const knj_kv_cache* cache, int type, const void* q, uint6
                        void* stream) {
   int rc = check_kv_cache(cache);
   if (rc) return rc;
-  const int eb = act_bytes(type);
-  KNJ_CHECK_ARG(eb, "activations must be F32, F16 or BF16");
-  KNJ_CHECK_ARG(q && out && prefix, "null pointer");
-  KNJ_CHECK_ARG(words_aligned(prefix, counts) && ((uintptr_t)mask & 7) == 0,
-                "prefix, counts and mask must be aligned to their types");
-  KNJ_CHECK_ARG(n_rows >= 0 && n_rows <= 1024, "n_rows must be in [0, 1024]");
-  KNJ_CHECK_ARG(n_head > 0 && n_head <= 1024 && n_head % cache->n_head_kv == 0,
-                "n_head must be a positive multiple of n_head_kv, at most 1024");
-  KNJ_CHECK_ARG(max_prefix >= 0 && (int64_t)max_prefix + n_rows <= cache->n_ctx,
-                "max_prefix and the drafts must fit into n_ctx");
-  KNJ_CHECK_ARG((int64_t)max_prefix + n_rows <= kMaxSlots, "max_prefix and the drafts must stay below 2^31 - 256");
-  KNJ_CHECK_ARG(scale >= 1e-6f && scale <= 1e6f, "the scale must be in [1e-6, 1e6]");
-  KNJ_CHECK_ARG((uint64_t)cache->n_seq * n_rows * n_head < (1ull << 31), "too many rows for one call");
-  const uint64_t width = (uint64_t)n_head * cache->head_dim;
-  KNJ_CHECK_ARG(q_stride >= width && out_stride >= width, "a row stride is below the row's width");
-  KNJ_CHECK_ARG(rows_aligned(q, q_stride, eb) && rows_aligned(out, out_stride, eb),
-                "rows must start on 16-byte boundaries");
-  KNJ_CHECK_ARG(q != out || q_stride == out_stride || (uint64_t)cache->n_seq * n_rows <= 1,
-                "an output in place takes its input's stride");
-  const uint64_t need = n_rows ? tree_partial_bytes(*cache, type, n_head, n_rows, max_prefix) : 0;
-  if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) {
-    set_error("knj_attention_tree: these sizes need a 16-byte aligned workspace of " + std::to_string(need) + " bytes");
-    return KNJ_E_ARG;
-  }
-  rc = require_device();
-  if (rc || n_rows == 0) return rc;
   TreeArgs a{with_stride(*cache), q, out, q_stride, out_stride, prefix, counts, mask, (float*)workspace, scale,
              n_head, n_rows, max_prefix, mask_shared, type};
+  rc = check_tree(a, workspace_bytes, "knj_attention_tree");
+  if (rc) return rc;
+  rc = require_device();
+  if (rc || n_rows == 0) return rc;
   KNJ_HIP(launch_attention_tree(a, (hipStream_t)stream));
   return KNJ_OK;
 }
 
 uint64_t knj_attention_tree_workspace(const knj_kv_cache* cache, int n_head, int n_rows, int max_prefix) {
-  if (check_kv_cache(cache) || n_head <= 0 || n_head > 1024 || n_head % cache->n_head_kv || n_rows <= 0 ||
-      n_rows > 1024 || max_prefix < 0 || (int64_t)max_prefix + n_rows > std::min<int64_t>(cache->n_ctx, kMaxSlots))
-    return 0;
-  // (enough for every type)
-  return std::max(tree_partial_bytes(*cache, KNJ_TYPE_F32, n_head, n_rows, max_prefix),
-                  tree_partial_bytes(*cache, KNJ_TYPE_F16, n_head, n_rows, max_prefix));
+  return check_kv_cache(cache) ? 0 : tree_workspace(*cache, n_head, n_rows, max_prefix);
 }
 
 }  // extern "C"

@@ -12,6 +12,7 @@
 #include "knj_common.h"
 #include "knj_dev.h"
 #include "knj_mfma.h"
+#include "knj_pages.h"
 
 namespace knj {
 
@@ -128,6 +129,12 @@ __device__ __forceinline__ uint4 lds_b128(uint32_t p) {
   return __builtin_bit_cast(uint4, *(lds_v4*)(uintptr_t)p);
 }
 
+__device__ __forceinline__ void lds_put_b128(uint32_t p, uint4 v) {
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) u32x4 lds_v4;
+  *(lds_v4*)(uintptr_t)p = __builtin_bit_cast(u32x4, v);
+}
+
 // Four results as activations.
 __device__ __forceinline__ uint2 pack4(int type, float4 v) {
   if (type == KNJ_TYPE_F16) return make_uint2(pack_act<KNJ_TYPE_F16>(v.x, v.y), pack_act<KNJ_TYPE_F16>(v.z, v.w));
@@ -208,9 +215,9 @@ typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 // chunk's DMA behind this one's reads (1 to 5 % slower).
 template <int D, int FORMAT, bool SPLIT, int NT, int WC, int WS, int SW>
 __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p) {
-  constexpr bool Q8 = FORMAT != KNJ_KV_F16;
+  constexpr bool PAGES = FORMAT == kFormatPages, Q8 = FORMAT == KNJ_KV_F8 || FORMAT == KNJ_KV_I8;
   constexpr int NW = WC * WS, NTH = 64 * NW, C = WS * SW, COLS = WC * NT * 16, ST = SW / 16;
-  constexpr int RB = Q8 ? D : 2 * D;                     // bytes of a cache row
+  constexpr int RB = Q8 ? D : 2 * D;                     // bytes of a chunk's row in LDS
   constexpr int RPB = 256 / RB, NSLOT = RB / 16, NPAIR = RB / 32, CB = C * RB;
   constexpr int NI = CB / 1024 / NW;                     // 1 KB DMA instructions per wave and matrix
   constexpr int SB = 2 * CB + (Q8 ? 8 * C : 0);          // bytes of a stage: K, V, scales of both
@@ -270,8 +277,57 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
            __builtin_amdgcn_readfirstlane(lds_addr(lds + st * SB + 2 * CB + wave % (2 * C / 64) * 256)));
     }
   };
+  // ---- chunk j of 4-bit pages: fetched into registers as it is, group by group, and put
+  // into a stage as f16 rows, permuted as above.  A thread has NG groups, of one slot:
+  // its key's and its value's, or with D 64, where there are half as many, one of them.
+  // The slot's page is looked up a chunk ahead of its fetch.
+  constexpr int GROUPS = C * D / 32, NG = 2 * GROUPS / NTH;  // groups of a matrix, and of a thread
+  static_assert(!PAGES || NG == 2 || NG == 1, "a thread's groups are of one slot");
+  using H = PageHead<D>;
+  const int pg = tid % GROUPS, prow = pg / (D / 32), pgroup = pg % (D / 32), pmat = NG == 1 ? tid / GROUPS : 0;
+  const int last_entry = a.n_table - 1;
+  int page = 0;  // of the next chunk to fetch
+  uint4 pcode[NG];
+  uint32_t pword[NG];
+  auto look_up = [&](int j) {
+    const int e = min((j * C + prow) >> a.page_shift, last_entry);
+    page = a.table[(uint64_t)s * a.n_table + e];
+  };
+  auto fetch = [&](int j) {
+    const bool in = page >= 0 && page < a.n_page;
+    const uint32_t head = H::kSlot << a.page_shift;
+    const uint8_t* at = a.pages + ((uint64_t)(in ? page : 0) * nk + kvh) * head;
+    const uint32_t row = (j * C + prow) & ((1 << a.page_shift) - 1);
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const int v = NG == 1 ? pmat : i;
+      pcode[i] = *reinterpret_cast<const uint4*>(at + H::codes(v, a.page_shift) + row * H::kCode + 16 * pgroup);
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(at + H::meta(v, a.page_shift) + row * H::kMeta + 4 * pgroup);
+      pword[i] = in ? w : kNanGroup;
+    }
+  };
+  auto put = [&](int st) {
+    const uint32_t to = lds_addr(lds + st * SB) + prow * RB;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const int v = NG == 1 ? pmat : i;
+      hx2 step, low;
+      group_word(pword[i], step, low);
+      const uint32_t perm = v ? ((prow / RPB) & (NPAIR - 1)) << 1 : (prow / RPB) & (NSLOT - 1);
+      const uint32_t c[4] = {pcode[i].x, pcode[i].y, pcode[i].z, pcode[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        lds_put_b128(to + (v ? CB : 0) + 16 * ((4 * pgroup + k) ^ perm), decode8(c[k], step, low));
+    }
+  };
   const int c0 = split * p.cps;
-  dma(c0, 0);
+  if constexpr (PAGES) {
+    look_up(c0);
+    fetch(c0);
+    look_up(c0 + 1);
+  } else {
+    dma(c0, 0);
+  }
 
   // ---- this lane's query columns.  Step c's dims 8 kq .. + 7 of 32; with 8 bits,
   // where a 16-byte piece of a K row is two steps', dims 64 (c/2) + 16 kq + 8 (c%2)
@@ -583,9 +639,18 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
   // then refills (past the range: fetched and not used).  A third stage, a chunk more
   // ahead, was 4 % slower (one draft over 32K int8 slots).
   int j = c0, stage = 0;
+  // With 4-bit pages chunk j + 1, fetched while j - 1 was computed, is put there now and
+  // j + 2 is fetched.
   auto ready = [&]() {
-    KNJ_BARRIER_AFTER(vm_lds_imm(0));
-    dma(j + 1, stage ^ 1);
+    if constexpr (PAGES) {
+      KNJ_BARRIER_AFTER(kLdsOnly);
+      put(stage ^ 1);
+      fetch(j + 2);
+      look_up(j + 3);
+    } else {
+      KNJ_BARRIER_AFTER(vm_lds_imm(0));
+      dma(j + 1, stage ^ 1);
+    }
   };
   auto next = [&]() {
     ++j;
@@ -593,6 +658,11 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
     if (j < c1) ready();
   };
   const int j_prefix = min(c1, P / C);  // chunks below lie in the prefix
+  if constexpr (PAGES) {
+    put(0);
+    fetch(c0 + 1);
+    look_up(c0 + 2);
+  }
   ready();
   while (j < c1) {
     // ---- the first chunk, those that reach the drafts or the end, and those of the

@@ -1,5 +1,6 @@
 // kanjoos_amd/csrc/knj_tree.hip -- plan, merge and launch of the drafts' attention.
 #include <algorithm>
+#include <string>
 
 #include "knj_tree.h"
 
@@ -12,6 +13,8 @@ template <>
 hipError_t launch_format<KNJ_KV_F8>(const TreeArgs&, const TreePlan&, int, hipStream_t);
 template <>
 hipError_t launch_format<KNJ_KV_I8>(const TreeArgs&, const TreePlan&, int, hipStream_t);
+template <>
+hipError_t launch_format<kFormatPages>(const TreeArgs&, const TreePlan&, int, hipStream_t);
 
 // Merge of a (draft, head)'s split records: M = max m, out = sum acc 2^(m - M) /
 // sum l 2^(m - M).  Thread = four dims of every NP-th split, eight splits' loads at
@@ -152,12 +155,49 @@ uint64_t tree_partial_bytes(const knj_kv_cache& c, int type, int n_head, int n_r
   return (uint64_t)q.p.units * q.p.n_tiles * q.cols * (c.head_dim + 4) * sizeof(float);
 }
 
+uint64_t tree_workspace(const knj_kv_cache& c, int n_head, int n_rows, int max_prefix) {
+  if (n_head <= 0 || n_head > 1024 || n_head % c.n_head_kv || n_rows <= 0 || n_rows > 1024 || max_prefix < 0 ||
+      (int64_t)max_prefix + n_rows > std::min<int64_t>(c.n_ctx, kMaxSlots))
+    return 0;
+  return std::max(tree_partial_bytes(c, KNJ_TYPE_F32, n_head, n_rows, max_prefix),
+                  tree_partial_bytes(c, KNJ_TYPE_F16, n_head, n_rows, max_prefix));
+}
+
+int check_tree(const TreeArgs& a, uint64_t workspace_bytes, const char* what) {
+  const int eb = act_bytes(a.type);
+  KNJ_CHECK_ARG(eb, "activations must be F32, F16 or BF16");
+  KNJ_CHECK_ARG(a.q && a.out && a.prefix, "null pointer");
+  KNJ_CHECK_ARG(words_aligned(a.prefix, a.counts) && ((uintptr_t)a.mask & 7) == 0,
+                "prefix, counts and mask must be aligned to their types");
+  KNJ_CHECK_ARG(a.n_rows >= 0 && a.n_rows <= 1024, "n_rows must be in [0, 1024]");
+  KNJ_CHECK_ARG(a.n_head > 0 && a.n_head <= 1024 && a.n_head % a.c.n_head_kv == 0,
+                "n_head must be a positive multiple of n_head_kv, at most 1024");
+  KNJ_CHECK_ARG(a.max_prefix >= 0 && (int64_t)a.max_prefix + a.n_rows <= a.c.n_ctx,
+                "max_prefix and the drafts must fit into n_ctx");
+  KNJ_CHECK_ARG((int64_t)a.max_prefix + a.n_rows <= kMaxSlots, "max_prefix and the drafts must stay below 2^31 - 256");
+  KNJ_CHECK_ARG(a.scale >= 1e-6f && a.scale <= 1e6f, "the scale must be in [1e-6, 1e6]");
+  KNJ_CHECK_ARG((uint64_t)a.c.n_seq * a.n_rows * a.n_head < (1ull << 31), "too many rows for one call");
+  const uint64_t width = (uint64_t)a.n_head * a.c.head_dim;
+  KNJ_CHECK_ARG(a.q_stride >= width && a.out_stride >= width, "a row stride is below the row's width");
+  KNJ_CHECK_ARG(rows_aligned(a.q, a.q_stride, eb) && rows_aligned(a.out, a.out_stride, eb),
+                "rows must start on 16-byte boundaries");
+  KNJ_CHECK_ARG(a.q != a.out || a.q_stride == a.out_stride || (uint64_t)a.c.n_seq * a.n_rows <= 1,
+                "an output in place takes its input's stride");
+  const uint64_t need = a.n_rows ? tree_partial_bytes(a.c, a.type, a.n_head, a.n_rows, a.max_prefix) : 0;
+  if (need && (!a.partial || workspace_bytes < need || ((uintptr_t)a.partial & 15))) {
+    set_error(std::string(what) + ": these sizes need a 16-byte aligned workspace of " + std::to_string(need) + " bytes");
+    return KNJ_E_ARG;
+  }
+  return KNJ_OK;
+}
+
 hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t s) {
   const tree::Planned q = tree::plan(a.c, a.type, a.n_head, a.n_rows, a.max_prefix);
   hipError_t e;
   if (a.c.format == KNJ_KV_F16) e = tree::launch_format<KNJ_KV_F16>(a, q.p, q.cols, s);
   else if (a.c.format == KNJ_KV_F8) e = tree::launch_format<KNJ_KV_F8>(a, q.p, q.cols, s);
-  else e = tree::launch_format<KNJ_KV_I8>(a, q.p, q.cols, s);
+  else if (a.c.format == KNJ_KV_I8) e = tree::launch_format<KNJ_KV_I8>(a, q.p, q.cols, s);
+  else e = tree::launch_format<kFormatPages>(a, q.p, q.cols, s);
   if (e != hipSuccess || q.p.n_split == 1) return e;
   // Few outputs or many splits: the splits over a workgroup's parts, for latency (one
   // draft over 4000 f16 slots 10.4 us a call, 16.8 with one part; 8 over 32K int8 28.9
