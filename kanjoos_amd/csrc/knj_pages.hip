@@ -123,11 +123,12 @@ __global__ __launch_bounds__(kBlock) void k_pages_load(PageRowsArgs a) {
     w[i] = *reinterpret_cast<const uint32_t*>(from + H::codes(i, g.shift) + c);
     meta[i] = *reinterpret_cast<const uint32_t*>(from + H::meta(i, g.shift) + m);
   }
+  const Decoder decode;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     hx2 step, low;
     group_word(meta[i], step, low);
-    const uint4 x = decode8(w[i], step, low);
+    const uint4 x = decode.eight(w[i], step, low);
     st4<TYPE>(i ? a.v : a.k, to, make_float4(h2f(x.x), h2f(x.x >> 16), h2f(x.y), h2f(x.y >> 16)));
     st4<TYPE>(i ? a.v : a.k, to + 4, make_float4(h2f(x.z), h2f(x.z >> 16), h2f(x.w), h2f(x.w >> 16)));
   }

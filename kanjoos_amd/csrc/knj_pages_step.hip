@@ -1,0 +1,347 @@
+// kanjoos_amd/csrc/knj_pages_step.hip -- attention over 4-bit pages for up to 16 columns a kv
+// head (a column is a row and a query head): decode steps and short chains of drafts.
+#include "knj_tree.h"
+
+namespace knj {
+namespace tree {
+namespace {
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// Eight weights as f16 high parts and remainders, two to an instruction.
+__device__ __forceinline__ void split8(const float (&w)[8], h16x8& hi, h16x8& lo) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const hx2 h = __builtin_convertvector(f32x2{w[i], w[i + 1]}, hx2);
+    const f32x2 r = {fmaf((float)h[0], -1.0f, w[i]), fmaf((float)h[1], -1.0f, w[i + 1])};
+    const hx2 l = __builtin_convertvector(r, hx2);
+    hi[i] = h[0];
+    hi[i + 1] = h[1];
+    lo[i] = l[0];
+    lo[i + 1] = l[1];
+  }
+}
+
+// The halves of a word that are infinite or NaN (0x7C00 and up) replaced by zero; the sign
+// bits of those that were.
+__device__ __forceinline__ uint32_t clear_nonfinite(uint32_t& w) {
+  const uint32_t m = ((w & 0x7FFF7FFFu) + 0x04000400u) & 0x80008000u;
+  w &= ~(m | (m - (m >> 15)));
+  return m;
+}
+
+// Workgroup = (sequence, split of the slots, kv head) of four waves that take its tiles of
+// 32 slots in turn, each by itself: no barrier until the end.  A lane (r = l % 16, kq =
+// l / 16) loads the part kq of rows r and 16 + r, decodes it, and
+//   scores  S[slot][col] = K (16 slots x 32 dims) x Q, keys from registers (a step's dims
+//           are D/4 kq + 8 c ..: whichever order, as long as the queries have the same);
+//   values  O^T[d][col] = V^T (16 dims x 32 slots) x E, the decoded rows through 8 KB of
+//           LDS of the wave's own, read back transposed.
+// The weights' reference, split and the records are k_tree's.
+// f32 queries take the registers of a fourth wave a SIMD.
+template <int D, bool SPLIT>
+__global__ __launch_bounds__(64 * kStepWaves, SPLIT ? 3 : 4) void k_pages_step(TreeArgs a, TreePlan p) {
+  using H = PageHead<D>;
+  constexpr int NW = kStepWaves;
+  constexpr int DT = D / 16, NC = D / 32;
+  constexpr int RS = 2 * D + 32;       // from a row in LDS to the next: 8 rows' 32 bytes on banks of their own
+  constexpr int LW = kStepTile * RS;   // bytes of a wave's LDS
+  using Codes = std::conditional_t<D == 128, uint4, uint2>;
+  __shared__ __align__(1024) uint8_t lds[NW * LW];
+  __shared__ float2 stats[NW][16];
+
+  const int nk = a.c.n_head_kv, G = p.by_group.d;
+  const int unit = blockIdx.y * gridDim.x + blockIdx.x;
+  if (unit >= p.units) return;
+  const int rest = p.by_nk.div(unit), kvh = unit - rest * nk;
+  const int s = p.by_split.div(rest), split = rest - s * p.n_split;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, kq = lane >> 4;
+
+  // ---- a tile's rows as they are: of one matrix, fetched again as soon as the tile before
+  // has been decoded.  The next tile's pages are looked up a tile ahead.
+  // (what is constant while the kernel runs, by scalar loads, whatever asm lies between)
+  typedef __attribute__((address_space(4))) const int32_t* Const;
+  const Const table = (Const)(uintptr_t)(a.table + (uint64_t)s * a.n_table);
+  const int given = ((Const)(uintptr_t)a.prefix)[s], count = a.counts ? ((Const)(uintptr_t)a.counts)[s] : a.n_rows;
+  const int shift = a.page_shift, last = a.n_table - 1;
+  const uint32_t head = (uint32_t)H::kSlot << shift;
+  const uint32_t codes_at = r * H::kCode + (D / 8) * kq, words_at = r * H::kMeta + (D == 128 ? 4 * kq : 4 * (kq >> 1));
+  struct Rows {
+    Codes c[2];
+    uint32_t w[2];
+    bool in[2];  // (of the whole wave: a slot without a page holds NaN)
+  };
+  int page[2];             // of the next tile, and what follows from them:
+  const uint8_t* base[2];  // its pages, and their first rows
+  uint32_t row[2];
+  bool in[2];
+  auto look_up = [&](int j) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st) page[st] = table[min((j * kStepTile + 16 * st) >> shift, last)];
+  };
+  auto place = [&](int j) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      in[st] = (uint32_t)page[st] < (uint32_t)a.n_page;
+      base[st] = a.pages + (uint64_t)(uint32_t)((in[st] ? page[st] : 0) * nk + kvh) * head;
+      row[st] = (j * kStepTile + 16 * st) & ((1 << shift) - 1);
+    }
+  };
+  auto load = [&](int v, Rows& t) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      t.in[st] = in[st];
+      const uint8_t* codes = base[st] + (H::codes(v, shift) + row[st] * H::kCode);
+      const uint8_t* words = base[st] + (H::meta(v, shift) + row[st] * H::kMeta);
+      // (scalar base and 32-bit offset: hoisted, the widened offset would take a register more)
+      uint32_t c = codes_at, w = words_at;
+      asm volatile("" : "+v"(c), "+v"(w));
+      t.c[st] = *reinterpret_cast<const Codes*>(codes + c);
+      t.w[st] = *reinterpret_cast<const uint32_t*>(words + w);
+    }
+  };
+  Rows K, V;
+  const int P = min(max(given, 0), a.max_prefix), N = min(max(count, 0), a.n_rows);
+  const int valid = P + N, n_cols = 16;
+  const int tiles = (valid + kStepTile - 1) / kStepTile, cps = p.even_cps(tiles);
+  const int c0 = split * cps, c1 = min(tiles, c0 + cps);
+  if (N == 0 || c0 >= c1) return;  // (all waves)
+  int j = c0 + wave;
+  look_up(j);
+  place(j);
+  load(1, V);
+  load(0, K);
+  look_up(j + NW < c1 ? j + NW : j);
+
+  // ---- the queries, read row by row (a lane's own parts of its column lie in 64 lines) and
+  // handed round in LDS.  Scaled by a power of two per column, as in k_tree.
+  constexpr int QS = 2 * D + 16, QP = D / 8;  // from a column to the next in LDS; pieces of eight of a column
+  static_assert((SPLIT ? 2 : 1) * 16 * QS <= NW * LW, "the queries fit");
+  __shared__ float scales[16];
+  if (threadIdx.x < 16 * QP) {
+    const int qc = threadIdx.x / QP, piece = threadIdx.x % QP, c = min(qc, a.n_rows * G - 1), t = p.by_group.div(c);
+    const uint64_t at = ((uint64_t)s * a.n_rows + t) * a.q_stride + (uint64_t)(kvh * G + c - t * G) * D + 8 * piece;
+    float4 x, y;
+    if constexpr (SPLIT) {
+      x = ld4<KNJ_TYPE_F32>(a.q, at);
+      y = ld4<KNJ_TYPE_F32>(a.q, at + 4);
+    } else if (a.type == KNJ_TYPE_F16) {
+      x = ld4<KNJ_TYPE_F16>(a.q, at);
+      y = ld4<KNJ_TYPE_F16>(a.q, at + 4);
+    } else {
+      x = ld4<KNJ_TYPE_BF16>(a.q, at);
+      y = ld4<KNJ_TYPE_BF16>(a.q, at + 4);
+    }
+    float am = fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))),
+                     fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+    am = group_max<QP>(am);
+    const int e = min(max((int)(__float_as_uint(am) >> 23) - 127, -126), 126);
+    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+    if (piece == 0)
+      scales[qc] = fminf(a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + e) << 23), 0x1.fffffep127f);
+    // (in decode8_mixed's order)
+    const float q[8] = {x.x * down, y.x * down, x.y * down, y.y * down, x.z * down, y.z * down, x.w * down, y.w * down};
+    h16x8 hi, lo;
+    split8(q, hi, lo);
+    lds_put_b128(lds_addr(lds) + qc * QS + 16 * piece, __builtin_bit_cast(uint4, hi));
+    if constexpr (SPLIT) lds_put_b128(lds_addr(lds) + 16 * QS + qc * QS + 16 * piece, __builtin_bit_cast(uint4, lo));
+  }
+  KNJ_BARRIER_AFTER(kLdsOnly);
+  const int trow = p.by_group.div(min(r, a.n_rows * G - 1));
+  h16x8 qh[NC], ql[SPLIT ? NC : 1];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    qh[c] = __builtin_bit_cast(h16x8, lds_b128(lds_addr(lds) + r * QS + 16 * (NC * kq + c)));
+    if constexpr (SPLIT) ql[c] = __builtin_bit_cast(h16x8, lds_b128(lds_addr(lds) + 16 * QS + r * QS + 16 * (NC * kq + c)));
+  }
+  const float s2 = scales[r];
+  KNJ_BARRIER_AFTER(kLdsOnly);
+  float m = -INFINITY, l = 0.0f;
+  bool spoilt = false;
+  f32x4 acc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const int words = (a.n_rows + 63) / 64;
+  const uint64_t* mask = a.mask ? a.mask + (a.mask_shared ? 0 : (uint64_t)s * a.n_rows) * words : nullptr;
+
+  const uint32_t mine = lds_addr(lds + wave * LW);
+  const uint32_t put = mine + r * RS + (D / 2) * kq, get = mine + (4 * kq + (r >> 2)) * RS + 8 * (r & 3);
+
+  auto words_of = [](const Codes& c, int i) {
+    if constexpr (D == 128) return i == 0 ? c.x : i == 1 ? c.y : i == 2 ? c.z : c.w;
+    else return i == 0 ? c.x : c.y;
+  };
+  for (; j < c1; j += NW) {
+    // (after the last tile it is fetched once more: loads on every path are waited for by
+    // their count, those on some only all at once)
+    const int next = j + NW < c1 ? j + NW : j;
+    const int p0 = j * kStepTile;
+    const bool drafts = p0 + kStepTile > P;
+    // the values' rows to LDS; beyond the prefix what is not finite there is dropped, and
+    // the rows that held it noted (slots past the rows are zeros)
+    uint32_t bad = 0;
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      hx2 step, low;
+      const int slot = p0 + 16 * st + r;
+      group_word(drafts && slot >= valid ? 0u : V.in[st] ? V.w[st] : kNanGroup, step, low);
+      uint4 x[NC];
+#pragma unroll
+      for (int i = 0; i < NC; ++i) x[i] = decode8_mixed(words_of(V.c[st], i), step, low);
+      if (drafts) {
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+          any |= clear_nonfinite(x[i].x) | clear_nonfinite(x[i].y) | clear_nonfinite(x[i].z) | clear_nonfinite(x[i].w);
+        // (of the prefix's rows in the tile too: every column sees them)
+        const uint64_t b = __ballot(any != 0);
+        bad |= (uint32_t)((b | b >> 16 | b >> 32 | b >> 48) & 0xFFFF) << (16 * st);
+      }
+#pragma unroll
+      for (int i = 0; i < NC; ++i) lds_put_b128(put + 16 * st * RS + 16 * i, x[i]);
+    }
+    place(next);
+    load(1, V);
+    __builtin_amdgcn_sched_barrier(0);
+    // scores, in units of 1 / s2
+    f32x4 sc[2];
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      sc[st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      hx2 step, low;
+      group_word(K.in[st] ? K.w[st] : kNanGroup, step, low);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const h16x8 ka = __builtin_bit_cast(h16x8, decode8_mixed(words_of(K.c[st], c), step, low));
+        sc[st] = mfma16(ka, qh[c], sc[st]);
+        if constexpr (SPLIT) sc[st] = mfma16(ka, ql[c], sc[st]);
+      }
+    }
+    load(0, K);
+    look_up(j + 2 * NW < c1 ? j + 2 * NW : j + NW);
+    __builtin_amdgcn_sched_barrier(0);
+    if (drafts) {
+      const uint64_t seen = seen64(mask ? mask + trow * words : nullptr, words, trow, N, p0 - P);
+      spoilt |= ((uint32_t)seen & bad) != 0;
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!((seen >> (16 * st + 4 * kq + i)) & 1)) sc[st][i] = -INFINITY;
+    }
+    // the reference moves where a score has passed it by kLag (a NaN or +inf carries)
+    float mx = max_nan(max_nan(max_nan(sc[0][0], sc[0][1]), max_nan(sc[0][2], sc[0][3])),
+                       max_nan(max_nan(sc[1][0], sc[1][1]), max_nan(sc[1][2], sc[1][3])));
+    const bool over = !(fmaf(mx, s2, -m) <= kLag) && m < INFINITY;
+    if (__ballot(over) != 0) {
+      const float2 m16 = pair16_f(mx);
+      mx = max_nan(m16.x, m16.y);
+      const float2 m32 = pair32_f(mx);
+      mx = max_nan(m32.x, m32.y);
+      const float old = m;
+      if (!(fmaf(mx, s2, -old) <= kLag)) m = max_nan(old, fmaf(mx, s2, -kLift));
+      const float alpha = __builtin_amdgcn_exp2f(old - (m == -INFINITY ? 0.0f : m));
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[dt][i] *= alpha;
+    }
+    // (the reference is -inf while the column has seen nothing: exponents then from 0)
+    const float mr = m == -INFINITY ? 0.0f : m;
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      w[i] = __builtin_amdgcn_exp2f(fmaf(sc[i >> 2][i & 3], s2, -mr));
+      l += w[i];
+    }
+    h16x8 eh, el;
+    split8(w, eh, el);
+    // four tiles of dims at a time, read before they are multiplied
+#pragma unroll
+    for (int b0 = 0; b0 < DT; b0 += 4) {
+      u32x2 v[4][2];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        v[b][0] = lds_tr16_at(get + 32 * (b0 + b));
+        v[b][1] = lds_tr16_at(get + 32 * (b0 + b) + 16 * RS);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const h16x8 vv = __builtin_bit_cast(h16x8, make_uint4(v[b][0].x, v[b][0].y, v[b][1].x, v[b][1].y));
+        acc[b0 + b] = mfma16(vv, eh, acc[b0 + b]);
+        acc[b0 + b] = mfma16(vv, el, acc[b0 + b]);
+      }
+    }
+  }
+
+  // ---- the waves joined: each leaves its columns in its own LDS, each takes dims of all
+  l += xor16_f(l);
+  l += xor32_f(l);
+  if (spoilt) l = NAN;
+  float4* mine4 = reinterpret_cast<float4*>(lds + wave * LW);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) {
+    // dims 0 4 1 5 of eight in the lanes of an even kq and 2 6 3 7 in those of kq + 1: 0 1 2 3
+    // and 4 5 6 7 by exchanges of 16 lanes with the next 16
+    const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[dt][0]), __float_as_uint(acc[dt][1]), false, false);
+    const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[dt][2]), __float_as_uint(acc[dt][3]), false, false);
+    mine4[64 * dt + lane] = make_float4(__uint_as_float(x[0]), __uint_as_float(y[0]), __uint_as_float(x[1]), __uint_as_float(y[1]));
+  }
+  if (kq == 0) stats[wave][r] = make_float2(m, l);
+  __syncthreads();
+  float M = -INFINITY, L = 0.0f, f[NW];
+#pragma unroll
+  for (int w = 0; w < NW; ++w) M = fmaxf(M, stats[w][r].x);
+  const float mr = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    const float2 ml = stats[w][r];
+    f[w] = __builtin_amdgcn_exp2f(ml.x - mr);
+    L += ml.y * f[w];
+  }
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // nothing seen: zeros
+  const int ocol = r;
+  if (ocol >= N * G) return;
+  for (int dt = wave; dt < DT; dt += NW) {
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float4 x = reinterpret_cast<const float4*>(lds + w * LW)[64 * dt + lane];
+      o = make_float4(o.x + x.x * f[w], o.y + x.y * f[w], o.z + x.z * f[w], o.w + x.w * f[w]);
+    }
+    const int d = 16 * dt + 4 * kq;
+    if (p.n_split > 1) {
+      float* rec = a.partial + ((((uint64_t)s * nk + kvh) * p.n_split + split) * n_cols + ocol) * (D + 4);
+      if (dt == 0 && kq == 0) *reinterpret_cast<float2*>(rec) = make_float2(M, L);
+      *reinterpret_cast<float4*>(rec + 4 + d) = o;
+      continue;
+    }
+    o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    const uint64_t to = ((uint64_t)s * a.n_rows + trow) * a.out_stride + (uint64_t)(kvh * G + ocol - trow * G) * D + d;
+    if constexpr (SPLIT) *reinterpret_cast<float4*>((float*)a.out + to) = o;
+    else *reinterpret_cast<uint2*>((uint16_t*)a.out + to) = pack4(a.type, o);
+  }
+}
+
+}  // namespace
+
+hipError_t launch_pages_step(const TreeArgs& a, const TreePlan& p, hipStream_t s) {
+  const unsigned y = (p.units + 65534u) / 65535u, x = (p.units + y - 1) / y;
+#define KNJ_STEP(DD, SPLIT) KNJ_LAUNCH((k_pages_step<DD, SPLIT>), dim3(x, y), dim3(64 * kStepWaves), 0, s, a, p)
+  const bool split = a.type == KNJ_TYPE_F32;
+  if (a.c.head_dim == 128) {
+    if (split) KNJ_STEP(128, true);
+    else KNJ_STEP(128, false);
+  } else {
+    if (split) KNJ_STEP(64, true);
+    else KNJ_STEP(64, false);
+  }
+#undef KNJ_STEP
+  return hipGetLastError();
+}
+
+}  // namespace tree
+}  // namespace knj

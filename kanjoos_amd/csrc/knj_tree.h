@@ -29,6 +29,10 @@ struct FastDiv {
   __device__ __forceinline__ uint32_t div(uint32_t n) const { return m ? __umulhi(n, m) >> sh : n; }
 };
 
+// Attention over 4-bit pages for up to 16 columns a kv head: workgroups of kStepWaves waves
+// that take tiles of kStepTile slots in turn.
+constexpr int kStepTile = 32, kStepWaves = 4;
+
 struct TreePlan {
   int cps;       // chunks per split of the slots
   int n_split;   // splits of the longest sequence
@@ -36,6 +40,13 @@ struct TreePlan {
   int units;     // n_seq * n_split * n_head_kv
   FastDiv by_nk, by_split, by_group;  // n_head_kv, n_split, query heads per kv head
   FastDiv by_head, by_rows, by_cps;   // n_head, n_rows, cps
+  bool even;     // of launch_pages_step: a sequence's own tiles are split evenly
+  // Tiles per split of a sequence: a multiple of the waves that take them in turn, and as
+  // many as it has splits for, so that a batch's shorter sequences keep as many workgroups
+  // busy as its longest.
+  __device__ __forceinline__ int even_cps(int tiles) const {
+    return max(((int)by_split.div(tiles + n_split - 1) + kStepWaves - 1) & -kStepWaves, kStepWaves);
+  }
 };
 
 namespace tree {
@@ -289,21 +300,22 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
   int page = 0;  // of the next chunk to fetch
   uint4 pcode[NG];
   uint32_t pword[NG];
+  const Decoder decode;
+  bool pin = false;  // (a slot without a page holds NaN)
   auto look_up = [&](int j) {
     const int e = min((j * C + prow) >> a.page_shift, last_entry);
     page = a.table[(uint64_t)s * a.n_table + e];
   };
   auto fetch = [&](int j) {
-    const bool in = page >= 0 && page < a.n_page;
+    pin = page >= 0 && page < a.n_page;
     const uint32_t head = H::kSlot << a.page_shift;
-    const uint8_t* at = a.pages + ((uint64_t)(in ? page : 0) * nk + kvh) * head;
+    const uint8_t* at = a.pages + ((uint64_t)(pin ? page : 0) * nk + kvh) * head;
     const uint32_t row = (j * C + prow) & ((1 << a.page_shift) - 1);
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
       const int v = NG == 1 ? pmat : i;
       pcode[i] = *reinterpret_cast<const uint4*>(at + H::codes(v, a.page_shift) + row * H::kCode + 16 * pgroup);
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(at + H::meta(v, a.page_shift) + row * H::kMeta + 4 * pgroup);
-      pword[i] = in ? w : kNanGroup;
+      pword[i] = *reinterpret_cast<const uint32_t*>(at + H::meta(v, a.page_shift) + row * H::kMeta + 4 * pgroup);
     }
   };
   auto put = [&](int st) {
@@ -312,12 +324,12 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
     for (int i = 0; i < NG; ++i) {
       const int v = NG == 1 ? pmat : i;
       hx2 step, low;
-      group_word(pword[i], step, low);
+      group_word(pin ? pword[i] : kNanGroup, step, low);
       const uint32_t perm = v ? ((prow / RPB) & (NPAIR - 1)) << 1 : (prow / RPB) & (NSLOT - 1);
       const uint32_t c[4] = {pcode[i].x, pcode[i].y, pcode[i].z, pcode[i].w};
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        lds_put_b128(to + (v ? CB : 0) + 16 * ((4 * pgroup + k) ^ perm), decode8(c[k], step, low));
+        lds_put_b128(to + (v ? CB : 0) + 16 * ((4 * pgroup + k) ^ perm), decode.eight(c[k], step, low));
     }
   };
   const int c0 = split * p.cps;
@@ -950,6 +962,8 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
     }
   }
 }
+
+hipError_t launch_pages_step(const TreeArgs& a, const TreePlan& p, hipStream_t s);
 
 // One launch of a format's kernel: D, split and the column tile's shape at run
 // time (columns per kv head up to 16, 32, 64 or more).

@@ -51,7 +51,14 @@ __global__ __launch_bounds__(kBlock) void k_tree_merge(TreeArgs a, TreePlan p, i
   fetch(0);
   int P, N;
   seq_lengths(a, s, P, N);
-  const int chunks = (P + N + chunk - 1) / chunk, used = p.by_cps.div(chunks + p.cps - 1);
+  const int chunks = (P + N + chunk - 1) / chunk;
+  int used;
+  if (p.even) {
+    const int cps = p.even_cps(chunks);
+    used = (chunks + cps - 1) / cps;
+  } else {
+    used = p.by_cps.div(chunks + p.cps - 1);
+  }
   float M = -INFINITY, L = 0.0f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = 0; i0 < used; i0 += B * NP) {
@@ -110,7 +117,8 @@ constexpr int kTreeChunk = 64;  // slots of a chunk in every shape
 
 struct Planned {
   TreePlan p;
-  int cols;  // columns of a tile
+  int cols;   // columns of a tile
+  int chunk;  // slots of a split's chunks
 };
 
 // Tiles of 32 columns (16 where there are no more) finish a chunk soonest; wider ones
@@ -129,8 +137,26 @@ struct Planned {
 // 4 drafts over 8,000 f16 slots (504) 16.8 against 12.5.
 constexpr int64_t kWideWork = 10000, kWideWorkF16 = 16000, kTwoWork = 2500;  // chunks of 32-column tiles, chunks of tiles
 
+// Of launch_pages_step.  A wave's tile takes 1.0 us and a merge 3: one workgroup a unit up to
+// four tiles a wave (32 sequences of 500 slots 10.2 us against 12.3 in four splits, 8 of
+// 200 7.4 against 9.6 in two; 32 of 2000, 16 tiles a wave, 22.9 against 17.1).  Else two
+// workgroups a CU (32 of 8000: 39.8 us; with one, three and four 44.6, 39.8 and 40.8) in up
+// to 64 splits, one batch of the merge's loads (one sequence of 32,700: 13.9; in 128 splits
+// 16.9, in 256 23.6).
+constexpr int kStepMerges = 16;
+Planned plan_step(const knj_kv_cache& c, int n_head, int n_rows, int max_prefix) {
+  const int tiles = (max_prefix + n_rows + kStepTile - 1) / kStepTile;
+  const int64_t units = (int64_t)c.n_seq * c.n_head_kv;
+  const int n_split = tiles <= kStepMerges ? 1 : (int)std::min<int64_t>({std::max<int64_t>(512 / units, 1), 64, tiles / kStepWaves});
+  const FastDiv none(1);
+  return {TreePlan{0, n_split, 1, (int)(units * n_split), FastDiv(c.n_head_kv), FastDiv(n_split),
+                   FastDiv(n_head / c.n_head_kv), FastDiv(n_head), FastDiv(n_rows), none, true},
+          16, kStepTile};
+}
+
 Planned plan(const knj_kv_cache& c, int type, int n_head, int n_rows, int max_prefix) {
   const int group = n_head / c.n_head_kv, n_cols = n_rows * group;
+  if (c.format == kFormatPages && n_cols <= 16) return plan_step(c, n_head, n_rows, max_prefix);
   const int chunks = (max_prefix + n_rows + kTreeChunk - 1) / kTreeChunk;
   const int64_t units = (int64_t)c.n_seq * c.n_head_kv;
   int cols = n_cols <= 16 ? 16 : 32;
@@ -142,8 +168,8 @@ Planned plan(const knj_kv_cache& c, int type, int n_head, int n_rows, int max_pr
   const int cps = (int)std::max<int64_t>(1, (chunks + want - 1) / want);
   const int n_split = (chunks + cps - 1) / cps;
   return {TreePlan{cps, n_split, tiles, (int)(units * n_split), FastDiv(c.n_head_kv), FastDiv(n_split), FastDiv(group),
-                   FastDiv(n_head), FastDiv(n_rows), FastDiv(cps)},
-          cols};
+                   FastDiv(n_head), FastDiv(n_rows), FastDiv(cps), false},
+          cols, kTreeChunk};
 }
 
 }  // namespace
@@ -194,7 +220,8 @@ int check_tree(const TreeArgs& a, uint64_t workspace_bytes, const char* what) {
 hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t s) {
   const tree::Planned q = tree::plan(a.c, a.type, a.n_head, a.n_rows, a.max_prefix);
   hipError_t e;
-  if (a.c.format == KNJ_KV_F16) e = tree::launch_format<KNJ_KV_F16>(a, q.p, q.cols, s);
+  if (q.p.even) e = tree::launch_pages_step(a, q.p, s);
+  else if (a.c.format == KNJ_KV_F16) e = tree::launch_format<KNJ_KV_F16>(a, q.p, q.cols, s);
   else if (a.c.format == KNJ_KV_F8) e = tree::launch_format<KNJ_KV_F8>(a, q.p, q.cols, s);
   else if (a.c.format == KNJ_KV_I8) e = tree::launch_format<KNJ_KV_I8>(a, q.p, q.cols, s);
   else e = tree::launch_format<kFormatPages>(a, q.p, q.cols, s);
@@ -208,7 +235,7 @@ hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t s) {
   const bool wide = n_out <= 512 || q.p.n_split > 8;
 #define KNJ_TREE_MERGE(DD, NP)                                                                                  \
   KNJ_LAUNCH((tree::k_tree_merge<DD, NP>), dim3((n_out + 1024 / (DD) / (NP) - 1) / (1024 / (DD) / (NP))),        \
-             dim3(dev::kBlock), 0, s, a, q.p, tree::kTreeChunk, n_cols, n_out)
+             dim3(dev::kBlock), 0, s, a, q.p, q.chunk, n_cols, n_out)
   if (a.c.head_dim == 128) {
     if (wide) KNJ_TREE_MERGE(128, 8);
     else KNJ_TREE_MERGE(128, 1);
