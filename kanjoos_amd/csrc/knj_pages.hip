@@ -13,6 +13,13 @@ namespace {
 
 using namespace dev;
 
+// Pieces of D/8 bytes: of a row four of codes a matrix and one of words.  (Vectors of the
+// compiler's own: arrays of its structs, loaded under a condition, end up in LDS.)
+typedef uint32_t u32v4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32v2 __attribute__((ext_vector_type(2)));
+template <int D>
+using Piece = std::conditional_t<D == 128, u32v4, u32v2>;
+
 // ---------------------------------------------------------------- rows
 // A row's kv head is D/8 lanes of eight dims, four lanes a group of 32; the same lanes
 // take its key and its value.  blockIdx.y is the sequence.
@@ -140,7 +147,8 @@ __device__ __forceinline__ int entries_of(const PageGeom& g, int slots) {
   return (int)(((int64_t)max(slots, 0) + g.size() - 1) >> g.shift);
 }
 
-// Entry (s, e) of the forked table into the workspace, its holder counted.
+// Entry (s, e) of the forked table into the workspace, its holder counted (where another page
+// comes: beams share most of theirs with their parents already).
 __global__ __launch_bounds__(kBlock) void k_pages_fork_read(PageGeom g, const int32_t* parent, const int32_t* keep,
                                                             int32_t* ws) {
   const uint32_t s = blockIdx.y, e = blockIdx.x * kBlock + threadIdx.x;
@@ -150,16 +158,17 @@ __global__ __launch_bounds__(kBlock) void k_pages_fork_read(PageGeom g, const in
   if (p >= 0 && p < g.n_seq && (!keep || (int)e < entries_of(g, keep[s]))) page = g.table[(uint64_t)p * g.n_table + e];
   if (page < 0 || page >= g.n_page) page = -1;
   ws[(uint64_t)s * g.n_table + e] = page;
-  if (page >= 0) atomicAdd(&g.refs[page], 1);
+  if (page >= 0 && page != g.table[(uint64_t)s * g.n_table + e]) atomicAdd(&g.refs[page], 1);
 }
 
 __global__ __launch_bounds__(kBlock) void k_pages_fork_write(PageGeom g, const int32_t* ws) {
   const uint32_t s = blockIdx.y, e = blockIdx.x * kBlock + threadIdx.x;
   if (e >= (uint32_t)g.n_table) return;
   const uint64_t i = (uint64_t)s * g.n_table + e;
-  const int old = g.table[i];
+  const int old = g.table[i], page = ws[i];
+  if (old == page) return;
   if (old >= 0 && old < g.n_page) atomicSub(&g.refs[old], 1);
-  g.table[i] = ws[i];
+  g.table[i] = page;
 }
 
 __global__ __launch_bounds__(kBlock) void k_pages_free(PageGeom g, const int32_t* keep) {
@@ -250,55 +259,69 @@ __global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
   }
   __syncthreads();
 
-  // entry number f: its place in the table, and the page that it holds (-1: none)
-  auto entry = [&](int f, int& s, int& e) {
+  // entry number f: its place in the table, the page that it holds (-1: none) and that page's
+  // holders.  A thread's first one is kept: a step's entries are rarely more.
+  struct Entry {
+    int at, e, s, page, holders;
+  };
+  auto find = [&](int f) {
+    Entry x;
     int lo = 0, hi = g.n_seq;  // first[lo] <= f < first[hi]
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (first[mid] <= f) lo = mid;
       else hi = mid;
     }
-    s = lo;
-    e = lowest[lo] + (f - first[lo]);
-    return s * g.n_table + e;
+    x.s = lo;
+    x.e = lowest[lo] + (f - first[lo]);
+    x.at = lo * g.n_table + x.e;
+    x.page = g.table[x.at];
+    if (x.page < 0 || x.page >= g.n_page) x.page = -1;
+    x.holders = x.page < 0 ? 0 : g.refs[x.page];
+    return x;
   };
-  auto held = [&](int at) {
-    const int p = g.table[at];
-    return p >= 0 && p < g.n_page ? p : -1;
-  };
+  Entry mine{0, 0, 0, -1, 0};
+  if (tid < n_asked) mine = find(tid);
+  auto entry = [&](int f) { return f == tid ? mine : find(f); };
   auto each_shared = [&](auto&& fn) {
     for (int f = tid; f < n_asked; f += kPlan) {
-      int s, e;
-      const int at = entry(f, s, e), p = held(at);
-      if (p >= 0 && g.refs[p] > 1) fn(at, p);
+      const Entry x = entry(f);
+      if (x.holders > 1) fn(x);
     }
     __builtin_amdgcn_s_waitcnt(0);  // (stores, then atomics, of one page by several waves)
     __syncthreads();
   };
-  each_shared([&](int, int p) {
-    ws.asked[p] = 0;
-    ws.last[p] = -1;
-  });
-  each_shared([&](int at, int p) {
-    atomicAdd(&ws.asked[p], 1);
-    atomicMax(&ws.last[p], at);
-  });
-  int n_fresh = 0;
+  // (any page with other holders at all?)
+  bool shared = mine.holders > 1;
+  for (int f = tid + kPlan; f < n_asked; f += kPlan) shared |= find(f).holders > 1;
+  if (__syncthreads_or(shared)) {
+    each_shared([&](const Entry& x) {
+      ws.asked[x.page] = 0;
+      ws.last[x.page] = -1;
+    });
+    each_shared([&](const Entry& x) {
+      atomicAdd(&ws.asked[x.page], 1);
+      atomicMax(&ws.last[x.page], x.at);
+    });
+  }
+  int n_fresh = 0, n_first = 0, rank = -1;  // of the first 1024 entries: how many, and this thread's number
   for (int f0 = 0; f0 < n_asked; f0 += kPlan) {
     const int f = f0 + tid;
     bool fresh = false;
-    int at = 0;
     if (f < n_asked) {
-      int s, e;
-      at = entry(f, s, e);
-      const int p = held(at);
-      fresh = p < 0;
-      if (p >= 0 && g.refs[p] > 1) fresh = ld_agent(&ws.asked[p]) != g.refs[p] || ld_agent(&ws.last[p]) != at;
+      const Entry x = entry(f);
+      fresh = x.page < 0;
+      if (x.holders > 1) fresh = ld_agent(&ws.asked[x.page]) != x.holders || ld_agent(&ws.last[x.page]) != x.at;
     }
     int n;
     const int i = n_fresh + flags_before(fresh, waves, n);
-    if (fresh && i < g.n_page) ws.fresh[i] = f;
     n_fresh += n;
+    if (f0 == 0) {
+      n_first = n_fresh;
+      if (fresh) rank = i;
+    } else if (fresh && i < g.n_page) {
+      ws.fresh[i] = f;
+    }
   }
   // the free pages, in order, until there are enough: four in a row of 64 lanes at a time
   int found = 0;
@@ -333,20 +356,20 @@ __global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
     }
     return;
   }
-  for (int i = tid; i < n_fresh; i += kPlan) {
-    int s, e;
-    const int at = entry(ws.fresh[i], s, e), old = held(at), page = ws.unused[i];
-    g.table[at] = page;
+  auto give = [&](const Entry& x, int page) {
+    g.table[x.at] = page;
     g.refs[page] = 1;
-    if (old < 0) continue;
-    atomicSub(&g.refs[old], 1);
-    const int64_t rows = min((int64_t)a.length[s] - ((int64_t)e << g.shift), (int64_t)g.size());
-    if (rows <= 0) continue;
+    if (x.page < 0) return;
+    atomicSub(&g.refs[x.page], 1);
+    const int64_t rows = min((int64_t)a.length[x.s] - ((int64_t)x.e << g.shift), (int64_t)g.size());
+    if (rows <= 0) return;
     int32_t* c = ws.copies + 3 * (uint64_t)atomicAdd(&n_copies, 1);
-    c[0] = old;
+    c[0] = x.page;
     c[1] = page;
     c[2] = (int)rows;
-  }
+  };
+  if (rank >= 0) give(mine, ws.unused[rank]);
+  for (int i = n_first + tid; i < n_fresh; i += kPlan) give(find(ws.fresh[i]), ws.unused[i]);
   __syncthreads();
   if (tid == 0) {
     *a.missing = 0;
@@ -359,7 +382,7 @@ __global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
 // of either's words.
 template <int D>
 __global__ __launch_bounds__(kBlock) void k_pages_cow(PageGeom g, int32_t* words, uint32_t pieces) {
-  using Piece = std::conditional_t<D == 128, uint4, uint2>;
+  using P = Piece<D>;
   const ReserveWs ws(words, g.n_page);
   const uint64_t n = (uint64_t)*ws.count * pieces;
   uint8_t* layer = g.data + (uint64_t)blockIdx.y * g.n_page * g.page_bytes();
@@ -368,8 +391,8 @@ __global__ __launch_bounds__(kBlock) void k_pages_cow(PageGeom g, int32_t* words
     const uint32_t rows = ws.copies[3 * (uint64_t)i + 2], units = 10 * rows;
     const uint32_t u = (uint32_t)(w - (uint64_t)i * pieces) * kBlock + threadIdx.x;
     if (u >= units * g.n_head_kv) continue;
-    const Piece* from = reinterpret_cast<const Piece*>(layer + (uint64_t)ws.copies[3 * (uint64_t)i] * g.page_bytes());
-    Piece* to = reinterpret_cast<Piece*>(layer + (uint64_t)ws.copies[3 * (uint64_t)i + 1] * g.page_bytes());
+    const P* from = reinterpret_cast<const P*>(layer + (uint64_t)ws.copies[3 * (uint64_t)i] * g.page_bytes());
+    P* to = reinterpret_cast<P*>(layer + (uint64_t)ws.copies[3 * (uint64_t)i + 1] * g.page_bytes());
     const uint32_t h = u / units, r = u - h * units;
     const uint32_t at = r < 4 * rows   ? r
                         : r < 8 * rows ? (4u << g.shift) + r - 4 * rows
@@ -380,57 +403,92 @@ __global__ __launch_bounds__(kBlock) void k_pages_cow(PageGeom g, int32_t* words
   }
 }
 
-// Rows moved together in place: a workgroup has one matrix of a layer's kv head of a
-// sequence and takes its rows in order, B at a time, which are read before any is written:
-// a row's new slot is at or below its old one, so that no row is overwritten before it
-// has been read.
-template <int D, int B>
-__global__ __launch_bounds__(B) void k_pages_compact(PageGeom g, const int32_t* start, const int32_t* rows,
-                                                     const int32_t* counts, int n_rows) {
-  using H = PageHead<D>;
-  using Piece = std::conditional_t<D == 128, uint4, uint2>;  // a quarter of a row's codes, or its words
-  const uint32_t s = blockIdx.z, h = blockIdx.x >> 1, v = blockIdx.x & 1;
-  const int n = counts ? min(max(counts[s], 0), n_rows) : n_rows;
-  const int64_t to0 = start[s];
+// Rows moved together in place.  A workgroup has `width` of the 10 n_head_kv pieces of a
+// layer's rows of a sequence (of a head: four of key codes, four of value codes, one of
+// either's words) and takes the rows in order, `batch` at a time, which are all read before
+// one is written: a row's new slot is at or below its old one, so none is overwritten before
+// it has been read, and the next batch is fetched while this one is written.
+constexpr int kMovePieces = 5;  // of a thread and batch
+struct MoveArgs {
+  PageGeom g;
+  const int32_t *start, *rows, *counts;
+  int n_rows, width, batch;
+  uint32_t by_width;  // 2^32 / width rounded up: i / width for i below 2^16
+};
+template <int D>
+__global__ __launch_bounds__(kBlock) void k_pages_compact(MoveArgs a) {
+  using P = Piece<D>;
+  const PageGeom& g = a.g;
+  const uint32_t s = blockIdx.z, q0 = blockIdx.x * a.width;
   const int tid = threadIdx.x;
-  uint8_t* head = g.data + (uint64_t)blockIdx.y * g.n_page * g.page_bytes() + (uint64_t)h * g.head_bytes();
-  __shared__ uint64_t src[B], dst[B];  // a row's piece numbers, all ones if it stays
-  constexpr uint64_t kStays = ~0ull;
-  for (int i0 = 0; i0 < n; i0 += B) {
+  const int64_t to0 = a.start[s];
+  const int n = a.counts ? min(max(a.counts[s], 0), a.n_rows) : a.n_rows;
+  if (n == 0) return;
+  P* layer = reinterpret_cast<P*>(g.data + (uint64_t)blockIdx.y * g.n_page * g.page_bytes());
+  const uint32_t head = 10u << g.shift, size = g.size();
+  // a batch's rows: pages and rows in them of the old slot and the new, page -1 if it stays
+  // (three buffers: a wave may look up the next batch while another writes the one before)
+  __shared__ int src[3][kBlock], dst[3][kBlock], src_row[3][kBlock];
+  auto look_up = [&](int i0, int buf) {
     const int i = i0 + tid;
-    uint64_t a = kStays, b = kStays;
+    if (tid >= a.batch) return;
+    int p = -1, q = -1, from = 0;
     if (i < n) {
-      const int from = rows[(uint64_t)s * n_rows + i];
-      const int64_t to = to0 + i;
-      const int p = page_of(g, s, from), q = page_of(g, s, to);
-      if (p >= 0 && q >= 0 && from != to) {
-        a = (uint64_t)p * g.page_bytes() / sizeof(Piece) + (from & (g.size() - 1));
-        b = (uint64_t)q * g.page_bytes() / sizeof(Piece) + (to & (g.size() - 1));
-      }
+      from = a.rows[(uint64_t)s * a.n_rows + i];
+      q = page_of(g, s, to0 + i);
+      p = from == to0 + i || q < 0 ? -1 : page_of(g, s, from);
     }
-    src[tid] = a;
-    dst[tid] = b;
-    __syncthreads();
-    const uint32_t codes = H::codes(v, g.shift) / sizeof(Piece), meta = H::meta(v, g.shift) / sizeof(Piece);
-    Piece* base = reinterpret_cast<Piece*>(head);
-    Piece x[4], m;
-    uint64_t to[4];
-    // (piece number of row r's codes: the page's, the block's and 4 r, of which a and b hold r)
-    auto code = [&](uint64_t at) { return (at & ~(uint64_t)(g.size() - 1)) + codes + 4 * (at & (g.size() - 1)); };
+    src[buf][tid] = p;
+    dst[buf][tid] = q;
+    src_row[buf][tid] = from & (size - 1);
+  };
+  // this thread's pieces: rows of a batch, and their places in a page (without the row)
+  int row[kMovePieces];
+  uint32_t at[kMovePieces], step[kMovePieces];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int r = (tid + B * k) >> 2;
-      const uint64_t f = src[r];
-      to[k] = dst[r];
-      if (f != kStays) x[k] = base[code(f) + (tid & 3)];
+  for (int k = 0; k < kMovePieces; ++k) {
+    const uint32_t i = tid + kBlock * k;
+    row[k] = (int)__umulhi(i, a.by_width);
+    const uint32_t q = q0 + i - row[k] * a.width, h = q / 10, r = q - 10 * h;
+    const bool in = row[k] < a.batch && q < 10u * g.n_head_kv;
+    if (!in) row[k] = -1;
+    step[k] = r < 8 ? 4 : 1;
+    at[k] = in ? h * head + (r < 4 ? r : r < 8 ? (4u << g.shift) + r - 4 : r << g.shift) : 0;
+  }
+  P x[2][kMovePieces];
+  // (a piece that stays is read all the same, from page 0)
+  auto fetch = [&](int buf, P (&x)[kMovePieces]) {
+#pragma unroll
+    for (int k = 0; k < kMovePieces; ++k) {
+      const int r = max(row[k], 0), p = max(src[buf][r], 0);
+      x[k] = layer[(uint64_t)p * g.n_head_kv * head + at[k] + step[k] * src_row[buf][r]];
     }
-    if (a != kStays) m = base[a + meta];
-    __builtin_amdgcn_s_waitcnt(0);  // every row of the B has been read
-    __syncthreads();
+  };
+  auto put = [&](int i0, int buf, const P (&x)[kMovePieces]) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (to[k] != kStays) base[code(to[k]) + (tid & 3)] = x[k];
-    if (b != kStays) base[b + meta] = m;
+    for (int k = 0; k < kMovePieces; ++k) {
+      if (row[k] < 0 || src[buf][row[k]] < 0) continue;
+      const uint32_t r = (uint32_t)(to0 + i0 + row[k]) & (size - 1);
+      layer[(uint64_t)dst[buf][row[k]] * g.n_head_kv * head + at[k] + step[k] * r] = x[k];
+    }
+  };
+  look_up(0, 0);
+  __syncthreads();
+  fetch(0, x[0]);
+  int buf = 0;
+  for (int i0 = 0; i0 < n; i0 += 2 * a.batch) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int i = i0 + b * a.batch, next = buf == 2 ? 0 : buf + 1;
+      if (i >= n) break;
+      const bool more = i + a.batch < n;
+      if (more) look_up(i + a.batch, next);
+      __builtin_amdgcn_s_waitcnt(0);  // every piece of this batch has been read
+      __syncthreads();
+      if (more) fetch(next, x[b ^ 1]);
+      put(i, buf, x[b]);
+      buf = next;
+    }
   }
 }
 
@@ -443,13 +501,12 @@ __global__ __launch_bounds__(kBlock) void k_pages_copy(PageGeom to, PageGeom fro
     const uint32_t i = (uint32_t)(w / pieces);
     const int p = src[i], q = dst[i];
     if (p < 0 || p >= from.n_page || q < 0 || q >= to.n_page) continue;
-    const uint4* f = reinterpret_cast<const uint4*>(from.data + ((uint64_t)blockIdx.y * from.n_page + p) * from.page_bytes());
-    uint4* t = reinterpret_cast<uint4*>(to.data + ((uint64_t)blockIdx.y * to.n_page + q) * to.page_bytes());
+    const u32v4* f = reinterpret_cast<const u32v4*>(from.data + ((uint64_t)blockIdx.y * from.n_page + p) * from.page_bytes());
+    u32v4* t = reinterpret_cast<u32v4*>(to.data + ((uint64_t)blockIdx.y * to.n_page + q) * to.page_bytes());
     const uint32_t u0 = (uint32_t)(w - (uint64_t)i * pieces) * kCopyPiece + threadIdx.x;
-    uint4 x[4];
+    u32v4 x[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (u0 + k * kBlock < units) x[k] = f[u0 + k * kBlock];
+    for (int k = 0; k < 4; ++k) x[k] = f[min(u0 + k * kBlock, units - 1)];
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (u0 + k * kBlock < units) t[u0 + k * kBlock] = x[k];
@@ -510,17 +567,15 @@ hipError_t launch_pages_free(const PageGeom& g, const int32_t* keep, hipStream_t
 
 hipError_t launch_pages_compact(const PageGeom& g, const int32_t* start, const int32_t* rows, const int32_t* counts,
                                 int n_rows, hipStream_t s) {
-  const dim3 grid(2 * g.n_head_kv, g.n_layer, g.n_seq);
-#define KNJ_PAGE_COMPACT(D, B) \
-  KNJ_LAUNCH((k_pages_compact<D, B>), grid, dim3(B), 0, s, g, start, rows, counts, n_rows)
-  if (g.head_dim == 128) {
-    if (n_rows <= 64) KNJ_PAGE_COMPACT(128, 64);
-    else KNJ_PAGE_COMPACT(128, 256);
-  } else {
-    if (n_rows <= 64) KNJ_PAGE_COMPACT(64, 64);
-    else KNJ_PAGE_COMPACT(64, 256);
-  }
-#undef KNJ_PAGE_COMPACT
+  // all of a layer's rows to a workgroup, or where those are few a head's or a matrix's
+  const int64_t all = (int64_t)g.n_layer * g.n_seq;
+  const int width = all >= 512 ? 10 * std::min(g.n_head_kv, 16) : all * g.n_head_kv >= 512 ? 10 : 5;
+  const int parts = (10 * g.n_head_kv + width - 1) / width;
+  const int batch = std::min(kMovePieces * dev::kBlock / width, dev::kBlock);
+  const MoveArgs a{g, start, rows, counts, n_rows, width, batch, (uint32_t)((0x100000000ull + width - 1) / width)};
+  const dim3 grid(parts, g.n_layer, g.n_seq);
+  if (g.head_dim == 128) KNJ_LAUNCH(k_pages_compact<128>, grid, dim3(kBlock), 0, s, a);
+  else KNJ_LAUNCH(k_pages_compact<64>, grid, dim3(kBlock), 0, s, a);
   return hipGetLastError();
 }
 
