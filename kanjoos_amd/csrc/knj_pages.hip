@@ -408,14 +408,14 @@ __global__ __launch_bounds__(kBlock) void k_pages_cow(PageGeom g, int32_t* words
 // either's words) and takes the rows in order, `batch` at a time, which are all read before
 // one is written: a row's new slot is at or below its old one, so none is overwritten before
 // it has been read, and the next batch is fetched while this one is written.
-constexpr int kMovePieces = 5;  // of a thread and batch
 struct MoveArgs {
   PageGeom g;
   const int32_t *start, *rows, *counts;
   int n_rows, width, batch;
   uint32_t by_width;  // 2^32 / width rounded up: i / width for i below 2^16
 };
-template <int D>
+constexpr int kMoveBatch = 2 * kBlock;  // at most
+template <int D, int PIECES>
 __global__ __launch_bounds__(kBlock) void k_pages_compact(MoveArgs a) {
   using P = Piece<D>;
   const PageGeom& g = a.g;
@@ -428,25 +428,28 @@ __global__ __launch_bounds__(kBlock) void k_pages_compact(MoveArgs a) {
   const uint32_t head = 10u << g.shift, size = g.size();
   // a batch's rows: pages and rows in them of the old slot and the new, page -1 if it stays
   // (three buffers: a wave may look up the next batch while another writes the one before)
-  __shared__ int src[3][kBlock], dst[3][kBlock], src_row[3][kBlock];
+  __shared__ int src[3][kMoveBatch], dst[3][kMoveBatch], src_row[3][kMoveBatch];
   auto look_up = [&](int i0, int buf) {
-    const int i = i0 + tid;
-    if (tid >= a.batch) return;
-    int p = -1, q = -1, from = 0;
-    if (i < n) {
-      from = a.rows[(uint64_t)s * a.n_rows + i];
-      q = page_of(g, s, to0 + i);
-      p = from == to0 + i || q < 0 ? -1 : page_of(g, s, from);
+#pragma unroll
+    for (int r = tid; r < kMoveBatch; r += kBlock) {
+      if (r >= a.batch) break;
+      const int i = i0 + r;
+      int p = -1, q = -1, from = 0;
+      if (i < n) {
+        from = a.rows[(uint64_t)s * a.n_rows + i];
+        q = page_of(g, s, to0 + i);
+        p = from == to0 + i || q < 0 ? -1 : page_of(g, s, from);
+      }
+      src[buf][r] = p;
+      dst[buf][r] = q;
+      src_row[buf][r] = from & (size - 1);
     }
-    src[buf][tid] = p;
-    dst[buf][tid] = q;
-    src_row[buf][tid] = from & (size - 1);
   };
   // this thread's pieces: rows of a batch, and their places in a page (without the row)
-  int row[kMovePieces];
-  uint32_t at[kMovePieces], step[kMovePieces];
+  int row[PIECES];
+  uint32_t at[PIECES], step[PIECES];
 #pragma unroll
-  for (int k = 0; k < kMovePieces; ++k) {
+  for (int k = 0; k < PIECES; ++k) {
     const uint32_t i = tid + kBlock * k;
     row[k] = (int)__umulhi(i, a.by_width);
     const uint32_t q = q0 + i - row[k] * a.width, h = q / 10, r = q - 10 * h;
@@ -455,18 +458,18 @@ __global__ __launch_bounds__(kBlock) void k_pages_compact(MoveArgs a) {
     step[k] = r < 8 ? 4 : 1;
     at[k] = in ? h * head + (r < 4 ? r : r < 8 ? (4u << g.shift) + r - 4 : r << g.shift) : 0;
   }
-  P x[2][kMovePieces];
+  P x[2][PIECES];
   // (a piece that stays is read all the same, from page 0)
-  auto fetch = [&](int buf, P (&x)[kMovePieces]) {
+  auto fetch = [&](int buf, P (&x)[PIECES]) {
 #pragma unroll
-    for (int k = 0; k < kMovePieces; ++k) {
+    for (int k = 0; k < PIECES; ++k) {
       const int r = max(row[k], 0), p = max(src[buf][r], 0);
       x[k] = layer[(uint64_t)p * g.n_head_kv * head + at[k] + step[k] * src_row[buf][r]];
     }
   };
-  auto put = [&](int i0, int buf, const P (&x)[kMovePieces]) {
+  auto put = [&](int i0, int buf, const P (&x)[PIECES]) {
 #pragma unroll
-    for (int k = 0; k < kMovePieces; ++k) {
+    for (int k = 0; k < PIECES; ++k) {
       if (row[k] < 0 || src[buf][row[k]] < 0) continue;
       const uint32_t r = (uint32_t)(to0 + i0 + row[k]) & (size - 1);
       layer[(uint64_t)dst[buf][row[k]] * g.n_head_kv * head + at[k] + step[k] * r] = x[k];
@@ -567,15 +570,23 @@ hipError_t launch_pages_free(const PageGeom& g, const int32_t* keep, hipStream_t
 
 hipError_t launch_pages_compact(const PageGeom& g, const int32_t* start, const int32_t* rows, const int32_t* counts,
                                 int n_rows, hipStream_t s) {
-  // all of a layer's rows to a workgroup, or where those are few a head's or a matrix's
+  // all of a layer's rows to a workgroup, or where those are few a head's or a matrix's;
+  // two pieces a thread where that takes all rows at once
   const int64_t all = (int64_t)g.n_layer * g.n_seq;
   const int width = all >= 512 ? 10 * std::min(g.n_head_kv, 16) : all * g.n_head_kv >= 512 ? 10 : 5;
   const int parts = (10 * g.n_head_kv + width - 1) / width;
-  const int batch = std::min(kMovePieces * dev::kBlock / width, dev::kBlock);
+  const int pieces = (int64_t)n_rows * width <= 2 * dev::kBlock ? 2 : 10;
+  const int batch = std::min(pieces * dev::kBlock / width, kMoveBatch);
   const MoveArgs a{g, start, rows, counts, n_rows, width, batch, (uint32_t)((0x100000000ull + width - 1) / width)};
   const dim3 grid(parts, g.n_layer, g.n_seq);
-  if (g.head_dim == 128) KNJ_LAUNCH(k_pages_compact<128>, grid, dim3(kBlock), 0, s, a);
-  else KNJ_LAUNCH(k_pages_compact<64>, grid, dim3(kBlock), 0, s, a);
+#define KNJ_PAGE_COMPACT(D)                                                                    \
+  do {                                                                                         \
+    if (pieces == 2) KNJ_LAUNCH((k_pages_compact<D, 2>), grid, dim3(kBlock), 0, s, a);         \
+    else KNJ_LAUNCH((k_pages_compact<D, 10>), grid, dim3(kBlock), 0, s, a);                    \
+  } while (0)
+  if (g.head_dim == 128) KNJ_PAGE_COMPACT(128);
+  else KNJ_PAGE_COMPACT(64);
+#undef KNJ_PAGE_COMPACT
   return hipGetLastError();
 }
 
