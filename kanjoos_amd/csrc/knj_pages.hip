@@ -171,6 +171,32 @@ __global__ __launch_bounds__(kBlock) void k_pages_fork_write(PageGeom g, const i
   g.table[i] = page;
 }
 
+// Both by one workgroup, of tables up to kForkOne entries.
+constexpr int kForkEach = 8, kForkOne = 1024 * kForkEach;
+__global__ __launch_bounds__(1024) void k_pages_fork(PageGeom g, const int32_t* parent, const int32_t* keep) {
+  const uint32_t total = (uint32_t)g.n_seq * g.n_table;
+  int old[kForkEach], page[kForkEach];
+#pragma unroll
+  for (int k = 0; k < kForkEach; ++k) {
+    const uint32_t i = threadIdx.x + 1024 * k, j = min(i, total - 1), s = j / g.n_table, e = j - s * g.n_table;
+    old[k] = g.table[j];
+    const int p = parent[s];
+    int v = -1;
+    if (p >= 0 && p < g.n_seq && (!keep || (int)e < entries_of(g, keep[s]))) v = g.table[(uint32_t)p * g.n_table + e];
+    page[k] = v >= 0 && v < g.n_page ? v : -1;
+  }
+  __builtin_amdgcn_s_waitcnt(0);  // every entry has been read
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kForkEach; ++k) {
+    const uint32_t i = threadIdx.x + 1024 * k;
+    if (i >= total || old[k] == page[k]) continue;
+    if (old[k] >= 0 && old[k] < g.n_page) atomicSub(&g.refs[old[k]], 1);
+    if (page[k] >= 0) atomicAdd(&g.refs[page[k]], 1);
+    g.table[i] = page[k];
+  }
+}
+
 __global__ __launch_bounds__(kBlock) void k_pages_free(PageGeom g, const int32_t* keep) {
   const uint32_t s = blockIdx.y, e = blockIdx.x * kBlock + threadIdx.x;
   const int n = keep[s];
@@ -191,7 +217,7 @@ struct ReserveWs {
         unused(fresh + n_page) {}
 };
 
-constexpr int kMaxSeq = 4096, kPlan = 1024, kPlanWaves = kPlan / 64;
+constexpr int kMaxSeq = 4096, kPlan = 1024, kPlanWaves = kPlan / 64, kPlanFew = 128;
 
 // How many of the workgroup's flags are set before this thread's, and in all.
 __device__ __forceinline__ int flags_before(bool f, int* waves, int& total) {
@@ -224,7 +250,16 @@ __global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
   __shared__ int first[kMaxSeq + 1];  // asked entries of the sequences before
   __shared__ int lowest[kMaxSeq];     // a sequence's first asked entry
   __shared__ int waves[kPlanWaves], counts[64], n_copies;
+  __shared__ int pages[kPlanFew], free_pages[kPlan];  // shared pages asked for (few entries); the first free ones
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // (of the first 4096 pages which are free, fetched before anything waits)
+  auto free_of = [&](int p0, int i) {
+    const int p = p0 + wave * 256 + 64 * i + lane;
+    return p < g.n_page && g.refs[p] <= 0;
+  };
+  bool free0[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) free0[i] = free_of(0, i);
 
   int n_asked = 0;
   for (int s0 = 0; s0 < g.n_seq; s0 += kPlan) {
@@ -291,18 +326,32 @@ __global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
     __builtin_amdgcn_s_waitcnt(0);  // (stores, then atomics, of one page by several waves)
     __syncthreads();
   };
-  // (any page with other holders at all?)
-  bool shared = mine.holders > 1;
-  for (int f = tid + kPlan; f < n_asked; f += kPlan) shared |= find(f).holders > 1;
-  if (__syncthreads_or(shared)) {
-    each_shared([&](const Entry& x) {
-      ws.asked[x.page] = 0;
-      ws.last[x.page] = -1;
-    });
-    each_shared([&](const Entry& x) {
-      atomicAdd(&ws.asked[x.page], 1);
-      atomicMax(&ws.last[x.page], x.at);
-    });
+  // How many entries ask to replace a page, and the last of them: with few entries each
+  // counts for itself, else by atomics (where any page has other holders).
+  const bool few = n_asked <= kPlanFew;
+  int asked = 0, last = -1;
+  if (few) {
+    if (tid < n_asked) pages[tid] = mine.holders > 1 ? mine.page : -1;
+    __syncthreads();
+    if (mine.holders > 1)
+      for (int i = 0; i < n_asked; ++i)
+        if (pages[i] == mine.page) {
+          ++asked;
+          last = i;  // (entries are numbered in the table's order)
+        }
+  } else {
+    bool shared = mine.holders > 1;
+    for (int f = tid + kPlan; f < n_asked; f += kPlan) shared |= find(f).holders > 1;
+    if (__syncthreads_or(shared)) {
+      each_shared([&](const Entry& x) {
+        ws.asked[x.page] = 0;
+        ws.last[x.page] = -1;
+      });
+      each_shared([&](const Entry& x) {
+        atomicAdd(&ws.asked[x.page], 1);
+        atomicMax(&ws.last[x.page], x.at);
+      });
+    }
   }
   int n_fresh = 0, n_first = 0, rank = -1;  // of the first 1024 entries: how many, and this thread's number
   for (int f0 = 0; f0 < n_asked; f0 += kPlan) {
@@ -311,7 +360,9 @@ __global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
     if (f < n_asked) {
       const Entry x = entry(f);
       fresh = x.page < 0;
-      if (x.holders > 1) fresh = ld_agent(&ws.asked[x.page]) != x.holders || ld_agent(&ws.last[x.page]) != x.at;
+      if (x.holders > 1)
+        fresh = few ? asked != x.holders || last != f
+                    : ld_agent(&ws.asked[x.page]) != x.holders || ld_agent(&ws.last[x.page]) != x.at;
     }
     int n;
     const int i = n_fresh + flags_before(fresh, waves, n);
@@ -329,8 +380,7 @@ __global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
     uint64_t b[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int p = p0 + wave * 256 + 64 * i + lane;
-      b[i] = __ballot(p < g.n_page && g.refs[p] <= 0);
+      b[i] = __ballot(p0 == 0 ? free0[i] : free_of(p0, i));
     }
     __syncthreads();
     if (lane < 4) counts[4 * wave + lane] = __popcll(lane == 0 ? b[0] : lane == 1 ? b[1] : lane == 2 ? b[2] : b[3]);
@@ -344,7 +394,10 @@ __global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int at = found + __shfl(sum, 4 * wave + i) - __popcll(b[i]) + __popcll(b[i] & ((1ull << lane) - 1));
-      if ((b[i] >> lane) & 1) ws.unused[at] = p0 + wave * 256 + 64 * i + lane;
+      const int p = p0 + wave * 256 + 64 * i + lane;
+      if (!((b[i] >> lane) & 1)) continue;
+      if (at < kPlan) free_pages[at] = p;
+      else ws.unused[at] = p;
     }
     found += __shfl(sum, 63);
   }
@@ -368,8 +421,8 @@ __global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
     c[1] = page;
     c[2] = (int)rows;
   };
-  if (rank >= 0) give(mine, ws.unused[rank]);
-  for (int i = n_first + tid; i < n_fresh; i += kPlan) give(find(ws.fresh[i]), ws.unused[i]);
+  if (rank >= 0) give(mine, free_pages[rank]);
+  for (int i = n_first + tid; i < n_fresh; i += kPlan) give(find(ws.fresh[i]), i < kPlan ? free_pages[i] : ws.unused[i]);
   __syncthreads();
   if (tid == 0) {
     *a.missing = 0;
@@ -548,9 +601,9 @@ uint64_t page_workspace_ints(const PageGeom& g) {
 hipError_t launch_pages_reserve(const PageReserveArgs& a, hipStream_t s) {
   KNJ_LAUNCH(k_pages_plan, dim3(1), dim3(kPlan), 0, s, a);
   // (how many pages are copied is known on the device only: as many workgroups as a page
-  // of each sequence needs, to a chipful)
+  // of each sequence needs, to eight a CU)
   const uint32_t pieces = (a.g.page_bytes() / (a.g.head_dim / 8) + kBlock - 1) / kBlock;
-  const uint64_t want = std::min<uint64_t>((uint64_t)pieces * a.g.n_seq, 8192 / a.g.n_layer);
+  const uint64_t want = std::min<uint64_t>((uint64_t)pieces * a.g.n_seq, 2048 / a.g.n_layer);
   const dim3 grid((uint32_t)std::max<uint64_t>(want, 1), a.g.n_layer);
   if (a.g.head_dim == 128) KNJ_LAUNCH(k_pages_cow<128>, grid, dim3(kBlock), 0, s, a.g, a.ws, pieces);
   else KNJ_LAUNCH(k_pages_cow<64>, grid, dim3(kBlock), 0, s, a.g, a.ws, pieces);
@@ -558,6 +611,11 @@ hipError_t launch_pages_reserve(const PageReserveArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_pages_fork(const PageGeom& g, const int32_t* parent, const int32_t* keep, int32_t* ws, hipStream_t s) {
+  // (one launch: 4 beams of 17 pages 2.4 us against 4.1 in two, 32 of 252 3.8 against 4.9)
+  if ((int64_t)g.n_seq * g.n_table <= kForkOne) {
+    KNJ_LAUNCH(k_pages_fork, dim3(1), dim3(1024), 0, s, g, parent, keep);
+    return hipGetLastError();
+  }
   KNJ_LAUNCH(k_pages_fork_read, table_grid(g), dim3(kBlock), 0, s, g, parent, keep, ws);
   KNJ_LAUNCH(k_pages_fork_write, table_grid(g), dim3(kBlock), 0, s, g, ws);
   return hipGetLastError();

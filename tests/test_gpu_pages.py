@@ -444,7 +444,7 @@ def reserve(p, start, length, want):
 
 @pytest.mark.parametrize("D,n_seq,n_page,page,n_table,seed", [
     (64, 5, 40, 16, 12, 0), (128, 9, 70, 32, 9, 1), (64, 33, 500, 16, 20, 2), (128, 3, 9, 256, 4, 3), (64, 70, 5000, 16, 70, 4),
-    (64, 1, 3000, 16, 2500, 5), (64, 1500, 9000, 16, 5, 6)])
+    (64, 1, 3000, 16, 2500, 5), (64, 1500, 9000, 16, 5, 6), (64, 300, 6000, 16, 40, 7)])
 def test_table_steps(device, D, n_seq, n_page, page, n_table, seed):
     """Random steps over one pool: reserve (with and without a start, with too few pages too), fork, free, store, compact,
     against the model after each."""
