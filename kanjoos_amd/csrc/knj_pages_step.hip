@@ -1,34 +1,10 @@
 // kanjoos_amd/csrc/knj_pages_step.hip -- attention over 4-bit pages for up to 16 columns a kv
 // head (a column is a row and a query head): decode steps and short chains of drafts.
-#include "knj_tree.h"
+#include "knj_pages_attn.h"
 
 namespace knj {
 namespace tree {
 namespace {
-
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-
-// Eight weights as f16 high parts and remainders, two to an instruction.
-__device__ __forceinline__ void split8(const float (&w)[8], h16x8& hi, h16x8& lo) {
-#pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    const hx2 h = __builtin_convertvector(f32x2{w[i], w[i + 1]}, hx2);
-    const f32x2 r = {fmaf((float)h[0], -1.0f, w[i]), fmaf((float)h[1], -1.0f, w[i + 1])};
-    const hx2 l = __builtin_convertvector(r, hx2);
-    hi[i] = h[0];
-    hi[i + 1] = h[1];
-    lo[i] = l[0];
-    lo[i + 1] = l[1];
-  }
-}
-
-// The halves of a word that are infinite or NaN (0x7C00 and up) replaced by zero; the sign
-// bits of those that were.
-__device__ __forceinline__ uint32_t clear_nonfinite(uint32_t& w) {
-  const uint32_t m = ((w & 0x7FFF7FFFu) + 0x04000400u) & 0x80008000u;
-  w &= ~(m | (m - (m >> 15)));
-  return m;
-}
 
 // Workgroup = (sequence, split of the slots, kv head) of four waves that take its tiles of
 // 32 slots in turn, each by itself: no barrier until the end.  A lane (r = l % 16, kq =
@@ -123,27 +99,12 @@ __global__ __launch_bounds__(64 * kStepWaves, SPLIT ? 3 : 4) void k_pages_step(T
     const int qc = threadIdx.x / QP, piece = threadIdx.x % QP, c = min(qc, a.n_rows * G - 1), t = p.by_group.div(c);
     const uint64_t at = ((uint64_t)s * a.n_rows + t) * a.q_stride + (uint64_t)(kvh * G + c - t * G) * D + 8 * piece;
     float4 x, y;
-    if constexpr (SPLIT) {
-      x = ld4<KNJ_TYPE_F32>(a.q, at);
-      y = ld4<KNJ_TYPE_F32>(a.q, at + 4);
-    } else if (a.type == KNJ_TYPE_F16) {
-      x = ld4<KNJ_TYPE_F16>(a.q, at);
-      y = ld4<KNJ_TYPE_F16>(a.q, at + 4);
-    } else {
-      x = ld4<KNJ_TYPE_BF16>(a.q, at);
-      y = ld4<KNJ_TYPE_BF16>(a.q, at + 4);
-    }
-    float am = fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))),
-                     fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
-    am = group_max<QP>(am);
-    const int e = min(max((int)(__float_as_uint(am) >> 23) - 127, -126), 126);
-    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-    if (piece == 0)
-      scales[qc] = fminf(a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + e) << 23), 0x1.fffffep127f);
-    // (in decode8_mixed's order)
-    const float q[8] = {x.x * down, y.x * down, x.y * down, y.y * down, x.z * down, y.z * down, x.w * down, y.w * down};
+    queries8<SPLIT>(a, at, x, y);
+    float down;
+    const float unit = column_unit(a.scale, group_max<QP>(largest8(x, y)), down);
+    if (piece == 0) scales[qc] = unit;
     h16x8 hi, lo;
-    split8(q, hi, lo);
+    pack_queries(x, y, down, hi, lo);
     lds_put_b128(lds_addr(lds) + qc * QS + 16 * piece, __builtin_bit_cast(uint4, hi));
     if constexpr (SPLIT) lds_put_b128(lds_addr(lds) + 16 * QS + qc * QS + 16 * piece, __builtin_bit_cast(uint4, lo));
   }
@@ -152,8 +113,8 @@ __global__ __launch_bounds__(64 * kStepWaves, SPLIT ? 3 : 4) void k_pages_step(T
   h16x8 qh[NC], ql[SPLIT ? NC : 1];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    qh[c] = __builtin_bit_cast(h16x8, lds_b128(lds_addr(lds) + r * QS + 16 * (NC * kq + c)));
-    if constexpr (SPLIT) ql[c] = __builtin_bit_cast(h16x8, lds_b128(lds_addr(lds) + 16 * QS + r * QS + 16 * (NC * kq + c)));
+    qh[c] = lds_h8(lds_addr(lds) + r * QS + 16 * (NC * kq + c));
+    if constexpr (SPLIT) ql[c] = lds_h8(lds_addr(lds) + 16 * QS + r * QS + 16 * (NC * kq + c));
   }
   const float s2 = scales[r];
   KNJ_BARRIER_AFTER(kLdsOnly);
@@ -283,13 +244,7 @@ __global__ __launch_bounds__(64 * kStepWaves, SPLIT ? 3 : 4) void k_pages_step(T
   if (spoilt) l = NAN;
   float4* mine4 = reinterpret_cast<float4*>(lds + wave * LW);
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) {
-    // dims 0 4 1 5 of eight in the lanes of an even kq and 2 6 3 7 in those of kq + 1: 0 1 2 3
-    // and 4 5 6 7 by exchanges of 16 lanes with the next 16
-    const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[dt][0]), __float_as_uint(acc[dt][1]), false, false);
-    const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[dt][2]), __float_as_uint(acc[dt][3]), false, false);
-    mine4[64 * dt + lane] = make_float4(__uint_as_float(x[0]), __uint_as_float(y[0]), __uint_as_float(x[1]), __uint_as_float(y[1]));
-  }
+  for (int dt = 0; dt < DT; ++dt) mine4[64 * dt + lane] = in_order(acc[dt]);
   if (kq == 0) stats[wave][r] = make_float2(m, l);
   __syncthreads();
   float M = -INFINITY, L = 0.0f, f[NW];

@@ -32,6 +32,8 @@ struct FastDiv {
 // Attention over 4-bit pages for up to 16 columns a kv head: workgroups of kStepWaves waves
 // that take tiles of kStepTile slots in turn.
 constexpr int kStepTile = 32, kStepWaves = 4;
+// For many: column tiles of 16 a wave over steps of kWideStep slots.
+constexpr int kWideStep = 64, kWideWaves = 8;
 
 struct TreePlan {
   int cps;       // chunks per split of the slots
@@ -964,6 +966,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
 }
 
 hipError_t launch_pages_step(const TreeArgs& a, const TreePlan& p, hipStream_t s);
+hipError_t launch_pages_wide(const TreeArgs& a, const TreePlan& p, hipStream_t s);
 
 // One launch of a format's kernel: D, split and the column tile's shape at run
 // time (columns per kv head up to 16, 32, 64 or more).
@@ -987,10 +990,16 @@ hipError_t launch_format(const TreeArgs& a, const TreePlan& p, int cols, hipStre
   }
 #define KNJ_TREE_COLS(DD, FORMAT, SPLIT)                                                             \
   do {                                                                                               \
-    if (cols == 16) KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, 1, 1, 4, 16);                                 \
-    else if (cols == 32) KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, 1, 2, 2, 32);                            \
+    if constexpr (FORMAT != kFormatPages) { /* (pages: launch_pages_step) */                         \
+      if (cols == 16) {                                                                              \
+        KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, 1, 1, 4, 16);                                             \
+        break;                                                                                       \
+      }                                                                                              \
+    }                                                                                                \
+    if (cols == 32) KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, 1, 2, 2, 32);                                 \
     else if (SPLIT || cols == 64) KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, 2, 2, 2, 32);                   \
-    else KNJ_TREE_LAUNCH(DD, FORMAT, false, 2, 4, 1, 64);                                            \
+    else if constexpr (FORMAT != kFormatPages || DD == 64) /* (pages: launch_pages_wide) */          \
+      KNJ_TREE_LAUNCH(DD, FORMAT, false, 2, 4, 1, 64);                                               \
   } while (0)
 #define KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, NT, WC, WS, SW) \
   KNJ_LAUNCH((k_tree<DD, FORMAT, SPLIT, NT, WC, WS, SW>), grid, dim3(64 * WC * WS), 0, s, a, p)

@@ -119,6 +119,7 @@ struct Planned {
   TreePlan p;
   int cols;   // columns of a tile
   int chunk;  // slots of a split's chunks
+  bool wide;  // launch_pages_wide's
 };
 
 // Tiles of 32 columns (16 where there are no more) finish a chunk soonest; wider ones
@@ -151,16 +152,38 @@ Planned plan_step(const knj_kv_cache& c, int n_head, int n_rows, int max_prefix)
   const FastDiv none(1);
   return {TreePlan{0, n_split, 1, (int)(units * n_split), FastDiv(c.n_head_kv), FastDiv(n_split),
                    FastDiv(n_head / c.n_head_kv), FastDiv(n_head), FastDiv(n_rows), none, true},
-          16, kStepTile};
+          16, kStepTile, false};
+}
+
+// Of launch_pages_wide, for heads of 128 and more than 64 columns: two workgroups a CU (one and
+// three: 141 and 129 us for 500 rows x 32 heads over 8000 slots, 121 with two).  It wins over
+// k_tree where there is work enough, in chunks of 32-column tiles: at 5,400, 7,028, 8,064 and
+// 9,216 of them 39.1, 32.1, 34.7 and 40.1 us against 35.1, 33.7, 37.0 and 41.4 (f32 queries
+// cross at 8,000); and, with a chain's upper triangle left out, earlier where the rows are
+// no fewer than the slots before them: 500 rows, nothing before (4,000) 27.4 against 47.9,
+// 300 before 34.5 against 64.1, 200 rows and nothing before (800) 16.4 against 16.2.
+constexpr int64_t kPagesWork = 7000, kPagesPrompt = 1500;
+Planned plan_wide(const knj_kv_cache& c, int n_head, int n_rows, int max_prefix) {
+  const int n_cols = n_rows * (n_head / c.n_head_kv), steps = (max_prefix + n_rows + kWideStep - 1) / kWideStep;
+  const int cols = 16 * kWideWaves, tiles = (n_cols + cols - 1) / cols;
+  const int64_t units = (int64_t)c.n_seq * c.n_head_kv, want = std::max<int64_t>(1, 512 / (units * tiles));
+  const int cps = (int)std::max<int64_t>(1, (steps + want - 1) / want), n_split = (steps + cps - 1) / cps;
+  return {TreePlan{cps, n_split, tiles, (int)(units * n_split), FastDiv(c.n_head_kv), FastDiv(n_split),
+                   FastDiv(n_head / c.n_head_kv), FastDiv(n_head), FastDiv(n_rows), FastDiv(cps), false},
+          cols, kWideStep, true};
 }
 
 Planned plan(const knj_kv_cache& c, int type, int n_head, int n_rows, int max_prefix) {
   const int group = n_head / c.n_head_kv, n_cols = n_rows * group;
-  if (c.format == kFormatPages && n_cols <= 16) return plan_step(c, n_head, n_rows, max_prefix);
   const int chunks = (max_prefix + n_rows + kTreeChunk - 1) / kTreeChunk;
   const int64_t units = (int64_t)c.n_seq * c.n_head_kv;
+  if (c.format == kFormatPages && n_cols <= 16) return plan_step(c, n_head, n_rows, max_prefix);
+  const int64_t work = units * ((n_cols + 31) / 32) * chunks;
+  if (c.format == kFormatPages && c.head_dim == 128 && n_cols > 64 &&
+      work >= (n_rows >= max_prefix ? kPagesPrompt : kPagesWork))
+    return plan_wide(c, n_head, n_rows, max_prefix);
   int cols = n_cols <= 16 ? 16 : 32;
-  if (n_cols > 32 && units * ((n_cols + 31) / 32) * chunks >= (c.format == KNJ_KV_F16 ? kWideWorkF16 : kWideWork))
+  if (n_cols > 32 && work >= (c.format == KNJ_KV_F16 ? kWideWorkF16 : kWideWork))
     cols = n_cols <= 64 || type == KNJ_TYPE_F32 ? 64 : 128;
   const int tiles = (n_cols + cols - 1) / cols;
   const int64_t wgs = units * tiles * chunks >= kTwoWork ? 512 : 256;
@@ -169,7 +192,7 @@ Planned plan(const knj_kv_cache& c, int type, int n_head, int n_rows, int max_pr
   const int n_split = (chunks + cps - 1) / cps;
   return {TreePlan{cps, n_split, tiles, (int)(units * n_split), FastDiv(c.n_head_kv), FastDiv(n_split), FastDiv(group),
                    FastDiv(n_head), FastDiv(n_rows), FastDiv(cps), false},
-          cols, kTreeChunk};
+          cols, kTreeChunk, false};
 }
 
 }  // namespace
@@ -221,6 +244,7 @@ hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t s) {
   const tree::Planned q = tree::plan(a.c, a.type, a.n_head, a.n_rows, a.max_prefix);
   hipError_t e;
   if (q.p.even) e = tree::launch_pages_step(a, q.p, s);
+  else if (q.wide) e = tree::launch_pages_wide(a, q.p, s);
   else if (a.c.format == KNJ_KV_F16) e = tree::launch_format<KNJ_KV_F16>(a, q.p, q.cols, s);
   else if (a.c.format == KNJ_KV_F8) e = tree::launch_format<KNJ_KV_F8>(a, q.p, q.cols, s);
   else if (a.c.format == KNJ_KV_I8) e = tree::launch_format<KNJ_KV_I8>(a, q.p, q.cols, s);

@@ -367,6 +367,106 @@ def test_attention_wide(device, t, D, T, nh, nk, P):
         close(got[:, i:i + 1], want, bound, f"row {i}")
 
 
+# A loose bound on the prefixes asks for many columns' kernel over short sequences too.
+LOOSE = 32000
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("T,nh,nk,page,prefixes", [
+    (66, 8, 4, 16, (0, 1, 61, 62, 63, 64, 126, 127, 500)), (25, 32, 2, 64, (190, 3, 64)), (130, 5, 1, 32, (0, 127, 128, 700)),
+    (17, 4, 1, 256, (100, 257, 0, 40, 1900)), (257, 3, 3, 128, (5, 255))])
+def test_attention_many_columns(device, t, T, nh, nk, page, prefixes):
+    """Trees with what not every row sees: NaN and huge values in unseen rows and past them, rows that see nothing,
+    rows that see a spoilt value; sequences with fewer rows, one of them with none."""
+    print(f"many columns type {t} T {T} heads {nh}/{nk} page {page} prefixes {prefixes}", flush=True)
+    rng = np.random.default_rng([T, nh, page, t])
+    n, D = len(prefixes), 128
+    pool = filled(rng, [m + T + 20 for m in prefixes], page, nk, D, extra=(LOOSE + T) // page + 1)
+    counts = np.array([T if s == 0 else max(T - 40 * s, 0) for s in range(n)])
+    sees = np.stack([tree_bits(rng, T) for _ in range(n)])
+    sees[:, :, 2:5] = False
+    sees[:, 0] = False
+    for s, P in enumerate(prefixes):
+        for slot in range(P + counts[s], P + T + 20):  # every byte past the rows set: NaN in step and lowest value
+            at = pool.where(s, slot)
+            for b in pool.blocks():
+                b[1, at[0], :, at[1]] = 0xFF
+        x = rng.normal(size=(3, 2, nk, D))
+        x[0, 1, :, 5], x[0, 0, :, 7] = np.inf, -np.inf
+        x[1, :, :, 100] = np.nan
+        x[2] *= 1e4
+        for r in range(min(3, counts[s] - 2)):
+            pool.put(1, s, P + 2 + r, *x[r])
+    sees[1 % n, 6, 2] = sees[0, 9, 3] = True  # a spoilt value seen
+    p = upload(pool)
+    kv = caches(pool, max(prefixes) + T)
+    q = decode(encode(1.5 * rng.normal(size=(n, T, nh, D)), t), t)
+    got, before = attend(p, t, q, T, prefixes, counts, sees, nh, pad=16, max_prefix=LOOSE)
+    with np.errstate(invalid="ignore", over="ignore"):
+        want, bound = tree64(q, kv, prefixes, counts, sees, D ** -0.5, t)
+    for s in range(n):
+        close(got[s, :counts[s]], want[s, :counts[s]], bound[s, :counts[s]], f"prefix {prefixes[s]}")
+        assert np.array_equal(got[s, counts[s]:], before[s, counts[s]:])  # rows past the drafts
+        if prefixes[s] == 0 and counts[s]:
+            assert np.all(got[s, 0] == 0)
+    again, _ = attend(p, t, q, T, prefixes, counts, sees, nh, pad=16, max_prefix=LOOSE, in_place=True)
+    for s in range(n):
+        assert np.array_equal(again[s, :counts[s]], got[s, :counts[s]], equal_nan=True)
+    same(p, pool)
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("T,nh,prefixes,loose", [(65, 6, (0, 77), True), (130, 2, (64, 1), True), (350, 12, (0, 41), False),
+                                                 (700, 8, (0,), False)])
+def test_attention_many_columns_chain(device, t, T, nh, prefixes, loose):
+    """No mask: row t sees rows 0..t, the same bits as with that mask, its own a sequence or one shared; a spoilt value
+    makes NaN of the rows from its own on, alike with a mask and without."""
+    print(f"many columns, chain: type {t} T {T} heads {nh} prefixes {prefixes}", flush=True)
+    rng = np.random.default_rng([T, nh, t])
+    nk, D, n = 1, 128, len(prefixes)
+    pool = filled(rng, [m + T for m in prefixes], 32, nk, D, extra=(LOOSE + T) // 32 + 1)
+    x = rng.normal(size=(2, nk, D))
+    x[1, :, 40] = np.inf
+    pool.put(1, n - 1, prefixes[-1] + T - 30, *x)
+    p = upload(pool)
+    kv = caches(pool, max(prefixes) + T)
+    q = decode(encode(rng.normal(size=(n, T, nh, D)), t), t)
+    sees = np.stack([np.tril(np.ones((T, T), bool))] * n)
+    limit = LOOSE if loose else None
+    got, _ = attend(p, t, q, T, prefixes, None, None, nh, max_prefix=limit)
+    with np.errstate(invalid="ignore"):
+        want, bound = tree64(q, kv, prefixes, [T] * n, sees, D ** -0.5, t)
+    close(got, want, bound, "chain")
+    assert np.isnan(got[n - 1, T - 30:]).all()
+    assert np.array_equal(attend(p, t, q, T, prefixes, None, sees, nh, max_prefix=limit)[0], got, equal_nan=True)
+    assert np.array_equal(attend(p, t, q, T, prefixes, None, sees[:1], nh, shared=True, max_prefix=limit)[0], got, equal_nan=True)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rising", [True, False])
+def test_attention_many_columns_drifting(device, t, rising):
+    """Scores that rise or fall along the slots by far more than f16 or an exponent's reference holds; a sequence
+    without a page beside it."""
+    rng = np.random.default_rng([t, rising])
+    T, nh, nk, D, P = 70, 8, 1, 128, 1500
+    pool = filled(rng, [P + T, 200 + T], 64, nk, D, extra=LOOSE // 64)
+    d = rng.normal(size=D)
+    drift = np.linspace(-40, 40, P + T) * (1 if rising else -1)
+    rows = np.stack([drift[:, None] * d / (d @ d) * 8 + rng.normal(size=(P + T, D)) * 0.3, rng.normal(size=(P + T, D))])
+    for slot in range(P + T):
+        pool.put(1, 0, slot, rows[0][slot][None], rows[1][slot][None])
+    pool.table[1, 2] = -7
+    pool.table[0, (P + T + 63) // 64:] = 2 ** 31 - 1  # behind the sequence's slots
+    p = upload(pool)
+    kv = [x[:1] for x in caches(pool, P + T)]
+    q = decode(encode(np.broadcast_to(4 * d, (2, T, nh, D)) + 0.1 * rng.normal(size=(2, T, nh, D)), t), t)
+    sees = np.stack([tree_bits(rng, T)] * 2)
+    got, _ = attend(p, t, q, T, [P, 200], None, sees, nh, max_prefix=LOOSE)
+    want, bound = tree64(q[:1], kv, [P], [T], sees[:1], D ** -0.5, t)
+    close(got[:1], want, bound, "drift")
+    assert np.isnan(got[1]).all()
+
+
 @pytest.mark.parametrize("T", [1, 3])
 def test_attention_long(device, T):
     """Long contexts of several splits; layers and pages beyond 2^32 bytes."""
