@@ -22,7 +22,7 @@ __device__ __forceinline__ h16x8 lds_h8(uint32_t p) {
 // makes it a conversion, of an upper half at half the rate, and a difference).
 __device__ __forceinline__ void split8(const float (&w)[8], h16x8& hi, h16x8& lo) {
   float minus = -1.0f;
-  asm("" : "+v"(minus));
+  asm("" : "+s"(minus));
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
     const hx2 h = __builtin_convertvector(f32x2{w[i], w[i + 1]}, hx2);

@@ -109,7 +109,6 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void k_pages_wide(TreeArgs a, T
       a, ((uint64_t)s * a.n_rows + trow) * a.q_stride + (uint64_t)(kvh * G + ccol - trow * G) * D + 8 * kq, 32, qh, ql);
 
   float m = -INFINITY, l = 0.0f;
-  bool spoilt = false;
   f32x4 acc[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -147,7 +146,7 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void k_pages_wide(TreeArgs a, T
           for (int i = 0; i < 4; ++i)
             if (!((seen >> (16 * st + 4 * kq + i)) & 1)) sc[st][i] = -INFINITY;
       }
-      spoilt |= (seen & bad) != 0;
+      if ((seen & bad) != 0) l = NAN;  // (and stays so)
     }
     // a weight beyond 2^kLag shows in the sum (and a column that has seen nothing yet in its
     // reference, -inf): the reference is moved and the weights formed again
@@ -205,7 +204,6 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void k_pages_wide(TreeArgs a, T
   // ---- results, or a split's record
   l += xor16_f(l);
   l += xor32_f(l);
-  if (spoilt) l = NAN;
   float4 o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = in_order(acc[dt]);

@@ -965,7 +965,7 @@ __global__ __launch_bounds__(64 * WC * WS, 2) void k_tree(TreeArgs a, TreePlan p
   }
 }
 
-hipError_t launch_pages_step(const TreeArgs& a, const TreePlan& p, hipStream_t s);
+hipError_t launch_pages_step(const TreeArgs& a, const TreePlan& p, int cols, hipStream_t s);
 hipError_t launch_pages_wide(const TreeArgs& a, const TreePlan& p, hipStream_t s);
 
 // One launch of a format's kernel: D, split and the column tile's shape at run

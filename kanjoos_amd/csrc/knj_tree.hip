@@ -144,7 +144,13 @@ constexpr int64_t kWideWork = 10000, kWideWorkF16 = 16000, kTwoWork = 2500;  // 
 // workgroups a CU (32 of 8000: 39.8 us; with one, three and four 44.6, 39.8 and 40.8) in up
 // to 64 splits, one batch of the merge's loads (one sequence of 32,700: 13.9; in 128 splits
 // 16.9, in 256 23.6).
-constexpr int kStepMerges = 16;
+// Columns 17 to 32 go there where that is work enough, or without a merge, and else, sooner
+// done, to k_tree (below): 4 drafts x 8 heads a kv head, 16 and 32 sequences of 2000 slots
+// (4,096 and 8,192 tiles) 18.8 and 23.5 us against 19.3 and 25.5, 16 of 1000 (2,048) 16.4
+// against 14.3; without a merge 16 and 32 of 200 and 450 9.8 and 13.3 against 10.8 and 14.9,
+// 8 of 300 11.1 against 9.6.
+constexpr int kStepMerges = 16, kStepUnits = 64;
+constexpr int64_t kStepWork = 4000;  // tiles
 Planned plan_step(const knj_kv_cache& c, int n_head, int n_rows, int max_prefix) {
   const int tiles = (max_prefix + n_rows + kStepTile - 1) / kStepTile;
   const int64_t units = (int64_t)c.n_seq * c.n_head_kv;
@@ -152,7 +158,7 @@ Planned plan_step(const knj_kv_cache& c, int n_head, int n_rows, int max_prefix)
   const FastDiv none(1);
   return {TreePlan{0, n_split, 1, (int)(units * n_split), FastDiv(c.n_head_kv), FastDiv(n_split),
                    FastDiv(n_head / c.n_head_kv), FastDiv(n_head), FastDiv(n_rows), none, true},
-          16, kStepTile, false};
+          n_rows * (n_head / c.n_head_kv) <= 16 ? 16 : 32, kStepTile, false};
 }
 
 // Of launch_pages_wide, for heads of 128 and more than 64 columns: two workgroups a CU (one and
@@ -177,7 +183,10 @@ Planned plan(const knj_kv_cache& c, int type, int n_head, int n_rows, int max_pr
   const int group = n_head / c.n_head_kv, n_cols = n_rows * group;
   const int chunks = (max_prefix + n_rows + kTreeChunk - 1) / kTreeChunk;
   const int64_t units = (int64_t)c.n_seq * c.n_head_kv;
-  if (c.format == kFormatPages && n_cols <= 16) return plan_step(c, n_head, n_rows, max_prefix);
+  const int64_t tiles32 = (max_prefix + n_rows + kStepTile - 1) / kStepTile;
+  if (c.format == kFormatPages &&
+      (n_cols <= 16 || (n_cols <= 32 && (units * tiles32 >= kStepWork || (tiles32 <= kStepMerges && units >= kStepUnits)))))
+    return plan_step(c, n_head, n_rows, max_prefix);
   const int64_t work = units * ((n_cols + 31) / 32) * chunks;
   if (c.format == kFormatPages && c.head_dim == 128 && n_cols > 64 &&
       work >= (n_rows >= max_prefix ? kPagesPrompt : kPagesWork))
@@ -243,7 +252,7 @@ int check_tree(const TreeArgs& a, uint64_t workspace_bytes, const char* what) {
 hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t s) {
   const tree::Planned q = tree::plan(a.c, a.type, a.n_head, a.n_rows, a.max_prefix);
   hipError_t e;
-  if (q.p.even) e = tree::launch_pages_step(a, q.p, s);
+  if (q.p.even) e = tree::launch_pages_step(a, q.p, q.cols, s);
   else if (q.wide) e = tree::launch_pages_wide(a, q.p, s);
   else if (a.c.format == KNJ_KV_F16) e = tree::launch_format<KNJ_KV_F16>(a, q.p, q.cols, s);
   else if (a.c.format == KNJ_KV_F8) e = tree::launch_format<KNJ_KV_F8>(a, q.p, q.cols, s);
