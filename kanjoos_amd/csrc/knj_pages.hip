@@ -22,7 +22,9 @@ using Piece = std::conditional_t<D == 128, u32v4, u32v2>;
 
 // ---------------------------------------------------------------- rows
 // A row's kv head is D/8 lanes of eight dims, four lanes a group of 32; the same lanes
-// take its key and its value.  blockIdx.y is the sequence.
+// take its key and its value.  blockIdx.y is the sequence.  Each element is read once and
+// written once: 4096 f32 rows of 4 kv heads, 19.4 MB either way, 7.1 us a call (2.7 TB/s, half
+// of it the launch's own latency; one row of 32 sequences takes 3.5 and 2.4).
 template <int D>
 struct PageUnit {
   static constexpr int T = D / 8;
@@ -217,7 +219,7 @@ struct ReserveWs {
         unused(fresh + n_page) {}
 };
 
-constexpr int kMaxSeq = 4096, kPlan = 1024, kPlanWaves = kPlan / 64, kPlanFew = 128;
+constexpr int kMaxSeq = 4096, kPlan = 1024, kPlanWaves = kPlan / 64, kPlanFew = 64;
 
 // How many of the workgroup's flags are set before this thread's, and in all.
 __device__ __forceinline__ int flags_before(bool f, int* waves, int& total) {
@@ -243,7 +245,8 @@ __device__ __forceinline__ int ld_agent(const int32_t* p) {
 // Which entries get which page, by one workgroup: the answer hangs on an order over all
 // sequences (lowest page first, all or none), and the entries of a step are few.  The
 // asked entries of all sequences are numbered through, and each thread takes every
-// 1024th.
+// 1024th.  Nothing but latency: 5 to 6 us for 4 to 32 sequences, a chain of lengths, table,
+// holders and stores with ten barriers between them.
 __global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
   const PageGeom& g = a.g;
   const ReserveWs ws(a.ws, g.n_page);
@@ -327,7 +330,8 @@ __global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
     __syncthreads();
   };
   // How many entries ask to replace a page, and the last of them: with few entries each
-  // counts for itself, else by atomics (where any page has other holders).
+  // counts for itself (32 entries 10.6 us a call against 11.6, 64 11.7 against 12.5; 128 12.6
+  // against 11.6), else by atomics (where any page has other holders).
   const bool few = n_asked <= kPlanFew;
   int asked = 0, last = -1;
   if (few) {
@@ -432,7 +436,7 @@ __global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
 
 // The first rows of pages copied, a layer per blockIdx.y, kBlock units of a page a
 // workgroup: units of D/8 bytes, of a row four of key codes, four of value codes and one
-// of either's words.
+// of either's words.  (Where nothing or one page a sequence is copied, 1.6 to 4 us, a launch.)
 template <int D>
 __global__ __launch_bounds__(kBlock) void k_pages_cow(PageGeom g, int32_t* words, uint32_t pieces) {
   using P = Piece<D>;
@@ -457,10 +461,13 @@ __global__ __launch_bounds__(kBlock) void k_pages_cow(PageGeom g, int32_t* words
 }
 
 // Rows moved together in place.  A workgroup has `width` of the 10 n_head_kv pieces of a
-// layer's rows of a sequence (of a head: four of key codes, four of value codes, one of
-// either's words) and takes the rows in order, `batch` at a time, which are all read before
-// one is written: a row's new slot is at or below its old one, so none is overwritten before
-// it has been read, and the next batch is fetched while this one is written.
+// layer's rows of a sequence (of a head: four of key codes and one of its words, the same of
+// values) and takes the rows in order, `batch` at a time, which are all read before one is
+// written: a row's new slot is at or below its old one, so none is overwritten before it has
+// been read, and the next batch is fetched while this one is written.
+// What bounds it: memory.  8000 of 16,000 slots, at random, in 48 layers of 4 kv heads are
+// 246 MB of rows, but lie in three quarters of the codes' lines of 128 bytes and in all of the
+// words': 450 MB fetched and 218 written by the counters, 120 us a call, 5.6 TB/s.
 struct MoveArgs {
   PageGeom g;
   const int32_t *start, *rows, *counts;
@@ -468,6 +475,7 @@ struct MoveArgs {
   uint32_t by_width;  // 2^32 / width rounded up: i / width for i below 2^16
 };
 constexpr int kMoveBatch = 2 * kBlock;  // at most
+constexpr int kMoveFew = 256;
 template <int D, int PIECES>
 __global__ __launch_bounds__(kBlock) void k_pages_compact(MoveArgs a) {
   using P = Piece<D>;
@@ -508,8 +516,9 @@ __global__ __launch_bounds__(kBlock) void k_pages_compact(MoveArgs a) {
     const uint32_t q = q0 + i - row[k] * a.width, h = q / 10, r = q - 10 * h;
     const bool in = row[k] < a.batch && q < 10u * g.n_head_kv;
     if (!in) row[k] = -1;
-    step[k] = r < 8 ? 4 : 1;
-    at[k] = in ? h * head + (r < 4 ? r : r < 8 ? (4u << g.shift) + r - 4 : r << g.shift) : 0;
+    const uint32_t v = r >= 5, part = r - 5 * v;  // of which matrix, which
+    step[k] = part < 4 ? 4 : 1;
+    at[k] = in ? h * head + (part < 4 ? (4 * v << g.shift) + part : (8 + v) << g.shift) : 0;
   }
   P x[2][PIECES];
   // (a piece that stays is read all the same, from page 0)
@@ -548,7 +557,8 @@ __global__ __launch_bounds__(kBlock) void k_pages_compact(MoveArgs a) {
   }
 }
 
-// Whole pages, a layer per blockIdx.y: 16 KB a workgroup, four 16-byte loads a thread.
+// Whole pages, a layer per blockIdx.y: 16 KB a workgroup, four 16-byte loads a thread (400
+// pages of 41 KB in 48 layers, 1.57 GB both ways: 298 us, 5.3 TB/s, as fast as a plain copy).
 constexpr int kCopyPiece = 4 * kBlock;  // of 16 bytes
 __global__ __launch_bounds__(kBlock) void k_pages_copy(PageGeom to, PageGeom from, const int32_t* dst, const int32_t* src,
                                                        uint32_t pieces, uint64_t n) {
@@ -611,7 +621,8 @@ hipError_t launch_pages_reserve(const PageReserveArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_pages_fork(const PageGeom& g, const int32_t* parent, const int32_t* keep, int32_t* ws, hipStream_t s) {
-  // (one launch: 4 beams of 17 pages 2.4 us against 4.1 in two, 32 of 252 3.8 against 4.9)
+  // (one launch: 4 beams of 17 pages 4.2 us against 6.5 in two, 32 of 126 4.3 against 6.0, 32 of
+  // 256 5.4 against 6.0)
   if ((int64_t)g.n_seq * g.n_table <= kForkOne) {
     KNJ_LAUNCH(k_pages_fork, dim3(1), dim3(1024), 0, s, g, parent, keep);
     return hipGetLastError();
@@ -628,12 +639,16 @@ hipError_t launch_pages_free(const PageGeom& g, const int32_t* keep, hipStream_t
 
 hipError_t launch_pages_compact(const PageGeom& g, const int32_t* start, const int32_t* rows, const int32_t* counts,
                                 int n_rows, hipStream_t s) {
-  // all of a layer's rows to a workgroup, or where those are few a head's or a matrix's;
-  // two pieces a thread where that takes all rows at once
-  const int64_t all = (int64_t)g.n_layer * g.n_seq;
-  const int width = all >= 512 ? 10 * std::min(g.n_head_kv, 16) : all * g.n_head_kv >= 512 ? 10 : 5;
+  // A head's rows to a workgroup.  Few rows: two pieces a thread (48 layers x 4 kv heads, 8, 12
+  // and 32 sequences of 60, 100 and 200 rows 7.4, 15.0 and 83 us against 11.4, 18.6 and 87 with
+  // ten; one of 500 10.4 against 8.7, of 8000 182 against 128), and so few that those of all
+  // heads fit at once, all of a layer's (32 of 8 rows 5.2 us against 9.9; 4 of 8 in 24 layers
+  // 5.0 and 4.8).  Many rows in few layers: a matrix's (one of 8000 in 24 layers 55 us against
+  // 70; in 48 layers 128 and 127).
+  const int all = 10 * std::min(g.n_head_kv, 16), pieces = n_rows <= kMoveFew ? 2 : 10;
+  const int64_t heads = (int64_t)g.n_layer * g.n_seq * g.n_head_kv;
+  const int width = (int64_t)n_rows * all <= 2 * dev::kBlock ? all : pieces == 10 && heads < 128 ? 5 : 10;
   const int parts = (10 * g.n_head_kv + width - 1) / width;
-  const int pieces = (int64_t)n_rows * width <= 2 * dev::kBlock ? 2 : 10;
   const int batch = std::min(pieces * dev::kBlock / width, kMoveBatch);
   const MoveArgs a{g, start, rows, counts, n_rows, width, batch, (uint32_t)((0x100000000ull + width - 1) / width)};
   const dim3 grid(parts, g.n_layer, g.n_seq);
