@@ -483,18 +483,19 @@ __global__ __launch_bounds__(kBlock) void k_pages_compact(MoveArgs a) {
   const uint32_t s = blockIdx.z, q0 = blockIdx.x * a.width;
   const int tid = threadIdx.x;
   const int64_t to0 = a.start[s];
-  const int n = a.counts ? min(max(a.counts[s], 0), a.n_rows) : a.n_rows;
+  // (unsigned: the first row past the last batch may lie beyond 2^31)
+  const uint32_t n = a.counts ? min(max(a.counts[s], 0), a.n_rows) : a.n_rows;
   if (n == 0) return;
   P* layer = reinterpret_cast<P*>(g.data + (uint64_t)blockIdx.y * g.n_page * g.page_bytes());
   const uint32_t head = 10u << g.shift, size = g.size();
   // a batch's rows: pages and rows in them of the old slot and the new, page -1 if it stays
   // (three buffers: a wave may look up the next batch while another writes the one before)
   __shared__ int src[3][kMoveBatch], dst[3][kMoveBatch], src_row[3][kMoveBatch];
-  auto look_up = [&](int i0, int buf) {
+  auto look_up = [&](uint32_t i0, int buf) {
 #pragma unroll
     for (int r = tid; r < kMoveBatch; r += kBlock) {
       if (r >= a.batch) break;
-      const int i = i0 + r;
+      const uint32_t i = i0 + r;
       int p = -1, q = -1, from = 0;
       if (i < n) {
         from = a.rows[(uint64_t)s * a.n_rows + i];
@@ -529,7 +530,7 @@ __global__ __launch_bounds__(kBlock) void k_pages_compact(MoveArgs a) {
       x[k] = layer[(uint64_t)p * g.n_head_kv * head + at[k] + step[k] * src_row[buf][r]];
     }
   };
-  auto put = [&](int i0, int buf, const P (&x)[PIECES]) {
+  auto put = [&](uint32_t i0, int buf, const P (&x)[PIECES]) {
 #pragma unroll
     for (int k = 0; k < PIECES; ++k) {
       if (row[k] < 0 || src[buf][row[k]] < 0) continue;
@@ -541,10 +542,11 @@ __global__ __launch_bounds__(kBlock) void k_pages_compact(MoveArgs a) {
   __syncthreads();
   fetch(0, x[0]);
   int buf = 0;
-  for (int i0 = 0; i0 < n; i0 += 2 * a.batch) {
+  for (uint32_t i0 = 0; i0 < n; i0 += 2 * a.batch) {
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      const int i = i0 + b * a.batch, next = buf == 2 ? 0 : buf + 1;
+      const uint32_t i = i0 + b * a.batch;
+      const int next = buf == 2 ? 0 : buf + 1;
       if (i >= n) break;
       const bool more = i + a.batch < n;
       if (more) look_up(i + a.batch, next);

@@ -467,6 +467,51 @@ def test_attention_many_columns_drifting(device, t, rising):
     assert np.isnan(got[1]).all()
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("D,T,nh,nk,page,prefixes,loose", [
+    (128, 4, 16, 2, 64, (0, 500, 31, 1900), True), (64, 17, 2, 2, 16, (64, 200), True), (128, 9, 6, 2, 32, (1, 1000), True),
+    (128, 3, 32, 4, 64, tuple(range(0, 500, 31)), False), (64, 8, 24, 8, 128, (0, 1, 30, 32, 33, 450, 64, 90), False)])
+def test_attention_two_column_tiles(device, t, D, T, nh, nk, page, prefixes, loose):
+    """17 to 32 columns with work enough: trees with what not every row sees, rows that see nothing, rows that see a
+    spoilt value, sequences with fewer rows; the same bits with a mask that sees all before it as without."""
+    print(f"two tiles type {t} D {D} T {T} heads {nh}/{nk} page {page} prefixes {prefixes}", flush=True)
+    rng = np.random.default_rng([T, nh, page, t])
+    n = len(prefixes)
+    pool = filled(rng, [m + T + 20 for m in prefixes], page, nk, D, extra=(LOOSE + T) // page + 1 if loose else 2)
+    counts = np.array([T if s % 3 == 0 else max(T - s, 0) for s in range(n)])
+    sees = np.stack([tree_bits(rng, T) for _ in range(n)])
+    sees[:, :, 1] = False
+    sees[:, 0] = False
+    for s, P in enumerate(prefixes):
+        for slot in range(P + counts[s], P + T + 20):  # every byte past the rows set: NaN in step and lowest value
+            at = pool.where(s, slot)
+            for b in pool.blocks():
+                b[1, at[0], :, at[1]] = 0xFF
+        x = rng.normal(size=(2, nk, D))
+        x[1, :, 5], x[0, :, 7] = np.inf, -np.inf
+        if counts[s] > 1:
+            pool.put(1, s, P + 1, *x)
+    sees[0, 2, 1] = True  # a spoilt value seen
+    p = upload(pool)
+    kv = caches(pool, max(prefixes) + T)
+    q = decode(encode(1.5 * rng.normal(size=(n, T, nh, D)), t), t)
+    limit = LOOSE if loose else None
+    got, before = attend(p, t, q, T, prefixes, counts, sees, nh, pad=16, max_prefix=limit)
+    with np.errstate(invalid="ignore", over="ignore"):
+        want, bound = tree64(q, kv, prefixes, counts, sees, D ** -0.5, t)
+    for s in range(n):
+        close(got[s, :counts[s]], want[s, :counts[s]], bound[s, :counts[s]], f"prefix {prefixes[s]}")
+        assert np.array_equal(got[s, counts[s]:], before[s, counts[s]:])  # rows past the drafts
+        if prefixes[s] == 0 and counts[s]:
+            assert np.all(got[s, 0] == 0)
+    assert np.isnan(got[0, 2]).all()
+    below = np.tril(np.ones((1, T, T), bool))
+    chain, _ = attend(p, t, q, T, prefixes, counts, None, nh, max_prefix=limit)
+    again, _ = attend(p, t, q, T, prefixes, counts, below, nh, shared=True, max_prefix=limit)
+    for s in range(n):
+        assert np.array_equal(again[s, :counts[s]], chain[s, :counts[s]], equal_nan=True)
+
+
 @pytest.mark.parametrize("T", [1, 3])
 def test_attention_long(device, T):
     """Long contexts of several splits; layers and pages beyond 2^32 bytes."""
