@@ -6,7 +6,7 @@ namespace knj {
 namespace tree {
 namespace {
 
-// Heads of 128.  Workgroup = (sequence, split of the slots, kv head, tile of 128 columns) of
+// Heads of 128.  Workgroup = (sequence, split of the slots, kv head, tile of up to 128 columns) of
 // eight waves of 16 columns each, over steps of 64 slots:
 //   scores  S[slot][col] = K (16 slots x 32 dims) x Q (32 dims x 16 columns);
 //   values  O^T[d][col] = V^T (16 dims x 32 slots) x E (32 slots x 16 columns),
@@ -17,8 +17,8 @@ namespace {
 // is computed: one barrier a step, the codes fetched two steps ahead, their pages looked up
 // three (a wave's 16 rows are of one page: scalar).  Rows are padded by 32 bytes.
 //
-// What bounds it (500 rows x 32 heads over 8000 slots of 4 kv heads, 70 GFLOP and a third
-// more for the remainders: 120 us a call, 8 of them the merge, 0.58 PFLOP/s): a SIMD's
+// What bounds it (500 rows x 32 heads over 8000 slots of 4 kv heads, 68 GFLOP and half
+// as many for the remainders: 120 us a call, 8 of them the merge, 0.56 PFLOP/s): a SIMD's
 // products take 43 % of its cycles and its other vector instructions 43 %, which hardly
 // overlap on one SIMD, whichever waves they come from.  Of a wave's vector instructions a
 // step (180) 48 form the weights, 32 split them and 44 decode its share of the rows.  Hence
@@ -28,7 +28,7 @@ namespace {
 template <bool SPLIT>
 __global__ __launch_bounds__(64 * kWideWaves, 4) void k_pages_wide(TreeArgs a, TreePlan p) {
   using H = PageHead<128>;
-  constexpr int D = 128, S = kWideStep, COLS = 16 * kWideWaves, DT = D / 16, NC = D / 32, ST = S / 16;
+  constexpr int D = 128, S = kWideStep, DT = D / 16, NC = D / 32, ST = S / 16;
   constexpr int RS = 2 * D + 32, SB = S * RS;      // bytes of a row in LDS, of a matrix's step
   static_assert(2 * S * NC == 64 * kWideWaves && S == 64, "a group a thread");
   __shared__ __align__(16) uint8_t lds[4 * SB];    // keys and values of even steps, of odd steps
@@ -44,12 +44,17 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void k_pages_wide(TreeArgs a, T
   const int r = lane & 15, kq = lane >> 4;
   int P, N;
   seq_lengths(a, s, P, N);
-  const int valid = P + N, n_cols = p.n_tiles * COLS;
+  const int valid = P + N, n_cols = p.n_tiles * 16 * kWideWaves;
   const int c0 = split * p.cps, steps = (valid + S - 1) / S;
-  if (tile * COLS >= N * G || c0 >= steps) return;
+  // the columns, 16 a wave, spread evenly over the tiles: a wave without any only decodes (25
+  // drafts x 8 heads, 7 and 6 waves with some, over 32,700 slots 41.6 us a call; with 8 and 5, or
+  // 8 and the last 3 computing what is not stored, 42.5 and 43.6)
+  const int each = ((a.n_rows * G + 15) / 16 + p.n_tiles - 1) / p.n_tiles, col0 = 16 * (tile * each + wave);
+  const bool mine = wave < each && col0 < N * G;
+  if (16 * tile * each >= N * G || c0 >= steps) return;
   // slots before `all` are seen by every row of the tile; a chain's tile goes no further than
   // its last row (a split that begins behind it has an empty record)
-  const int row_0 = p.by_group.div(tile * COLS), row_1 = p.by_group.div(min(tile * COLS + COLS, N * G) - 1);
+  const int row_0 = p.by_group.div(16 * tile * each), row_1 = p.by_group.div(min(16 * (tile + 1) * each, N * G) - 1);
   const int all = a.mask ? P : P + row_0 + 1;
   const int c1 = min(min(a.mask ? steps : (P + row_1) / S + 1, steps), c0 + p.cps);
 
@@ -102,7 +107,7 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void k_pages_wide(TreeArgs a, T
   look_up(c0 + 1);
 
   // ---- this lane's query column: step c's dims 32 c + 8 kq .. + 7, in decode8_mixed's order
-  const int col = tile * COLS + wave * 16 + r, ccol = min(col, a.n_rows * G - 1);  // (past the rows: not stored)
+  const int col = col0 + r, ccol = min(col, a.n_rows * G - 1);  // (past the rows: not stored)
   const int trow = p.by_group.div(ccol);
   h16x8 qh[NC], ql[NC];
   const float s2 = column<D, SPLIT>(
@@ -122,80 +127,82 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void k_pages_wide(TreeArgs a, T
   look_up(c0 + 2);
   for (int h = c0; h < c1; ++h) {
     KNJ_BARRIER_AFTER(kLdsOnly);
-    const uint32_t stage = 2 * (h & 1) * SB;
-    f32x4 sc[ST];
+    if (mine) {
+      const uint32_t stage = 2 * (h & 1) * SB;
+      f32x4 sc[ST];
 #pragma unroll
-    for (int st = 0; st < ST; ++st) sc[st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int st = 0; st < ST; ++st) sc[st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int st = 0; st < ST; ++st) {
-        const h16x8 ka = lds_h8(kat + stage + 16 * st * RS + 64 * c);
-        sc[st] = mfma16(ka, qh[c], sc[st]);
-        if constexpr (SPLIT) sc[st] = mfma16(ka, ql[c], sc[st]);
+        for (int st = 0; st < ST; ++st) {
+          const h16x8 ka = lds_h8(kat + stage + 16 * st * RS + 64 * c);
+          sc[st] = mfma16(ka, qh[c], sc[st]);
+          if constexpr (SPLIT) sc[st] = mfma16(ka, ql[c], sc[st]);
+        }
+      if (__builtin_expect((h + 1) * S > P, 0)) {
+        uint64_t seen = ~0ull, bad = 0;
+#pragma unroll
+        for (int st = 0; st < ST; ++st) bad |= (uint64_t)poison[h & 1][st] << (16 * st);
+        if ((h + 1) * S > all) {
+          seen = seen64(mask ? mask + (uint64_t)trow * words : nullptr, words, trow, N, h * S - P);
+#pragma unroll
+          for (int st = 0; st < ST; ++st)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (!((seen >> (16 * st + 4 * kq + i)) & 1)) sc[st][i] = -INFINITY;
+        }
+        if ((seen & bad) != 0) l = NAN;  // (and stays so)
       }
-    if (__builtin_expect((h + 1) * S > P, 0)) {
-      uint64_t seen = ~0ull, bad = 0;
+      // a weight beyond 2^kLag shows in the sum (and a column that has seen nothing yet in its
+      // reference, -inf): the reference is moved and the weights formed again
+      float w[4 * ST], sum;
+      auto weights = [&]() __attribute__((always_inline)) {
+        const float mr = m == -INFINITY ? 0.0f : m;
+        sum = 0.0f;
 #pragma unroll
-      for (int st = 0; st < ST; ++st) bad |= (uint64_t)poison[h & 1][st] << (16 * st);
-      if ((h + 1) * S > all) {
-        seen = seen64(mask ? mask + (uint64_t)trow * words : nullptr, words, trow, N, h * S - P);
+        for (int i = 0; i < 4 * ST; ++i) {
+          w[i] = __builtin_amdgcn_exp2f(fmaf(sc[i >> 2][i & 3], s2, -mr));
+          sum += w[i];
+        }
+      };
+      weights();
+      if (__builtin_expect(__ballot((!(sum <= 0x1p13f) | (m == -INFINITY)) & (m < INFINITY)) != 0, 0)) {
+        float mx = -INFINITY;
 #pragma unroll
         for (int st = 0; st < ST; ++st)
+          mx = max_nan(max_nan(max_nan(mx, sc[st][0]), max_nan(sc[st][1], sc[st][2])), sc[st][3]);
+        const float2 m16 = pair16_f(mx);
+        const float2 m32 = pair32_f(max_nan(m16.x, m16.y));
+        mx = max_nan(m32.x, m32.y);
+        const float old = m;
+        if (!(fmaf(mx, s2, -old) <= kLag)) m = max_nan(old, fmaf(mx, s2, -kLift));
+        const float alpha = __builtin_amdgcn_exp2f(old - (m == -INFINITY ? 0.0f : m));
+        l *= alpha;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (!((seen >> (16 * st + 4 * kq + i)) & 1)) sc[st][i] = -INFINITY;
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[dt][i] *= alpha;
+        weights();
       }
-      if ((seen & bad) != 0) l = NAN;  // (and stays so)
-    }
-    // a weight beyond 2^kLag shows in the sum (and a column that has seen nothing yet in its
-    // reference, -inf): the reference is moved and the weights formed again
-    float w[4 * ST], sum;
-    auto weights = [&]() __attribute__((always_inline)) {
-      const float mr = m == -INFINITY ? 0.0f : m;
-      sum = 0.0f;
+      l += sum;
+      h16x8 eh[ST / 2], el[ST / 2];
 #pragma unroll
-      for (int i = 0; i < 4 * ST; ++i) {
-        w[i] = __builtin_amdgcn_exp2f(fmaf(sc[i >> 2][i & 3], s2, -mr));
-        sum += w[i];
+      for (int e = 0; e < ST / 2; ++e) {
+        const float x[8] = {w[8 * e], w[8 * e + 1], w[8 * e + 2], w[8 * e + 3], w[8 * e + 4], w[8 * e + 5], w[8 * e + 6], w[8 * e + 7]};
+        split8(x, eh[e], el[e]);
       }
-    };
-    weights();
-    if (__builtin_expect(__ballot((!(sum <= 0x1p13f) | (m == -INFINITY)) & (m < INFINITY)) != 0, 0)) {
-      float mx = -INFINITY;
 #pragma unroll
-      for (int st = 0; st < ST; ++st)
-        mx = max_nan(max_nan(max_nan(mx, sc[st][0]), max_nan(sc[st][1], sc[st][2])), sc[st][3]);
-      const float2 m16 = pair16_f(mx);
-      const float2 m32 = pair32_f(max_nan(m16.x, m16.y));
-      mx = max_nan(m32.x, m32.y);
-      const float old = m;
-      if (!(fmaf(mx, s2, -old) <= kLag)) m = max_nan(old, fmaf(mx, s2, -kLift));
-      const float alpha = __builtin_amdgcn_exp2f(old - (m == -INFINITY ? 0.0f : m));
-      l *= alpha;
+      for (int e = 0; e < ST / 2; ++e)
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[dt][i] *= alpha;
-      weights();
+        for (int dt = 0; dt < DT; ++dt) {
+          const uint32_t at = vat + stage + 32 * e * RS + 32 * dt;
+          const u32x2 v0 = lds_tr16_at(at), v1 = lds_tr16_at(at + 16 * RS);
+          const h16x8 v = __builtin_bit_cast(h16x8, make_uint4(v0.x, v0.y, v1.x, v1.y));
+          acc[dt] = mfma16(v, eh[e], acc[dt]);
+          acc[dt] = mfma16(v, el[e], acc[dt]);
+        }
     }
-    l += sum;
-    h16x8 eh[ST / 2], el[ST / 2];
-#pragma unroll
-    for (int e = 0; e < ST / 2; ++e) {
-      const float x[8] = {w[8 * e], w[8 * e + 1], w[8 * e + 2], w[8 * e + 3], w[8 * e + 4], w[8 * e + 5], w[8 * e + 6], w[8 * e + 7]};
-      split8(x, eh[e], el[e]);
-    }
-#pragma unroll
-    for (int e = 0; e < ST / 2; ++e)
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const uint32_t at = vat + stage + 32 * e * RS + 32 * dt;
-        const u32x2 v0 = lds_tr16_at(at), v1 = lds_tr16_at(at + 16 * RS);
-        const h16x8 v = __builtin_bit_cast(h16x8, make_uint4(v0.x, v0.y, v1.x, v1.y));
-        acc[dt] = mfma16(v, eh[e], acc[dt]);
-        acc[dt] = mfma16(v, el[e], acc[dt]);
-      }
     put(h + 1);
     fetch(h + 2);
     look_up(h + 3);
@@ -207,7 +214,7 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void k_pages_wide(TreeArgs a, T
   float4 o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = in_order(acc[dt]);
-  if (col >= N * G) return;
+  if (!mine || col >= N * G) return;
   if (p.n_split > 1) {
     float* rec = a.partial + ((((uint64_t)s * nk + kvh) * p.n_split + split) * n_cols + col) * (D + 4);
     if (kq == 0) *reinterpret_cast<float2*>(rec) = make_float2(m, l);
