@@ -130,13 +130,17 @@ struct Planned {
 // 12,032 40.3 and 48.0 against 39.0 and 49.4 (int8 with f32 queries crosses there too);
 // over f16, where nothing is decoded, 64 drafts at 12,096 and 16,064 38.8 and 44.4
 // against 37.4 and 45.1, 25 at 14,028 and 28,028 43.5 and 69.0 against 40.9 and 72.3
-// (with f32 queries between 12,000, for many sequences, and 30,000, for one).
+// (with f32 queries between 12,000, for many sequences, and 30,000, for one); over 4-bit
+// pages, where decoding costs most, 8 drafts x 8 heads of 32 sequences at 8,192, 12,288 and
+// 16,384 35.9, 43.9 and 54.7 against 37.9, 48.3 and 60.1, heads of 64 at 8,192 and 33,250 25.0
+// and 53.6 against 26.9 and 122 (at 4,032 18.3 against 19.4, with f32 queries 22.0 against 20.3).
 // Two workgroups a CU where each then has several chunks, else one, with fewer records
 // to merge: two against one for 16 drafts x 8 heads over 8,000, 12,000 and 16,000 f16
 // slots (2,016, 3,008 and 4,016 chunks of tiles) 16.0, 18.3 and 20.6 against 15.6, 19.1
 // and 22.2 us, over int8 with f32 queries 21.8, 25.4 and 29.5 against 22.5, 28.2 and 34.0;
 // 4 drafts over 8,000 f16 slots (504) 16.8 against 12.5.
-constexpr int64_t kWideWork = 10000, kWideWorkF16 = 16000, kTwoWork = 2500;  // chunks of 32-column tiles, chunks of tiles
+constexpr int64_t kWideWork = 10000, kWideWorkF16 = 16000, kWideWorkPages = 8000;  // chunks of 32-column tiles
+constexpr int64_t kTwoWork = 2500;  // chunks of tiles
 
 // Of launch_pages_step.  A wave's tile takes 1.0 us and a merge 3: one workgroup a unit up to
 // four tiles a wave (32 sequences of 500 slots 10.2 us against 12.3 in four splits, 8 of
@@ -192,7 +196,8 @@ Planned plan(const knj_kv_cache& c, int type, int n_head, int n_rows, int max_pr
       work >= (n_rows >= max_prefix ? kPagesPrompt : kPagesWork))
     return plan_wide(c, n_head, n_rows, max_prefix);
   int cols = n_cols <= 16 ? 16 : 32;
-  if (n_cols > 32 && work >= (c.format == KNJ_KV_F16 ? kWideWorkF16 : kWideWork))
+  const int64_t wide = c.format == KNJ_KV_F16 ? kWideWorkF16 : c.format == kFormatPages ? kWideWorkPages : kWideWork;
+  if (n_cols > 32 && work >= wide)
     cols = n_cols <= 64 || type == KNJ_TYPE_F32 ? 64 : 128;
   const int tiles = (n_cols + cols - 1) / cols;
   const int64_t wgs = units * tiles * chunks >= kTwoWork ? 512 : 256;

@@ -372,15 +372,16 @@ LOOSE = 32000
 
 
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("T,nh,nk,page,prefixes", [
-    (66, 8, 4, 16, (0, 1, 61, 62, 63, 64, 126, 127, 500)), (25, 32, 2, 64, (190, 3, 64)), (130, 5, 1, 32, (0, 127, 128, 700)),
-    (17, 4, 1, 256, (100, 257, 0, 40, 1900)), (257, 3, 3, 128, (5, 255))])
-def test_attention_many_columns(device, t, T, nh, nk, page, prefixes):
+@pytest.mark.parametrize("T,nh,nk,page,prefixes,D", [
+    (66, 8, 4, 16, (0, 1, 61, 62, 63, 64, 126, 127, 500), 128), (25, 32, 2, 64, (190, 3, 64), 128),
+    (130, 5, 1, 32, (0, 127, 128, 700), 128), (17, 4, 1, 256, (100, 257, 0, 40, 1900), 128), (257, 3, 3, 128, (5, 255), 128),
+    (25, 4, 2, 32, (0, 64, 500, 63), 128), (44, 8, 2, 16, (0, 127, 300), 64), (20, 6, 2, 64, (1, 64, 130, 0), 64)])
+def test_attention_many_columns(device, t, T, nh, nk, page, prefixes, D):
     """Trees with what not every row sees: NaN and huge values in unseen rows and past them, rows that see nothing,
     rows that see a spoilt value; sequences with fewer rows, one of them with none."""
-    print(f"many columns type {t} T {T} heads {nh}/{nk} page {page} prefixes {prefixes}", flush=True)
+    print(f"many columns type {t} D {D} T {T} heads {nh}/{nk} page {page} prefixes {prefixes}", flush=True)
     rng = np.random.default_rng([T, nh, page, t])
-    n, D = len(prefixes), 128
+    n = len(prefixes)
     pool = filled(rng, [m + T + 20 for m in prefixes], page, nk, D, extra=(LOOSE + T) // page + 1)
     counts = np.array([T if s == 0 else max(T - 40 * s, 0) for s in range(n)])
     sees = np.stack([tree_bits(rng, T) for _ in range(n)])
@@ -393,7 +394,7 @@ def test_attention_many_columns(device, t, T, nh, nk, page, prefixes):
                 b[1, at[0], :, at[1]] = 0xFF
         x = rng.normal(size=(3, 2, nk, D))
         x[0, 1, :, 5], x[0, 0, :, 7] = np.inf, -np.inf
-        x[1, :, :, 100] = np.nan
+        x[1, :, :, D - 28] = np.nan
         x[2] *= 1e4
         for r in range(min(3, counts[s] - 2)):
             pool.put(1, s, P + 2 + r, *x[r])
