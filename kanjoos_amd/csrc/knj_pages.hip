@@ -297,10 +297,11 @@ __global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
   }
   __syncthreads();
 
-  // entry number f: its place in the table, the page that it holds (-1: none) and that page's
-  // holders.  A thread's first one is kept: a step's entries are rarely more.
+  // entry number f: its place in the table, the page that it holds (-1: none), that page's
+  // holders and its sequence's length.  A thread's first one is kept: a step's entries are
+  // rarely more.
   struct Entry {
-    int at, e, s, page, holders;
+    int at, e, length, page, holders;
   };
   auto find = [&](int f) {
     Entry x;
@@ -310,7 +311,7 @@ __global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
       if (first[mid] <= f) lo = mid;
       else hi = mid;
     }
-    x.s = lo;
+    x.length = a.length[lo];
     x.e = lowest[lo] + (f - first[lo]);
     x.at = lo * g.n_table + x.e;
     x.page = g.table[x.at];
@@ -330,8 +331,8 @@ __global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
     __syncthreads();
   };
   // How many entries ask to replace a page, and the last of them: with few entries each
-  // counts for itself (32 entries 10.6 us a call against 11.6, 64 11.7 against 12.5; 128 12.6
-  // against 11.6), else by atomics (where any page has other holders).
+  // counts for itself (32 entries 9.2 us a call against 10.2, 64 10.9 against 12.0; of 128 1.0
+  // more), else by atomics (where any page has other holders).
   const bool few = n_asked <= kPlanFew;
   int asked = 0, last = -1;
   if (few) {
@@ -418,7 +419,7 @@ __global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
     g.refs[page] = 1;
     if (x.page < 0) return;
     atomicSub(&g.refs[x.page], 1);
-    const int64_t rows = min((int64_t)a.length[x.s] - ((int64_t)x.e << g.shift), (int64_t)g.size());
+    const int64_t rows = min((int64_t)x.length - ((int64_t)x.e << g.shift), (int64_t)g.size());
     if (rows <= 0) return;
     int32_t* c = ws.copies + 3 * (uint64_t)atomicAdd(&n_copies, 1);
     c[0] = x.page;

@@ -704,7 +704,8 @@ def test_entries_that_are_none(device):
 
 
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("n_rows,page,nk", [(1, 16, 1), (7, 64, 4), (64, 16, 2), (65, 32, 1), (256, 256, 3), (257, 16, 2), (900, 64, 1)])
+@pytest.mark.parametrize("n_rows,page,nk", [(1, 16, 1), (7, 64, 4), (64, 16, 2), (65, 32, 1), (256, 256, 3), (257, 16, 2), (900, 64, 1), (400, 16, 12),
+                                            (3, 16, 20), (600, 32, 11)])
 def test_compact(device, D, n_rows, page, nk):
     """Rows moved over one another, from one slot on to far; sequences that move nothing, or all of theirs by one."""
     print(f"compact D {D} rows {n_rows} page {page} nk {nk}", flush=True)
