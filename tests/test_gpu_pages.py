@@ -908,12 +908,13 @@ class Step:
                 self.p.refs.download(np.int32), self.missing.download(np.int32)]
 
 
-SHAPES = [dict(D=64, page=16, T=4), dict(D=128, page=64, T=1)]
+SHAPES = [dict(D=64, page=16, T=4), dict(D=128, page=64, T=1), dict(D=128, page=128, T=300)]
 
 
-def test_two_streams_at_once(streams):
+@pytest.mark.parametrize("pair", [(0, 1), (2, 1)])
+def test_two_streams_at_once(streams, pair):
     """Two steps on two streams, workspaces each, give what each gives alone."""
-    steps = [Step(np.random.default_rng(i), streams[i], **SHAPES[i]) for i in range(2)]
+    steps = [Step(np.random.default_rng(i), streams[i], **SHAPES[pair[i]]) for i in range(2)]
     want = []
     for st in steps:
         for _ in range(6):
@@ -931,10 +932,11 @@ def test_two_streams_at_once(streams):
             assert np.array_equal(a, b)
 
 
-def test_steps_in_graphs(streams):
+@pytest.mark.parametrize("pair", [(0, 1), (2, 1)])
+def test_steps_in_graphs(streams, pair):
     """Captured steps, replayed with inputs changed in between and eager work between replays."""
     h, stream = hip(), streams[0]
-    steps = [Step(np.random.default_rng(i), stream, **SHAPES[i]) for i in range(2)]
+    steps = [Step(np.random.default_rng(i), stream, **SHAPES[pair[i]]) for i in range(2)]
     graphs = []
     for st in steps:
         st.run()
