@@ -763,6 +763,60 @@ def test_copy(device, D, nk, page, n_layer):
     same(p, a)
 
 
+def test_offsets_beyond_32_bits(device):
+    """Pages 2.4 GB into a layer, layers 2.4 GB apart: rows, attention of one and of many, copied, moved."""
+    n_page, page, nk, nh, D, n_layer, T = 60000, 64, 4, 32, 128, 3, 150
+    rng = np.random.default_rng(5)
+    p = K.KvPages.allocate(n_layer, n_page, page, nk, D, 2, 16)
+    refs = np.ones(n_page, np.int32)
+    refs[-20:] = 0
+    p.refs.upload(refs)
+    ws, missing = K.DeviceBuffer(K.pages_workspace(p)), i32([5])
+    K.pages_reserve(p, i32([0, 0]), i32([300, 200]), missing, ws)
+    table = p.table.download(np.int32).reshape(2, 16)
+    assert missing.download(np.int32)[0] == 0
+    assert table[0, :5].tolist() == list(range(n_page - 20, n_page - 15)) and table[1, :4].tolist() == list(range(n_page - 15, n_page - 11))
+    x = rng.normal(size=(n_layer, 2, 2, 300, nk, D)).astype(np.float32)
+    for layer in range(n_layer):
+        bufs = [put(a) for a in x[layer]]
+        K.pages_store(p, layer, F32, bufs[0], bufs[1], i32([0, 0]), 300, counts=i32([300, 200]))
+    held = values(*groups(x.astype(np.float64)))
+
+    def check(s, n, want, what):
+        """Slots below n of sequence s hold want [n_layer][2][n][nk][D]."""
+        for layer in range(n_layer):
+            out = [K.DeviceBuffer(2 * 300 * nk * D * 4) for _ in range(2)]
+            K.pages_load(p, layer, F32, out[0], out[1], 300)
+            for i in range(2):
+                got = out[i].download(np.float32).reshape(2, 300, nk, D)[s, :n]
+                assert np.array_equal(got, want[layer, i].astype(np.float32)), (what, layer, i)
+
+    check(0, 300, held[:, :, 0], "rows")
+    check(1, 200, held[:, :, 1, :200], "rows")
+    kv = [held[2, i].transpose(0, 2, 1, 3) for i in range(2)]
+    for rows, prefixes in ((1, [299, 199]), (4, [296, 196]), (T, [150, 50])):
+        q = rng.normal(size=(2, rows, nh, D)).astype(np.float32).astype(np.float64)
+        got, _ = attend(p, F32, q, rows, prefixes, None, None, nh, layer=2)
+        want, bound = tree64(q, kv, prefixes, [rows] * 2, np.stack([np.tril(np.ones((rows, rows), bool))] * 2), D ** -0.5, F32)
+        close(got, want, bound, f"{rows} rows")
+    # the first sequence's start shared, its third page copied
+    K.pages_fork(p, i32([0, 0]), ws, keep=i32([300, 130]))
+    K.pages_reserve(p, i32([300, 130]), i32([300, 140]), missing, ws)
+    table = p.table.download(np.int32).reshape(2, 16)
+    assert table[1, :2].tolist() == table[0, :2].tolist() and table[1, 2] == n_page - 15
+    check(1, 130, held[:, :, 0, :130], "copied")
+    # 100 of its rows moved together
+    moved = np.sort(rng.choice(np.arange(160, 300), 100, False))
+    K.pages_compact(p, i32([130, 0]), i32(np.stack([moved, np.arange(100)])), 100, counts=i32([100, 0]))
+    now = held[:, :, 0, :230].copy()
+    now[:, :, 130:] = held[:, :, 0, moved]
+    check(0, 230, now, "moved")
+    K.pages_copy(p, p, i32([7, n_page - 1]), i32([n_page - 20, n_page - 19]), 2)
+    table[1, :2] = [7, n_page - 1]
+    p.table.upload(table)
+    check(1, 128, held[:, :, 0, :128], "pages copied")
+
+
 # ------------------------------------------------------------------ together
 
 class Serving:
