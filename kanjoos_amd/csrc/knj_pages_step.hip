@@ -13,8 +13,9 @@ namespace {
 //           are D/4 kq + 8 c ..: whichever order, as long as the queries have the same);
 //   values  O^T[d][col] = V^T (16 dims x 32 slots) x E, the decoded rows through 9 KB of
 //           LDS of the wave's own, read back transposed.
-// The weights' reference, split and the records are k_tree's.  f32 queries take the
-// registers of a fourth wave a SIMD, and 17 to 32 columns those of a third.
+// The weights' reference, split and the records are k_tree's.  Registers are those of three
+// waves a SIMD (held to four it spills: 32 sequences over 8000 slots 40.4 us a call against
+// 39.1, over 500 10.2 against 9.9), with 17 to 32 columns of two.
 //
 // What bounds it (32 sequences of up to 8000 slots, 32 heads over 4 kv heads, 144 MB: 39 us a
 // call, 3.7 TB/s; the loads alone, nothing decoded or multiplied, 34): 250 tiles a unit over
@@ -24,7 +25,7 @@ namespace {
 // and two launches.  Four drafts instead of one cost 7 us more (46; k_tree, which shares a
 // chunk's rows between waves behind barriers, 57).
 template <int D, bool SPLIT, int NT>
-__global__ __launch_bounds__(64 * kStepWaves, NT == 2 ? 2 : SPLIT ? 3 : 4) void k_pages_step(TreeArgs a, TreePlan p) {
+__global__ __launch_bounds__(64 * kStepWaves, NT == 2 ? 2 : 3) void k_pages_step(TreeArgs a, TreePlan p) {
   using H = PageHead<D>;
   constexpr int NW = kStepWaves;
   constexpr int DT = D / 16, NC = D / 32;
