@@ -19,7 +19,7 @@ namespace {
 //
 // What bounds it (32 sequences of up to 8000 slots, 32 heads over 4 kv heads, 144 MB: 39 us a
 // call, 3.7 TB/s; the loads alone, nothing decoded or multiplied, 34): 250 tiles a unit over
-// two workgroups a CU, each wave some 450 vector instructions a tile of which 190 decode, in
+// two workgroups a CU, each wave some 280 vector instructions a tile of which 190 decode, in
 // waves that the memory keeps waiting; 4 of the 39 are the merge.  A step over 1000 slots,
 // 9.2 us, is one tile a wave (1.0 us), the prologue's chain of loads (lengths, table, rows)
 // and two launches.  Four drafts instead of one cost 7 us more (46; k_tree, which shares a
