@@ -335,7 +335,8 @@ int knj_pages_load(const knj_kv_pages* pages, int layer, int type, const int32_t
 /* knj_attention_pages: knj_attention_tree over one layer of pages: its arguments, masks and
  *   limits (n_ctx is n_table * page_size; a decode step is n_rows 1 with its own key stored, a
  *   piece of a prompt n_rows up to 1024 without a mask).  A slot without a page holds NaN.
- *   f32 queries keep 22 bits; weights keep 22 bits with any activations, and queries are of
+ *   A value group of a prefix slot that reads back as NaN makes its own 32 dims NaN, of every
+ *   row; of a draft's slot, as there, all dims of the rows that see it.  f32 queries keep 22 bits; weights keep 22 bits with any activations, and queries are of
  *   any size that leaves the scores, scale q.k, below 2^25 in magnitude with scale |q| below
  *   2^126. */
 int knj_attention_pages(const knj_kv_pages* pages, int layer, int type, const void* q,

@@ -36,9 +36,9 @@ __device__ __forceinline__ void split8(const float (&w)[8], h16x8& hi, h16x8& lo
 }
 
 // The halves of a word that are infinite or NaN (0x7C00 and up) replaced by zero; the sign
-// bits of those that were.
-__device__ __forceinline__ uint32_t clear_nonfinite(uint32_t& w) {
-  const uint32_t m = ((w & 0x7FFF7FFFu) + 0x04000400u) & 0x80008000u;
+// bits of those that were.  `signs` has both halves' sign bits, or none: then nothing is.
+__device__ __forceinline__ uint32_t clear_nonfinite(uint32_t& w, uint32_t signs) {
+  const uint32_t m = ((w & 0x7FFF7FFFu) + 0x04000400u) & signs;
   w &= ~(m | (m - (m >> 15)));
   return m;
 }

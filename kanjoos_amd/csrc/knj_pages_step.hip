@@ -161,8 +161,9 @@ __global__ __launch_bounds__(64 * kStepWaves, NT == 2 ? 2 : 3) void k_pages_step
     const int next = j + NW < c1 ? j + NW : j;
     const int p0 = j * kStepTile;
     const bool drafts = p0 + kStepTile > P;
-    // the values' rows to LDS; beyond the prefix what is not finite there is dropped, and
-    // the rows that held it noted (slots past the rows are zeros)
+    // the values' rows to LDS; of slots beyond the prefix what is not finite there is dropped,
+    // and the rows that held it noted (slots past the rows are zeros; a prefix slot is seen
+    // by every column and keeps its group's NaN)
     uint32_t bad = 0;
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
@@ -174,10 +175,11 @@ __global__ __launch_bounds__(64 * kStepWaves, NT == 2 ? 2 : 3) void k_pages_step
       for (int i = 0; i < NC; ++i) x[i] = decode8_mixed(words_of(V.c[st], i), step, low);
       if (drafts) {
         uint32_t any = 0;
+        const uint32_t signs = slot >= P ? 0x80008000u : 0u;
 #pragma unroll
         for (int i = 0; i < NC; ++i)
-          any |= clear_nonfinite(x[i].x) | clear_nonfinite(x[i].y) | clear_nonfinite(x[i].z) | clear_nonfinite(x[i].w);
-        // (of the prefix's rows in the tile too: every column sees them)
+          any |= clear_nonfinite(x[i].x, signs) | clear_nonfinite(x[i].y, signs) | clear_nonfinite(x[i].z, signs) |
+                 clear_nonfinite(x[i].w, signs);
         const uint64_t b = __ballot(any != 0);
         bad |= (uint32_t)((b | b >> 16 | b >> 32 | b >> 48) & 0xFFFF) << (16 * st);
       }

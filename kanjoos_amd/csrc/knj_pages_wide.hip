@@ -77,7 +77,8 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void k_pages_wide(TreeArgs a, T
     word = *reinterpret_cast<const uint32_t*>(base + H::meta(matrix, shift) + slot * H::kMeta + 4 * group);
   };
   // Step x's group, decoded, into its buffer.  Of values behind the prefix what is not finite
-  // is dropped and the rows that held it noted; slots past the rows are zeros.
+  // is dropped and the rows that held it noted; slots past the rows are zeros.  (A prefix slot
+  // is seen by every column and keeps its group's NaN.)
   const uint32_t put_at = lds_addr(lds) + matrix * SB + row * RS + 64 * group;
   auto put = [&](int x) __attribute__((always_inline)) {
     const bool drafts = matrix == 1 && (x + 1) * S > P;
@@ -88,9 +89,11 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void k_pages_wide(TreeArgs a, T
                   decode8_mixed(code.z, st, low), decode8_mixed(code.w, st, low)};
     if (drafts) {
       uint32_t any = 0;
+      const uint32_t signs = x * S + row >= P ? 0x80008000u : 0u;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        any |= clear_nonfinite(v[k].x) | clear_nonfinite(v[k].y) | clear_nonfinite(v[k].z) | clear_nonfinite(v[k].w);
+        any |= clear_nonfinite(v[k].x, signs) | clear_nonfinite(v[k].y, signs) | clear_nonfinite(v[k].z, signs) |
+               clear_nonfinite(v[k].w, signs);
       uint64_t b = __ballot(any != 0);  // four bits a row: into one
       b |= b >> 1;
       b |= b >> 2;

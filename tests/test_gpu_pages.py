@@ -289,6 +289,40 @@ def test_attention_unseen_slots(device, t, T, nh):
     assert np.all(got[0, 0] == 0)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("D,T,nh,nk,page,prefixes,limit", [
+    (128, 1, 16, 2, 64, (101, 128, 135, 129), None), (64, 2, 16, 2, 16, (1000, 111, 130, 160), None),  # up to 16 columns
+    (128, 3, 32, 4, 32, (101, 128, 131, 130) * 4, None), (64, 17, 2, 2, 64, (101, 200), 32000),  # 17 to 32
+    (64, 9, 16, 2, 64, (101, 128, 131, 200), None), (128, 20, 6, 2, 16, (101, 160), None),  # more
+    (128, 66, 4, 2, 64, (101, 192, 163, 161), 32000), (128, 130, 2, 1, 128, (129, 101, 190), 32000)])  # many, work enough
+def test_attention_prefix_value_not_held(device, t, D, T, nh, nk, page, prefixes, limit):
+    """One value group of a prefix slot that is not held, the last slot's or the hundredth before the drafts: NaN in
+    that group's dims of every row of its kv head, whichever tile the slot falls into, and nowhere else."""
+    print(f"prefix value not held: type {t} D {D} T {T} heads {nh}/{nk} prefixes {prefixes}", flush=True)
+    rng = np.random.default_rng([D, T, nh, t])
+    n = len(prefixes)
+    pool = filled(rng, [m + T for m in prefixes], page, nk, D, extra=0 if limit is None else (limit + T) // page + 1)
+    clean = caches(pool, max(prefixes) + T)
+    spoilt = np.zeros((n, nk, D), bool)
+    for s, P in enumerate(prefixes):
+        slot, h, g = P - 1 if s % 2 == 0 else P - 100, s % nk, (s // 2) % (D // 32)
+        at = pool.where(s, slot)
+        pool.blocks()[3][1, at[0], h, at[1]].view(np.uint32)[g] = 0x7E000000
+        spoilt[s, h, 32 * g:32 * g + 32] = True
+    p = upload(pool)
+    kv = caches(pool, max(prefixes) + T)
+    q = decode(encode(rng.normal(size=(n, T, nh, D)), t), t)
+    for chain in (True, False):
+        sees = np.stack([np.tril(np.ones((T, T), bool)) if chain else tree_bits(rng, T) for _ in range(n)])
+        got, _ = attend(p, t, q, T, prefixes, None, None if chain else sees, nh, max_prefix=limit)
+        want, bound = tree64(q, kv, prefixes, [T] * n, sees, D ** -0.5, t)
+        without, off = tree64(q, clean, prefixes, [T] * n, sees, D ** -0.5, t)
+        by_head = np.repeat(spoilt, nh // nk, 1)[:, None]
+        assert np.array_equal(np.isnan(want), np.broadcast_to(by_head, want.shape))
+        close(got, want, bound, "spoilt")
+        close(np.where(by_head, 0.0, got), np.where(by_head, 0.0, without), off, "the rest")
+
+
 @pytest.mark.parametrize("T,nh", [(1, 8), (3, 8), (20, 8)])
 def test_attention_without_a_page(device, T, nh):
     """Slots whose page is outside the pool hold NaN: sequences that reach one are NaN, others and rows past the slots
