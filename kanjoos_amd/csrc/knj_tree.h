@@ -990,18 +990,21 @@ hipError_t launch_format(const TreeArgs& a, const TreePlan& p, int cols, hipStre
     }                                                                                                    \
     return hipGetLastError();                                                                            \
   }
+// (Shapes of pages that are not built are those of launch_pages_step and launch_pages_wide; `plan`
+// asserts that it gives none of them to this.)
 #define KNJ_TREE_COLS(DD, FORMAT, SPLIT)                                                             \
   do {                                                                                               \
-    if constexpr (FORMAT != kFormatPages) { /* (pages: launch_pages_step) */                         \
-      if (cols == 16) {                                                                              \
-        KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, 1, 1, 4, 16);                                             \
-        break;                                                                                       \
-      }                                                                                              \
+    if (cols == 16) {                                                                                \
+      if constexpr (FORMAT != kFormatPages) KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, 1, 1, 4, 16);         \
+      else return hipErrorInvalidValue;                                                              \
+    } else if (cols == 32) {                                                                         \
+      KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, 1, 2, 2, 32);                                               \
+    } else if (SPLIT || cols == 64) {                                                                \
+      KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, 2, 2, 2, 32);                                               \
+    } else {                                                                                         \
+      if constexpr (FORMAT != kFormatPages || DD == 64) KNJ_TREE_LAUNCH(DD, FORMAT, false, 2, 4, 1, 64); \
+      else return hipErrorInvalidValue;                                                              \
     }                                                                                                \
-    if (cols == 32) KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, 1, 2, 2, 32);                                 \
-    else if (SPLIT || cols == 64) KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, 2, 2, 2, 32);                   \
-    else if constexpr (FORMAT != kFormatPages || DD == 64) /* (pages: launch_pages_wide) */          \
-      KNJ_TREE_LAUNCH(DD, FORMAT, false, 2, 4, 1, 64);                                               \
   } while (0)
 #define KNJ_TREE_LAUNCH(DD, FORMAT, SPLIT, NT, WC, WS, SW) \
   KNJ_LAUNCH((k_tree<DD, FORMAT, SPLIT, NT, WC, WS, SW>), grid, dim3(64 * WC * WS), 0, s, a, p)

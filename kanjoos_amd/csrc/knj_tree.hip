@@ -173,6 +173,8 @@ Planned plan_step(const knj_kv_cache& c, int n_head, int n_rows, int max_prefix)
 // no fewer than the slots before them: 500 rows, nothing before (4,000) 27.4 against 47.9,
 // 300 before 34.5 against 64.1, 200 rows and nothing before (800) 16.4 against 16.2.
 constexpr int64_t kPagesWork = 7000, kPagesPrompt = 1500;
+static_assert(kPagesWork <= kWideWorkPages && kPagesPrompt <= kWideWorkPages,
+              "over pages of heads of 128 k_tree has no tile of 128 columns: launch_pages_wide takes them first");
 Planned plan_wide(const knj_kv_cache& c, int n_head, int n_rows, int max_prefix) {
   const int n_cols = n_rows * (n_head / c.n_head_kv), steps = (max_prefix + n_rows + kWideStep - 1) / kWideStep;
   const int cols = 16 * kWideWaves, tiles = (n_cols + cols - 1) / cols;
