@@ -311,7 +311,7 @@ uint64_t knj_token_logprobs_workspace(int n_rows, int n_vocab);
  *   (all but reserve, fork and free) take NULL there.
  * page_size: a power of two from 16 to 256.  n_layer at most 1024, n_seq at most 4096, n_head_kv
  *   at most 64, n_page below 2^26, n_table * page_size below 2^31 - 256, n_seq * n_table below
- *   2^31.  data is 16-byte aligned.
+ *   2^31 - 1024.  data is 16-byte aligned.
  * knj_pages_bytes: bytes of data (0: sizes that are refused); pointers are not looked at. */
 typedef struct knj_kv_pages {
   void* data;

@@ -696,7 +696,8 @@ static int check_page_sizes(const knj_kv_pages* p) {
   KNJ_CHECK_ARG(p->n_seq > 0 && p->n_seq <= kMaxSeq, "n_seq must be in [1, 4096]");
   KNJ_CHECK_ARG(p->n_table > 0 && (int64_t)p->n_table * p->page_size < kMaxSlots,
                 "n_table must be positive and its slots fewer than 2^31 - 256");
-  KNJ_CHECK_ARG((int64_t)p->n_seq * p->n_table < (1ll << 31), "the table must have fewer than 2^31 entries");
+  // (k_pages_plan's threads count entries in 32 bits, kPlan further than the last)
+  KNJ_CHECK_ARG((int64_t)p->n_seq * p->n_table < (1ll << 31) - kPlan, "the table must have fewer than 2^31 - 1024 entries");
   return KNJ_OK;
 }
 

@@ -102,6 +102,21 @@ def test_pool_refusals(kw, match):
         assert getattr(K.lib(), f)(None) == 0
 
 
+def test_most_entries():
+    """Entries are counted in 32 bits, 1024 at a time: a table whose last step would pass 2^31 is refused."""
+    def kw(entries, n_seq):
+        return dict(n_seq=n_seq, n_table=entries // n_seq, n_page=2 ** 20, page_size=16)
+    most = pages(**kw(2 ** 31 - 1025, 3729))
+    assert most.desc.n_seq * most.desc.n_table == 2 ** 31 - 1025
+    assert K.lib().knj_pages_bytes(most.ref) > 0 and K.pages_workspace(most) > 0
+    for entries, n_seq in ((2 ** 31 - 1024, 4064), (2 ** 31 - 128, 4095), (2 ** 31 - 512, 4094)):
+        p = pages(**kw(entries, n_seq))
+        assert p.desc.n_seq * p.desc.n_table == entries
+        for call in every_call(p):
+            refused(call, "entries")
+        assert K.lib().knj_pages_bytes(p.ref) == 0 and K.pages_workspace(p) == 0
+
+
 def test_missing_tables():
     for call in every_call(pages(table=None))[:-2]:
         refused(call, "null")
