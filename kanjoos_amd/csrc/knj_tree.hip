@@ -166,14 +166,26 @@ Planned plan_step(const knj_kv_cache& c, int n_head, int n_rows, int max_prefix)
 }
 
 // Of launch_pages_wide, for heads of 128 and more than 64 columns: two workgroups a CU (one and
-// three: 141 and 129 us for 500 rows x 32 heads over 8000 slots, 121 with two).  It wins over
-// k_tree where there is work enough, in chunks of 32-column tiles: at 5,400, 7,028, 8,064 and
-// 9,216 of them 39.1, 32.1, 34.7 and 40.1 us against 35.1, 33.7, 37.0 and 41.4 (f32 queries
-// cross at 8,000); and, with a chain's upper triangle left out, earlier where the rows are
-// no fewer than the slots before them: 500 rows, nothing before (4,000) 27.4 against 47.9,
-// 300 before 34.5 against 64.1, 200 rows and nothing before (800) 16.4 against 16.2.
-constexpr int64_t kPagesWork = 7000, kPagesPrompt = 1500;
-static_assert(kPagesWork <= kWideWorkPages && kPagesPrompt <= kWideWorkPages,
+// three: 141 and 129 us for 500 rows x 32 heads over 8000 slots, 121 with two).  It against
+// k_tree, bf16, rows x query heads a kv head, in us:
+// - where there is work enough, in chunks of 32-column tiles: at 5,400, 7,028, 8,064 and 9,216 of
+//   them (25 drafts) 39.1, 32.1, 34.7 and 40.1 against 35.1, 33.7, 37.0 and 41.4 (f32 queries
+//   cross at 8,000);
+// - with more than 2,048 columns, 64 of k_tree's tiles, whatever the work: those of one split
+//   and kv head share an XCD, whose 32 CUs hold two each.  At 2,080 (260 x 8 of 4 kv heads,
+//   nothing before) 22.1 against 28.1, 2,240 (70 x 32 of one, 1,500 before) 30.5 and 30.9, 2,400
+//   (300 x 8 of 4, 800 before) 30.0 and 56.7; at 1,920 (60 x 32 of one, 1,500 before) 27.4 and
+//   19.6, 2,000 (250 x 8 of 4, 250 before; 500 x 4 of 8, 200 before) 25.9 and 34.5 against 22.4
+//   and 30.2;
+// - where it has no splits to merge, from 600 chunks on: 20 sequences of 32 x 8 of 4 behind 20
+//   slots (640), 64 of 16 behind 16 (1,024) and 32 of 64 behind 64 (4,096) 10.6, 10.8 and 19.8
+//   against 12.1, 14.4 and 31.5; 16 of 32 behind 30 (512) 10.3 against 8.5.  (In splits 4 of 100
+//   behind 100, 1,600, take 25.0 against 14.7, 8 of 25 behind 900, 3,360, 25.3 against 21.5.)
+// With a mask, which leaves no upper triangle out, they cross at the same places (2,000 and 2,080
+// columns 26.8 and 23.6 against 22.7 and 28.9).
+constexpr int64_t kPagesWork = 7000, kPagesUnsplit = 600;
+constexpr int kPagesCols = 2048;
+static_assert(kPagesWork <= kWideWorkPages && kPagesUnsplit <= kPagesWork,
               "over pages of heads of 128 k_tree has no tile of 128 columns: launch_pages_wide takes them first");
 Planned plan_wide(const knj_kv_cache& c, int n_head, int n_rows, int max_prefix) {
   const int n_cols = n_rows * (n_head / c.n_head_kv), steps = (max_prefix + n_rows + kWideStep - 1) / kWideStep;
@@ -194,9 +206,10 @@ Planned plan(const knj_kv_cache& c, int type, int n_head, int n_rows, int max_pr
       (n_cols <= 16 || (n_cols <= 32 && (units * tiles32 >= kStepWork || (tiles32 <= kStepMerges && units >= kStepUnits)))))
     return plan_step(c, n_head, n_rows, max_prefix);
   const int64_t work = units * ((n_cols + 31) / 32) * chunks;
-  if (c.format == kFormatPages && c.head_dim == 128 && n_cols > 64 &&
-      work >= (n_rows >= max_prefix ? kPagesPrompt : kPagesWork))
-    return plan_wide(c, n_head, n_rows, max_prefix);
+  if (c.format == kFormatPages && c.head_dim == 128 && n_cols > 64) {
+    const Planned q = plan_wide(c, n_head, n_rows, max_prefix);
+    if (n_cols > kPagesCols || work >= (q.p.n_split == 1 ? kPagesUnsplit : kPagesWork)) return q;
+  }
   int cols = n_cols <= 16 ? 16 : 32;
   const int64_t wide = c.format == KNJ_KV_F16 ? kWideWorkF16 : c.format == kFormatPages ? kWideWorkPages : kWideWork;
   if (n_cols > 32 && work >= wide)

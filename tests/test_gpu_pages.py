@@ -478,6 +478,36 @@ def test_attention_many_columns_chain(device, t, T, nh, prefixes, loose):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("T,nh,nk,page,prefixes", [
+    (20, 32, 4, 16, tuple(range(33))), (16, 48, 4, 32, (0, 1, 15, 17, 48) * 8), (40, 16, 4, 16, (0, 30, 60, 88) * 14),  # no merge
+    (70, 32, 1, 64, (0, 61)), (17, 128, 1, 16, (0,)), (260, 8, 1, 32, (30,))])  # more than 2048 columns
+def test_attention_many_columns_short(device, t, T, nh, nk, page, prefixes):
+    """Many columns over few slots, of many sequences (no split to merge) or of one (more columns than an XCD holds at
+    once): trees and chains, sequences with fewer rows; a sample of the rows is compared."""
+    print(f"many columns, short: type {t} T {T} heads {nh}/{nk} prefixes {len(prefixes)}", flush=True)
+    rng = np.random.default_rng([T, nh, page, t])
+    n, D = len(prefixes), 128
+    pool = filled(rng, [m + T for m in prefixes], page, nk, D)
+    p = upload(pool)
+    kv = caches(pool, max(prefixes) + T)
+    counts = np.array([T if s % 3 == 0 else max(T - s, 0) for s in range(n)])
+    q = decode(encode(1.5 * rng.normal(size=(n, T, nh, D)), t), t)
+    trees = np.stack([tree_bits(rng, T) for _ in range(n)])
+    trees[:, 1] = False  # the prefix alone
+    below = np.tril(np.ones((T, T), bool))
+    for sees, mask in ((trees, trees), (np.stack([below] * n), None)):
+        got, before = attend(p, t, q, T, prefixes, counts, mask, nh, pad=16)
+        for s in range(n):
+            assert np.array_equal(got[s, counts[s]:], before[s, counts[s]:])  # rows past the drafts
+            h = np.unique(rng.integers(0, nh, 4))  # (heads one by one: each has its kv head's cache)
+            for x in h if counts[s] else []:
+                one = [c[s:s + 1, x * nk // nh:x * nk // nh + 1] for c in kv]
+                want, bound = tree64(q[s:s + 1, :, x:x + 1], one, [prefixes[s]], [counts[s]], sees[s:s + 1], D ** -0.5, t)
+                close(got[s:s + 1, :counts[s], x:x + 1], want[:, :counts[s]], bound[:, :counts[s]], f"sequence {s} head {x}")
+    assert np.array_equal(attend(p, t, q, T, prefixes, counts, below[None], nh, shared=True, pad=16)[0], got)
+
+
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("rising", [True, False])
 def test_attention_many_columns_drifting(device, t, rising):
     """Scores that rise or fall along the slots by far more than f16 or an exponent's reference holds; a sequence
