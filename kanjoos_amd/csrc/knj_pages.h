@@ -33,7 +33,8 @@ __device__ __forceinline__ void group_word(uint32_t m, hx2& step, hx2& low) {
   low = hx2{w[1], w[1]};
 }
 
-// Eight codes as f16(low + step * code), one rounding each, in order of the dims.  A
+// Eight codes as f16(low + step * code), one rounding each, in order of the dims: of rows that
+// are loaded, and of k_tree, whose operands take any cache's rows in that order.  A
 // code's bits become the low bits of 1024's significand, or, four bits up, of 64's
 // (steps of 1 and of 1/16: 64 + code), from which the offset is taken off exactly.
 // The two exponents are kept in vector registers, so that one instruction masks and joins
@@ -54,8 +55,10 @@ struct Decoder {
   }
 };
 
-// The same in the order 0 4 1 5 2 6 3 7 of the dims: a code as a byte is the e4m3 number code
-// * 2^-9 (subnormal or not), which the conversion of two takes back to the whole number.
+// The same in the order 0 4 1 5 2 6 3 7 of the dims, for kernels that pack their queries and
+// put their results in order to suit (pack_queries, in_order): a code as a byte is the e4m3
+// number code * 2^-9 (subnormal or not), which the conversion of two takes back to the whole
+// number.
 __device__ __forceinline__ uint4 decode8_mixed(uint32_t w, hx2 step, hx2 low) {
   const uint32_t a = w & 0x0F0F0F0Fu, b = (w >> 4) & 0x0F0F0F0Fu;
   auto value = [&](hx2 x) { return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x, step, low)); };

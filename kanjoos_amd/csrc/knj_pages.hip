@@ -24,7 +24,8 @@ using Piece = std::conditional_t<D == 128, u32v4, u32v2>;
 // A row's kv head is D/8 lanes of eight dims, four lanes a group of 32; the same lanes
 // take its key and its value.  blockIdx.y is the sequence.  Each element is read once and
 // written once: 4096 f32 rows of 4 kv heads, 19.4 MB either way, 7.1 us a call (2.7 TB/s, half
-// of it the launch's own latency; one row of 32 sequences takes 3.5 and 2.4).
+// of it the launch's own latency; one row of 32 sequences takes 3.5 and 2.4; 65,536 rows, 310 MB,
+// stored 56 and loaded 63, 5.6 and 4.9 TB/s).
 template <int D>
 struct PageUnit {
   static constexpr int T = D / 8;
@@ -246,7 +247,11 @@ __device__ __forceinline__ int ld_agent(const int32_t* p) {
 // sequences (lowest page first, all or none), and the entries of a step are few.  The
 // asked entries of all sequences are numbered through, and each thread takes every
 // 1024th.  Nothing but latency: 5 to 6 us for 4 to 32 sequences, a chain of lengths, table,
-// holders and stores with ten barriers between them.
+// holders and stores with ten barriers between them, while enough free pages lie among the
+// first 4096, whose counts are fetched ahead.  Each 4096 further are a round trip more: with the
+// free pages last, a call over 4,000, 60,000, 250,000 and 1,000,000 pages takes 6, 24, 86 and
+// 326 us.  So do entries past the first 1024, which each pass looks up anew: 1,024, 4,032 and
+// 32,256 of them 7, 15 and 119 us.
 __global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
   const PageGeom& g = a.g;
   const ReserveWs ws(a.ws, g.n_page);
@@ -437,7 +442,10 @@ __global__ __launch_bounds__(kPlan) void k_pages_plan(PageReserveArgs a) {
 
 // The first rows of pages copied, a layer per blockIdx.y, kBlock units of a page a
 // workgroup: units of D/8 bytes, of a row four of key codes, four of value codes and one
-// of either's words.  (Where nothing or one page a sequence is copied, 1.6 to 4 us, a launch.)
+// of either's words.  (Where nothing or one page a sequence is copied, 1.6 to 4 us, a launch.
+// One load a thread is in flight, behind the count, the copy's entry and its rows: a reservation
+// that copies 250 pages of 41 KB in 48 layers takes 262 us, 3.7 TB/s, where k_pages_copy, with
+// four, moves them in 182.)
 template <int D>
 __global__ __launch_bounds__(kBlock) void k_pages_cow(PageGeom g, int32_t* words, uint32_t pieces) {
   using P = Piece<D>;
@@ -468,7 +476,8 @@ __global__ __launch_bounds__(kBlock) void k_pages_cow(PageGeom g, int32_t* words
 // been read, and the next batch is fetched while this one is written.
 // What bounds it: memory.  8000 of 16,000 slots, at random, in 48 layers of 4 kv heads are
 // 246 MB of rows, but lie in three quarters of the codes' lines of 128 bytes and in all of the
-// words': 450 MB fetched and 218 written by the counters, 120 us a call, 5.6 TB/s.
+// words': by the counters 3.07 million lines, 393 MB, read and 246 MB written, 132 us a call,
+// 4.8 TB/s (4858 and 6984 kept 86 and 118).
 struct MoveArgs {
   PageGeom g;
   const int32_t *start, *rows, *counts;

@@ -19,8 +19,9 @@ namespace {
 //
 // What bounds it (500 rows x 32 heads over 8000 slots of 4 kv heads, 68 GFLOP and half
 // as many for the remainders: 120 us a call, 8 of them the merge, 0.56 PFLOP/s): a SIMD's
-// products take 43 % of its cycles and its other vector instructions 43 %, which hardly
-// overlap on one SIMD, whichever waves they come from.  Of a wave's vector instructions a
+// products take 43 % of its cycles and its other vector instructions 43 %, one after the
+// other (a loop of a step's 48 products and 180 other instructions alone, four waves a SIMD:
+// 344 and 311 ns a wave apart, 560 together).  Of a wave's vector instructions a
 // step (180) 48 form the weights, 32 split them and 44 decode its share of the rows.  Hence
 // many columns to a workgroup: k_tree with as many in four waves, which decode twice as much
 // each, takes 135.  Nothing gained: codes by DMA, decoded behind the products or between
