@@ -505,6 +505,9 @@ def test_attention_many_columns_short(device, t, T, nh, nk, page, prefixes):
                 want, bound = tree64(q[s:s + 1, :, x:x + 1], one, [prefixes[s]], [counts[s]], sees[s:s + 1], D ** -0.5, t)
                 close(got[s:s + 1, :counts[s], x:x + 1], want[:, :counts[s]], bound[:, :counts[s]], f"sequence {s} head {x}")
     assert np.array_equal(attend(p, t, q, T, prefixes, counts, below[None], nh, shared=True, pad=16)[0], got)
+    again, _ = attend(p, t, q, T, prefixes, counts, None, nh, pad=16, in_place=True)
+    for s in range(n):
+        assert np.array_equal(again[s, :counts[s]], got[s, :counts[s]])
 
 
 @pytest.mark.parametrize("t", TYPES)
